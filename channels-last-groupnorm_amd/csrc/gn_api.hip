@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "../../include/gnnhwc.h"
+#include "gn_error.h"
 #include "gn_host.h"
 
 namespace gn {
@@ -19,6 +20,7 @@ namespace {
 
 thread_local char g_error[512] = "";
 
+}  // namespace
 int fail(int code, const char *fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -26,6 +28,7 @@ int fail(int code, const char *fmt, ...) {
   va_end(ap);
   return code;
 }
+namespace {
 
 int env_int(const char *name, int fallback) {
   const char *v = getenv(name);

@@ -1,0 +1,275 @@
+// Rotary positions with several axes, optionally behind a root-mean-square norm of each head.
+//
+//   (u, v) -> (u cos a - v sin a, u sin a + v cos a),    a = position[axis of the pair] * frequency[pair]
+// backward (the turn is orthogonal): the gradient turned by -a; behind a norm, with d that gradient, h = t r and g = d w,
+//   dt = r (g - h mean(g h)),        dw = sum over heads and tokens of d h
+//
+// Memory bounds them: q and k are read once and written once; angles come from a position and P frequencies per token and
+// are not read from tables.  A group of lanes (a power of two, W >= pairs / S) takes one head at a time, each lane S pairs as
+// two lane vectors; it turns every `groups`-th head of its token, so that one set of sines and cosines serves several heads
+// and neighbouring groups read neighbouring memory.
+#pragma once
+#include "gn_rms.h"
+
+namespace gn {
+
+// sin and cos of pos * freq.  The product is carried as an exact pair of floats and turned into revolutions with 1 / (2 pi) as
+// a pair, so that the reduction loses nothing however long the angle is; then polynomials in z^2 on an eighth of a revolution
+// (fits at Chebyshev nodes, errors 2.5e-9 and 5e-11).  About 30 instructions, where a float sine of a long angle takes a loop.
+__device__ __forceinline__ void angle_sincos(float pos, float freq, float &sn, float &cs) {
+  float p = pos * freq;
+  pin(p);  // (the products and the errors below must be the rounded ones')
+  const float pl = __builtin_fmaf(pos, freq, -p);
+  constexpr float kTurn = 0.15915494f, kTurnLow = (float)(0.15915494309189533577 - (double)0.15915494f);
+  float t = p * kTurn;
+  pin(t);
+  const float low = __builtin_fmaf(p, kTurn, -t) + (p * kTurnLow + pl * kTurn);
+  const float r = (t - __builtin_rintf(t)) + low;
+  const float m = __builtin_rintf(4.0f * r);
+  const float z = __builtin_fmaf(m, -0.25f, r), z2 = z * z;
+  const float s = z * __builtin_fmaf(z2, __builtin_fmaf(z2, __builtin_fmaf(z2, -75.39976950f, 81.59250773f), -41.34166241f), 6.283185288f);
+  const float c = __builtin_fmaf(z2, __builtin_fmaf(z2, __builtin_fmaf(z2, __builtin_fmaf(z2, 59.21866124f, -85.44280388f), 64.93931580f), -19.73920865f), 1.0f);
+  const int quarter = (int)m;
+  const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
+  sn = quarter & 2 ? -a : a;
+  cs = (quarter + 1) & 2 ? -b : b;
+}
+__device__ __forceinline__ void angle_sincos(double pos, double freq, double &sn, double &cs) {
+  const double a = pos * freq;
+  sn = sin(a);
+  cs = cos(a);
+}
+
+__device__ __forceinline__ float position_at(const void *p, int64_t i, int type) {
+  switch (type) {
+    case 0: return (float)load_global<int32_t>((const int32_t *)p + i);
+    case 1: return (float)load_global<int64_t>((const int64_t *)p + i);
+    default: return load_global<float>((const float *)p + i);
+  }
+}
+
+// The pairs of one lane: S of them as two lane vectors of S channels.
+template <typename T, int S, bool NEAR> struct PairLane {
+  using A = acc_of_t<T>;
+  int j0, at0, at1, P;
+  __device__ __forceinline__ PairLane(const RotaryArgs &q, int lane) : P(q.P) {
+    const int v = lane < q.nvec ? lane : q.nvec - 1;  // spare lanes repeat the last vector and store nothing
+    j0 = v * S;
+    const bool far = !NEAR && j0 < P;  // (S divides P where pairs are far)
+    at0 = far ? j0 : 2 * j0;
+    at1 = far ? j0 + P : 2 * j0 + S;
+  }
+  __device__ __forceinline__ void angles(const RotaryArgs &q, int b, int l, A (&sn)[S], A (&cs)[S]) const {
+    const int64_t at = (int64_t)b * q.pos_stride[0] + (int64_t)l * q.pos_stride[1];
+    float pos[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) pos[a] = a < q.axes ? position_at(q.pos, at + a, q.pos_type) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int j = j0 + i;
+      const float f = load_global<float>(q.freq + (j < P ? j : P - 1));
+      float p = pos[0];
+#pragma unroll
+      for (int a = 1; a < 4; ++a) p = j >= q.ends[a - 1] && a < q.axes ? pos[a] : p;
+      angle_sincos((A)p, (A)f, sn[i], cs[i]);
+      sn[i] *= (A)q.sign;
+    }
+  }
+  __device__ __forceinline__ void load(const T *p, typename LaneVec<T, S>::raw_t (&r)[2]) const {
+    r[0] = load_loose<LaneVec<T, S>>(p + at0);
+    r[1] = load_loose<LaneVec<T, S>>(p + at1);
+  }
+  __device__ __forceinline__ static void unpack(const typename LaneVec<T, S>::raw_t (&r)[2], A (&v)[2 * S]) {
+    A t[S];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      LaneVec<T, S>::unpack(r[h], t);
+#pragma unroll
+      for (int i = 0; i < S; ++i) v[h * S + i] = t[i];
+    }
+  }
+  __device__ __forceinline__ void store(T *p, const A (&v)[2 * S]) const {
+    A t[S];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < S; ++i) t[i] = v[h * S + i];
+      store_loose<LaneVec<T, S>>(p + (h ? at1 : at0), LaneVec<T, S>::pack(t));
+    }
+  }
+  template <typename W> __device__ __forceinline__ void weights(const W *w, A (&v)[2 * S]) const {
+    A t[S];
+    load_params<W, S>(w + at0, t);
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[i] = t[i];
+    load_params<W, S>(w + at1, t);
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[S + i] = t[i];
+  }
+  // (channels behind the pairs are selected, not multiplied by one and zero: an infinity there stays one)
+  __device__ __forceinline__ void turn(A (&v)[2 * S], const A (&sn)[S], const A (&cs)[S], bool partial) const {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      A &x = v[NEAR ? 2 * i : i], &y = v[NEAR ? 2 * i + 1 : S + i];
+      const A u = x * cs[i] - y * sn[i], w = x * sn[i] + y * cs[i];
+      const bool keep = partial && j0 + i >= P;
+      x = keep ? x : u;
+      y = keep ? y : w;
+    }
+  }
+};
+
+// Heads of one token for one group of lanes.
+struct HeadWalk {
+  bool live;
+  int which, first, step, count, b, l;  // which: 0 q, 1 k; heads first, first + step, ...
+};
+__device__ __forceinline__ HeadWalk head_walk(const RotaryArgs &q, int group) {
+  HeadWalk w;
+  w.live = group < q.tokens * q.groups;
+  group = w.live ? group : 0;
+  const int token = div_by(group, q.by_groups);
+  const int g = group - token * q.groups;
+  w.which = g >= q.side[0].groups ? 1 : 0;
+  w.first = w.which ? g - q.side[0].groups : g;
+  w.step = w.which ? q.side[1].groups : q.side[0].groups;
+  w.count = w.which ? q.side[1].heads : q.side[0].heads;
+  w.b = div_by(token, q.by_L);
+  w.l = token - w.b * q.L;
+  return w;
+}
+// q's or k's tensors, field by field: both are scalar loads of the argument block and a selection.
+struct Side {
+  const void *in, *grad, *weight;
+  void *out;
+  int64_t in_stride[3], grad_stride[3], out_stride[3];
+};
+__device__ __forceinline__ Side side_of(const RotaryArgs &q, int which) {
+  const RotarySide &a = q.side[0], &b = q.side[1];
+  Side s;
+  s.in = which ? b.in : a.in;
+  s.grad = which ? b.grad : a.grad;
+  s.weight = which ? b.weight : a.weight;
+  s.out = which ? b.out : a.out;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    s.in_stride[i] = which ? b.in_stride[i] : a.in_stride[i];
+    s.grad_stride[i] = which ? b.grad_stride[i] : a.grad_stride[i];
+    s.out_stride[i] = which ? b.out_stride[i] : a.out_stride[i];
+  }
+  return s;
+}
+__device__ __forceinline__ int64_t head_at(const int64_t (&s)[3], int b, int l) { return b * s[0] + l * s[1]; }
+
+template <typename T, typename P, int S, bool NEAR, bool NORM>
+__global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
+  using A = acc_of_t<T>;
+  constexpr int kHeads = 4;  // heads whose loads are in flight together
+  const int lane = threadIdx.x & (q.lanes - 1);
+  const HeadWalk walk = head_walk(q, (int)(blockIdx.x * (kBlock >> q.lanes_log2)) + (int)(threadIdx.x >> q.lanes_log2));
+  const PairLane<T, S, NEAR> pl(q, lane);
+  const Side side = side_of(q, walk.which);
+  const bool stores = walk.live && lane < q.nvec, partial = 2 * q.P < q.D;
+  const T *in = (const T *)side.in + head_at(side.in_stride, walk.b, walk.l);
+  T *out = (T *)side.out + head_at(side.out_stride, walk.b, walk.l);
+  const int64_t in_head = side.in_stride[2], out_head = side.out_stride[2];
+  A sn[S], cs[S], w[2 * S];
+  pl.angles(q, walk.b, walk.l, sn, cs);
+  if constexpr (NORM) pl.weights((const P *)side.weight, w);
+  for (int h0 = walk.first; h0 < walk.count; h0 += kHeads * walk.step) {
+    typename LaneVec<T, S>::raw_t r[kHeads][2];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int h = h0 + i * walk.step;
+      if (h < walk.count) pl.load(in + h * in_head, r[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int h = h0 + i * walk.step;
+      A v[2 * S];
+      pl.unpack(r[i], v);
+      if constexpr (NORM) {
+        A ss = 0;
+#pragma unroll
+        for (int c = 0; c < 2 * S; ++c) ss += v[c] * v[c];
+        ss = segment_sum(lane < q.nvec ? ss : (A)0, q.lanes);
+        const A rstd = exact_rsqrt(ss * (A)q.inv_d + (A)q.eps);
+#pragma unroll
+        for (int c = 0; c < 2 * S; ++c) v[c] = v[c] * rstd * w[c];
+      }
+      pl.turn(v, sn, cs, partial);
+      if (stores && h < walk.count) pl.store(out + h * out_head, v);
+    }
+  }
+}
+
+// Backward behind a norm.  A group keeps its place among the heads (and so q or k) while it walks over tokens, and its share
+// of dw in registers; a workgroup leaves one partial row of 2 D values (q's, k's).
+template <typename T, typename P, int S, bool NEAR>
+__global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArgs q) {
+  using A = acc_of_t<T>;
+  extern __shared__ char lds_dyn[];
+  const int lane = threadIdx.x & (q.lanes - 1), sub = threadIdx.x >> q.lanes_log2, subs = kBlock >> q.lanes_log2;
+  const PairLane<T, S, NEAR> pl(q, lane);
+  const bool partial = 2 * q.P < q.D;
+  const int start = (int)blockIdx.x * subs + sub;
+  // (groups that do not fill a whole set of heads stay idle)
+  HeadWalk walk = head_walk(q, start < q.walkers ? start : 0);
+  const bool works = start < q.walkers;
+  const Side side = side_of(q, walk.which);
+  A w[2 * S], dw[2 * S], sn[S], cs[S];
+  pl.weights((const P *)side.weight, w);
+#pragma unroll
+  for (int c = 0; c < 2 * S; ++c) dw[c] = 0;
+  int token = div_by(works ? start : 0, q.by_groups);
+  if (works)
+    for (; token < q.tokens; token += q.token_step) {
+      const int b = div_by(token, q.by_L), l = token - b * q.L;
+      pl.angles(q, b, l, sn, cs);
+      const T *in = (const T *)side.in + head_at(side.in_stride, b, l), *grad = (const T *)side.grad + head_at(side.grad_stride, b, l);
+      T *out = (T *)side.out + head_at(side.out_stride, b, l);
+      for (int h = walk.first; h < walk.count; h += walk.step) {
+        typename LaneVec<T, S>::raw_t rt[2], rd[2];
+        pl.load(in + h * side.in_stride[2], rt);
+        pl.load(grad + h * side.grad_stride[2], rd);
+        A t[2 * S], d[2 * S], ss = 0, gt = 0;
+        pl.unpack(rt, t);
+        pl.unpack(rd, d);
+        pl.turn(d, sn, cs, partial);
+#pragma unroll
+        for (int c = 0; c < 2 * S; ++c) {
+          ss += t[c] * t[c];
+          gt += d[c] * w[c] * t[c];
+        }
+        if (lane >= q.nvec) ss = gt = 0;
+        segment_sum2(ss, gt, q.lanes);
+        const A r = exact_rsqrt(ss * (A)q.inv_d + (A)q.eps), m = r * gt * (A)q.inv_d;
+#pragma unroll
+        for (int c = 0; c < 2 * S; ++c) {
+          const A hn = t[c] * r;
+          dw[c] += d[c] * hn;
+          d[c] = r * (d[c] * w[c] - hn * m);
+        }
+        if (lane < q.nvec) pl.store(out + h * side.out_stride[2], d);
+      }
+    }
+  // the workgroup's groups, q's and k's apart
+  A *box = (A *)lds_dyn;  // [subs][D]
+  int *kind = (int *)(box + subs * q.D);
+  if (lane < q.nvec)
+#pragma unroll
+    for (int c = 0; c < S; ++c) {
+      box[sub * q.D + pl.at0 + c] = dw[c];
+      box[sub * q.D + pl.at1 + c] = dw[S + c];
+    }
+  if (lane == 0) kind[sub] = works ? walk.which : 2;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * q.D; i += kBlock) {
+    const int which = i >= q.D ? 1 : 0, c = i - which * q.D;
+    A acc = 0;
+    for (int g = 0; g < subs; ++g) acc += kind[g] == which ? box[g * q.D + c] : (A)0;
+    store_global<A>((A *)q.part + (int64_t)blockIdx.x * 2 * q.D + i, acc);
+  }
+}
+
+}  // namespace gn

@@ -1,0 +1,87 @@
+// Kernels of the rotary positions (gn_rotary.h) instantiated and launched for ONE element type, selected with
+// -DGN_INST_DTYPE=0..3 (f32, f64, f16, bf16).
+#include "gn_rotary.h"
+
+#ifndef GN_INST_DTYPE
+#error "compile with -DGN_INST_DTYPE=<0|1|2|3>"
+#endif
+
+namespace gn {
+
+#if GN_INST_DTYPE == 0
+typedef float elem_t;
+typedef float wide_param_t;
+#define GN_SUFFIX f32
+#elif GN_INST_DTYPE == 1
+typedef double elem_t;
+typedef double wide_param_t;
+#define GN_SUFFIX f64
+#elif GN_INST_DTYPE == 2
+typedef f16_t elem_t;
+typedef float wide_param_t;
+#define GN_SUFFIX f16
+#else
+typedef bf16_t elem_t;
+typedef float wide_param_t;
+#define GN_SUFFIX bf16
+#endif
+#define GN_CAT2(a, b) a##b
+#define GN_CAT(a, b) GN_CAT2(a, b)
+
+namespace {
+
+typedef acc_of_t<elem_t> A;
+
+template <typename P, int S, bool NEAR> void launch_one(const RotaryArgs &a, bool norm, hipStream_t stream) {
+  const int per_block = kBlock >> a.lanes_log2;
+  const dim3 grid((unsigned)(((int64_t)a.tokens * a.groups + per_block - 1) / per_block));
+  if (norm) hipLaunchKernelGGL((rotary_kernel<elem_t, P, S, NEAR, true>), grid, dim3(kBlock), 0, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<elem_t, P, S, NEAR, false>), grid, dim3(kBlock), 0, stream, a);
+}
+template <typename P, int S, bool NEAR> void launch_bwd(const RotaryArgs &a, int blocks, hipStream_t stream) {
+  const int per_block = kBlock >> a.lanes_log2;
+  const size_t lds = (size_t)per_block * a.D * sizeof(A) + (size_t)per_block * sizeof(int);
+  hipLaunchKernelGGL((rotary_norm_bwd_kernel<elem_t, P, S, NEAR>), dim3((unsigned)blocks), dim3(kBlock), lds, stream, a);
+}
+// Calls f<pairs a lane, near>() for the pairs that the plan chose.
+template <typename F> void with_pairs(int pairs, bool near, F &&f) {
+  auto go = [&](auto s) {
+    if (near) f(s, std::true_type());
+    else f(s, std::false_type());
+  };
+  if (pairs == 1) return go(std::integral_constant<int, 1>());
+#if GN_INST_DTYPE == 1
+  return go(std::integral_constant<int, 2>());
+#else
+#if GN_INST_DTYPE >= 2
+  if (pairs == 8) return go(std::integral_constant<int, 8>());
+#endif
+  return go(std::integral_constant<int, 4>());
+#endif
+}
+
+}  // namespace
+
+hipError_t GN_CAT(launch_rotary_, GN_SUFFIX)(const RotaryArgs &a, int pairs, bool near, bool norm, int pdtype, hipStream_t stream) {
+  with_pairs(pairs, near, [&](auto s, auto n) {
+    if (!norm || pdtype == GN_INST_DTYPE) launch_one<elem_t, decltype(s)::value, decltype(n)::value>(a, norm, stream);
+    else launch_one<wide_param_t, decltype(s)::value, decltype(n)::value>(a, norm, stream);
+  });
+  return hipGetLastError();
+}
+
+hipError_t GN_CAT(launch_rotary_norm_bwd_, GN_SUFFIX)(const RotaryArgs &a, int pairs, bool near, int pdtype, int blocks, void *const (&dw)[2],
+                                                       hipStream_t stream) {
+  if (blocks > 0) with_pairs(pairs, near, [&](auto s, auto n) {  // (no tokens: the weights' gradients are zero)
+    if (pdtype == GN_INST_DTYPE) launch_bwd<elem_t, decltype(s)::value, decltype(n)::value>(a, blocks, stream);
+    else launch_bwd<wide_param_t, decltype(s)::value, decltype(n)::value>(a, blocks, stream);
+  });
+  for (int i = 0; i < 2; ++i) {
+    if (!dw[i]) continue;
+    const PartialSum p = {(const A *)a.part + i * a.D, dw[i], blocks, a.D, pdtype, 2 * a.D};
+    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((a.D + 15) / 16)), dim3(256), 0, stream, p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace gn

@@ -1,0 +1,110 @@
+// Host-side interface of the operators for token streams: argument blocks shared by the C ABI (gn_tokens.hip) and the
+// kernels' launchers (gn_rms.hip, gn_rotary.hip: compiled once per element type; gn_clip.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+#include "../../include/gnnhwc_tokens.h"
+#include "gn_plan.h"
+
+namespace gn {
+
+enum { GN_F8 = GNNHWC_F8E4M3, GN_I8 = GNNHWC_I8 };
+
+// Rows of the norms: C channels as nvec lane vectors, dealt to lpr = 2^lpr_log2 lanes.
+struct RowCut {
+  int vec, nvec, lpr, lpr_log2, nv, threads;
+  bool ragged;
+};
+
+struct RmsFwd {
+  const void *x, *res, *w;
+  void *sum, *y;
+  float *scales;
+  int64_t rows, x_stride, res_stride;
+  double eps, inv_c;
+  int C, nvec, lpr, lpr_log2;
+  int block_lanes, nblocks, qtype;  // quantised: lanes per scale (0: one scale per row), scales per row, type
+  float q_most;
+};
+struct RmsBwd {
+  const void *dy, *ds, *s, *w;
+  void *dx, *part;
+  int64_t rows, dy_stride, ds_stride, s_stride;
+  double eps, inv_c;
+  int C, nvec, lpr, lpr_log2;
+};
+
+struct RotarySide {  // q or k
+  const void *in, *grad, *weight;
+  void *out;
+  int64_t in_stride[3], grad_stride[3], out_stride[3];  // batch, token, head
+  int heads, groups;  // groups of lanes that share a token's heads
+};
+struct RotaryArgs {
+  RotarySide side[2];
+  const void *pos;
+  int64_t pos_stride[2];
+  const float *freq;
+  int pos_type, axes, ends[4], P, D;
+  int nvec, lanes, lanes_log2;  // lane vectors of half a head, lanes of a group
+  int tokens, L, groups;        // batch * tokens, tokens of a sample, groups of a token (q's, then k's)
+  Divisor by_groups, by_L;
+  int walkers, token_step;      // backward behind a norm: groups that work, tokens between two of a group
+  double eps, inv_d;
+  float sign;                   // -1: turn back
+  void *part;
+};
+
+// Sums of `count` rows of partial results, C values each, in a fixed order (gn_rms.hip).
+struct PartialSum {
+  const void *part;
+  void *out;
+  int count, C, out_dtype;
+  int pitch;  // values from one row to the next
+};
+
+RowCut rms_cut(int64_t C, int esize, int most_vectors, int least_lanes);
+int rms_bwd_blocks(int64_t rows, const RowCut &cut);
+constexpr int kMostChannels = 16384;
+constexpr int kFwdVectors = 8, kBwdVectors = 4;  // most lane vectors of a row per lane
+
+#define GN_DECLARE_TOKENS(S)                                                                            \
+  hipError_t launch_rms_fwd_##S(const RmsFwd &a, const RowCut &cut, int pdtype, bool quant, hipStream_t stream);   \
+  hipError_t launch_rms_bwd_##S(const RmsBwd &a, const RowCut &cut, int pdtype, int blocks, void *dw, hipStream_t stream); \
+  hipError_t launch_rotary_##S(const RotaryArgs &a, int pairs, bool near, bool norm, int pdtype, hipStream_t stream);       \
+  hipError_t launch_rotary_norm_bwd_##S(const RotaryArgs &a, int pairs, bool near, int pdtype, int blocks, void *const (&dw)[2], hipStream_t stream);
+// Gradients of one launch; the whole table travels as a kernel argument.
+struct ClipEntry {
+  const void *in;
+  void *out;
+  int64_t n;
+  unsigned first_chunk;
+  int types;  // dtype | out dtype << 8
+};
+constexpr int kClipEntries = 112;
+struct ClipTable {
+  ClipEntry e[kClipEntries];
+  int count;
+  unsigned chunks;
+};
+constexpr int kClipChunk = 8192;     // elements
+constexpr int kClipPartials = 1024;  // partial sums over all launches (and one more for each launch)
+struct ClipFinish {
+  const double *part;
+  int parts;
+  double max_norm, eps, grad_scale;
+  void *total;
+  int total_dtype;
+  bool in_place;
+};
+hipError_t launch_clip_norm(const ClipTable &t, double *part, int blocks, hipStream_t stream);
+hipError_t launch_clip_apply(const ClipTable &t, const ClipFinish &f, int blocks, hipStream_t stream);
+
+GN_DECLARE_TOKENS(f32)
+GN_DECLARE_TOKENS(f64)
+GN_DECLARE_TOKENS(f16)
+GN_DECLARE_TOKENS(bf16)
+#undef GN_DECLARE_TOKENS
+
+}  // namespace gn

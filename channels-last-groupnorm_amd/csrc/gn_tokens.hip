@@ -1,0 +1,436 @@
+// C ABI of the operators for token streams (declared in include/gnnhwc_tokens.h): argument checks, launch planning,
+// element-type dispatch.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "gn_error.h"
+#include "gn_tokens.h"
+
+namespace gn {
+namespace {
+
+int elem_size(int64_t dtype) {
+  switch (dtype) {
+    case GN_F32: return 4;
+    case GN_F64: return 8;
+    case GN_F16: return 2;
+    case GN_BF16: return 2;
+    default: return 0;
+  }
+}
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int log2_of(int v) {
+  int l = 0;
+  while ((1 << l) < v) ++l;
+  return l;
+}
+int invalid(const char *what) { return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s", what); }
+int launched(hipError_t e, const char *what) {
+  return e == hipSuccess ? GNNHWC_OK : fail(GNNHWC_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+
+int check_types(int64_t dtype, int64_t param_dtype) {
+  if (!elem_size(dtype)) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "unknown dtype code %lld", (long long)dtype);
+  const bool half = dtype == GN_F16 || dtype == GN_BF16;
+  if (param_dtype != dtype && !(half && param_dtype == GN_F32))
+    return fail(GNNHWC_ERR_INVALID_ARGUMENT, "weight dtype %lld does not go with dtype %lld (the same, or f32 for 16-bit data)",
+                (long long)param_dtype, (long long)dtype);
+  return GNNHWC_OK;
+}
+int check_rows(int64_t rows, int64_t C, int dtype, int param_dtype) {
+  if (const int rc = check_types(dtype, param_dtype)) return rc;
+  const int64_t most = dtype == GN_F64 ? kMostChannels / 2 : kMostChannels;
+  if (C < 1 || C > most)
+    return fail(GNNHWC_ERR_INVALID_ARGUMENT, "rows of %lld channels: 1 to %lld are supported", (long long)C, (long long)most);
+  if (rows < 0 || rows > 0x7fffffff)
+    return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%lld rows: 0 to 2^31 - 1 are supported", (long long)rows);
+  return GNNHWC_OK;
+}
+// (eps may be zero: a row of zeros then gives NaN, as the formula does)
+int check_eps(double eps) { return eps >= 0 && eps < INFINITY ? GNNHWC_OK : invalid("eps must be finite and not negative"); }
+
+#define GN_BY_TYPE(dtype, call)                 \
+  ((dtype) == GN_F32   ? call(f32)              \
+   : (dtype) == GN_F64 ? call(f64)              \
+   : (dtype) == GN_F16 ? call(f16)              \
+                       : call(bf16))
+
+RmsFwd fwd_args(const void *x, const void *residual, const void *weight, void *sum_out, void *y, int64_t rows, int64_t C,
+                int64_t x_stride, int64_t residual_stride, double eps, const RowCut &cut) {
+  RmsFwd a = {};
+  a.x = x; a.res = residual; a.w = weight;
+  a.sum = sum_out; a.y = y;
+  a.rows = rows; a.x_stride = x_stride; a.res_stride = residual_stride;
+  a.eps = eps; a.inv_c = 1.0 / (double)C;
+  a.C = (int)C; a.nvec = cut.nvec; a.lpr = cut.lpr; a.lpr_log2 = cut.lpr_log2;
+  return a;
+}
+int check_fwd(const void *x, const void *residual, void *sum_out, const void *y, int64_t rows) {
+  if (rows > 0 && (!x || !y)) return invalid("null tensor");
+  if (sum_out && !residual) return invalid("sum_out without a residual");
+  return GNNHWC_OK;
+}
+
+}  // namespace
+
+// How a row's lane vectors are dealt to lanes: among the powers of two that leave each lane at most `most_vectors`, the one that
+// leaves the fewest lanes idle, and of those alike the one inside a wavefront.
+RowCut rms_cut(int64_t C, int esize, int most_vectors, int least_lanes) {
+  const int vec = 16 / esize;
+  RowCut c;
+  c.vec = C < vec ? 1 : vec;
+  c.nvec = (int)ceil_div(C, c.vec);
+  c.ragged = C % c.vec != 0;
+  double best = -1;
+  c.lpr = c.nv = 0;
+  for (int lpr = std::max(8, least_lanes); lpr <= 1024; lpr <<= 1) {
+    int nv = (int)ceil_div(c.nvec, lpr);
+    if (nv == 7) nv = 8;
+    const int most = lpr > 256 ? kMostChannels / (esize == 8 ? 2 : 1) / (vec * 1024) : most_vectors;
+    if (nv > most) continue;
+    const double used = (double)c.nvec / ((double)lpr * nv) - (lpr > 64 ? 0.1 : 0.0);
+    if (used > best + 0.02) {
+      best = used;
+      c.lpr = lpr;
+      c.nv = nv;
+    }
+  }
+  c.lpr_log2 = log2_of(c.lpr);
+  c.threads = c.lpr > 256 ? c.lpr : 256;
+  return c;
+}
+// Workgroups of the backward's walk: two per CU, or one for each step of rows where there are fewer.
+int rms_bwd_blocks(int64_t rows, const RowCut &cut) {
+  const int64_t steps = ceil_div(rows, cut.threads / cut.lpr);
+  return (int)std::min<int64_t>(steps, 2 * kNumCU);
+}
+
+namespace {
+
+// ---- rotary ----
+struct RotaryPlan {
+  RotaryArgs a;
+  int pairs;   // of a lane
+  int blocks;  // of the backward behind a norm
+  bool empty;
+};
+int64_t partial_bytes(const RotaryPlan &p, int64_t dtype) {
+  return (int64_t)p.blocks * 2 * p.a.D * (dtype == GN_F64 ? 8 : 4);
+}
+
+int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
+  if (!c) return invalid("null call");
+  if (const int rc = check_types(c->dtype, c->q_weight ? c->param_dtype : c->dtype)) return rc;
+  if (c->batch < 0 || c->tokens < 0 || c->heads < 1 || c->kv_heads < 0) return invalid("batch, tokens or heads out of range");
+  if (c->heads > 65535 || c->kv_heads > 65535) return invalid("heads out of range: at most 65535");
+  if (c->head_dim < 2 || c->head_dim > 256 || c->head_dim % 2) return invalid("head_dim must be even and 2 to 256");
+  if (c->axes < 1 || c->axes > 4) return invalid("1 to 4 axes are supported");
+  int64_t last = 0;
+  for (int i = 0; i < c->axes; ++i) {
+    if (c->section_end[i] < last) return invalid("section_end must not descend");
+    last = c->section_end[i];
+  }
+  if (last < 1 || 2 * last > c->head_dim) return invalid("sections must hold 1 to head_dim / 2 pairs");
+  if (c->position_type < 0 || c->position_type > 2) return invalid("position_type must be 0 (int32), 1 (int64) or 2 (float)");
+  if ((c->kv_heads > 0) != (c->k_out != nullptr) && c->batch * c->tokens > 0) return invalid("kv_heads without k_out, or the reverse");
+  if (c->kv_heads > 0 && (c->q_weight != nullptr) != (c->k_weight != nullptr)) return invalid("q_weight and k_weight go together");
+  const bool norm = c->q_weight != nullptr;
+  if (const int rc = check_eps(norm ? c->eps : 0)) return rc;
+  p = {};
+  RotaryArgs &a = p.a;
+  p.empty = c->batch == 0 || c->tokens == 0;
+  a.D = (int)c->head_dim;
+  a.P = (int)last;
+  const int half = a.D / 2, most = c->dtype == GN_F64 ? 2 : c->dtype == GN_F32 ? 4 : 8;
+  // the widest lane vector that the pairs are a multiple of; half of 16 bytes for half-precision heads such as 40
+  p.pairs = 1;
+  for (int s = most; s > 1; s >>= 1)
+    if (!(s == 2 && most != 2) && half % s == 0 && (c->interleaved || a.P % s == 0)) {
+      p.pairs = s;
+      break;
+    }
+  a.nvec = half / p.pairs;
+  if (a.nvec > 64) return invalid("heads of more than 128 channels must have a multiple of 8 channels, and so must their pairs");
+  a.lanes_log2 = log2_of(a.nvec);
+  a.lanes = 1 << a.lanes_log2;
+  if (p.empty) return GNNHWC_OK;
+
+  if (c->batch > 0x7fffffff / c->tokens || c->batch * c->tokens > 0x40000000) return invalid("too many tokens: at most 2^30");
+  const int64_t tokens = c->batch * c->tokens;
+  if (!c->positions || !c->frequencies) return invalid("null positions or frequencies");
+  if (!c->q_out || (c->kv_heads && !c->k_out)) return invalid("null output");
+  const bool reads = !backward || norm;
+  if (reads && (!c->q || (c->kv_heads && !c->k))) return invalid("null tensor");
+  if (backward && (!c->q_grad || (c->kv_heads && !c->k_grad))) return invalid("null gradient");
+  const int64_t heads[2] = {c->heads, c->kv_heads};
+  // heads a group takes one after the other: up to eight as long as the groups fill the device four times
+  int take = 8;
+  while (take > 1 && tokens * (ceil_div(heads[0], take) + ceil_div(heads[1], take)) * a.lanes < (int64_t)4 * kNumCU * kBlock) take >>= 1;
+  const void *in[2] = {c->q, c->k}, *grad[2] = {c->q_grad, c->k_grad}, *weight[2] = {c->q_weight, c->k_weight};
+  void *out[2] = {c->q_out, c->k_out};
+  const int64_t *is[2] = {c->q_stride, c->k_stride}, *gs[2] = {c->q_grad_stride, c->k_grad_stride}, *os[2] = {c->q_out_stride, c->k_out_stride};
+  for (int i = 0; i < 2; ++i) {
+    RotarySide &s = a.side[i];
+    const bool turns_grad = backward && !norm;  // the gradient is what is turned
+    s.in = turns_grad ? grad[i] : in[i];
+    s.grad = grad[i];
+    s.weight = weight[i];
+    s.out = out[i];
+    for (int d = 0; d < 3; ++d) {
+      s.in_stride[d] = turns_grad ? gs[i][d] : is[i][d];
+      s.grad_stride[d] = gs[i][d];
+      s.out_stride[d] = os[i][d];
+    }
+    s.heads = (int)heads[i];
+    s.groups = (int)ceil_div(heads[i], take);
+  }
+  a.groups = a.side[0].groups + a.side[1].groups;
+  if (tokens * a.groups > 0x7fff0000) return invalid("too many tokens and heads for one call");
+  a.pos = c->positions;
+  a.pos_stride[0] = c->position_stride[0];
+  a.pos_stride[1] = c->position_stride[1];
+  a.freq = c->frequencies;
+  a.pos_type = (int)c->position_type;
+  a.axes = (int)c->axes;
+  for (int i = 0; i < 4; ++i) a.ends[i] = (int)(i < c->axes ? c->section_end[i] : last);
+  a.tokens = (int)tokens;
+  a.L = (int)c->tokens;
+  a.by_groups = make_divisor(a.groups, 0);
+  a.by_L = make_divisor(a.L, 0);
+  a.eps = c->eps;
+  a.inv_d = 1.0 / a.D;
+  a.sign = backward ? -1.0f : 1.0f;
+  if (backward && norm) {
+    // a walk of whole sets of groups: two workgroups per CU, or as many as there are tokens
+    const int64_t subs = kBlock / a.lanes;
+    const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(tokens, 2 * kNumCU * subs / a.groups));
+    a.token_step = (int)steps;
+    a.walkers = (int)(steps * a.groups);
+    p.blocks = (int)ceil_div(a.walkers, subs);
+  }
+  return GNNHWC_OK;
+}
+
+}  // namespace
+}  // namespace gn
+
+using namespace gn;
+
+extern "C" {
+
+int gnnhwc_rms_fwd(const void *x, const void *residual, const void *weight, void *sum_out, void *y, int64_t rows, int64_t C,
+                   int64_t x_stride, int64_t residual_stride, double eps, int dtype, int param_dtype, void *stream) {
+  if (const int rc = check_rows(rows, C, dtype, weight ? param_dtype : dtype)) return rc;
+  if (const int rc = check_eps(eps)) return rc;
+  if (const int rc = check_fwd(x, residual, sum_out, y, rows)) return rc;
+  if (rows == 0) return GNNHWC_OK;
+  const RowCut cut = rms_cut(C, elem_size(dtype), kFwdVectors, 8);
+  const RmsFwd a = fwd_args(x, residual, weight, sum_out, y, rows, C, x_stride, residual_stride, eps, cut);
+  const int pt = weight ? param_dtype : dtype;
+#define GN_CALL(S) launch_rms_fwd_##S(a, cut, pt, false, (hipStream_t)stream)
+  return launched(GN_BY_TYPE(dtype, GN_CALL), "gnnhwc_rms_fwd");
+#undef GN_CALL
+}
+
+int gnnhwc_rms_fwd_quant(const void *x, const void *residual, const void *weight, void *sum_out, void *q, float *scales,
+                         int64_t rows, int64_t C, int64_t x_stride, int64_t residual_stride, int64_t block, double eps, int dtype,
+                         int param_dtype, int q_dtype, void *stream) {
+  if (const int rc = check_rows(rows, C, dtype, weight ? param_dtype : dtype)) return rc;
+  if (dtype == GN_F64) return invalid("8-bit results take f32, f16 or bf16 data");
+  if (q_dtype != GNNHWC_F8E4M3 && q_dtype != GNNHWC_I8) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "unknown 8-bit type %d", q_dtype);
+  if (const int rc = check_eps(eps)) return rc;
+  if (const int rc = check_fwd(x, residual, sum_out, q, rows)) return rc;
+  if (rows > 0 && !scales) return invalid("null scales");
+  const bool by_row = block == 0 || block >= C;
+  if (!by_row && (block < 16 || block > 256 || (block & (block - 1))))
+    return fail(GNNHWC_ERR_INVALID_ARGUMENT, "a block of %lld channels: a power of two from 16 to 256, or 0 for whole rows", (long long)block);
+  if (rows == 0) return GNNHWC_OK;
+  const int lanes = by_row ? 0 : (int)block / (16 / elem_size(dtype));
+  const RowCut cut = rms_cut(C, elem_size(dtype), kFwdVectors, std::max(8, lanes));
+  RmsFwd a = fwd_args(x, residual, weight, sum_out, q, rows, C, x_stride, residual_stride, eps, cut);
+  a.scales = scales;
+  a.block_lanes = lanes;
+  a.nblocks = by_row ? 1 : (int)ceil_div(C, block);
+  a.qtype = q_dtype;
+  a.q_most = q_dtype == GNNHWC_F8E4M3 ? 448.0f : 127.0f;
+  const int pt = weight ? param_dtype : dtype;
+#define GN_CALL(S) launch_rms_fwd_##S(a, cut, pt, true, (hipStream_t)stream)
+  return launched(GN_BY_TYPE(dtype, GN_CALL), "gnnhwc_rms_fwd_quant");
+#undef GN_CALL
+}
+
+size_t gnnhwc_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype) {
+  if (check_rows(rows, C, dtype, dtype)) return 0;
+  const RowCut cut = rms_cut(C, elem_size(dtype), kBwdVectors, 8);
+  return 256 + (size_t)rms_bwd_blocks(rows, cut) * (size_t)C * (dtype == GN_F64 ? 8 : 4);
+}
+
+int gnnhwc_rms_bwd(const void *dy, const void *ds, const void *s, const void *weight, void *dx, void *dweight, int64_t rows, int64_t C,
+                   int64_t dy_stride, int64_t ds_stride, int64_t s_stride, double eps, int dtype, int param_dtype, void *workspace,
+                   size_t workspace_bytes, void *stream) {
+  if (const int rc = check_rows(rows, C, dtype, weight || dweight ? param_dtype : dtype)) return rc;
+  if (const int rc = check_eps(eps)) return rc;
+  if (rows > 0 && (!dy || !s)) return invalid("null tensor");
+  if (!dx && !dweight) return GNNHWC_OK;
+  if (dweight && (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < gnnhwc_rms_bwd_workspace_bytes(rows, C, dtype)))
+    return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_rms_bwd_workspace_bytes");
+  const RowCut cut = rms_cut(C, elem_size(dtype), kBwdVectors, 8);
+  RmsBwd a = {};
+  a.dy = dy; a.ds = ds; a.s = s; a.w = weight;
+  a.dx = dx; a.part = dweight ? workspace : nullptr;
+  a.rows = rows; a.dy_stride = dy_stride; a.ds_stride = ds_stride; a.s_stride = s_stride;
+  a.eps = eps; a.inv_c = 1.0 / (double)C;
+  a.C = (int)C; a.nvec = cut.nvec; a.lpr = cut.lpr; a.lpr_log2 = cut.lpr_log2;
+  const int pt = weight || dweight ? param_dtype : dtype, blocks = rms_bwd_blocks(rows, cut);
+  if (rows == 0 && !dweight) return GNNHWC_OK;
+#define GN_CALL(S) launch_rms_bwd_##S(a, cut, pt, blocks, dweight, (hipStream_t)stream)
+  return launched(GN_BY_TYPE(dtype, GN_CALL), "gnnhwc_rms_bwd");
+#undef GN_CALL
+}
+
+int gnnhwc_rotary(const gnnhwc_rotary_call *c, void *stream) {
+  RotaryPlan p;
+  if (const int rc = plan_rotary(c, false, p)) return rc;
+  if (p.empty) return GNNHWC_OK;
+  const bool norm = c->q_weight != nullptr;
+#define GN_CALL(S) launch_rotary_##S(p.a, p.pairs, c->interleaved != 0, norm, (int)c->param_dtype, (hipStream_t)stream)
+  return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary");
+#undef GN_CALL
+}
+
+size_t gnnhwc_rotary_bwd_workspace_bytes(const gnnhwc_rotary_call *c) {
+  RotaryPlan p;
+  if (plan_rotary(c, true, p)) return 0;
+  return 256 + (size_t)partial_bytes(p, c->dtype);
+}
+
+int gnnhwc_rotary_bwd(const gnnhwc_rotary_call *c, void *workspace, size_t workspace_bytes, void *stream) {
+  RotaryPlan p;
+  if (const int rc = plan_rotary(c, true, p)) return rc;
+  const bool norm = c->q_weight != nullptr;
+  if (p.empty && !norm) return GNNHWC_OK;
+  if (!norm) {
+#define GN_CALL(S) launch_rotary_##S(p.a, p.pairs, c->interleaved != 0, false, (int)c->dtype, (hipStream_t)stream)
+    return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary_bwd");
+#undef GN_CALL
+  }
+  if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < 256 + (size_t)partial_bytes(p, c->dtype))
+    return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_rotary_bwd_workspace_bytes");
+  p.a.part = workspace;
+  void *const dw[2] = {c->q_dweight, c->kv_heads ? c->k_dweight : nullptr};
+#define GN_CALL(S) launch_rotary_norm_bwd_##S(p.a, p.pairs, c->interleaved != 0, (int)c->param_dtype, p.blocks, dw, (hipStream_t)stream)
+  return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary_bwd");
+#undef GN_CALL
+}
+
+size_t gnnhwc_clip_workspace_bytes(int64_t count) {
+  if (count < 0) {
+    invalid("negative count");
+    return 0;
+  }
+  return (size_t)(kClipPartials + ceil_div(count, kClipEntries) + 1) * sizeof(double);
+}
+
+int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const int *dtype, const int *out_dtype, int64_t count,
+                double max_norm, double eps, double grad_scale, void *total, int total_dtype, void *workspace, size_t workspace_bytes,
+                void *stream) try {
+  if (count < 0 || (count > 0 && (!in || !n || !dtype || (out && !out_dtype)))) return invalid("null array or negative count");
+  if (!(max_norm >= 0)) return invalid("max_norm must not be negative");
+  if (const int rc = check_eps(eps)) return rc;
+  if (!(fabs(grad_scale) < INFINITY)) return invalid("grad_scale must be finite");
+  if (!total) return invalid("null total");
+  if (total_dtype != GN_F32 && total_dtype != GN_F64) return invalid("total must be f32 or f64");
+  if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < gnnhwc_clip_workspace_bytes(count))
+    return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_clip_workspace_bytes");
+  struct Range {
+    uintptr_t from, to;
+    int64_t i;
+    bool written;
+  };
+  const bool scales = out || grad_scale != 1.0 || max_norm < INFINITY;
+  std::vector<ClipEntry> list;
+  std::vector<Range> ranges;
+  list.reserve((size_t)count);
+  if (scales) ranges.reserve((size_t)(out ? 2 * count : count));
+  for (int64_t i = 0; i < count; ++i) {
+    const int es = elem_size(dtype[i]), os = out ? elem_size(out_dtype[i]) : es;
+    if (!es || !os) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "tensor %lld: unknown dtype code", (long long)i);
+    if (n[i] < 0 || n[i] > ((int64_t)1 << 42)) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "tensor %lld: size out of range", (long long)i);
+    if (n[i] == 0) continue;
+    if (!in[i] || (out && !out[i])) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "tensor %lld: null", (long long)i);
+    ClipEntry e = {in[i], out ? out[i] : const_cast<void *>(in[i]), n[i], 0, dtype[i] | (out ? out_dtype[i] : dtype[i]) << 8};
+    const uintptr_t a = (uintptr_t)e.in, b = (uintptr_t)e.out;
+    if (scales) {
+      const bool same = a == b && es == os;
+      ranges.push_back({b, b + (uintptr_t)n[i] * os, i, true});
+      if (!same) ranges.push_back({a, a + (uintptr_t)n[i] * es, i, false});
+    }
+    // neighbours in memory are one tensor (the gradients of a bucket)
+    if (!list.empty()) {
+      ClipEntry &l = list.back();
+      if (l.types == e.types && (uintptr_t)l.in + (uintptr_t)l.n * es == a && (uintptr_t)l.out + (uintptr_t)l.n * os == b) {
+        l.n += e.n;
+        continue;
+      }
+    }
+    list.push_back(e);
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.from < b.from; });
+  // against the furthest end so far of what is written, and of everything
+  uintptr_t any_to = 0, written_to = 0;
+  for (const Range &r : ranges) {
+    if (r.from < written_to || (r.written && r.from < any_to))
+      return fail(GNNHWC_ERR_INVALID_ARGUMENT, "tensor %lld overlaps another one that is written", (long long)r.i);
+    any_to = std::max(any_to, r.to);
+    if (r.written) written_to = std::max(written_to, r.to);
+  }
+
+  int64_t chunks = 0;
+  for (const ClipEntry &e : list) chunks += ceil_div(e.n, kClipChunk);
+  if (chunks > 0x7fffffff) return invalid("more gradients than one call takes");
+  double *part = (double *)workspace;
+  ClipFinish f = {};
+  f.part = part;
+  f.max_norm = max_norm; f.eps = eps; f.grad_scale = grad_scale;
+  f.total = total; f.total_dtype = total_dtype;
+  f.in_place = !out;
+  // tables of up to kClipEntries tensors; a table's workgroups in proportion to its chunks
+  auto table_at = [&](size_t first, ClipTable &t) {
+    t.count = (int)std::min<size_t>(list.size() - first, kClipEntries);
+    t.chunks = 0;
+    for (int i = 0; i < t.count; ++i) {
+      t.e[i] = list[first + (size_t)i];
+      t.e[i].first_chunk = t.chunks;
+      t.chunks += (unsigned)ceil_div(t.e[i].n, kClipChunk);
+    }
+  };
+  auto blocks_of = [&](const ClipTable &t) {
+    const int64_t share = chunks <= kClipPartials ? t.chunks : (int64_t)t.chunks * kClipPartials / chunks;
+    return (int)std::max<int64_t>(1, share);
+  };
+  ClipTable t;
+  for (size_t at = 0; at < list.size(); at += kClipEntries) {
+    table_at(at, t);
+    const int blocks = blocks_of(t);
+    if (const hipError_t e = launch_clip_norm(t, part + f.parts, blocks, (hipStream_t)stream)) return launched(e, "gnnhwc_clip");
+    f.parts += blocks;
+  }
+  if (!scales || list.empty()) {
+    t.count = 0;
+    t.chunks = 0;
+    return launched(launch_clip_apply(t, f, 1, (hipStream_t)stream), "gnnhwc_clip");
+  }
+  for (size_t at = 0; at < list.size(); at += kClipEntries) {
+    if (list.size() > kClipEntries) table_at(at, t);
+    if (const hipError_t e = launch_clip_apply(t, f, blocks_of(t), (hipStream_t)stream)) return launched(e, "gnnhwc_clip");
+    f.total = nullptr;  // written by the first launch
+  }
+  return GNNHWC_OK;
+} catch (...) {
+  return fail(GNNHWC_ERR_LAUNCH, "gnnhwc_clip: out of host memory");
+}
+
+}  // extern "C"

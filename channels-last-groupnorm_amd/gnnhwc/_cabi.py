@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_CSRC, "libgnnhwc_hip_trace.so" if TRACING else "libgnnh
 
 # dtype / activation codes of include/gnnhwc.h
 F32, F64, F16, BF16 = 0, 1, 2, 3
+F8E4M3, I8 = 4, 5  # 8-bit result types of include/gnnhwc_tokens.h
 STATIC_SCRATCH_BYTES = 4 << 20  # GNNHWC_STATIC_SCRATCH_BYTES
 NUM_KERNEL_KINDS = 15
 
@@ -44,7 +45,30 @@ SYMBOLS = (
     "gnnhwc_debug_backward_sets",
     "gnnhwc_debug_last_launch",
     "gnnhwc_debug_load_tile",
+    "gnnhwc_rms_fwd",
+    "gnnhwc_rms_fwd_quant",
+    "gnnhwc_rms_bwd_workspace_bytes",
+    "gnnhwc_rms_bwd",
+    "gnnhwc_rotary",
+    "gnnhwc_rotary_bwd_workspace_bytes",
+    "gnnhwc_rotary_bwd",
+    "gnnhwc_clip_workspace_bytes",
+    "gnnhwc_clip",
 )
+
+
+class RotaryCall(ctypes.Structure):
+    """gnnhwc_rotary_call of include/gnnhwc_tokens.h."""
+
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("q", "k", "q_grad", "k_grad", "q_out", "k_out")]
+        + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "q_grad_stride", "k_grad_stride", "q_out_stride", "k_out_stride")]
+        + [(n, ctypes.c_int64) for n in ("batch", "tokens", "heads", "kv_heads", "head_dim", "axes")]
+        + [("section_end", ctypes.c_int64 * 4), ("interleaved", ctypes.c_int64), ("positions", ctypes.c_void_p),
+           ("position_stride", ctypes.c_int64 * 2), ("position_type", ctypes.c_int64)]
+        + [(n, ctypes.c_void_p) for n in ("frequencies", "q_weight", "k_weight", "q_dweight", "k_dweight")]
+        + [("eps", ctypes.c_double), ("dtype", ctypes.c_int64), ("param_dtype", ctypes.c_int64)]
+    )
 
 
 def _load():
@@ -108,6 +132,25 @@ def _load():
     lib.gnnhwc_debug_backward_sets.restype = ci
     lib.gnnhwc_debug_last_launch.argtypes = [ctypes.POINTER(i64)]
     lib.gnnhwc_debug_last_launch.restype = ci
+    lib.gnnhwc_rms_fwd.argtypes = [vp] * 5 + [i64] * 4 + [dbl, ci, ci, vp]
+    lib.gnnhwc_rms_fwd.restype = ci
+    lib.gnnhwc_rms_fwd_quant.argtypes = [vp] * 6 + [i64] * 5 + [dbl, ci, ci, ci, vp]
+    lib.gnnhwc_rms_fwd_quant.restype = ci
+    lib.gnnhwc_rms_bwd_workspace_bytes.argtypes = [i64, i64, ci]
+    lib.gnnhwc_rms_bwd_workspace_bytes.restype = sz
+    lib.gnnhwc_rms_bwd.argtypes = [vp] * 6 + [i64] * 5 + [dbl, ci, ci, vp, sz, vp]
+    lib.gnnhwc_rms_bwd.restype = ci
+    rotary = ctypes.POINTER(RotaryCall)
+    lib.gnnhwc_rotary.argtypes = [rotary, vp]
+    lib.gnnhwc_rotary.restype = ci
+    lib.gnnhwc_rotary_bwd_workspace_bytes.argtypes = [rotary]
+    lib.gnnhwc_rotary_bwd_workspace_bytes.restype = sz
+    lib.gnnhwc_rotary_bwd.argtypes = [rotary, vp, sz, vp]
+    lib.gnnhwc_rotary_bwd.restype = ci
+    lib.gnnhwc_clip_workspace_bytes.argtypes = [i64]
+    lib.gnnhwc_clip_workspace_bytes.restype = sz
+    lib.gnnhwc_clip.argtypes = [vp, vp, vp, vp, vp, i64, dbl, dbl, dbl, vp, ci, vp, sz, vp]
+    lib.gnnhwc_clip.restype = ci
     lib.gnnhwc_kernel_kind_name.argtypes = [ci]
     lib.gnnhwc_kernel_kind_name.restype = ctypes.c_char_p
     return lib
