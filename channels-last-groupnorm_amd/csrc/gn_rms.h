@@ -336,7 +336,7 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dx[i] += u[i];
       }
-      if (live && cut.has(k)) store_loose<LV>((T *)q.dx + row * q.C + cut.start(k), LV::pack(dx));
+      if (q.dx && live && cut.has(k)) store_loose<LV>((T *)q.dx + row * q.C + cut.start(k), LV::pack(dx));
     }
   }
   if (!q.part) return;

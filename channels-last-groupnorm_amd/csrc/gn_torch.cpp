@@ -6,27 +6,11 @@
 // group_norm() takes ordinary eager calls only -- plain device tensors in one of the two dense layouts, no mode, transform,
 // tracer or tangent that would want to see the individual torch operations -- and answers NotImplemented to everything
 // else, errors included; the caller then runs the Python implementation, which remains the general one.
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/record_function.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include "../../include/gnnhwc.h"
+#include "gn_torch.h"
 
 namespace {
 
-using at::Tensor;
-using std::optional;
+using namespace gn_torch;
 
 // The C ABI's entry points, handed over by address: the Python binding decides which library is loaded.
 struct Entry {
@@ -41,16 +25,6 @@ struct Entry {
   decltype(&gnnhwc_bwd_nchw) bwd_nchw;
 } abi = {};
 
-int code_of(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return GNNHWC_F32;
-    case at::kDouble: return GNNHWC_F64;
-    case at::kHalf: return GNNHWC_F16;
-    case at::kBFloat16: return GNNHWC_BF16;
-    default: return -1;
-  }
-}
-bool is_half(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 // 16-bit data keep their statistics in float32
 at::ScalarType stats_type(at::ScalarType t) { return is_half(t) ? at::kFloat : t; }
 
@@ -88,7 +62,6 @@ Shape shape_of(const Tensor &x) {
   for (int64_t d = 2; d < x.dim(); ++d) s.R *= x.size(d);
   return s;
 }
-void *stream_of(const Tensor &x) { return (void *)c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
 // Scratch memory of one call, from the caching allocator: in stream order, and part of a graph's own pool under capture.
 Tensor workspace(size_t bytes, const Tensor &x, const char *what) {
   TORCH_CHECK(bytes != 0, what, ": ", abi.last_error());
@@ -123,17 +96,6 @@ Tensor in_layout(const Tensor &t, bool first) {
   const Orders o = orders_of(t.dim());
   return t.permute(o.last).contiguous().permute(o.back);
 }
-
-// The operator's name in torch's profiler, around one call.
-class OperatorRange {
- public:
-  explicit OperatorRange(const char *what) : range_(at::RecordScope::FUNCTION) {
-    if (range_.isActive()) range_.before(what);
-  }
-
- private:
-  at::RecordFunction range_;
-};
 
 struct Added {  // pre-additions of the forward (group_norm_nhwc)
   optional<Tensor> residual, channel_bias;
@@ -172,31 +134,6 @@ Tensor run_forward(const Tensor &x, const optional<Tensor> &weight, const option
                       code_of(st), code_of(out), ws.data_ptr(), bytes, stream_of(x));
   check(rc, what);
   return y;
-}
-
-// Dispatch keys of a plain device tensor; any other key (a subclass, a transform's wrapper, a lazy conjugate ...) declines.
-const c10::DispatchKeySet &plain_keys() {
-  static const c10::DispatchKeySet keys = c10::DispatchKeySet(c10::DispatchKey::CUDA) |
-                                          c10::DispatchKeySet(c10::DispatchKey::AutogradCUDA) |
-                                          c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView) |
-                                          c10::DispatchKeySet(c10::DispatchKey::AutocastCUDA);
-  return keys;
-}
-// Keys that are switched on for every thread, or by autocast (which has no rule for this operation).
-const c10::DispatchKeySet &plain_tls() {
-  static const c10::DispatchKeySet keys =
-      c10::default_included_set | c10::autocast_dispatch_keyset | c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView);
-  return keys;
-}
-// (by the bits: the sets' difference keeps the bits of the backends)
-bool only(c10::DispatchKeySet keys, c10::DispatchKeySet allowed) { return (keys.raw_repr() & ~allowed.raw_repr()) == 0; }
-bool ordinary_dispatch() {
-  return !c10::impl::TorchDispatchModeTLS::any_modes_set() && only(c10::impl::tls_local_dispatch_key_set().included_, plain_tls());
-}
-bool ordinary_thread() { return at::impl::PythonTorchFunctionTLS::stack_len() == 0 && ordinary_dispatch(); }
-bool plain(const Tensor &t, const c10::Device &device) {
-  return t.defined() && t.is_cuda() && t.device() == device && t.layout() == at::kStrided && only(t.key_set(), plain_keys()) &&
-         !t._fw_grad(0).defined();
 }
 
 // Memory the kernels can be given, whatever else the tensor carries.
@@ -309,28 +246,6 @@ struct GroupNormNode : public torch::autograd::Function<GroupNormNode> {
 };
 
 // ---- what group_norm() takes -----------------------------------------------------------------------------------------
-// While it lives, other Python threads run: allocations may have to wait for the device, launches for a full queue or for
-// another thread's.  (Saved-tensor hooks and operators implemented in Python take the lock again by themselves.)
-class WithoutGil {
- public:
-  WithoutGil() : state_(PyEval_SaveThread()) {}
-  ~WithoutGil() { PyEval_RestoreThread(state_); }
-  WithoutGil(const WithoutGil &) = delete;
-  WithoutGil &operator=(const WithoutGil &) = delete;
-
- private:
-  PyThreadState *state_;
-};
-bool needs_grad(const optional<Tensor> &t) { return t.has_value() && t->requires_grad(); }
-
-// None -> no value; an exact torch.Tensor / Parameter -> its tensor; anything else -> false.
-bool tensor_or_none(PyObject *o, optional<Tensor> &t) {
-  if (o == Py_None) return true;
-  if (!THPVariable_CheckExact(o)) return false;
-  t = THPVariable_Unpack(o);
-  return true;
-}
-
 // group_norm(x, weight, bias, num_groups, eps, act_code, out_dtype, residual, channel_bias, return_sum[, functional])
 //   -> y, (y, sum), or NotImplemented.  functional: on behalf of group_norm_nhwc, whose derivative is the operators' own.
 PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -445,4 +360,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__native(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__native(void) {
+  PyObject *m = PyModule_Create(&module);
+  if (m && gn_torch::add_token_methods(m) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

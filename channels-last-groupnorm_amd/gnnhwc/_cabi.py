@@ -158,13 +158,16 @@ def _load():
 
 lib = _load()
 try:
-    from . import _native  # csrc/gn_torch.cpp: the eager calls of GN_NHWC and group_norm_nhwc
+    from . import _native  # csrc/gn_torch.cpp, gn_tokens_torch.cpp: the ordinary eager calls
 except ImportError as exc:
     raise ImportError("gnnhwc: the _native extension is not built or does not load (make -C %s native): %s" % (_CSRC, exc)) from exc
 # the entry points the extension calls, in the order it binds them
 NATIVE_ENTRY_POINTS = ("last_error", "fwd_workspace_bytes", "bwd_workspace_bytes", "nchw_workspace_bytes", "fwd_cast", "bwd_cast",
                        "fwd_add", "fwd_nchw", "bwd_nchw")
 _native.bind(*[ctypes.cast(getattr(lib, "gnnhwc_" + name), ctypes.c_void_p).value for name in NATIVE_ENTRY_POINTS])
+TOKEN_ENTRY_POINTS = ("last_error", "rms_fwd", "rms_fwd_quant", "rms_bwd_workspace_bytes", "rms_bwd", "rotary", "rotary_bwd_workspace_bytes",
+                      "rotary_bwd", "clip_workspace_bytes", "clip")
+_native.bind_tokens(*[ctypes.cast(getattr(lib, "gnnhwc_" + name), ctypes.c_void_p).value for name in TOKEN_ENTRY_POINTS])
 
 
 def last_error():

@@ -3,8 +3,9 @@
 with several axes, optionally behind a norm of each head) and ``clip_gradients`` / ``clip_grad_norm_``.  The reference has no
 counterpart to any of them.
 
-The kernels are those of include/gnnhwc_tokens.h in libgnnhwc_hip.so, reached through ``gnop::`` operators, which carry meta
-kernels and autograd formulas.
+The kernels are those of include/gnnhwc_tokens.h in libgnnhwc_hip.so.  Ordinary eager calls run in native code
+(csrc/gn_tokens_torch.cpp); what that declines -- tracing, subclasses, tensors in other layouts, and every error -- comes
+here, through the ``gnop::`` operators, which carry meta kernels and autograd formulas.
 """
 import ctypes
 import math
@@ -12,7 +13,7 @@ import math
 import torch
 import torch.nn as nn
 
-from . import _cabi
+from . import _cabi, _native
 from .custom_gn import _check_device, _current_stream_ptr, _dtype_code, _DTYPE_CODE, _on_device, _op_lib, _workspace
 
 _POSITION_TYPE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -198,6 +199,10 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, return_sum=False, channel_
     front would, and is what is normalised.  With return_sum=True the call returns (y, s), so that s is the next residual
     (without a residual, s is x).  Means and products are in float32 (float64).  Differentiable in x, residual and weight;
     the gradients of s reach x and residual too."""
+    if not torch.compiler.is_compiling() and channel_dim == -1:
+        out = _native.rms_norm(x, weight, eps, residual, return_sum)
+        if out is not NotImplemented:
+            return out
     if channel_dim != -1:
         x, residual = _channels_last_dim(x, channel_dim), _channels_last_dim(residual, channel_dim)
     want = residual is not None and (return_sum or _needs_grad(x, residual, weight))
@@ -217,6 +222,10 @@ def rms_norm_quant(x, weight=None, eps=1e-6, residual=None, return_sum=False, ou
     scale = max(max |y| / most, 2^-126) per row (block=None; scales are (..., 1)) or per `block` consecutive channels (a power of
     two from 16 to 256; scales are (..., ceil(C / block))), most = 448 for torch.float8_e4m3fn and 127 for torch.int8;
     q = y / scale, rounded to nearest even from float32.  For serving: it has no derivative."""
+    if not torch.compiler.is_compiling():
+        out = _native.rms_norm_quant(x, weight, eps, residual, return_sum, out_dtype, block)
+        if out is not NotImplemented:
+            return out
     if _needs_grad(x, residual, weight):
         raise RuntimeError("rms_norm_quant has no derivative: call it under torch.no_grad()")
     if block is not None and block < 1:
@@ -446,6 +455,10 @@ def rotary(q, k, positions, frequencies, sections=None, interleaved=False, q_wei
     With q_weight / k_weight, (D,) in q's dtype or float32 beside half precision, every head is first normalised over its D
     channels, t / sqrt(mean(t^2) + eps) * weight, in the same pass.  Everything in between is float32 (float64).
     Differentiable in q, k and the weights."""
+    if not torch.compiler.is_compiling():
+        out = _native.rotary(q, k, positions, frequencies, sections, interleaved, q_weight, k_weight, eps)
+        if out is not NotImplemented:
+            return out
     sections = (frequencies.numel(),) if sections is None else tuple(int(n) for n in sections)
     qo, ko = torch.ops.gnop.rotary(q, k, positions, frequencies, sections, bool(interleaved), q_weight, k_weight, float(eps))
     return qo if k is None else (qo, ko)
@@ -510,6 +523,9 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
         raise RuntimeError("out must have as many tensors as grads")
     if not grads:
         return torch.zeros(())
+    result = _native.clip_gradients(grads, float(max_norm), outs, float(grad_scale), float(eps))
+    if result is not NotImplemented:
+        return result
     dev = grads[0].device
     keep, back = [], []
     for i, g in enumerate(grads):
@@ -552,6 +568,8 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
     _cabi.check(rc, "clip_gradients")
     for t, c in back:
         t.copy_(c)
+    if out is not None or grad_scale != 1.0 or max_norm < math.inf:
+        torch.autograd.graph.increment_version([t for t in (grads if outs is None else outs) if not t.is_inference()])
     return total
 
 
