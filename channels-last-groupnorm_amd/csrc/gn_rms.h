@@ -26,14 +26,25 @@ template <typename LV, typename T> __device__ __forceinline__ typename LV::raw_t
   typedef typename loose<typename LV::raw_t, sizeof(T)>::type U;
   return *(const global_mem<U> *)p;
 }
+// STREAM: without a place in the caches, for tensors that no cache can hold until somebody reads them again.
+template <typename LV, bool STREAM, typename T> __device__ __forceinline__ typename LV::raw_t load_once(const T *p) {
+  typedef typename loose<typename LV::raw_t, sizeof(T)>::type U;
+  if constexpr (STREAM) return __builtin_nontemporal_load((const global_mem<U> *)p);
+  else return *(const global_mem<U> *)p;
+}
 template <typename LV, typename T> __device__ __forceinline__ void store_loose(T *p, typename LV::raw_t r) {
   typedef typename loose<typename LV::raw_t, sizeof(T)>::type U;
   __builtin_nontemporal_store((U)r, (global_mem<U> *)p);
 }
 
 template <typename T> using acc_of_t = typename acc_of<T>::type;
-__device__ __forceinline__ float exact_rsqrt(float v) { return 1.0f / __builtin_sqrtf(v); }
-__device__ __forceinline__ double exact_rsqrt(double v) { return 1.0 / __builtin_sqrt(v); }
+// 1 / sqrt(v) within an ulp or so: the hardware's estimate and one Newton step (six instructions, where a root and a division
+// take about thirty), except where the step would meet a zero, an infinity or a subnormal.
+__device__ __forceinline__ float row_rsqrt(float v) {
+  if (v > 0x1p-100f && v < 0x1p+120f) return fast_rsqrt(v);
+  return 1.0f / __builtin_sqrtf(v);
+}
+__device__ __forceinline__ double row_rsqrt(double v) { return 1.0 / __builtin_sqrt(v); }
 
 // One lane vector's worth of VEC parameters of type P, as accumulators.
 template <typename P, int VEC, typename A> __device__ __forceinline__ void load_params(const P *w, A (&v)[VEC]) {
@@ -151,7 +162,7 @@ template <int VEC> __device__ __forceinline__ Bytes<VEC> pack_bytes(const float 
   return r;
 }
 
-template <typename T, typename P, int VEC, int NV, int THREADS, bool RAGGED, bool RES, bool QUANT>
+template <typename T, typename P, int VEC, int NV, int THREADS, bool RAGGED, bool RES, bool QUANT, bool STREAM>
 __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
   using A = acc_of_t<T>;
   using LV = LaneVec<T, VEC>;
@@ -168,8 +179,8 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
   raw_t s[NV], r[RES ? NV : 1];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    s[k] = load_loose<LV>(x + cut.start(k));
-    if constexpr (RES) r[k] = load_loose<LV>(res + cut.start(k));
+    s[k] = load_once<LV, STREAM>(x + cut.start(k));
+    if constexpr (RES) r[k] = load_once<LV, STREAM>(res + cut.start(k));
   }
   A ss = 0, none = 0;
 #pragma unroll
@@ -193,7 +204,7 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
     ss += cut.has(k) ? part : (A)0;
   }
   row_sum2(ss, none, q.lpr, lds, 0);
-  const A rstd = exact_rsqrt(ss * (A)q.inv_c + (A)q.eps);
+  const A rstd = row_rsqrt(ss * (A)q.inv_c + (A)q.eps);
 
   if constexpr (!QUANT) {
 #pragma unroll
@@ -265,7 +276,7 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
 // Backward.  A workgroup walks over rows and keeps its share of dw in registers, in a fixed order, and leaves one partial row
 // of dw; rms_dw_kernel adds those.  r is computed again from s, whose sum of squares rides along with that of g s, so that the
 // forward saves no statistics:  with G = sum g s,  mean(g h) = r G / C.
-template <typename T, typename P, int VEC, int NV, int THREADS, bool RAGGED, bool DS>
+template <typename T, typename P, int VEC, int NV, int THREADS, bool RAGGED, bool DS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
   using A = acc_of_t<T>;
   using LV = LaneVec<T, VEC>;
@@ -286,7 +297,8 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
   }
   int turn = 0;
   // (the bound does not depend on the lane: all wavefronts meet at the same barriers)
-  for (int64_t base = (int64_t)blockIdx.x * rows_per_step; base < q.rows; base += (int64_t)gridDim.x * rows_per_step) {
+  const int64_t stride = (int64_t)gridDim.x * rows_per_step;
+  for (int64_t base = (int64_t)blockIdx.x * rows_per_step; base < q.rows; base += stride, turn ^= 1) {
     const bool live = base + sub < q.rows;
     const int64_t row = live ? base + sub : q.rows - 1;
     const T *sp = (const T *)q.s + row * q.s_stride, *dyp = (const T *)q.dy + row * q.dy_stride;
@@ -294,9 +306,9 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
     raw_t s[NV], dy[NV], ds[DS ? NV : 1];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      s[k] = load_loose<LV>(sp + cut.start(k));
-      dy[k] = load_loose<LV>(dyp + cut.start(k));
-      if constexpr (DS) ds[k] = load_loose<LV>(dsp + cut.start(k));
+      s[k] = load_once<LV, STREAM>(sp + cut.start(k));
+      dy[k] = load_once<LV, STREAM>(dyp + cut.start(k));
+      if constexpr (DS) ds[k] = load_once<LV, STREAM>(dsp + cut.start(k));
     }
     A ss = 0, gs = 0;
 #pragma unroll
@@ -316,9 +328,10 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
       gs += cut.has(k) ? p1 : (A)0;
     }
     row_sum2(ss, gs, q.lpr, lds, turn);
-    turn ^= 1;
-    const A r = exact_rsqrt(ss * (A)q.inv_c + (A)q.eps);
-    const A c = r * gs * (A)q.inv_c;
+    // r (g - h mean(g h)) = r g - s (r^3 G / C)
+    const A r = row_rsqrt(ss * (A)q.inv_c + (A)q.eps);
+    const A c = -r * r * r * gs * (A)q.inv_c;
+    if (!live) continue;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       A sv[VEC], dv[VEC], dx[VEC];
@@ -326,9 +339,9 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
       LV::unpack(dy[k], dv);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const A h = sv[i] * r;
-        dx[i] = r * (dv[i] * w[k][i] - h * c);
-        dw[k][i] += live ? dv[i] * h : (A)0;
+        const A dr = dv[i] * r;
+        dw[k][i] += dr * sv[i];
+        dx[i] = dr * w[k][i] + sv[i] * c;
       }
       if constexpr (DS) {
         A u[VEC];
@@ -336,7 +349,7 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dx[i] += u[i];
       }
-      if (q.dx && live && cut.has(k)) store_loose<LV>((T *)q.dx + row * q.C + cut.start(k), LV::pack(dx));
+      if (q.dx && cut.has(k)) store_loose<LV>((T *)q.dx + row * q.C + cut.start(k), LV::pack(dx));
     }
   }
   if (!q.part) return;
@@ -373,21 +386,23 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
   }
 }
 
-// Sums of `count` rows of C partial results, in a fixed order: 16 columns a workgroup (a line of memory), 16 threads a column.
-template <typename A> __global__ __launch_bounds__(256) void partial_sum_kernel(const PartialSum q) {
-  __shared__ A lds[16][17];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), sub = threadIdx.x >> 4;
+// Sums of `count` rows of C partial results, in a fixed order: 16 columns a workgroup (half a line of memory), 64 threads a
+// column, so that the few hundred rows there are take a handful of loads a thread, all in flight at once.
+template <typename A> __global__ __launch_bounds__(1024) void partial_sum_kernel(const PartialSum q) {
+  __shared__ A lds[64][17];
+  const int lane = threadIdx.x & 15, sub = threadIdx.x >> 4, col = blockIdx.x * 16 + lane;
   const A *p = (const A *)q.part + (col < q.C ? col : q.C - 1);
   A acc = 0;
 #pragma unroll 8
-  for (int i = sub; i < q.count; i += 16) acc += load_global<A>(p + (int64_t)i * q.pitch);
-  lds[sub][threadIdx.x & 15] = acc;
+  for (int i = sub; i < q.count; i += 64) acc += load_global<A>(p + (int64_t)i * q.C);
+  lds[sub][lane] = acc;
   __syncthreads();
   if (sub != 0 || col >= q.C) return;
   acc = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc += lds[i][threadIdx.x & 15];
-  store_scalar<A>(q.out, col, q.out_dtype, acc);
+  for (int i = 0; i < 64; ++i) acc += lds[i][lane];
+  void *out = col < q.split ? q.out[0] : q.out[1];
+  if (out) store_scalar<A>(out, col < q.split ? col : col - q.split, q.out_dtype, acc);
 }
 
 }  // namespace gn

@@ -1,5 +1,7 @@
 // Kernels of the root-mean-square norm (gn_rms.h) instantiated and launched for ONE element type, selected with
 // -DGN_INST_DTYPE=0..3 (f32, f64, f16, bf16).
+#include <type_traits>
+
 #include "gn_rms.h"
 
 #ifndef GN_INST_DTYPE
@@ -35,67 +37,63 @@ constexpr int kVec = vec_of<elem_t>::value;
 // Most lane vectors of a row of 1024 lanes.
 constexpr int kWideVectors = kMostChannels / (sizeof(elem_t) == 8 ? 2 : 1) / (kVec * 1024);
 
-// ---- forward ----
-template <typename P, int VEC, int NV, int THREADS, bool RAGGED, bool QUANT>
-void fwd_launch(const RmsFwd &a, hipStream_t stream, unsigned grid, int threads) {
-  if (a.res) hipLaunchKernelGGL((rms_fwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, true, QUANT>), dim3(grid), dim3(threads), 0, stream, a);
-  else hipLaunchKernelGGL((rms_fwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, false, QUANT>), dim3(grid), dim3(threads), 0, stream, a);
+// Calls f with the vectors of a lane and the threads of a workgroup as constants.
+template <typename F> void with_width(const RowCut &cut, F &&f) {
+  typedef std::integral_constant<int, 256> Narrow;
+  typedef std::integral_constant<int, 1024> Wide;
+  typedef std::integral_constant<int, 1> One;
+  typedef std::integral_constant<int, 2> Two;
+  typedef std::integral_constant<int, 3> Three;
+  if (cut.threads <= 256) {
+    if (cut.nv <= 1) return f(One(), Narrow());
+    if (cut.nv == 2) return f(Two(), Narrow());
+    return f(Three(), Narrow());
+  }
+  // rows longer than 256 lanes of three vectors hold
+  if (cut.nv == 2) return f(Two(), Wide());
+  if constexpr (kWideVectors > 3) {
+    if (cut.nv > 3) return f(std::integral_constant<int, 4>(), Wide());
+  }
+  return f(Three(), Wide());
 }
-template <typename P, bool RAGGED, bool QUANT> void fwd_width(const RmsFwd &a, const RowCut &cut, hipStream_t stream, unsigned grid) {
-  if (cut.vec == 1) return fwd_launch<P, 1, 1, 256, false, QUANT>(a, stream, grid, cut.threads);
-  if (cut.threads > 256) {
-    if (cut.nv == 1) return fwd_launch<P, kVec, 1, 1024, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    if (kWideVectors < 3 || cut.nv == 2) return fwd_launch<P, kVec, 2, 1024, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    if constexpr (kWideVectors >= 3) {
-      if (cut.nv == 3) return fwd_launch<P, kVec, 3, 1024, RAGGED, QUANT>(a, stream, grid, cut.threads);
-      return fwd_launch<P, kVec, 4, 1024, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    }
-  }
-  switch (cut.nv) {
-    case 1: return fwd_launch<P, kVec, 1, 256, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    case 2: return fwd_launch<P, kVec, 2, 256, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    case 3: return fwd_launch<P, kVec, 3, 256, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    case 4: return fwd_launch<P, kVec, 4, 256, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    case 5: return fwd_launch<P, kVec, 5, 256, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    case 6: return fwd_launch<P, kVec, 6, 256, RAGGED, QUANT>(a, stream, grid, cut.threads);
-    default: return fwd_launch<P, kVec, 8, 256, RAGGED, QUANT>(a, stream, grid, cut.threads);
-  }
+
+// ---- forward ----
+template <typename P, int VEC, int NV, int THREADS, bool RAGGED, bool QUANT, bool STREAM>
+void fwd_launch(const RmsFwd &a, const RowCut &cut, hipStream_t stream) {
+  const int rows = cut.threads / cut.lpr;
+  const dim3 grid((unsigned)((a.rows + rows - 1) / rows)), block(cut.threads);
+  if (a.res) hipLaunchKernelGGL((rms_fwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, true, QUANT, STREAM>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((rms_fwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, false, QUANT, STREAM>), grid, block, 0, stream, a);
 }
 template <typename P, bool QUANT> void fwd_params(const RmsFwd &a, const RowCut &cut, hipStream_t stream) {
-  const int rows = cut.threads / cut.lpr;
-  const unsigned grid = (unsigned)((a.rows + rows - 1) / rows);
-  if (cut.ragged) fwd_width<P, true, QUANT>(a, cut, stream, grid);
-  else fwd_width<P, false, QUANT>(a, cut, stream, grid);
+  const bool streams = a.rows * a.C * (int64_t)sizeof(elem_t) * (a.res ? 2 : 1) > kCachedBytes;
+  if (cut.vec == 1) return fwd_launch<P, 1, 1, 256, false, QUANT, false>(a, cut, stream);
+  with_width(cut, [&](auto nv, auto threads) {
+    constexpr int NV = decltype(nv)::value, THREADS = decltype(threads)::value;
+    if (cut.ragged) fwd_launch<P, kVec, NV, THREADS, true, QUANT, false>(a, cut, stream);
+    else if (streams) fwd_launch<P, kVec, NV, THREADS, false, QUANT, true>(a, cut, stream);
+    else fwd_launch<P, kVec, NV, THREADS, false, QUANT, false>(a, cut, stream);
+  });
 }
 
 // ---- backward ----
-template <typename P, int VEC, int NV, int THREADS, bool RAGGED>
-void bwd_launch(const RmsBwd &a, hipStream_t stream, unsigned grid, const RowCut &cut) {
+template <typename P, int VEC, int NV, int THREADS, bool RAGGED, bool STREAM>
+void bwd_launch(const RmsBwd &a, const RowCut &cut, hipStream_t stream, int blocks) {
   const int lanes = cut.lpr < 64 ? 64 : cut.lpr, groups = cut.threads / lanes;
   const size_t lds = (size_t)(groups / 2) * NV * VEC * lanes * sizeof(A);
-  if (a.ds) hipLaunchKernelGGL((rms_bwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, true>), dim3(grid), dim3(cut.threads), lds, stream, a);
-  else hipLaunchKernelGGL((rms_bwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, false>), dim3(grid), dim3(cut.threads), lds, stream, a);
+  const dim3 grid((unsigned)blocks), block(cut.threads);
+  if (a.ds) hipLaunchKernelGGL((rms_bwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, true, STREAM>), grid, block, lds, stream, a);
+  else hipLaunchKernelGGL((rms_bwd_kernel<elem_t, P, VEC, NV, THREADS, RAGGED, false, STREAM>), grid, block, lds, stream, a);
 }
-template <typename P, bool RAGGED> void bwd_width(const RmsBwd &a, const RowCut &cut, hipStream_t stream, unsigned grid) {
-  if (cut.vec == 1) return bwd_launch<P, 1, 1, 256, false>(a, stream, grid, cut);
-  if (cut.threads > 256) {
-    if (cut.nv == 1) return bwd_launch<P, kVec, 1, 1024, RAGGED>(a, stream, grid, cut);
-    if (kWideVectors < 3 || cut.nv == 2) return bwd_launch<P, kVec, 2, 1024, RAGGED>(a, stream, grid, cut);
-    if constexpr (kWideVectors >= 3) {
-      if (cut.nv == 3) return bwd_launch<P, kVec, 3, 1024, RAGGED>(a, stream, grid, cut);
-      return bwd_launch<P, kVec, 4, 1024, RAGGED>(a, stream, grid, cut);
-    }
-  }
-  switch (cut.nv) {
-    case 1: return bwd_launch<P, kVec, 1, 256, RAGGED>(a, stream, grid, cut);
-    case 2: return bwd_launch<P, kVec, 2, 256, RAGGED>(a, stream, grid, cut);
-    case 3: return bwd_launch<P, kVec, 3, 256, RAGGED>(a, stream, grid, cut);
-    default: return bwd_launch<P, kVec, 4, 256, RAGGED>(a, stream, grid, cut);
-  }
-}
-template <typename P> void bwd_params(const RmsBwd &a, const RowCut &cut, hipStream_t stream, unsigned grid) {
-  if (cut.ragged) bwd_width<P, true>(a, cut, stream, grid);
-  else bwd_width<P, false>(a, cut, stream, grid);
+template <typename P> void bwd_params(const RmsBwd &a, const RowCut &cut, hipStream_t stream, int blocks) {
+  const bool streams = a.rows * a.C * (int64_t)sizeof(elem_t) * (a.ds ? 3 : 2) > kCachedBytes;
+  if (cut.vec == 1) return bwd_launch<P, 1, 1, 256, false, false>(a, cut, stream, blocks);
+  with_width(cut, [&](auto nv, auto threads) {
+    constexpr int NV = decltype(nv)::value, THREADS = decltype(threads)::value;
+    if (cut.ragged) bwd_launch<P, kVec, NV, THREADS, true, false>(a, cut, stream, blocks);
+    else if (streams) bwd_launch<P, kVec, NV, THREADS, false, true>(a, cut, stream, blocks);
+    else bwd_launch<P, kVec, NV, THREADS, false, false>(a, cut, stream, blocks);
+  });
 }
 
 }  // namespace
@@ -115,11 +113,11 @@ hipError_t GN_CAT(launch_rms_fwd_, GN_SUFFIX)(const RmsFwd &a, const RowCut &cut
 
 hipError_t GN_CAT(launch_rms_bwd_, GN_SUFFIX)(const RmsBwd &a, const RowCut &cut, int pdtype, int blocks, void *dw, hipStream_t stream) {
   if (blocks == 0) {  // no rows: dw is zero
-  } else if (pdtype == GN_INST_DTYPE) bwd_params<elem_t>(a, cut, stream, (unsigned)blocks);
-  else bwd_params<wide_param_t>(a, cut, stream, (unsigned)blocks);
+  } else if (pdtype == GN_INST_DTYPE) bwd_params<elem_t>(a, cut, stream, blocks);
+  else bwd_params<wide_param_t>(a, cut, stream, blocks);
   if (dw) {
-    const PartialSum p = {a.part, dw, blocks, a.C, pdtype, a.C};
-    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((a.C + 15) / 16)), dim3(256), 0, stream, p);
+    const PartialSum p = {a.part, {dw, nullptr}, blocks, a.C, a.C, pdtype};
+    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, stream, p);
   }
   return hipGetLastError();
 }

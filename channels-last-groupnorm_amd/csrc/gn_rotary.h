@@ -40,39 +40,68 @@ __device__ __forceinline__ void angle_sincos(double pos, double freq, double &sn
   cs = cos(a);
 }
 
-__device__ __forceinline__ float position_at(const void *p, int64_t i, int type) {
-  switch (type) {
-    case 0: return (float)load_global<int32_t>((const int32_t *)p + i);
-    case 1: return (float)load_global<int64_t>((const int64_t *)p + i);
-    default: return load_global<float>((const float *)p + i);
+// Position on one axis, without control flow: all types are read as one word, integers of 64 bits by their lower half.
+__device__ __forceinline__ float position_at(const RotaryArgs &q, int64_t at) {
+  const uint32_t word = load_global<uint32_t>((const uint32_t *)q.pos + (at << (q.pos_type == 1 ? 1 : 0)));
+  return q.pos_type == 2 ? __builtin_bit_cast(float, word) : (float)(int32_t)word;
+}
+
+// Sine and cosine of all pairs of the tokens that a workgroup works on, in LDS: [token - first][pair].  Each is computed once a
+// workgroup; lanes that compute those of their own pairs take more instructions for them than for turning four heads.
+// Pairs behind the turning ones get the identity.
+template <typename A> struct SinCos {
+  A sn, cs;
+};
+template <typename A> __device__ __forceinline__ void fill_angles(const RotaryArgs &q, int first, int tokens, SinCos<A> *table) {
+  const int half = q.D >> 1;
+  for (int i = threadIdx.x; i < tokens * half; i += kBlock) {
+    const int t = div_by(i, q.by_half), j = i - t * half;
+    const int token = first + t < q.tokens ? first + t : q.tokens - 1;
+    const int b = div_by(token, q.by_L), l = token - b * q.L;
+    int axis = 0;
+#pragma unroll
+    for (int a = 0; a < 3; ++a) axis += j >= q.ends[a] ? 1 : 0;
+    const int at = axis < q.axes ? axis : q.axes - 1;
+    const float pos = position_at(q, (int64_t)b * q.pos_stride[0] + (int64_t)l * q.pos_stride[1] + at);
+    const float f = load_global<float>(q.freq + (j < q.P ? j : q.P - 1));
+    SinCos<A> v;
+    angle_sincos((A)pos, (A)f, v.sn, v.cs);
+    v.sn = j < q.P ? v.sn * (A)q.sign : (A)0;
+    v.cs = j < q.P ? v.cs : (A)1;
+    table[i] = v;
   }
 }
 
-// The pairs of one lane: S of them as two lane vectors of S channels.
+// The pairs of one lane: S of them as two lane vectors of S channels.  Neighbouring lanes hold neighbouring vectors, so that one
+// access of a group is one run of memory: far pairs (j, j + P) have a vector from either half of the turning channels, near
+// pairs (2j, 2j + 1) one from either half of the head, with S / 2 pairs each.  (A lane with all its near pairs behind each other
+// reads every line twice: float16 (46800, 24 + 24 heads, 128) 286 us.)
 template <typename T, int S, bool NEAR> struct PairLane {
   using A = acc_of_t<T>;
-  int j0, at0, at1, P;
+  static constexpr bool kHalves = NEAR && S > 1;
+  int j0, j1, at0, at1, P;  // j1: first pair of the second vector, where that has pairs of its own
   __device__ __forceinline__ PairLane(const RotaryArgs &q, int lane) : P(q.P) {
     const int v = lane < q.nvec ? lane : q.nvec - 1;  // spare lanes repeat the last vector and store nothing
-    j0 = v * S;
-    const bool far = !NEAR && j0 < P;  // (S divides P where pairs are far)
-    at0 = far ? j0 : 2 * j0;
-    at1 = far ? j0 + P : 2 * j0 + S;
+    if constexpr (kHalves) {
+      j0 = v * (S / 2);
+      j1 = (q.nvec + v) * (S / 2);
+      at0 = 2 * j0;
+      at1 = 2 * j1;
+    } else {
+      j0 = v * S;
+      j1 = 0;
+      const bool far = !NEAR && j0 < P;  // (S divides P where pairs are far)
+      at0 = far ? j0 : 2 * j0;
+      at1 = far ? j0 + P : 2 * j0 + S;
+    }
   }
-  __device__ __forceinline__ void angles(const RotaryArgs &q, int b, int l, A (&sn)[S], A (&cs)[S]) const {
-    const int64_t at = (int64_t)b * q.pos_stride[0] + (int64_t)l * q.pos_stride[1];
-    float pos[4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a) pos[a] = a < q.axes ? position_at(q.pos, at + a, q.pos_type) : 0.0f;
+  __device__ __forceinline__ int pair(int i) const { return kHalves && i >= S / 2 ? j1 + i - S / 2 : j0 + i; }
+  __device__ __forceinline__ void angles(const SinCos<A> *row, A (&sn)[S], A (&cs)[S]) const {
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const int j = j0 + i;
-      const float f = load_global<float>(q.freq + (j < P ? j : P - 1));
-      float p = pos[0];
-#pragma unroll
-      for (int a = 1; a < 4; ++a) p = j >= q.ends[a - 1] && a < q.axes ? pos[a] : p;
-      angle_sincos((A)p, (A)f, sn[i], cs[i]);
-      sn[i] *= (A)q.sign;
+      const SinCos<A> v = row[pair(i)];
+      sn[i] = v.sn;
+      cs[i] = v.cs;
     }
   }
   __device__ __forceinline__ void load(const T *p, typename LaneVec<T, S>::raw_t (&r)[2]) const {
@@ -106,36 +135,45 @@ template <typename T, int S, bool NEAR> struct PairLane {
 #pragma unroll
     for (int i = 0; i < S; ++i) v[S + i] = t[i];
   }
-  // (channels behind the pairs are selected, not multiplied by one and zero: an infinity there stays one)
   __device__ __forceinline__ void turn(A (&v)[2 * S], const A (&sn)[S], const A (&cs)[S], bool partial) const {
+    A was[2 * S];
+#pragma unroll
+    for (int c = 0; c < 2 * S; ++c) was[c] = v[c];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      A &x = v[NEAR ? 2 * i : i], &y = v[NEAR ? 2 * i + 1 : S + i];
-      const A u = x * cs[i] - y * sn[i], w = x * sn[i] + y * cs[i];
-      const bool keep = partial && j0 + i >= P;
-      x = keep ? x : u;
-      y = keep ? y : w;
+      const int a = NEAR ? 2 * i : i, b = NEAR ? 2 * i + 1 : S + i;
+      v[a] = was[a] * cs[i] - was[b] * sn[i];
+      v[b] = was[a] * sn[i] + was[b] * cs[i];
     }
+    // channels behind the pairs are taken back, not multiplied by one and zero: an infinity there stays one
+    if (partial)
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const int a = NEAR ? 2 * i : i, b = NEAR ? 2 * i + 1 : S + i;
+        const bool keep = pair(i) >= P;
+        v[a] = keep ? was[a] : v[a];
+        v[b] = keep ? was[b] : v[b];
+      }
   }
 };
 
 // Heads of one token for one group of lanes.
 struct HeadWalk {
   bool live;
-  int which, first, step, count, b, l;  // which: 0 q, 1 k; heads first, first + step, ...
+  int token, which, first, step, count, b, l;  // which: 0 q, 1 k; heads first, first + step, ...
 };
 __device__ __forceinline__ HeadWalk head_walk(const RotaryArgs &q, int group) {
   HeadWalk w;
   w.live = group < q.tokens * q.groups;
-  group = w.live ? group : 0;
-  const int token = div_by(group, q.by_groups);
-  const int g = group - token * q.groups;
+  group = w.live ? group : q.tokens * q.groups - 1;  // (the last one again: its token is in the workgroup's span)
+  w.token = div_by(group, q.by_groups);
+  const int g = group - w.token * q.groups;
   w.which = g >= q.side[0].groups ? 1 : 0;
   w.first = w.which ? g - q.side[0].groups : g;
   w.step = w.which ? q.side[1].groups : q.side[0].groups;
   w.count = w.which ? q.side[1].heads : q.side[0].heads;
-  w.b = div_by(token, q.by_L);
-  w.l = token - w.b * q.L;
+  w.b = div_by(w.token, q.by_L);
+  w.l = w.token - w.b * q.L;
   return w;
 }
 // q's or k's tensors, field by field: both are scalar loads of the argument block and a selection.
@@ -164,42 +202,47 @@ __device__ __forceinline__ int64_t head_at(const int64_t (&s)[3], int b, int l) 
 template <typename T, typename P, int S, bool NEAR, bool NORM>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
   using A = acc_of_t<T>;
-  constexpr int kHeads = 4;  // heads whose loads are in flight together
-  const int lane = threadIdx.x & (q.lanes - 1);
-  const HeadWalk walk = head_walk(q, (int)(blockIdx.x * (kBlock >> q.lanes_log2)) + (int)(threadIdx.x >> q.lanes_log2));
+  constexpr int kHeads = kRotaryHeads;
+  extern __shared__ char lds_dyn[];
+  SinCos<A> *const table = (SinCos<A> *)lds_dyn;
+  const int lane = threadIdx.x & (q.lanes - 1), sub = threadIdx.x >> q.lanes_log2, subs = kBlock >> q.lanes_log2;
+  const int start = (int)blockIdx.x * subs;
+  const HeadWalk walk = head_walk(q, start + sub);
   const PairLane<T, S, NEAR> pl(q, lane);
   const Side side = side_of(q, walk.which);
   const bool stores = walk.live && lane < q.nvec, partial = 2 * q.P < q.D;
   const T *in = (const T *)side.in + head_at(side.in_stride, walk.b, walk.l);
   T *out = (T *)side.out + head_at(side.out_stride, walk.b, walk.l);
   const int64_t in_head = side.in_stride[2], out_head = side.out_stride[2];
+  // all heads are asked for first and are on their way while the angles are computed
+  typename LaneVec<T, S>::raw_t r[kHeads][2];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = walk.first + i * walk.step;
+    pl.load(in + (h < walk.count ? h : walk.first) * in_head, r[i]);
+  }
   A sn[S], cs[S], w[2 * S];
-  pl.angles(q, walk.b, walk.l, sn, cs);
   if constexpr (NORM) pl.weights((const P *)side.weight, w);
-  for (int h0 = walk.first; h0 < walk.count; h0 += kHeads * walk.step) {
-    typename LaneVec<T, S>::raw_t r[kHeads][2];
+  const int first = div_by(start, q.by_groups);
+  fill_angles(q, first, q.span, table);
+  __syncthreads();
+  pl.angles(table + (walk.token - first) * (q.D >> 1), sn, cs);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int h = h0 + i * walk.step;
-      if (h < walk.count) pl.load(in + h * in_head, r[i]);
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = walk.first + i * walk.step;
+    A v[2 * S];
+    pl.unpack(r[i], v);
+    if constexpr (NORM) {
+      A ss = 0;
+#pragma unroll
+      for (int c = 0; c < 2 * S; ++c) ss += v[c] * v[c];
+      ss = segment_sum(lane < q.nvec ? ss : (A)0, q.lanes);
+      const A rstd = row_rsqrt(ss * (A)q.inv_d + (A)q.eps);
+#pragma unroll
+      for (int c = 0; c < 2 * S; ++c) v[c] = v[c] * rstd * w[c];
     }
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int h = h0 + i * walk.step;
-      A v[2 * S];
-      pl.unpack(r[i], v);
-      if constexpr (NORM) {
-        A ss = 0;
-#pragma unroll
-        for (int c = 0; c < 2 * S; ++c) ss += v[c] * v[c];
-        ss = segment_sum(lane < q.nvec ? ss : (A)0, q.lanes);
-        const A rstd = exact_rsqrt(ss * (A)q.inv_d + (A)q.eps);
-#pragma unroll
-        for (int c = 0; c < 2 * S; ++c) v[c] = v[c] * rstd * w[c];
-      }
-      pl.turn(v, sn, cs, partial);
-      if (stores && h < walk.count) pl.store(out + h * out_head, v);
-    }
+    pl.turn(v, sn, cs, partial);
+    if (stores && h < walk.count) pl.store(out + h * out_head, v);
   }
 }
 
@@ -208,51 +251,67 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
 template <typename T, typename P, int S, bool NEAR>
 __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArgs q) {
   using A = acc_of_t<T>;
+  constexpr int kHeads = kRotaryBwdHeads;
   extern __shared__ char lds_dyn[];
   const int lane = threadIdx.x & (q.lanes - 1), sub = threadIdx.x >> q.lanes_log2, subs = kBlock >> q.lanes_log2;
   const PairLane<T, S, NEAR> pl(q, lane);
   const bool partial = 2 * q.P < q.D;
-  const int start = (int)blockIdx.x * subs + sub;
-  // (groups that do not fill a whole set of heads stay idle)
-  HeadWalk walk = head_walk(q, start < q.walkers ? start : 0);
-  const bool works = start < q.walkers;
+  const int start = (int)blockIdx.x * subs;
+  const bool works = start + sub < q.walkers;  // (groups that do not fill a whole set of heads stay idle)
+  const HeadWalk walk = head_walk(q, works ? start + sub : start);
   const Side side = side_of(q, walk.which);
-  A w[2 * S], dw[2 * S], sn[S], cs[S];
+  SinCos<A> *const tables = (SinCos<A> *)lds_dyn;
+  const int first = div_by(start, q.by_groups), half = q.D >> 1;
+  A w[2 * S], dw[2 * S];
   pl.weights((const P *)side.weight, w);
 #pragma unroll
   for (int c = 0; c < 2 * S; ++c) dw[c] = 0;
-  int token = div_by(works ? start : 0, q.by_groups);
-  if (works)
-    for (; token < q.tokens; token += q.token_step) {
-      const int b = div_by(token, q.by_L), l = token - b * q.L;
-      pl.angles(q, b, l, sn, cs);
-      const T *in = (const T *)side.in + head_at(side.in_stride, b, l), *grad = (const T *)side.grad + head_at(side.grad_stride, b, l);
-      T *out = (T *)side.out + head_at(side.out_stride, b, l);
-      for (int h = walk.first; h < walk.count; h += walk.step) {
-        typename LaneVec<T, S>::raw_t rt[2], rd[2];
-        pl.load(in + h * side.in_stride[2], rt);
-        pl.load(grad + h * side.grad_stride[2], rd);
-        A t[2 * S], d[2 * S], ss = 0, gt = 0;
-        pl.unpack(rt, t);
-        pl.unpack(rd, d);
-        pl.turn(d, sn, cs, partial);
+  int turn = 0;
+  // (the bound is the workgroup's: all wavefronts meet at the same barriers; two tables in turn, so that one is enough)
+  for (int at = 0; first + at < q.tokens; at += q.token_step, turn ^= 1) {
+    const bool there = works && walk.token + at < q.tokens;
+    const int token = there ? walk.token + at : q.tokens - 1, b = div_by(token, q.by_L), l = token - b * q.L;
+    const T *in = (const T *)side.in + head_at(side.in_stride, b, l), *grad = (const T *)side.grad + head_at(side.grad_stride, b, l);
+    T *out = (T *)side.out + head_at(side.out_stride, b, l);
+    typename LaneVec<T, S>::raw_t rt[kHeads][2], rd[kHeads][2];
 #pragma unroll
-        for (int c = 0; c < 2 * S; ++c) {
-          ss += t[c] * t[c];
-          gt += d[c] * w[c] * t[c];
-        }
-        if (lane >= q.nvec) ss = gt = 0;
-        segment_sum2(ss, gt, q.lanes);
-        const A r = exact_rsqrt(ss * (A)q.inv_d + (A)q.eps), m = r * gt * (A)q.inv_d;
-#pragma unroll
-        for (int c = 0; c < 2 * S; ++c) {
-          const A hn = t[c] * r;
-          dw[c] += d[c] * hn;
-          d[c] = r * (d[c] * w[c] - hn * m);
-        }
-        if (lane < q.nvec) pl.store(out + h * side.out_stride[2], d);
-      }
+    for (int i = 0; i < kHeads; ++i) {
+      const int h = walk.first + i * walk.step < walk.count ? walk.first + i * walk.step : walk.first;
+      pl.load(in + h * side.in_stride[2], rt[i]);
+      pl.load(grad + h * side.grad_stride[2], rd[i]);
     }
+    SinCos<A> *const table = tables + turn * q.span * half;
+    fill_angles(q, first + at, q.span, table);
+    __syncthreads();
+    A sn[S], cs[S];
+    pl.angles(table + (walk.token - first) * half, sn, cs);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int h = walk.first + i * walk.step;
+      if (!there || h >= walk.count) continue;
+      A t[2 * S], d[2 * S], ss = 0, gt = 0;
+      pl.unpack(rt[i], t);
+      pl.unpack(rd[i], d);
+      pl.turn(d, sn, cs, partial);
+#pragma unroll
+      for (int c = 0; c < 2 * S; ++c) {
+        ss += t[c] * t[c];
+        gt += d[c] * w[c] * t[c];
+      }
+      if (lane >= q.nvec) ss = gt = 0;
+      segment_sum2(ss, gt, q.lanes);
+      // with h = t r and mean(g h) = r gt / D:  r (g - h mean) = r g - t (r^3 gt / D)
+      const A r = row_rsqrt(ss * (A)q.inv_d + (A)q.eps), m = -r * r * r * gt * (A)q.inv_d;
+#pragma unroll
+      for (int c = 0; c < 2 * S; ++c) {
+        const A dr = d[c] * r;
+        dw[c] += dr * t[c];
+        d[c] = dr * w[c] + t[c] * m;
+      }
+      if (lane < q.nvec) pl.store(out + h * side.out_stride[2], d);
+    }
+  }
+  __syncthreads();
   // the workgroup's groups, q's and k's apart
   A *box = (A *)lds_dyn;  // [subs][D]
   int *kind = (int *)(box + subs * q.D);

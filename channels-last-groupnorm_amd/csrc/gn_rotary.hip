@@ -35,12 +35,16 @@ typedef acc_of_t<elem_t> A;
 template <typename P, int S, bool NEAR> void launch_one(const RotaryArgs &a, bool norm, hipStream_t stream) {
   const int per_block = kBlock >> a.lanes_log2;
   const dim3 grid((unsigned)(((int64_t)a.tokens * a.groups + per_block - 1) / per_block));
-  if (norm) hipLaunchKernelGGL((rotary_kernel<elem_t, P, S, NEAR, true>), grid, dim3(kBlock), 0, stream, a);
-  else hipLaunchKernelGGL((rotary_kernel<elem_t, P, S, NEAR, false>), grid, dim3(kBlock), 0, stream, a);
+  const size_t lds = (size_t)a.span * (a.D / 2) * sizeof(SinCos<A>);
+  if (norm) hipLaunchKernelGGL((rotary_kernel<elem_t, P, S, NEAR, true>), grid, dim3(kBlock), lds, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<elem_t, P, S, NEAR, false>), grid, dim3(kBlock), lds, stream, a);
 }
 template <typename P, int S, bool NEAR> void launch_bwd(const RotaryArgs &a, int blocks, hipStream_t stream) {
   const int per_block = kBlock >> a.lanes_log2;
-  const size_t lds = (size_t)per_block * a.D * sizeof(A) + (size_t)per_block * sizeof(int);
+  // the walk's two tables of angles, and after it the groups' sums
+  const size_t tables = (size_t)2 * a.span * (a.D / 2) * sizeof(SinCos<A>);
+  const size_t sums = (size_t)per_block * a.D * sizeof(A) + (size_t)per_block * sizeof(int);
+  const size_t lds = tables > sums ? tables : sums;
   hipLaunchKernelGGL((rotary_norm_bwd_kernel<elem_t, P, S, NEAR>), dim3((unsigned)blocks), dim3(kBlock), lds, stream, a);
 }
 // Calls f<pairs a lane, near>() for the pairs that the plan chose.
@@ -76,10 +80,9 @@ hipError_t GN_CAT(launch_rotary_norm_bwd_, GN_SUFFIX)(const RotaryArgs &a, int p
     if (pdtype == GN_INST_DTYPE) launch_bwd<elem_t, decltype(s)::value, decltype(n)::value>(a, blocks, stream);
     else launch_bwd<wide_param_t, decltype(s)::value, decltype(n)::value>(a, blocks, stream);
   });
-  for (int i = 0; i < 2; ++i) {
-    if (!dw[i]) continue;
-    const PartialSum p = {(const A *)a.part + i * a.D, dw[i], blocks, a.D, pdtype, 2 * a.D};
-    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((a.D + 15) / 16)), dim3(256), 0, stream, p);
+  if (dw[0] || dw[1]) {
+    const PartialSum p = {a.part, {dw[0], dw[1]}, blocks, 2 * a.D, a.D, pdtype};
+    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((2 * a.D + 15) / 16)), dim3(1024), 0, stream, p);
   }
   return hipGetLastError();
 }

@@ -17,7 +17,7 @@ struct RowCut {
   bool ragged;
 };
 
-struct RmsFwd {
+struct RmsFwd {  // (see gn_rms.h)
   const void *x, *res, *w;
   void *sum, *y;
   float *scales;
@@ -35,6 +35,7 @@ struct RmsBwd {
   int C, nvec, lpr, lpr_log2;
 };
 
+constexpr int kRotaryHeads = 4, kRotaryBwdHeads = 2;  // most heads of a token that a group of lanes turns
 struct RotarySide {  // q or k
   const void *in, *grad, *weight;
   void *out;
@@ -49,25 +50,28 @@ struct RotaryArgs {
   int pos_type, axes, ends[4], P, D;
   int nvec, lanes, lanes_log2;  // lane vectors of half a head, lanes of a group
   int tokens, L, groups;        // batch * tokens, tokens of a sample, groups of a token (q's, then k's)
-  Divisor by_groups, by_L;
+  int span;                     // most tokens that a workgroup's groups belong to
+  Divisor by_groups, by_L, by_half;
   int walkers, token_step;      // backward behind a norm: groups that work, tokens between two of a group
   double eps, inv_d;
   float sign;                   // -1: turn back
   void *part;
 };
 
-// Sums of `count` rows of partial results, C values each, in a fixed order (gn_rms.hip).
+// Sums of `count` rows of partial results, C values each, in a fixed order (gn_rms.h).
 struct PartialSum {
   const void *part;
-  void *out;
-  int count, C, out_dtype;
-  int pitch;  // values from one row to the next
+  void *out[2];  // columns below and from `split` on; null: not wanted
+  int count, C, split, out_dtype;
 };
 
-RowCut rms_cut(int64_t C, int esize, int most_vectors, int least_lanes);
+RowCut rms_cut(int64_t C, int esize, int least_lanes);
 int rms_bwd_blocks(int64_t rows, const RowCut &cut);
 constexpr int kMostChannels = 16384;
-constexpr int kFwdVectors = 8, kBwdVectors = 4;  // most lane vectors of a row per lane
+constexpr int kRowVectors = 3;  // most lane vectors of a row per lane, but for the longest rows
+// What the memory-side cache is counted on to hold until the next kernel.  Inputs beyond it are read past the caches: forward of
+// float16 (65536, 2560) 229 -> 221 us, its backward 235 -> 229; but bf16 (16384, 1280), which the cache can hold, 26 -> 30.
+constexpr int64_t kCachedBytes = (int64_t)224 << 20;
 
 #define GN_DECLARE_TOKENS(S)                                                                            \
   hipError_t launch_rms_fwd_##S(const RmsFwd &a, const RowCut &cut, int pdtype, bool quant, hipStream_t stream);   \

@@ -76,36 +76,26 @@ int check_fwd(const void *x, const void *residual, void *sum_out, const void *y,
 
 }  // namespace
 
-// How a row's lane vectors are dealt to lanes: among the powers of two that leave each lane at most `most_vectors`, the one that
-// leaves the fewest lanes idle, and of those alike the one inside a wavefront.
-RowCut rms_cut(int64_t C, int esize, int most_vectors, int least_lanes) {
+// How a row's lane vectors are dealt to lanes: the fewest lanes (a power of two) that leave none more than three (forward of
+// float16 (65536, 2560): 223 us with three, 228 with five; bf16 in 8 bits, 128 channels a block, (16384, 2560): 54 and 61).
+RowCut rms_cut(int64_t C, int esize, int least_lanes) {
   const int vec = 16 / esize;
   RowCut c;
   c.vec = C < vec ? 1 : vec;
   c.nvec = (int)ceil_div(C, c.vec);
   c.ragged = C % c.vec != 0;
-  double best = -1;
-  c.lpr = c.nv = 0;
-  for (int lpr = std::max(8, least_lanes); lpr <= 1024; lpr <<= 1) {
-    int nv = (int)ceil_div(c.nvec, lpr);
-    if (nv == 7) nv = 8;
-    const int most = lpr > 256 ? kMostChannels / (esize == 8 ? 2 : 1) / (vec * 1024) : most_vectors;
-    if (nv > most) continue;
-    const double used = (double)c.nvec / ((double)lpr * nv) - (lpr > 64 ? 0.1 : 0.0);
-    if (used > best + 0.02) {
-      best = used;
-      c.lpr = lpr;
-      c.nv = nv;
-    }
-  }
+  c.lpr = std::max(8, least_lanes);
+  while (c.lpr < 1024 && c.nvec > kRowVectors * c.lpr) c.lpr <<= 1;
+  c.nv = (int)ceil_div(c.nvec, c.lpr);
   c.lpr_log2 = log2_of(c.lpr);
   c.threads = c.lpr > 256 ? c.lpr : 256;
   return c;
 }
-// Workgroups of the backward's walk: two per CU, or one for each step of rows where there are fewer.
+// Workgroups of the backward's walk: as many as walk equally far, up to two per CU (with three or four, float16 (65536, 2560)
+// takes 251 and 274 us instead of 235, bf16 (16384, 1280) 37 and 42 instead of 38).
 int rms_bwd_blocks(int64_t rows, const RowCut &cut) {
   const int64_t steps = ceil_div(rows, cut.threads / cut.lpr);
-  return (int)std::min<int64_t>(steps, 2 * kNumCU);
+  return steps == 0 ? 0 : (int)ceil_div(steps, ceil_div(steps, 2 * kNumCU));
 }
 
 namespace {
@@ -167,7 +157,7 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   if (backward && (!c->q_grad || (c->kv_heads && !c->k_grad))) return invalid("null gradient");
   const int64_t heads[2] = {c->heads, c->kv_heads};
   // heads a group takes one after the other: up to eight as long as the groups fill the device four times
-  int take = 8;
+  int take = backward && norm ? kRotaryBwdHeads : kRotaryHeads;
   while (take > 1 && tokens * (ceil_div(heads[0], take) + ceil_div(heads[1], take)) * a.lanes < (int64_t)4 * kNumCU * kBlock) take >>= 1;
   const void *in[2] = {c->q, c->k}, *grad[2] = {c->q_grad, c->k_grad}, *weight[2] = {c->q_weight, c->k_weight};
   void *out[2] = {c->q_out, c->k_out};
@@ -200,15 +190,18 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   a.L = (int)c->tokens;
   a.by_groups = make_divisor(a.groups, 0);
   a.by_L = make_divisor(a.L, 0);
+  a.by_half = make_divisor(half, 0);
+  const int subs = kBlock / a.lanes;
+  a.span = (int)std::min<int64_t>(tokens, (subs - 1 + a.groups - 1) / a.groups + 1);
   a.eps = c->eps;
   a.inv_d = 1.0 / a.D;
   a.sign = backward ? -1.0f : 1.0f;
   if (backward && norm) {
-    // a walk of whole sets of groups: two workgroups per CU, or as many as there are tokens
-    const int64_t subs = kBlock / a.lanes;
-    const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(tokens, 2 * kNumCU * subs / a.groups));
-    a.token_step = (int)steps;
-    a.walkers = (int)(steps * a.groups);
+    // a walk of whole sets of groups: three workgroups per CU, or as many as there are tokens, alike in length
+    const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(tokens, 3 * kNumCU * subs / a.groups));
+    const int64_t turns = (tokens + steps / 2) / steps;
+    a.token_step = (int)ceil_div(tokens, std::max<int64_t>(turns, 1));
+    a.walkers = a.token_step * a.groups;
     p.blocks = (int)ceil_div(a.walkers, subs);
   }
   return GNNHWC_OK;
@@ -227,7 +220,7 @@ int gnnhwc_rms_fwd(const void *x, const void *residual, const void *weight, void
   if (const int rc = check_eps(eps)) return rc;
   if (const int rc = check_fwd(x, residual, sum_out, y, rows)) return rc;
   if (rows == 0) return GNNHWC_OK;
-  const RowCut cut = rms_cut(C, elem_size(dtype), kFwdVectors, 8);
+  const RowCut cut = rms_cut(C, elem_size(dtype), 8);
   const RmsFwd a = fwd_args(x, residual, weight, sum_out, y, rows, C, x_stride, residual_stride, eps, cut);
   const int pt = weight ? param_dtype : dtype;
 #define GN_CALL(S) launch_rms_fwd_##S(a, cut, pt, false, (hipStream_t)stream)
@@ -249,7 +242,7 @@ int gnnhwc_rms_fwd_quant(const void *x, const void *residual, const void *weight
     return fail(GNNHWC_ERR_INVALID_ARGUMENT, "a block of %lld channels: a power of two from 16 to 256, or 0 for whole rows", (long long)block);
   if (rows == 0) return GNNHWC_OK;
   const int lanes = by_row ? 0 : (int)block / (16 / elem_size(dtype));
-  const RowCut cut = rms_cut(C, elem_size(dtype), kFwdVectors, std::max(8, lanes));
+  const RowCut cut = rms_cut(C, elem_size(dtype), std::max(8, lanes));
   RmsFwd a = fwd_args(x, residual, weight, sum_out, q, rows, C, x_stride, residual_stride, eps, cut);
   a.scales = scales;
   a.block_lanes = lanes;
@@ -264,7 +257,7 @@ int gnnhwc_rms_fwd_quant(const void *x, const void *residual, const void *weight
 
 size_t gnnhwc_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype) {
   if (check_rows(rows, C, dtype, dtype)) return 0;
-  const RowCut cut = rms_cut(C, elem_size(dtype), kBwdVectors, 8);
+  const RowCut cut = rms_cut(C, elem_size(dtype), 8);
   return 256 + (size_t)rms_bwd_blocks(rows, cut) * (size_t)C * (dtype == GN_F64 ? 8 : 4);
 }
 
@@ -277,7 +270,7 @@ int gnnhwc_rms_bwd(const void *dy, const void *ds, const void *s, const void *we
   if (!dx && !dweight) return GNNHWC_OK;
   if (dweight && (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < gnnhwc_rms_bwd_workspace_bytes(rows, C, dtype)))
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_rms_bwd_workspace_bytes");
-  const RowCut cut = rms_cut(C, elem_size(dtype), kBwdVectors, 8);
+  const RowCut cut = rms_cut(C, elem_size(dtype), 8);
   RmsBwd a = {};
   a.dy = dy; a.ds = ds; a.s = s; a.w = weight;
   a.dx = dx; a.part = dweight ? workspace : nullptr;
