@@ -84,7 +84,17 @@ __global__ __launch_bounds__(kBlock) void clip_norm_kernel(const ClipTable t, do
   if (threadIdx.x == 0) store_global<double>(part + blockIdx.x, sum);
 }
 
-template <typename T, typename U> __device__ void chunk_scale(const T *p, U *o, int n, double factor) {
+// One sum of many partial ones, in their place: for lists of more tables than kClipTables.
+__global__ __launch_bounds__(kBlock) void clip_sum_kernel(double *part, int parts) {
+  __shared__ double lds[4];
+  double sum = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < parts; i += kBlock) sum += load_global<double>(part + i);
+  sum = block_sum(sum, lds);
+  if (threadIdx.x == 0) store_global<double>(part, sum);
+}
+
+template <bool STREAM, typename T, typename U> __device__ void chunk_scale(const T *p, U *o, int n, double factor) {
   constexpr int VT = vec_of<T>::value, VU = vec_of<U>::value, VEC = VT < VU ? VT : VU;
   using LV = LaneVec<T, VEC>;
   using LU = LaneVec<U, VEC>;
@@ -107,7 +117,7 @@ template <typename T, typename U> __device__ void chunk_scale(const T *p, U *o, 
     for (int k0 = 0; k0 < kClipChunk / (VEC * kBlock); k0 += kSteps) {
       typename LV::raw_t r[kSteps];
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) r[k] = load_loose<LV>(p + ((k0 + k) * kBlock + (int)threadIdx.x) * VEC);
+      for (int k = 0; k < kSteps; ++k) r[k] = load_once<LV, STREAM>(p + ((k0 + k) * kBlock + (int)threadIdx.x) * VEC);
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) one(r[k], (k0 + k) * kBlock + (int)threadIdx.x);
     }
@@ -122,16 +132,16 @@ template <typename T, typename U> __device__ void chunk_scale(const T *p, U *o, 
     LaneVec<U, 1>::store(o + i, LaneVec<U, 1>::pack(u));
   }
 }
-template <typename T> __device__ __forceinline__ void scale_to(const T *p, void *o, int64_t at, int n, double f, int type) {
+template <bool STREAM, typename T> __device__ __forceinline__ void scale_to(const T *p, void *o, int64_t at, int n, double f, int type) {
   switch (type) {
-    case GN_F32: chunk_scale(p, (float *)o + at, n, f); break;
-    case GN_F64: chunk_scale(p, (double *)o + at, n, f); break;
-    case GN_F16: chunk_scale(p, (f16_t *)o + at, n, f); break;
-    default: chunk_scale(p, (bf16_t *)o + at, n, f); break;
+    case GN_F32: chunk_scale<STREAM>(p, (float *)o + at, n, f); break;
+    case GN_F64: chunk_scale<STREAM>(p, (double *)o + at, n, f); break;
+    case GN_F16: chunk_scale<STREAM>(p, (f16_t *)o + at, n, f); break;
+    default: chunk_scale<STREAM>(p, (bf16_t *)o + at, n, f); break;
   }
 }
 
-__global__ __launch_bounds__(kBlock) void clip_apply_kernel(const ClipTable t, const ClipFinish q) {
+template <bool STREAM> __global__ __launch_bounds__(kBlock) void clip_apply_kernel(const ClipTable t, const ClipFinish q) {
   __shared__ double lds[4];
   double sum = 0;
   for (int i = threadIdx.x; i < q.parts; i += kBlock) sum += load_global<double>(q.part + i);
@@ -150,10 +160,10 @@ __global__ __launch_bounds__(kBlock) void clip_apply_kernel(const ClipTable t, c
     const int n = (int)(e.n - at < kClipChunk ? e.n - at : kClipChunk);
     const int to = e.types >> 8;
     switch (e.types & 0xff) {
-      case GN_F32: scale_to((const float *)e.in + at, e.out, at, n, factor, to); break;
-      case GN_F64: scale_to((const double *)e.in + at, e.out, at, n, factor, to); break;
-      case GN_F16: scale_to((const f16_t *)e.in + at, e.out, at, n, factor, to); break;
-      default: scale_to((const bf16_t *)e.in + at, e.out, at, n, factor, to); break;
+      case GN_F32: scale_to<STREAM>((const float *)e.in + at, e.out, at, n, factor, to); break;
+      case GN_F64: scale_to<STREAM>((const double *)e.in + at, e.out, at, n, factor, to); break;
+      case GN_F16: scale_to<STREAM>((const f16_t *)e.in + at, e.out, at, n, factor, to); break;
+      default: scale_to<STREAM>((const bf16_t *)e.in + at, e.out, at, n, factor, to); break;
     }
   }
 }
@@ -164,8 +174,13 @@ hipError_t launch_clip_norm(const ClipTable &t, double *part, int blocks, hipStr
   hipLaunchKernelGGL(clip_norm_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, stream, t, part);
   return hipGetLastError();
 }
-hipError_t launch_clip_apply(const ClipTable &t, const ClipFinish &f, int blocks, hipStream_t stream) {
-  hipLaunchKernelGGL(clip_apply_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, stream, t, f);
+hipError_t launch_clip_sum(double *part, int parts, hipStream_t stream) {
+  hipLaunchKernelGGL(clip_sum_kernel, dim3(1), dim3(kBlock), 0, stream, part, parts);
+  return hipGetLastError();
+}
+hipError_t launch_clip_apply(const ClipTable &t, const ClipFinish &f, bool streams, int blocks, hipStream_t stream) {
+  if (streams) hipLaunchKernelGGL(clip_apply_kernel<true>, dim3((unsigned)blocks), dim3(kBlock), 0, stream, t, f);
+  else hipLaunchKernelGGL(clip_apply_kernel<false>, dim3((unsigned)blocks), dim3(kBlock), 0, stream, t, f);
   return hipGetLastError();
 }
 

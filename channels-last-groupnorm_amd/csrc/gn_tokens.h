@@ -92,8 +92,9 @@ struct ClipTable {
   int count;
   unsigned chunks;
 };
-constexpr int kClipChunk = 8192;     // elements
-constexpr int kClipPartials = 1024;  // partial sums over all launches (and one more for each launch)
+constexpr int kClipChunk = 16384;   // elements
+constexpr int kClipBlocks = 1024;   // workgroups of a norm's launch, each with a partial sum
+constexpr int kClipTables = 4;       // tables whose partial sums every workgroup of the second pass adds itself
 struct ClipFinish {
   const double *part;
   int parts;
@@ -103,7 +104,8 @@ struct ClipFinish {
   bool in_place;
 };
 hipError_t launch_clip_norm(const ClipTable &t, double *part, int blocks, hipStream_t stream);
-hipError_t launch_clip_apply(const ClipTable &t, const ClipFinish &f, int blocks, hipStream_t stream);
+hipError_t launch_clip_sum(double *part, int parts, hipStream_t stream);
+hipError_t launch_clip_apply(const ClipTable &t, const ClipFinish &f, bool streams, int blocks, hipStream_t stream);
 
 GN_DECLARE_TOKENS(f32)
 GN_DECLARE_TOKENS(f64)

@@ -156,7 +156,8 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   if (reads && (!c->q || (c->kv_heads && !c->k))) return invalid("null tensor");
   if (backward && (!c->q_grad || (c->kv_heads && !c->k_grad))) return invalid("null gradient");
   const int64_t heads[2] = {c->heads, c->kv_heads};
-  // heads a group takes one after the other: up to eight as long as the groups fill the device four times
+  // Heads that a group turns: as many as it has registers for, each of them on its way at once, as long as the groups fill the
+  // device four times.
   int take = backward && norm ? kRotaryBwdHeads : kRotaryHeads;
   while (take > 1 && tokens * (ceil_div(heads[0], take) + ceil_div(heads[1], take)) * a.lanes < (int64_t)4 * kNumCU * kBlock) take >>= 1;
   const void *in[2] = {c->q, c->k}, *grad[2] = {c->q_grad, c->k_grad}, *weight[2] = {c->q_weight, c->k_weight};
@@ -324,7 +325,8 @@ size_t gnnhwc_clip_workspace_bytes(int64_t count) {
     invalid("negative count");
     return 0;
   }
-  return (size_t)(kClipPartials + ceil_div(count, kClipEntries) + 1) * sizeof(double);
+  // (sums of more tables than these are added up on the way)
+  return (size_t)(std::min<int64_t>(ceil_div(count, kClipEntries), kClipTables) * kClipBlocks + 1) * sizeof(double);
 }
 
 int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const int *dtype, const int *out_dtype, int64_t count,
@@ -390,7 +392,8 @@ int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const
   f.max_norm = max_norm; f.eps = eps; f.grad_scale = grad_scale;
   f.total = total; f.total_dtype = total_dtype;
   f.in_place = !out;
-  // tables of up to kClipEntries tensors; a table's workgroups in proportion to its chunks
+  // tables of up to kClipEntries tensors, each with a launch of its own
+  int64_t bytes = 0;
   auto table_at = [&](size_t first, ClipTable &t) {
     t.count = (int)std::min<size_t>(list.size() - first, kClipEntries);
     t.chunks = 0;
@@ -400,25 +403,27 @@ int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const
       t.chunks += (unsigned)ceil_div(t.e[i].n, kClipChunk);
     }
   };
-  auto blocks_of = [&](const ClipTable &t) {
-    const int64_t share = chunks <= kClipPartials ? t.chunks : (int64_t)t.chunks * kClipPartials / chunks;
-    return (int)std::max<int64_t>(1, share);
-  };
   ClipTable t;
   for (size_t at = 0; at < list.size(); at += kClipEntries) {
     table_at(at, t);
-    const int blocks = blocks_of(t);
+    for (int i = 0; i < t.count; ++i) bytes += t.e[i].n * elem_size(t.e[i].types & 0xff);
+    const int blocks = (int)std::min<int64_t>(t.chunks, kClipBlocks);
+    if (f.parts + blocks > kClipTables * kClipBlocks + 1) {
+      if (const hipError_t e = launch_clip_sum(part, f.parts, (hipStream_t)stream)) return launched(e, "gnnhwc_clip");
+      f.parts = 1;
+    }
     if (const hipError_t e = launch_clip_norm(t, part + f.parts, blocks, (hipStream_t)stream)) return launched(e, "gnnhwc_clip");
     f.parts += blocks;
   }
   if (!scales || list.empty()) {
     t.count = 0;
     t.chunks = 0;
-    return launched(launch_clip_apply(t, f, 1, (hipStream_t)stream), "gnnhwc_clip");
+    return launched(launch_clip_apply(t, f, false, 1, (hipStream_t)stream), "gnnhwc_clip");
   }
   for (size_t at = 0; at < list.size(); at += kClipEntries) {
     if (list.size() > kClipEntries) table_at(at, t);
-    if (const hipError_t e = launch_clip_apply(t, f, blocks_of(t), (hipStream_t)stream)) return launched(e, "gnnhwc_clip");
+    const int blocks = (int)std::min<int64_t>(t.chunks, 2 * kClipBlocks);
+    if (const hipError_t e = launch_clip_apply(t, f, bytes > kCachedBytes, blocks, (hipStream_t)stream)) return launched(e, "gnnhwc_clip");
     f.total = nullptr;  // written by the first launch
   }
   return GNNHWC_OK;

@@ -505,7 +505,6 @@ def _dense(t):
     return True
 
 
-@torch.no_grad()
 def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
     """The Euclidean norm over all tensors of `grads`, and their clipping to `max_norm`; returns the norm as a tensor on the
     device (nothing waits for it).
@@ -526,6 +525,11 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
     result = _native.clip_gradients(grads, float(max_norm), outs, float(grad_scale), float(eps))
     if result is not NotImplemented:
         return result
+    with torch.no_grad():
+        return _clip_general(grads, outs, max_norm, grad_scale, eps)
+
+
+def _clip_general(grads, outs, max_norm, grad_scale, eps):
     dev = grads[0].device
     keep, back = [], []
     for i, g in enumerate(grads):
@@ -534,8 +538,8 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
         if g.layout != torch.strided or g.device != dev:
             raise RuntimeError("gradient %d must be a dense tensor on %s" % (i, dev))
         if outs is None:
-            if not _dense(g):  # a slice with gaps: through a copy
-                c = g.contiguous()
+            if not _dense(g) or g.is_neg():  # a slice with gaps, or a view that only stands for negated memory: through a copy
+                c = g.resolve_neg().contiguous()
                 back.append((g, c))
                 g = c
             keep.append((g, g))
@@ -545,9 +549,10 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
         _dtype_code(o, "out %d" % i)
         if o.shape != g.shape or o.device != dev or o.layout != torch.strided:
             raise RuntimeError("out %d must have the gradient's shape %s on %s" % (i, tuple(g.shape), dev))
-        if not (_dense(g) and _dense(o) and (g.stride() == o.stride() or g.is_contiguous() and o.is_contiguous())):
+        g = g.resolve_neg()
+        if not (_dense(g) and _dense(o) and not o.is_neg() and (g.stride() == o.stride() or g.is_contiguous() and o.is_contiguous())):
             g = g.contiguous()
-            if not o.is_contiguous():
+            if not o.is_contiguous() or o.is_neg():
                 c = torch.empty(o.shape, dtype=o.dtype, device=dev)
                 back.append((o, c))
                 o = c
@@ -568,7 +573,7 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
     _cabi.check(rc, "clip_gradients")
     for t, c in back:
         t.copy_(c)
-    if out is not None or grad_scale != 1.0 or max_norm < math.inf:
+    if outs is not None or grad_scale != 1.0 or max_norm < math.inf:
         torch.autograd.graph.increment_version([t for t in (grads if outs is None else outs) if not t.is_inference()])
     return total
 

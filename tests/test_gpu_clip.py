@@ -56,7 +56,7 @@ def test_in_place_and_elsewhere(dtypes, max_norm, device):
         assert all(torch.equal(a, b) for a, b in zip(grads, before))
 
 
-@pytest.mark.parametrize("count,size", [(1, 3_000_001), (500, 97), (260, 8200), (113, 1), (112, 5)])
+@pytest.mark.parametrize("count,size", [(1, 3_000_001), (500, 97), (260, 8200), (113, 1), (112, 5), (1300, 65)])
 def test_many_and_large(count, size, device):
     """More tensors than one table holds; gradients far apart in memory and neighbours in a bucket."""
     for packed in (False, True):
@@ -134,6 +134,19 @@ def test_layouts(device):
     _check_total(clip_gradients(grads, 2.0), want)
     _check_scaled(grads, before, 2.0 / (want + 1e-6))
     assert torch.equal(wide[:, [0, 1, 9, 10, 11]], rest)
+
+
+def test_negated_views(device):
+    """The imaginary part of a conjugate is a view whose memory holds the negated values."""
+    z = torch.complex(*_grads([(50,), (50,)], [F32, F32], device, 12)).conj()
+    grads = [z.imag, torch.ones(3, device=device)]
+    assert grads[0].is_neg()
+    before, want = [g.clone() for g in grads], _norm(grads)
+    out = [torch.empty(50, device=device), torch.empty(3, device=device)]
+    _check_total(clip_gradients(grads, 0.5, out=out), want)
+    _check_scaled(out, before, 0.5 / (want + 1e-6))
+    clip_gradients(grads, 0.5)
+    _check_scaled(grads, before, 0.5 / (want + 1e-6))
 
 
 def test_parameters(device):

@@ -115,6 +115,17 @@ def test_saved_tensor_hooks(data):
     assert torch.equal(a, b)
 
 
+def test_negated_views(device):
+    """Views that only stand for negated memory go through the dispatcher, which resolves them."""
+    z = torch.complex(torch.randn(4, 64, device=device), torch.randn(4, 64, device=device)).conj()
+    x = z.imag
+    assert x.is_neg()
+    assert torch.equal(rms_norm(x), rms_norm(x.clone())) and torch.equal(rms_norm(x, residual=x), rms_norm(x.clone(), residual=x.clone()))
+    f, p = rotary_frequencies((4,), device=device), torch.arange(4, device=device)
+    q = x.as_strided((1, 4, 8, 8), (512, x.stride(0), 8 * x.stride(1), x.stride(1)))
+    assert torch.equal(rotary(q, None, p, f), rotary(q.clone(), None, p, f))
+
+
 def test_modules(device):
     m = gnnhwc.RMSNorm(64).to(device).bfloat16()
     x = torch.randn(3, 64, device=device).bfloat16()
