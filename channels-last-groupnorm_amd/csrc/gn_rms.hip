@@ -50,11 +50,11 @@ template <typename F> void with_width(const RowCut &cut, F &&f) {
     return f(Three(), Narrow());
   }
   // rows longer than 256 lanes of three vectors hold
-  if (cut.nv == 2) return f(Two(), Wide());
-  if constexpr (kWideVectors > 3) {
+  if constexpr (kWideVectors > 2) {
+    if (cut.nv == 3) return f(Three(), Wide());
     if (cut.nv > 3) return f(std::integral_constant<int, 4>(), Wide());
   }
-  return f(Three(), Wide());
+  return f(Two(), Wide());
 }
 
 // ---- forward ----

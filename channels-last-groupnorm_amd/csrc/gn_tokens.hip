@@ -52,6 +52,9 @@ int check_rows(int64_t rows, int64_t C, int dtype, int param_dtype) {
 // (eps may be zero: a row of zeros then gives NaN, as the formula does)
 int check_eps(double eps) { return eps >= 0 && eps < INFINITY ? GNNHWC_OK : invalid("eps must be finite and not negative"); }
 
+// A launch has fewer than 2^32 threads: calls with more rows than that go out in pieces.
+int64_t rows_per_launch(const RowCut &cut) { return ((int64_t)1 << 31) / cut.lpr; }
+
 #define GN_BY_TYPE(dtype, call)                 \
   ((dtype) == GN_F32   ? call(f32)              \
    : (dtype) == GN_F64 ? call(f64)              \
@@ -67,6 +70,21 @@ RmsFwd fwd_args(const void *x, const void *residual, const void *weight, void *s
   a.eps = eps; a.inv_c = 1.0 / (double)C;
   a.C = (int)C; a.nvec = cut.nvec; a.lpr = cut.lpr; a.lpr_log2 = cut.lpr_log2;
   return a;
+}
+int launch_fwd(RmsFwd a, const RowCut &cut, int dtype, int param_dtype, bool quant, hipStream_t stream, const char *what) {
+  const int64_t rows = a.rows, most = rows_per_launch(cut), es = elem_size(dtype);
+  for (int64_t at = 0; at < rows; at += most) {
+    a.rows = std::min(most, rows - at);
+#define GN_CALL(S) launch_rms_fwd_##S(a, cut, param_dtype, quant, stream)
+    if (const hipError_t e = GN_BY_TYPE(dtype, GN_CALL)) return launched(e, what);
+#undef GN_CALL
+    a.x = (const char *)a.x + most * a.x_stride * es;
+    if (a.res) a.res = (const char *)a.res + most * a.res_stride * es;
+    if (a.sum) a.sum = (char *)a.sum + most * a.C * es;
+    a.y = (char *)a.y + most * a.C * (quant ? 1 : es);
+    if (a.scales) a.scales += most * a.nblocks;
+  }
+  return GNNHWC_OK;
 }
 int check_fwd(const void *x, const void *residual, void *sum_out, const void *y, int64_t rows) {
   if (rows > 0 && (!x || !y)) return invalid("null tensor");
@@ -85,7 +103,8 @@ RowCut rms_cut(int64_t C, int esize, int least_lanes) {
   c.nvec = (int)ceil_div(C, c.vec);
   c.ragged = C % c.vec != 0;
   c.lpr = std::max(8, least_lanes);
-  while (c.lpr < 1024 && c.nvec > kRowVectors * c.lpr) c.lpr <<= 1;
+  // (two where a workgroup is wider than 256: a third does not fit the registers of 1024 threads in the backward)
+  while (c.lpr < 1024 && c.nvec > (c.lpr > 256 ? 2 : kRowVectors) * c.lpr) c.lpr <<= 1;
   c.nv = (int)ceil_div(c.nvec, c.lpr);
   c.lpr_log2 = log2_of(c.lpr);
   c.threads = c.lpr > 256 ? c.lpr : 256;
@@ -179,7 +198,7 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
     s.groups = (int)ceil_div(heads[i], take);
   }
   a.groups = a.side[0].groups + a.side[1].groups;
-  if (tokens * a.groups > 0x7fff0000) return invalid("too many tokens and heads for one call");
+  if (tokens * a.groups > 0x7fff0000 || tokens * a.groups * a.lanes > 0xffff0000) return invalid("too many tokens and heads for one call");
   a.pos = c->positions;
   a.pos_stride[0] = c->position_stride[0];
   a.pos_stride[1] = c->position_stride[1];
@@ -222,11 +241,8 @@ int gnnhwc_rms_fwd(const void *x, const void *residual, const void *weight, void
   if (const int rc = check_fwd(x, residual, sum_out, y, rows)) return rc;
   if (rows == 0) return GNNHWC_OK;
   const RowCut cut = rms_cut(C, elem_size(dtype), 8);
-  const RmsFwd a = fwd_args(x, residual, weight, sum_out, y, rows, C, x_stride, residual_stride, eps, cut);
-  const int pt = weight ? param_dtype : dtype;
-#define GN_CALL(S) launch_rms_fwd_##S(a, cut, pt, false, (hipStream_t)stream)
-  return launched(GN_BY_TYPE(dtype, GN_CALL), "gnnhwc_rms_fwd");
-#undef GN_CALL
+  RmsFwd a = fwd_args(x, residual, weight, sum_out, y, rows, C, x_stride, residual_stride, eps, cut);
+  return launch_fwd(a, cut, dtype, weight ? param_dtype : dtype, false, (hipStream_t)stream, "gnnhwc_rms_fwd");
 }
 
 int gnnhwc_rms_fwd_quant(const void *x, const void *residual, const void *weight, void *sum_out, void *q, float *scales,
@@ -250,10 +266,7 @@ int gnnhwc_rms_fwd_quant(const void *x, const void *residual, const void *weight
   a.nblocks = by_row ? 1 : (int)ceil_div(C, block);
   a.qtype = q_dtype;
   a.q_most = q_dtype == GNNHWC_F8E4M3 ? 448.0f : 127.0f;
-  const int pt = weight ? param_dtype : dtype;
-#define GN_CALL(S) launch_rms_fwd_##S(a, cut, pt, true, (hipStream_t)stream)
-  return launched(GN_BY_TYPE(dtype, GN_CALL), "gnnhwc_rms_fwd_quant");
-#undef GN_CALL
+  return launch_fwd(a, cut, dtype, weight ? param_dtype : dtype, true, (hipStream_t)stream, "gnnhwc_rms_fwd_quant");
 }
 
 size_t gnnhwc_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype) {
