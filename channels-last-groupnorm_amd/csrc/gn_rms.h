@@ -182,6 +182,12 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
     s[k] = load_once<LV, STREAM>(x + cut.start(k));
     if constexpr (RES) r[k] = load_once<LV, STREAM>(res + cut.start(k));
   }
+  // Asked for here, so that it is there when the sum is, and without a branch, at whose end the compiler would wait for all that
+  // is on its way: without a weight P is T, and the row's own memory is read instead.
+  const P *wp = q.w ? (const P *)q.w : (const P *)x;
+  A w[NV][VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) load_params<P, VEC>(wp + cut.start(k), w[k]);
   A ss = 0, none = 0;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -196,11 +202,18 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
       if (q.sum && live && cut.has(k)) store_loose<LV>((T *)q.sum + row * q.C + cut.start(k), s[k]);
       LV::unpack(s[k], v);
     }
-    const int skip = cut.doubled(k);
     A part = 0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (!RAGGED || i >= skip) part += v[i] * v[i];
+    for (int i = 0; i < VEC; ++i) part += v[i] * v[i];
+    if constexpr (RAGGED) {
+      const int skip = cut.doubled(k);
+      if (skip > 0) {  // one lane a row: a branch of its own is cheaper than a selection for every element of all
+        issue_order_fence();
+        part = 0;
+#pragma unroll
+        for (int i = 1; i < VEC; ++i) part += i >= skip ? v[i] * v[i] : (A)0;
+      }
+    }
     ss += cut.has(k) ? part : (A)0;
   }
   row_sum2(ss, none, q.lpr, lds, 0);
@@ -209,11 +222,10 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
   if constexpr (!QUANT) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      A v[VEC], w[VEC];
+      A v[VEC];
       LV::unpack(s[k], v);
-      if (q.w) load_params<P, VEC>((const P *)q.w + cut.start(k), w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = q.w ? v[i] * rstd * w[i] : v[i] * rstd;
+      for (int i = 0; i < VEC; ++i) v[i] = q.w ? v[i] * rstd * w[k][i] : v[i] * rstd;
       if (live && cut.has(k)) store_loose<LV>((T *)q.y + row * q.C + cut.start(k), LV::pack(v));
     }
   } else {
@@ -221,16 +233,25 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
     uint32_t most[NV], whole = 0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      float w[VEC];
       LV::unpack(s[k], y[k]);
-      if (q.w) load_params<P, VEC>((const P *)q.w + cut.start(k), w);
-      const int skip = cut.doubled(k);
       most[k] = 0;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        y[k][i] = q.w ? y[k][i] * rstd * w[i] : y[k][i] * rstd;
+        y[k][i] = q.w ? y[k][i] * rstd * w[k][i] : y[k][i] * rstd;
         const uint32_t b = magnitude_bits(y[k][i]);
-        if ((!RAGGED || i >= skip) && b > most[k]) most[k] = b;
+        most[k] = b > most[k] ? b : most[k];
+      }
+      if constexpr (RAGGED) {
+        const int skip = cut.doubled(k);
+        if (skip > 0) {  // (the doubled elements may belong to another block)
+          issue_order_fence();
+          most[k] = 0;
+#pragma unroll
+          for (int i = 1; i < VEC; ++i) {
+            const uint32_t b = i >= skip ? magnitude_bits(y[k][i]) : 0;
+            most[k] = b > most[k] ? b : most[k];
+          }
+        }
       }
       if (!cut.has(k)) most[k] = 0;
       whole = most[k] > whole ? most[k] : whole;
