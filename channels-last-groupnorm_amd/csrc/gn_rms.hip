@@ -117,7 +117,7 @@ hipError_t GN_CAT(launch_rms_bwd_, GN_SUFFIX)(const RmsBwd &a, const RowCut &cut
   else bwd_params<wide_param_t>(a, cut, stream, blocks);
   if (dw) {
     const PartialSum p = {a.part, {dw, nullptr}, blocks, a.C, a.C, pdtype};
-    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, stream, p);
+    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((a.C + kSumColumns - 1) / kSumColumns)), dim3(kSumThreads), 0, stream, p);
   }
   return hipGetLastError();
 }

@@ -82,7 +82,7 @@ hipError_t GN_CAT(launch_rotary_norm_bwd_, GN_SUFFIX)(const RotaryArgs &a, int p
   });
   if (dw[0] || dw[1]) {
     const PartialSum p = {a.part, {dw[0], dw[1]}, blocks, 2 * a.D, a.D, pdtype};
-    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((2 * a.D + 15) / 16)), dim3(1024), 0, stream, p);
+    hipLaunchKernelGGL((partial_sum_kernel<A>), dim3((unsigned)((2 * a.D + kSumColumns - 1) / kSumColumns)), dim3(kSumThreads), 0, stream, p);
   }
   return hipGetLastError();
 }
