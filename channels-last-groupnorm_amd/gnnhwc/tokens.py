@@ -186,10 +186,6 @@ def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _channels_last_dim(t, channel_dim):
-    return t if t is None or channel_dim in (-1, t.dim() - 1) else t.movedim(channel_dim, -1)
-
-
 def rms_norm(x, weight=None, eps=1e-6, residual=None, return_sum=False, channel_dim=-1):
     """s / sqrt(mean(s^2) + eps) * weight over the channels, s = x + residual.
 
@@ -199,20 +195,19 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, return_sum=False, channel_
     front would, and is what is normalised.  With return_sum=True the call returns (y, s), so that s is the next residual
     (without a residual, s is x).  Means and products are in float32 (float64).  Differentiable in x, residual and weight;
     the gradients of s reach x and residual too."""
-    if not torch.compiler.is_compiling() and channel_dim == -1:
+    if channel_dim != -1 and channel_dim != x.dim() - 1:
+        last = [None if t is None else t.movedim(channel_dim, -1) for t in (x, residual)]
+        out = rms_norm(last[0], weight, eps, last[1], return_sum)
+        return tuple(t.movedim(-1, channel_dim) for t in out) if return_sum else out.movedim(-1, channel_dim)
+    if not torch.compiler.is_compiling():
         out = _native.rms_norm(x, weight, eps, residual, return_sum)
         if out is not NotImplemented:
             return out
-    if channel_dim != -1:
-        x, residual = _channels_last_dim(x, channel_dim), _channels_last_dim(residual, channel_dim)
     want = residual is not None and (return_sum or _needs_grad(x, residual, weight))
     y, s = torch.ops.gnop.rms_norm(x, residual, weight, eps, want)
-    if residual is None:
-        s = x
-    if channel_dim != -1:
-        y = y.movedim(-1, channel_dim)
-        s = s.movedim(-1, channel_dim) if return_sum else s
-    return (y, s) if return_sum else y
+    if not return_sum:
+        return y
+    return y, x if residual is None else s
 
 
 def rms_norm_quant(x, weight=None, eps=1e-6, residual=None, return_sum=False, out_dtype=torch.float8_e4m3fn, block=None):
@@ -447,7 +442,7 @@ def rotary(q, k, positions, frequencies, sections=None, interleaved=False, q_wei
 
     q: (B, L, heads, D), k: (B, L, kv_heads, D) or None, with any strides as long as a head's channels are contiguous (slices of
     one packed projection are read where they are); D even, up to 256.  positions: (L, axes) or (B, L, axes), int32, int64 or
-    float32 (with one axis also (L,) or (B, L)).  frequencies: float32, one for each turning pair, see rotary_frequencies;
+    float32, whole numbers within 32 bits and exact to 2^24 (with one axis also (L,) or (B, L)).  frequencies: float32, one for each turning pair, see rotary_frequencies;
     sections: how many of them belong to each axis, in order (None: all to one axis).  Pair j of a head is its channels
     (2 j, 2 j + 1) if `interleaved`, else (j, j + P), P = sum(sections); it is turned by positions[axis] * frequencies[j].
     Channels behind the 2 P first stay as they are.

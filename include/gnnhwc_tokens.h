@@ -94,7 +94,7 @@ typedef struct gnnhwc_rotary_call {
   int64_t interleaved;
   const void *positions;                        /* (batch, tokens, axes), axes contiguous */
   int64_t position_stride[2];                   /* batch (0: the same for all), token */
-  int64_t position_type;                        /* 0 int32, 1 int64, 2 float; exact up to 2^24 */
+  int64_t position_type;                        /* 0 int32, 1 int64 (within 32 bits), 2 float; exact up to 2^24 */
   const float *frequencies;                     /* P */
   const void *q_weight, *k_weight;              /* both or none (k_weight only with k) */
   void *q_dweight, *k_dweight;

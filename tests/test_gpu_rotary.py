@@ -1,9 +1,11 @@
 """GPU tests of rotary against its formula in float64 (tests/token_refs.py has the bounds and where they come from)."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+from gnnhwc import _cabi
 from gnnhwc import Rotary, rotary, rotary_frequencies
 from tests import token_refs as ref
 
@@ -210,6 +212,52 @@ def test_empty(device):
     y = rotary(q, None, torch.zeros((3, 1), device=device), f, q_weight=w)
     dq, dw = torch.autograd.grad(y, [q, w], torch.zeros_like(y))
     assert dq.shape == q.shape and torch.equal(dw, torch.zeros(8, device=device))
+
+
+@pytest.mark.parametrize("near", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_in_place_through_the_c_abi(norm, near, device):
+    """Outputs in the place of the inputs they replace, in a packed projection; and of the incoming gradients in the backward."""
+    B, L, H, Kh, D = 3, 37, 5, 2, 80
+    f, sections = rotary_frequencies((10, 20), device=device), (10, 20)
+    p = torch.randint(0, 300, (L, 2), generator=torch.Generator().manual_seed(1)).to(device)
+    packed = _normal((B, L, (H + 2 * Kh) * D), BF16, device, 2)
+    w = [(1 + 0.2 * _normal((D,), F64, "cpu", 3 + i)).to(BF16).to(device).requires_grad_(True) for i in range(2)] if norm else [None, None]
+    view = lambda t: (t[..., :H * D].view(B, L, H, D), t[..., H * D:(H + Kh) * D].view(B, L, Kh, D))  # noqa: E731
+    q, k = (t.clone().requires_grad_(True) for t in view(packed))
+    want = rotary(q, k, p, f, sections, near, *w, EPS)
+    grads = _normal(q.shape, BF16, device, 5), _normal(k.shape, BF16, device, 6)
+    want_back = torch.autograd.grad(want, [q, k] + [t for t in w if t is not None], grads)
+
+    def call(**tensors):
+        c = _cabi.RotaryCall()
+        c.batch, c.tokens, c.heads, c.kv_heads, c.head_dim, c.axes, c.interleaved = B, L, H, Kh, D, 2, int(near)
+        c.section_end[0], c.section_end[1] = 10, 30
+        c.positions, c.position_type, c.frequencies, c.eps, c.dtype, c.param_dtype = p.data_ptr(), 1, f.data_ptr(), EPS, _cabi.BF16, _cabi.BF16
+        c.position_stride[0], c.position_stride[1] = 0, 2
+        if norm:
+            c.q_weight, c.k_weight = w[0].data_ptr(), w[1].data_ptr()
+        for name, t in tensors.items():
+            setattr(c, name, t.data_ptr())
+            if t.dim() == 4:
+                setattr(c, name + "_stride", (ctypes.c_int64 * 3)(*t.stride()[:3]))
+        return c
+
+    stream = torch.cuda.current_stream().cuda_stream
+    rest = packed[..., (H + Kh) * D:].clone()
+    a, b = view(packed)
+    _cabi.check(_cabi.lib.gnnhwc_rotary(ctypes.byref(call(q=a, k=b, q_out=a, k_out=b)), stream), "gnnhwc_rotary")
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1]) and torch.equal(packed[..., (H + Kh) * D:], rest)
+    gq, gk = (g.clone() for g in grads)
+    dw = [torch.empty(D, dtype=BF16, device=device) for _ in range(2)]
+    tensors = dict(q_grad=gq, k_grad=gk, q_out=gq, k_out=gk)
+    if norm:
+        tensors.update(q=q.detach(), k=k.detach(), q_dweight=dw[0], k_dweight=dw[1])
+    c = call(**tensors)
+    ws = torch.empty(_cabi.lib.gnnhwc_rotary_bwd_workspace_bytes(ctypes.byref(c)), dtype=torch.uint8, device=device)
+    _cabi.check(_cabi.lib.gnnhwc_rotary_bwd(ctypes.byref(c), ws.data_ptr(), ws.numel(), stream), "gnnhwc_rotary_bwd")
+    got = [gq, gk] + (dw if norm else [])
+    assert all(torch.equal(x, y) for x, y in zip(got, want_back))
 
 
 def test_graph_stream_and_compile(device):

@@ -93,6 +93,29 @@ def test_versions_move_on(device):
         assert t._version == before
 
 
+def test_operators_pass_torchs_checks(data):
+    """Schemas, fake tensors, autograd registration and tracing with dynamic shapes."""
+    leaf = lambda t: t.detach().clone().requires_grad_(True)  # noqa: E731
+    ops, check = torch.ops.gnop, torch.library.opcheck
+    x, r, w, q, k, p, f = (data[n] for n in ("x", "r", "w", "q", "k", "p", "f"))
+    check(ops.rms_norm.default, (leaf(x), leaf(r), leaf(w), 1e-6, True))
+    check(ops.rms_norm.default, (leaf(x), leaf(r), None, 1e-6, False))
+    check(ops.rms_norm_bwd.default, (x, r, x, w, 1e-6))
+    check(ops.rms_norm_quant.default, (x, r, w, 1e-6, 32, torch.int8, True))
+    check(ops.rotary.default, (leaf(q), leaf(k), p, f, [8, 12, 12], True, leaf(data["qw"]), leaf(data["kw"]), 1e-6))
+    check(ops.rotary.default, (leaf(q), None, p, f, [8, 12, 12], False, None, None, 1e-6))
+    check(ops.rotary_bwd.default, (q, k, q, k, p, f, [8, 12, 12], True, data["qw"], data["kw"], 1e-6))
+
+
+def test_images_are_native(data, monkeypatch, device):
+    """Channels-last images reach the native call as the rows they are."""
+    monkeypatch.setattr(torch.ops.gnop, "rms_norm", None)
+    image = torch.randn(2, 160, 3, 4, device=device).to(memory_format=torch.channels_last).requires_grad_(True)
+    y, s = rms_norm(image, data["w"], residual=image, return_sum=True, channel_dim=1)
+    assert y.shape == image.shape and y.is_contiguous(memory_format=torch.channels_last) and torch.equal(s, image + image)
+    assert torch.autograd.grad(y.sum(), image)[0].shape == image.shape
+
+
 def test_saved_tensor_hooks(data):
     """Tensors offloaded to the host between forward and backward, and gradients in other layouts."""
     x, w = data["x"].detach().clone().requires_grad_(True), data["w"].detach().clone().requires_grad_(True)
