@@ -144,6 +144,7 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   }
   if (last < 1 || 2 * last > c->head_dim) return invalid("sections must hold 1 to head_dim / 2 pairs");
   if (c->position_type < 0 || c->position_type > 2) return invalid("position_type must be 0 (int32), 1 (int64) or 2 (float)");
+  if (c->tokens > 0 && c->batch > 0x40000000 / c->tokens) return invalid("too many tokens: at most 2^30");
   if ((c->kv_heads > 0) != (c->k_out != nullptr) && c->batch * c->tokens > 0) return invalid("kv_heads without k_out, or the reverse");
   if (c->kv_heads > 0 && (c->q_weight != nullptr) != (c->k_weight != nullptr)) return invalid("q_weight and k_weight go together");
   const bool norm = c->q_weight != nullptr;
@@ -167,7 +168,6 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   a.lanes = 1 << a.lanes_log2;
   if (p.empty) return GNNHWC_OK;
 
-  if (c->batch > 0x7fffffff / c->tokens || c->batch * c->tokens > 0x40000000) return invalid("too many tokens: at most 2^30");
   const int64_t tokens = c->batch * c->tokens;
   if (!c->positions || !c->frequencies) return invalid("null positions or frequencies");
   if (!c->q_out || (c->kv_heads && !c->k_out)) return invalid("null output");

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <vector>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include "../../include/gnnhwc_tokens.h"
@@ -29,9 +30,13 @@ struct Entry {
 } abi = {};
 
 void check(int rc, const char *what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, "): ", abi.last_error()); }
+// Memory on like's device from the caching allocator, without the dispatcher: small calls are bound by the host.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
 Tensor workspace(size_t bytes, const Tensor &like, const char *what) {
   TORCH_CHECK(bytes != 0, what, ": ", abi.last_error());
-  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+  return fresh({(int64_t)bytes}, at::kByte, like);
 }
 PyObject *decline() { Py_RETURN_NOTIMPLEMENTED; }
 Tensor defined(const optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
@@ -116,8 +121,8 @@ void run_norm(const NormCall &c, bool want_sum, Tensor &y, Tensor &sum) {
   const c10::DeviceGuard guard(c.x.device());
   const at::AutoDispatchBelowADInplaceOrView below;
   const OperatorRange range("gnop::rms_norm");
-  y = at::empty(c.x.sizes(), c.x.options());
-  if (want_sum && c.residual.defined()) sum = at::empty(c.x.sizes(), c.x.options());
+  y = fresh(c.x.sizes(), c.x.scalar_type(), c.x);
+  if (want_sum && c.residual.defined()) sum = fresh(c.x.sizes(), c.x.scalar_type(), c.x);
   check(abi.rms_fwd(c.x.data_ptr(), ptr(c.residual), ptr(c.weight), ptr(sum), y.data_ptr(), c.xr.count, c.xr.C, c.xr.stride, c.rr.stride, c.eps,
                     code_of(c.x.scalar_type()), param_code(c.weight, c.x), stream_of(c.x)),
         "gnop::rms_norm");
@@ -159,11 +164,11 @@ struct NormNode : public torch::autograd::Function<NormNode> {
       const int dt = code_of(s.scalar_type());
       // (edges count the inputs that are there: x, weight, residual)
       const bool wants_dx = ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(weight.defined() ? 2 : 1));
-      if (wants_dx) dx = at::empty(s.sizes(), s.options());
+      if (wants_dx) dx = fresh(s.sizes(), s.scalar_type(), s);
       Tensor ws;
       size_t bytes = 0;
       if (weight.defined() && ctx->needs_input_grad(1)) {
-        dw = at::empty({sr.C}, weight.options());
+        dw = fresh({sr.C}, weight.scalar_type(), weight);
         bytes = abi.rms_bwd_workspace_bytes(sr.count, sr.C, dt);
         ws = workspace(bytes, s, "gnop::rms_norm_bwd");
       }
@@ -228,10 +233,10 @@ PyObject *rms_norm_quant(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const at::AutoDispatchBelowADInplaceOrView below;
     const OperatorRange range("gnop::rms_norm_quant");
     c10::SmallVector<int64_t, 6> shape(c.x.sizes().begin(), c.x.sizes().end());
-    q = at::empty(shape, c.x.options().dtype(out));
+    q = fresh(shape, out, c.x);
     shape.back() = block == 0 || block >= c.xr.C ? 1 : (c.xr.C + block - 1) / block;
-    scales = at::empty(shape, c.x.options().dtype(at::kFloat));
-    if (return_sum && c.residual.defined()) sum = at::empty(c.x.sizes(), c.x.options());
+    scales = fresh(shape, at::kFloat, c.x);
+    if (return_sum && c.residual.defined()) sum = fresh(c.x.sizes(), c.x.scalar_type(), c.x);
     check(abi.rms_fwd_quant(c.x.data_ptr(), ptr(c.residual), ptr(c.weight), ptr(sum), q.data_ptr(), (float *)scales.data_ptr(), c.xr.count, c.xr.C,
                             c.xr.stride, c.rr.stride, block, c.eps, code_of(c.x.scalar_type()), param_code(c.weight, c.x),
                             out == at::kChar ? GNNHWC_I8 : GNNHWC_F8E4M3, stream_of(c.x)),
@@ -316,13 +321,13 @@ void run_rotary(const Tensor &q, const Tensor &k, gnnhwc_rotary_call &c, Tensor 
   const c10::DeviceGuard guard(q.device());
   const at::AutoDispatchBelowADInplaceOrView below;
   const OperatorRange range("gnop::rotary");
-  qo = at::empty(q.sizes(), q.options());
+  qo = fresh(q.sizes(), q.scalar_type(), q);
   c.q = q.data_ptr();
   c.q_out = qo.data_ptr();
   put_strides(q, c.q_stride);
   put_strides(qo, c.q_out_stride);
   if (k.defined()) {
-    ko = at::empty(k.sizes(), k.options());
+    ko = fresh(k.sizes(), k.scalar_type(), k);
     c.k = k.data_ptr();
     c.k_out = ko.data_ptr();
     put_strides(k, c.k_stride);
@@ -371,13 +376,13 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
       const c10::DeviceGuard guard(device);
       const at::AutoDispatchBelowADInplaceOrView below;
       const OperatorRange range("gnop::rotary_bwd");
-      dq = at::empty(gq.sizes(), gq.options());
+      dq = fresh(gq.sizes(), gq.scalar_type(), gq);
       c.q_grad = gq.data_ptr();
       c.q_out = dq.data_ptr();
       put_strides(gq, c.q_grad_stride);
       put_strides(dq, c.q_out_stride);
       if (has_k) {
-        dk = at::empty(gk.sizes(), gk.options());
+        dk = fresh(gk.sizes(), gk.scalar_type(), gk);
         c.k_grad = gk.data_ptr();
         c.k_out = dk.data_ptr();
         put_strides(gk, c.k_grad_stride);
@@ -388,12 +393,12 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
       if (norm) {
         c.q = q.data_ptr();
         put_strides(q, c.q_stride);
-        dqw = at::empty({c.head_dim}, qw.options());
+        dqw = fresh({c.head_dim}, qw.scalar_type(), qw);
         c.q_dweight = dqw.data_ptr();
         if (has_k) {
           c.k = k.data_ptr();
           put_strides(k, c.k_stride);
-          dkw = at::empty({c.head_dim}, kw.options());
+          dkw = fresh({c.head_dim}, kw.scalar_type(), kw);
           c.k_dweight = dkw.data_ptr();
         }
         bytes = abi.rotary_bwd_workspace_bytes(&c);
@@ -512,7 +517,7 @@ PyObject *clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const c10::DeviceGuard guard(first.device());
     const at::AutoDispatchBelowADInplaceOrView below;
     const OperatorRange range("gnop::clip_gradients");
-    total = at::empty({}, first.options().dtype(all_double ? at::kDouble : at::kFloat));
+    total = fresh({}, all_double ? at::kDouble : at::kFloat, first);
     const size_t bytes = abi.clip_workspace_bytes(n);
     const Tensor ws = workspace(bytes, first, "clip_gradients");
     check(abi.clip(in.data(), elsewhere ? out.data() : nullptr, sizes.data(), types.data(), elsewhere ? out_types.data() : nullptr, n, max_norm, eps,

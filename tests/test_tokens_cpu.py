@@ -93,7 +93,7 @@ def _call(**change):
                                          (dict(position_type=3), "position_type"), (dict(heads=0), "heads"), (dict(heads=70000, kv_heads=0, k_out=None), "heads"),
                                          (dict(kv_heads=0), "kv_heads"), (dict(k_out=None), "kv_heads"), (dict(dtype=7), "dtype"),
                                          (dict(q_weight="p"), "together"), (dict(positions=None), "null"), (dict(frequencies=None), "null"),
-                                         (dict(q=None), "null"), (dict(k=None), "null"), (dict(batch=2 ** 31, tokens=4), "tokens"),
+                                         (dict(q=None), "null"), (dict(k=None), "null"), (dict(batch=2 ** 31, tokens=4), "tokens"), (dict(batch=2 ** 40, tokens=2 ** 40), "tokens"),
                                          (dict(batch=-1), "batch"), (dict(q_weight="p", k_weight="p", eps=-1.0), "eps"),
                                          (dict(q_weight="p", k_weight="p", param_dtype=F16), "weight dtype"),
                                          (dict(head_dim=254, ends=(8, 16)), "multiple of 8")])
