@@ -106,9 +106,9 @@ template <typename T, int S, bool NEAR> struct PairLane {
       cs[i] = v.cs;
     }
   }
-  __device__ __forceinline__ void load(const T *p, typename LaneVec<T, S>::raw_t (&r)[2]) const {
-    r[0] = load_loose<LaneVec<T, S>>(p + at0);
-    r[1] = load_loose<LaneVec<T, S>>(p + at1);
+  template <bool STREAM = false> __device__ __forceinline__ void load(const T *p, typename LaneVec<T, S>::raw_t (&r)[2]) const {
+    r[0] = load_once<LaneVec<T, S>, STREAM>(p + at0);
+    r[1] = load_once<LaneVec<T, S>, STREAM>(p + at1);
   }
   __device__ __forceinline__ static void unpack(const typename LaneVec<T, S>::raw_t (&r)[2], A (&v)[2 * S]) {
     A t[S];
@@ -201,7 +201,7 @@ __device__ __forceinline__ Side side_of(const RotaryArgs &q, int which) {
 }
 __device__ __forceinline__ int64_t head_at(const int64_t (&s)[3], int b, int l) { return b * s[0] + l * s[1]; }
 
-template <typename T, typename P, int S, bool NEAR, bool NORM>
+template <typename T, typename P, int S, bool NEAR, bool NORM, bool STREAM>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
   using A = acc_of_t<T>;
   constexpr int kHeads = kRotaryHeads;
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = walk.first + i * walk.step;
-    pl.load(in + (h < walk.count ? h : walk.first) * in_head, r[i]);
+    pl.template load<STREAM>(in + (h < walk.count ? h : walk.first) * in_head, r[i]);
   }
   A sn[S], cs[S], w[2 * S];
   if constexpr (NORM) pl.weights((const P *)side.weight, w);
@@ -232,6 +232,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = walk.first + i * walk.step;
+    if (h >= walk.count) continue;
     A v[2 * S];
     pl.unpack(r[i], v);
     if constexpr (NORM) {
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
       for (int c = 0; c < 2 * S; ++c) v[c] = v[c] * rstd * w[c];
     }
     pl.turn(v, sn, cs, partial);
-    if (stores && h < walk.count) pl.store(out + h * out_head, v);
+    if (stores) pl.store(out + h * out_head, v);
   }
 }
 
