@@ -5,7 +5,7 @@
 //   dt = r (g - h mean(g h)),        dw = sum over heads and tokens of d h
 //
 // Memory bounds them: q and k are read once and written once; angles come from a position and P frequencies per token and are
-// not read from tables: float16 (46800 tokens, 24 + 24 heads, 128) 202 us, 5.7 TB/s, a copy's rate; bf16 (16384, 20 + 20, 64)
+// not read from tables: float16 (46800 tokens, 24 + 24 heads, 128) 192 us, 6.0 TB/s (a copy: 5.7); bf16 (16384, 20 + 20, 64)
 // with a norm 35 us, 4.7 (a copy of that size: 5.1), its backward 50, 5.0.  A group of lanes (a power of two, W >= pairs / S)
 // takes one head at a time, each lane S pairs as two lane vectors; it turns every `groups`-th head of its token, so that one
 // set of sines and cosines serves several heads and neighbouring groups read neighbouring memory.
