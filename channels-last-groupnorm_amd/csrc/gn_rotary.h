@@ -6,9 +6,9 @@
 //
 // Memory bounds them: q and k are read once and written once; angles come from a position and P frequencies per token and are
 // not read from tables: float16 (46800 tokens, 24 + 24 heads, 128) 192 us, 6.0 TB/s (a copy: 5.7); bf16 (16384, 20 + 20, 64)
-// with a norm 35 us, 4.7 (a copy of that size: 5.1), its backward 50, 5.0.  A group of lanes (a power of two, W >= pairs / S)
-// takes one head at a time, each lane S pairs as two lane vectors; it turns every `groups`-th head of its token, so that one
-// set of sines and cosines serves several heads and neighbouring groups read neighbouring memory.
+// with a norm 31 us, 5.4 (a copy of that size: 5.1), its backward 46, 5.4.  A group of lanes (a power of two) takes one head at
+// a time, each lane one or two lane vectors of it; it turns every `groups`-th head of its token, so that one set of sines and
+// cosines serves several heads and neighbouring groups read neighbouring memory.
 #pragma once
 #include "gn_rms.h"
 
@@ -74,75 +74,88 @@ template <typename A> __device__ __forceinline__ void fill_angles(const RotaryAr
   }
 }
 
-// The pairs of one lane: S of them as two lane vectors of S channels.  Neighbouring lanes hold neighbouring vectors, so that
-// one access of a group is one run of memory: far pairs (j, j + P) have a vector from either half of the turning channels, near
-// pairs (2j, 2j + 1) one from either half of the head, with S / 2 pairs each.  (A lane with all its near pairs behind each other
-// reads every line twice: float16 (46800, 24 + 24 heads, 128) 286 us.)
+// Whether a lane holds one vector of a head, with its near pairs inside (the host's plan decides alike).  Of 16 bits alone: halves
+// of a head, 64 bytes at 32 channels each, made the stores write 16 to 25 % more than the head (bf16 (16384, 20 + 20, 64) 36.5 us,
+// whole 31; its backward behind a norm 51 and 47; float16 (65536, 8 + 8, 80) 71 and 59), while halves of 32 bits are longer and a
+// workgroup of half as many heads costs more: float32 (308142, 2 + 1, 96) 129 us, whole 150; (770, 24 + 12, 40) 4.9 and 5.3.
+template <typename T, int S, bool NEAR> constexpr bool kNearWhole = NEAR && S > 1 && sizeof(T) == 2;
+
+// What one lane holds of a head: one or two lane vectors of S channels, neighbouring lanes neighbouring vectors, so that one
+// access of a group is one run of memory.  Far pairs (j, j + P) have a vector from either half of the turning channels; near
+// pairs (2j, 2j + 1) lie inside a vector, and where there are two, they come from either half of the head.  (Two vectors behind
+// each other read every line twice: float16 (46800, 24 + 24 heads, 128) 286 us.)
 template <typename T, int S, bool NEAR> struct PairLane {
   using A = acc_of_t<T>;
-  static constexpr bool kHalves = NEAR && S > 1;
+  static constexpr bool kWhole = kNearWhole<T, S, NEAR>;
+  static constexpr int kVecs = kWhole ? 1 : 2, kPairs = kWhole ? S / 2 : S, kWidth = kVecs * S;
+  static constexpr bool kHalves = NEAR && S > 1 && !kWhole;
   int j0, j1, at0, at1, P;  // j1: first pair of the second vector, where that has pairs of its own
   __device__ __forceinline__ PairLane(const RotaryArgs &q, int lane) : P(q.P) {
     const int v = lane < q.nvec ? lane : q.nvec - 1;  // spare lanes repeat the last vector and store nothing
-    if constexpr (kHalves) {
+    j1 = at1 = 0;
+    if constexpr (kWhole) {
+      j0 = v * (S / 2);
+      at0 = v * S;
+    } else if constexpr (kHalves) {
       j0 = v * (S / 2);
       j1 = (q.nvec + v) * (S / 2);
       at0 = 2 * j0;
       at1 = 2 * j1;
     } else {
       j0 = v * S;
-      j1 = 0;
       const bool far = !NEAR && j0 < P;  // (S divides P where pairs are far)
       at0 = far ? j0 : 2 * j0;
       at1 = far ? j0 + P : 2 * j0 + S;
     }
   }
   __device__ __forceinline__ int pair(int i) const { return kHalves && i >= S / 2 ? j1 + i - S / 2 : j0 + i; }
-  __device__ __forceinline__ void angles(const SinCos<A> *row, A (&sn)[S], A (&cs)[S]) const {
+  __device__ __forceinline__ int at(int k) const { return k ? at1 : at0; }
+  typedef typename LaneVec<T, S>::raw_t raw_t;
+  __device__ __forceinline__ void angles(const SinCos<A> *row, A (&sn)[kPairs], A (&cs)[kPairs]) const {
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
+    for (int i = 0; i < kPairs; ++i) {
       const SinCos<A> v = row[pair(i)];
       sn[i] = v.sn;
       cs[i] = v.cs;
     }
   }
-  template <bool STREAM = false> __device__ __forceinline__ void load(const T *p, typename LaneVec<T, S>::raw_t (&r)[2]) const {
-    r[0] = load_once<LaneVec<T, S>, STREAM>(p + at0);
-    r[1] = load_once<LaneVec<T, S>, STREAM>(p + at1);
+  template <bool STREAM = false> __device__ __forceinline__ void load(const T *p, raw_t (&r)[kVecs]) const {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) r[k] = load_once<LaneVec<T, S>, STREAM>(p + at(k));
   }
-  __device__ __forceinline__ static void unpack(const typename LaneVec<T, S>::raw_t (&r)[2], A (&v)[2 * S]) {
+  __device__ __forceinline__ static void unpack(const raw_t (&r)[kVecs], A (&v)[kWidth]) {
     A t[S];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      LaneVec<T, S>::unpack(r[h], t);
+    for (int k = 0; k < kVecs; ++k) {
+      LaneVec<T, S>::unpack(r[k], t);
 #pragma unroll
-      for (int i = 0; i < S; ++i) v[h * S + i] = t[i];
+      for (int i = 0; i < S; ++i) v[k * S + i] = t[i];
     }
   }
-  __device__ __forceinline__ void store(T *p, const A (&v)[2 * S]) const {
+  __device__ __forceinline__ void store(T *p, const A (&v)[kWidth]) const {
     A t[S];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int k = 0; k < kVecs; ++k) {
 #pragma unroll
-      for (int i = 0; i < S; ++i) t[i] = v[h * S + i];
-      store_loose<LaneVec<T, S>>(p + (h ? at1 : at0), LaneVec<T, S>::pack(t));
+      for (int i = 0; i < S; ++i) t[i] = v[k * S + i];
+      store_loose<LaneVec<T, S>>(p + at(k), LaneVec<T, S>::pack(t));
     }
   }
-  template <typename W> __device__ __forceinline__ void weights(const W *w, A (&v)[2 * S]) const {
+  template <typename W> __device__ __forceinline__ void weights(const W *w, A (&v)[kWidth]) const {
     A t[S];
-    load_params<W, S>(w + at0, t);
 #pragma unroll
-    for (int i = 0; i < S; ++i) v[i] = t[i];
-    load_params<W, S>(w + at1, t);
+    for (int k = 0; k < kVecs; ++k) {
+      load_params<W, S>(w + at(k), t);
 #pragma unroll
-    for (int i = 0; i < S; ++i) v[S + i] = t[i];
+      for (int i = 0; i < S; ++i) v[k * S + i] = t[i];
+    }
   }
-  __device__ __forceinline__ void turn(A (&v)[2 * S], const A (&sn)[S], const A (&cs)[S], bool partial) const {
-    A was[2 * S];
+  __device__ __forceinline__ void turn(A (&v)[kWidth], const A (&sn)[kPairs], const A (&cs)[kPairs], bool partial) const {
+    A was[kWidth];
 #pragma unroll
-    for (int c = 0; c < 2 * S; ++c) was[c] = v[c];
+    for (int c = 0; c < kWidth; ++c) was[c] = v[c];
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
+    for (int i = 0; i < kPairs; ++i) {
       const int a = NEAR ? 2 * i : i, b = NEAR ? 2 * i + 1 : S + i;
       v[a] = was[a] * cs[i] - was[b] * sn[i];
       v[b] = was[a] * sn[i] + was[b] * cs[i];
@@ -150,7 +163,7 @@ template <typename T, int S, bool NEAR> struct PairLane {
     // channels behind the pairs are taken back, not multiplied by one and zero: an infinity there stays one
     if (partial)
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
+      for (int i = 0; i < kPairs; ++i) {
         const int a = NEAR ? 2 * i : i, b = NEAR ? 2 * i + 1 : S + i;
         const bool keep = pair(i) >= P;
         v[a] = keep ? was[a] : v[a];
@@ -204,26 +217,27 @@ __device__ __forceinline__ int64_t head_at(const int64_t (&s)[3], int b, int l) 
 template <typename T, typename P, int S, bool NEAR, bool NORM, bool STREAM>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
   using A = acc_of_t<T>;
+  using Lane = PairLane<T, S, NEAR>;
   constexpr int kHeads = kRotaryHeads;
   extern __shared__ char lds_dyn[];
   SinCos<A> *const table = (SinCos<A> *)lds_dyn;
   const int lane = threadIdx.x & (q.lanes - 1), sub = threadIdx.x >> q.lanes_log2, subs = kBlock >> q.lanes_log2;
   const int start = (int)blockIdx.x * subs;
   const HeadWalk walk = head_walk(q, start + sub);
-  const PairLane<T, S, NEAR> pl(q, lane);
+  const Lane pl(q, lane);
   const Side side = side_of(q, walk.which);
   const bool stores = walk.live && lane < q.nvec, partial = 2 * q.P < q.D;
   const T *in = (const T *)side.in + head_at(side.in_stride, walk.b, walk.l);
   T *out = (T *)side.out + head_at(side.out_stride, walk.b, walk.l);
   const int64_t in_head = side.in_stride[2], out_head = side.out_stride[2];
   // all heads are asked for first and are on their way while the angles are computed
-  typename LaneVec<T, S>::raw_t r[kHeads][2];
+  typename Lane::raw_t r[kHeads][Lane::kVecs];
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = walk.first + i * walk.step;
     pl.template load<STREAM>(in + (h < walk.count ? h : walk.first) * in_head, r[i]);
   }
-  A sn[S], cs[S], w[2 * S];
+  A sn[Lane::kPairs], cs[Lane::kPairs], w[Lane::kWidth];
   if constexpr (NORM) pl.weights((const P *)side.weight, w);
   const int first = div_by(start, q.by_groups);
   fill_angles(q, first, q.span, table);
@@ -233,32 +247,34 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
   for (int i = 0; i < kHeads; ++i) {
     const int h = walk.first + i * walk.step;
     if (h >= walk.count) continue;
-    A v[2 * S];
+    A v[Lane::kWidth];
     pl.unpack(r[i], v);
     if constexpr (NORM) {
       A ss = 0;
 #pragma unroll
-      for (int c = 0; c < 2 * S; ++c) ss += v[c] * v[c];
+      for (int c = 0; c < Lane::kWidth; ++c) ss += v[c] * v[c];
       ss = segment_sum(lane < q.nvec ? ss : (A)0, q.lanes);
       const A rstd = row_rsqrt(ss * (A)q.inv_d + (A)q.eps);
 #pragma unroll
-      for (int c = 0; c < 2 * S; ++c) v[c] = v[c] * rstd * w[c];
+      for (int c = 0; c < Lane::kWidth; ++c) v[c] = v[c] * rstd * w[c];
     }
     pl.turn(v, sn, cs, partial);
     if (stores) pl.store(out + h * out_head, v);
   }
 }
 
-// Backward behind a norm: two heads of q or k and of their gradients at once (four take the registers of a third workgroup a
-// CU: 59 us instead of 50 for bf16 (16384, 20 + 20, 64)).  A group keeps its place among the heads (and so q or k) while it
-// walks over tokens, and its share of dw in registers; a workgroup leaves one partial row of 2 D values (q's, k's).
+// Backward behind a norm: four lane vectors of q or k and four of their gradients at once (bf16 (16384, 20 + 20, 64): eight take
+// the registers of a third workgroup a CU, 59 us instead of 50 with far pairs; two take 51 instead of 47 with near ones).  A group
+// keeps its place among the heads (and so q or k) while it walks over tokens, and its share of dw in registers; a workgroup
+// leaves one partial row of 2 D values (q's, k's).
 template <typename T, typename P, int S, bool NEAR>
 __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArgs q) {
   using A = acc_of_t<T>;
-  constexpr int kHeads = kRotaryBwdHeads;
+  using Lane = PairLane<T, S, NEAR>;
+  constexpr int kHeads = kRotaryBwdVecs / Lane::kVecs, kWidth = Lane::kWidth;
   extern __shared__ char lds_dyn[];
   const int lane = threadIdx.x & (q.lanes - 1), sub = threadIdx.x >> q.lanes_log2, subs = kBlock >> q.lanes_log2;
-  const PairLane<T, S, NEAR> pl(q, lane);
+  const Lane pl(q, lane);
   const bool partial = 2 * q.P < q.D;
   const int start = (int)blockIdx.x * subs;
   const bool works = start + sub < q.walkers;  // (groups that do not fill a whole set of heads stay idle)
@@ -266,10 +282,10 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
   const Side side = side_of(q, walk.which);
   SinCos<A> *const tables = (SinCos<A> *)lds_dyn;
   const int first = div_by(start, q.by_groups), half = q.D >> 1;
-  A w[2 * S], dw[2 * S];
+  A w[kWidth], dw[kWidth];
   pl.weights((const P *)side.weight, w);
 #pragma unroll
-  for (int c = 0; c < 2 * S; ++c) dw[c] = 0;
+  for (int c = 0; c < kWidth; ++c) dw[c] = 0;
   int turn = 0;
   // (the bound is the workgroup's: all wavefronts meet at the same barriers; two tables in turn, so that one is enough)
   for (int at = 0; first + at < q.tokens; at += q.token_step, turn ^= 1) {
@@ -277,7 +293,7 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
     const int token = there ? walk.token + at : q.tokens - 1, b = div_by(token, q.by_L), l = token - b * q.L;
     const T *in = (const T *)side.in + head_at(side.in_stride, b, l), *grad = (const T *)side.grad + head_at(side.grad_stride, b, l);
     T *out = (T *)side.out + head_at(side.out_stride, b, l);
-    typename LaneVec<T, S>::raw_t rt[kHeads][2], rd[kHeads][2];
+    typename Lane::raw_t rt[kHeads][Lane::kVecs], rd[kHeads][Lane::kVecs];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       const int h = walk.first + i * walk.step < walk.count ? walk.first + i * walk.step : walk.first;
@@ -287,18 +303,18 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
     SinCos<A> *const table = tables + turn * q.span * half;
     fill_angles(q, first + at, q.span, table);
     __syncthreads();
-    A sn[S], cs[S];
+    A sn[Lane::kPairs], cs[Lane::kPairs];
     pl.angles(table + (walk.token - first) * half, sn, cs);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       const int h = walk.first + i * walk.step;
       if (!there || h >= walk.count) continue;
-      A t[2 * S], d[2 * S], ss = 0, gt = 0;
+      A t[kWidth], d[kWidth], ss = 0, gt = 0;
       pl.unpack(rt[i], t);
       pl.unpack(rd[i], d);
       pl.turn(d, sn, cs, partial);
 #pragma unroll
-      for (int c = 0; c < 2 * S; ++c) {
+      for (int c = 0; c < kWidth; ++c) {
         ss += t[c] * t[c];
         gt += d[c] * w[c] * t[c];
       }
@@ -307,7 +323,7 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
       // with h = t r and mean(g h) = r gt / D:  r (g - h mean) = r g - t (r^3 gt / D)
       const A r = row_rsqrt(ss * (A)q.inv_d + (A)q.eps), m = -r * r * r * gt * (A)q.inv_d;
 #pragma unroll
-      for (int c = 0; c < 2 * S; ++c) {
+      for (int c = 0; c < kWidth; ++c) {
         const A dr = d[c] * r;
         dw[c] += dr * t[c];
         d[c] = dr * w[c] + t[c] * m;
@@ -321,10 +337,7 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
   int *kind = (int *)(box + subs * q.D);
   if (lane < q.nvec)
 #pragma unroll
-    for (int c = 0; c < S; ++c) {
-      box[sub * q.D + pl.at0 + c] = dw[c];
-      box[sub * q.D + pl.at1 + c] = dw[S + c];
-    }
+    for (int c = 0; c < kWidth; ++c) box[sub * q.D + pl.at(c / S) + c % S] = dw[c];
   if (lane == 0) kind[sub] = works ? walk.which : 2;
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * q.D; i += kBlock) {

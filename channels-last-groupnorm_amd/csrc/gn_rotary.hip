@@ -55,18 +55,18 @@ template <typename P, int S, bool NEAR> void launch_bwd(const RotaryArgs &a, int
   const size_t lds = tables > sums ? tables : sums;
   hipLaunchKernelGGL((rotary_norm_bwd_kernel<elem_t, P, S, NEAR>), dim3((unsigned)blocks), dim3(kBlock), lds, stream, a);
 }
-// Calls f<pairs a lane, near>() for the pairs that the plan chose.
-template <typename F> void with_pairs(int pairs, bool near, F &&f) {
+// Calls f<channels of a lane vector, near>() for the width that the plan chose.
+template <typename F> void with_vec(int vec, bool near, F &&f) {
   auto go = [&](auto s) {
     if (near) f(s, std::true_type());
     else f(s, std::false_type());
   };
-  if (pairs == 1) return go(std::integral_constant<int, 1>());
+  if (vec == 1) return go(std::integral_constant<int, 1>());
 #if GN_INST_DTYPE == 1
   return go(std::integral_constant<int, 2>());
 #else
 #if GN_INST_DTYPE >= 2
-  if (pairs == 8) return go(std::integral_constant<int, 8>());
+  if (vec == 8) return go(std::integral_constant<int, 8>());
 #endif
   return go(std::integral_constant<int, 4>());
 #endif
@@ -74,8 +74,8 @@ template <typename F> void with_pairs(int pairs, bool near, F &&f) {
 
 }  // namespace
 
-hipError_t GN_CAT(launch_rotary_, GN_SUFFIX)(const RotaryArgs &a, int pairs, bool near, bool norm, int pdtype, hipStream_t stream) {
-  with_pairs(pairs, near, [&](auto s, auto n) {
+hipError_t GN_CAT(launch_rotary_, GN_SUFFIX)(const RotaryArgs &a, int vec, bool near, bool norm, int pdtype, hipStream_t stream) {
+  with_vec(vec, near, [&](auto s, auto n) {
     if (!norm) launch_one<elem_t, decltype(s)::value, decltype(n)::value, false>(a, stream);
     else if (pdtype == GN_INST_DTYPE) launch_one<elem_t, decltype(s)::value, decltype(n)::value, true>(a, stream);
     else launch_one<wide_param_t, decltype(s)::value, decltype(n)::value, true>(a, stream);
@@ -83,9 +83,9 @@ hipError_t GN_CAT(launch_rotary_, GN_SUFFIX)(const RotaryArgs &a, int pairs, boo
   return hipGetLastError();
 }
 
-hipError_t GN_CAT(launch_rotary_norm_bwd_, GN_SUFFIX)(const RotaryArgs &a, int pairs, bool near, int pdtype, int blocks, void *const (&dw)[2],
+hipError_t GN_CAT(launch_rotary_norm_bwd_, GN_SUFFIX)(const RotaryArgs &a, int vec, bool near, int pdtype, int blocks, void *const (&dw)[2],
                                                        hipStream_t stream) {
-  if (blocks > 0) with_pairs(pairs, near, [&](auto s, auto n) {  // (no tokens: the weights' gradients are zero)
+  if (blocks > 0) with_vec(vec, near, [&](auto s, auto n) {  // (no tokens: the weights' gradients are zero)
     if (pdtype == GN_INST_DTYPE) launch_bwd<elem_t, decltype(s)::value, decltype(n)::value>(a, blocks, stream);
     else launch_bwd<wide_param_t, decltype(s)::value, decltype(n)::value>(a, blocks, stream);
   });

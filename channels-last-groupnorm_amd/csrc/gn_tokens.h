@@ -35,7 +35,8 @@ struct RmsBwd {
   int C, nvec, lpr, lpr_log2;
 };
 
-constexpr int kRotaryHeads = 4, kRotaryBwdHeads = 2;  // most heads of a token that a group of lanes turns
+// Most heads of a token that a group of lanes turns; backward, most lane vectors of x (and as many of its gradient) that a lane holds.
+constexpr int kRotaryHeads = 4, kRotaryBwdVecs = 4;
 struct RotarySide {  // q or k
   const void *in, *grad, *weight;
   void *out;
@@ -48,7 +49,7 @@ struct RotaryArgs {
   int64_t pos_stride[2];
   const float *freq;
   int pos_type, axes, ends[4], P, D;
-  int nvec, lanes, lanes_log2;  // lane vectors of half a head, lanes of a group
+  int nvec, lanes, lanes_log2;  // lanes that a head takes, lanes of a group
   int tokens, L, groups;        // batch * tokens, tokens of a sample, groups of a token (q's, then k's)
   int span;                     // most tokens that a workgroup's groups belong to
   Divisor by_groups, by_L, by_half;
@@ -76,8 +77,8 @@ constexpr int64_t kCachedBytes = (int64_t)224 << 20;
 #define GN_DECLARE_TOKENS(S)                                                                            \
   hipError_t launch_rms_fwd_##S(const RmsFwd &a, const RowCut &cut, int pdtype, bool quant, hipStream_t stream);   \
   hipError_t launch_rms_bwd_##S(const RmsBwd &a, const RowCut &cut, int pdtype, int blocks, void *dw, hipStream_t stream); \
-  hipError_t launch_rotary_##S(const RotaryArgs &a, int pairs, bool near, bool norm, int pdtype, hipStream_t stream);       \
-  hipError_t launch_rotary_norm_bwd_##S(const RotaryArgs &a, int pairs, bool near, int pdtype, int blocks, void *const (&dw)[2], hipStream_t stream);
+  hipError_t launch_rotary_##S(const RotaryArgs &a, int vec, bool near, bool norm, int pdtype, hipStream_t stream);         \
+  hipError_t launch_rotary_norm_bwd_##S(const RotaryArgs &a, int vec, bool near, int pdtype, int blocks, void *const (&dw)[2], hipStream_t stream);
 // Gradients of one launch; the whole table travels as a kernel argument.
 struct ClipEntry {
   const void *in;

@@ -122,7 +122,7 @@ namespace {
 // ---- rotary ----
 struct RotaryPlan {
   RotaryArgs a;
-  int pairs;   // of a lane
+  int vec;     // channels of a lane vector
   int blocks;  // of the backward behind a norm
   bool empty;
 };
@@ -155,14 +155,17 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   a.D = (int)c->head_dim;
   a.P = (int)last;
   const int half = a.D / 2, most = c->dtype == GN_F64 ? 2 : c->dtype == GN_F32 ? 4 : 8;
-  // the widest lane vector that the pairs are a multiple of; half of 16 bytes for half-precision heads such as 40
-  p.pairs = 1;
+  // The widest lane vector that divides half of a head and far pairs, or (near pairs of 16 bits, kNearWhole) a head; half of 16
+  // bytes for half-precision heads such as 40 with far pairs.
+  const bool whole = c->interleaved && (c->dtype == GN_F16 || c->dtype == GN_BF16);
+  p.vec = 1;
   for (int s = most; s > 1; s >>= 1)
-    if (!(s == 2 && most != 2) && half % s == 0 && (c->interleaved || a.P % s == 0)) {
-      p.pairs = s;
+    if (!(s == 2 && most != 2) && (whole ? a.D % s == 0 : half % s == 0 && (c->interleaved || a.P % s == 0))) {
+      p.vec = s;
       break;
     }
-  a.nvec = half / p.pairs;
+  const int vecs = whole && p.vec > 1 ? 1 : 2;
+  a.nvec = a.D / (vecs * p.vec);
   if (a.nvec > 64) return invalid("heads of more than 128 channels must have a multiple of 8 channels, and so must their pairs");
   a.lanes_log2 = log2_of(a.nvec);
   a.lanes = 1 << a.lanes_log2;
@@ -177,7 +180,7 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   const int64_t heads[2] = {c->heads, c->kv_heads};
   // Heads that a group turns: as many as it has registers for, each of them on its way at once, as long as the groups fill the
   // device four times.
-  int take = backward && norm ? kRotaryBwdHeads : kRotaryHeads;
+  int take = backward && norm ? kRotaryBwdVecs / vecs : kRotaryHeads;
   while (take > 1 && tokens * (ceil_div(heads[0], take) + ceil_div(heads[1], take)) * a.lanes < (int64_t)4 * kNumCU * kBlock) take >>= 1;
   const void *in[2] = {c->q, c->k}, *grad[2] = {c->q_grad, c->k_grad}, *weight[2] = {c->q_weight, c->k_weight};
   void *out[2] = {c->q_out, c->k_out};
@@ -217,10 +220,11 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   a.inv_d = 1.0 / a.D;
   a.sign = backward ? -1.0f : 1.0f;
   if (backward && norm) {
-    // a walk of whole sets of groups: three workgroups per CU, or as many as there are tokens, alike in length
-    const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(tokens, 3 * kNumCU * subs / a.groups));
-    const int64_t turns = (tokens + steps / 2) / steps;
-    a.token_step = (int)ceil_div(tokens, std::max<int64_t>(turns, 1));
+    // A walk of whole sets of groups, alike in length: at most three workgroups per CU (a few more than that leave some CUs with
+    // four: 151 us instead of 123 for float16 (65536, 8 + 8, 80)), or four where that spares the second turn.
+    const int64_t steps = std::max<int64_t>(1, 3 * kNumCU * subs / a.groups);
+    const int64_t turns = tokens <= steps + steps / 3 ? 1 : ceil_div(tokens, steps);
+    a.token_step = (int)ceil_div(tokens, turns);
     a.walkers = a.token_step * a.groups;
     p.blocks = (int)ceil_div(a.walkers, subs);
   }
@@ -303,7 +307,7 @@ int gnnhwc_rotary(const gnnhwc_rotary_call *c, void *stream) {
   if (const int rc = plan_rotary(c, false, p)) return rc;
   if (p.empty) return GNNHWC_OK;
   const bool norm = c->q_weight != nullptr;
-#define GN_CALL(S) launch_rotary_##S(p.a, p.pairs, c->interleaved != 0, norm, (int)c->param_dtype, (hipStream_t)stream)
+#define GN_CALL(S) launch_rotary_##S(p.a, p.vec, c->interleaved != 0, norm, (int)c->param_dtype, (hipStream_t)stream)
   return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary");
 #undef GN_CALL
 }
@@ -320,7 +324,7 @@ int gnnhwc_rotary_bwd(const gnnhwc_rotary_call *c, void *workspace, size_t works
   const bool norm = c->q_weight != nullptr;
   if (p.empty && !norm) return GNNHWC_OK;
   if (!norm) {
-#define GN_CALL(S) launch_rotary_##S(p.a, p.pairs, c->interleaved != 0, false, (int)c->dtype, (hipStream_t)stream)
+#define GN_CALL(S) launch_rotary_##S(p.a, p.vec, c->interleaved != 0, false, (int)c->dtype, (hipStream_t)stream)
     return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary_bwd");
 #undef GN_CALL
   }
@@ -328,7 +332,7 @@ int gnnhwc_rotary_bwd(const gnnhwc_rotary_call *c, void *workspace, size_t works
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_rotary_bwd_workspace_bytes");
   p.a.part = workspace;
   void *const dw[2] = {c->q_dweight, c->kv_heads ? c->k_dweight : nullptr};
-#define GN_CALL(S) launch_rotary_norm_bwd_##S(p.a, p.pairs, c->interleaved != 0, (int)c->param_dtype, p.blocks, dw, (hipStream_t)stream)
+#define GN_CALL(S) launch_rotary_norm_bwd_##S(p.a, p.vec, c->interleaved != 0, (int)c->param_dtype, p.blocks, dw, (hipStream_t)stream)
   return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary_bwd");
 #undef GN_CALL
 }

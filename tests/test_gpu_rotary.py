@@ -121,6 +121,22 @@ def test_many_tokens(B, L, H, Kh, D, sections, norm, device):
     _check(B, L, H, Kh, D, sections, False, norm, F32, F32, device, train=False)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D,sections", [(12, (5,)), (36, (18,)), (52, (7, 9, 9)), (200, (100,)), (200, (33,)), (248, (31, 62))])
+def test_near_pairs_in_heads_that_lane_vectors_divide(D, sections, dtype, device):
+    """Half of the head need not be whole vectors where a lane holds the pairs of one."""
+    for norm in (False, True):
+        _check(2, 45, 5, 3, D, sections, True, norm, dtype, F32, device)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("L", [768, 769, 1024, 1025, 2049])
+def test_walks_of_the_backward(L, dtype, device):
+    """Walks of one turn and more, and last turns that not every group has."""
+    for near in (False, True):
+        _check(1, L, 16, 16, 64, (16, 16), near, True, dtype, dtype, device)
+
+
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64, F32])
 def test_long_positions(kind, device):
     """Angles of hundreds of thousands of radians, to 2^24: only the position and the frequency are in 32 bits."""
