@@ -74,26 +74,32 @@ template <typename A> __device__ __forceinline__ void fill_angles(const RotaryAr
   }
 }
 
-// Whether a lane holds one vector of a head, with its near pairs inside (the host's plan decides alike).  Of 16 bits alone: halves
-// of a head, 64 bytes at 32 channels each, made the stores write 16 to 25 % more than the head (bf16 (16384, 20 + 20, 64) 36.5 us,
-// whole 31; its backward behind a norm 51 and 47; float16 (65536, 8 + 8, 80) 71 and 59), while halves of 32 bits are longer and a
-// workgroup of half as many heads costs more: float32 (308142, 2 + 1, 96) 129 us, whole 150; (770, 24 + 12, 40) 4.9 and 5.3.
-template <typename T, int S, bool NEAR> constexpr bool kNearWhole = NEAR && S > 1 && sizeof(T) == 2;
-
-// What one lane holds of a head: one or two lane vectors of S channels, neighbouring lanes neighbouring vectors, so that one
-// access of a group is one run of memory.  Far pairs (j, j + P) have a vector from either half of the turning channels; near
-// pairs (2j, 2j + 1) lie inside a vector, and where there are two, they come from either half of the head.  (Two vectors behind
-// each other read every line twice: float16 (46800, 24 + 24 heads, 128) 286 us.)
-template <typename T, int S, bool NEAR> struct PairLane {
+// What one lane holds of a head: lane vectors of S channels, neighbouring lanes neighbouring vectors, so that one access of a
+// group is one run of memory.
+// - Two vectors: far pairs (j, j + P) have one from either half of the turning channels, near pairs (2j, 2j + 1) one from either
+//   half of the head.  (Two near vectors behind each other read every line twice: float16 (46800, 24 + 24 heads, 128) 286 us.)
+// - One vector (WHOLE), and the access is the whole head: near pairs lie inside it, far ones trade values with the lane that
+//   holds the other half.  Halves that are not whole lines of memory made the stores write 16 to 25 % more than the heads.
+// The host's plan (gn_tokens.hip) chooses, and says what each takes.
+template <typename T, int S, bool NEAR, bool WHOLE> struct PairLane {
   using A = acc_of_t<T>;
-  static constexpr bool kWhole = kNearWhole<T, S, NEAR>;
-  static constexpr int kVecs = kWhole ? 1 : 2, kPairs = kWhole ? S / 2 : S, kWidth = kVecs * S;
-  static constexpr bool kHalves = NEAR && S > 1 && !kWhole;
-  int j0, j1, at0, at1, P;  // j1: first pair of the second vector, where that has pairs of its own
+  static constexpr int kVecs = WHOLE ? 1 : 2, kPairs = WHOLE && NEAR ? S / 2 : S, kWidth = kVecs * S;
+  static constexpr bool kHalves = NEAR && S > 1 && !WHOLE;
+  static constexpr bool kTrade = WHOLE && !NEAR;  // the other halves of the pairs are another lane's
+  int j0, j1, at0, at1, P, other;
+  bool first, turns; // j1: first pair of the second vector, where that has pairs of its own
   __device__ __forceinline__ PairLane(const RotaryArgs &q, int lane) : P(q.P) {
     const int v = lane < q.nvec ? lane : q.nvec - 1;  // spare lanes repeat the last vector and store nothing
-    j1 = at1 = 0;
-    if constexpr (kWhole) {
+    j1 = at1 = other = 0;
+    first = turns = true;
+    if constexpr (kTrade) {
+      at0 = v * S;
+      first = at0 < P;
+      turns = at0 < 2 * P;  // (S divides P)
+      j0 = first ? at0 : turns ? at0 - P : 0;
+      const int partner = first ? at0 + P : turns ? at0 - P : at0;
+      other = ((int)threadIdx.x - lane + partner / S) * 4;
+    } else if constexpr (WHOLE) {
       j0 = v * (S / 2);
       at0 = v * S;
     } else if constexpr (kHalves) {
@@ -115,7 +121,7 @@ template <typename T, int S, bool NEAR> struct PairLane {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       const SinCos<A> v = row[pair(i)];
-      sn[i] = v.sn;
+      sn[i] = kTrade && first ? -v.sn : v.sn;
       cs[i] = v.cs;
     }
   }
@@ -154,6 +160,15 @@ template <typename T, int S, bool NEAR> struct PairLane {
     A was[kWidth];
 #pragma unroll
     for (int c = 0; c < kWidth; ++c) was[c] = v[c];
+    if constexpr (kTrade) {
+#pragma unroll
+      for (int c = 0; c < kWidth; ++c) {
+        const A o = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(other, __builtin_bit_cast(int, v[c])));
+        v[c] = was[c] * cs[c] + o * sn[c];
+        v[c] = turns ? v[c] : was[c];
+      }
+      return;
+    } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       const int a = NEAR ? 2 * i : i, b = NEAR ? 2 * i + 1 : S + i;
@@ -169,6 +184,7 @@ template <typename T, int S, bool NEAR> struct PairLane {
         v[a] = keep ? was[a] : v[a];
         v[b] = keep ? was[b] : v[b];
       }
+    }
   }
 };
 
@@ -214,10 +230,10 @@ __device__ __forceinline__ Side side_of(const RotaryArgs &q, int which) {
 }
 __device__ __forceinline__ int64_t head_at(const int64_t (&s)[3], int b, int l) { return b * s[0] + l * s[1]; }
 
-template <typename T, typename P, int S, bool NEAR, bool NORM, bool STREAM>
+template <typename T, typename P, int S, bool NEAR, bool WHOLE, bool NORM, bool STREAM>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
   using A = acc_of_t<T>;
-  using Lane = PairLane<T, S, NEAR>;
+  using Lane = PairLane<T, S, NEAR, WHOLE>;
   constexpr int kHeads = kRotaryHeads;
   extern __shared__ char lds_dyn[];
   SinCos<A> *const table = (SinCos<A> *)lds_dyn;
@@ -267,10 +283,10 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
 // the registers of a third workgroup a CU, 59 us instead of 50 with far pairs; two take 51 instead of 47 with near ones).  A group
 // keeps its place among the heads (and so q or k) while it walks over tokens, and its share of dw in registers; a workgroup
 // leaves one partial row of 2 D values (q's, k's).
-template <typename T, typename P, int S, bool NEAR>
+template <typename T, typename P, int S, bool NEAR, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArgs q) {
   using A = acc_of_t<T>;
-  using Lane = PairLane<T, S, NEAR>;
+  using Lane = PairLane<T, S, NEAR, WHOLE>;
   constexpr int kHeads = kRotaryBwdVecs / Lane::kVecs, kWidth = Lane::kWidth;
   extern __shared__ char lds_dyn[];
   const int lane = threadIdx.x & (q.lanes - 1), sub = threadIdx.x >> q.lanes_log2, subs = kBlock >> q.lanes_log2;

@@ -35,6 +35,12 @@ struct RmsBwd {
   int C, nvec, lpr, lpr_log2;
 };
 
+// How lanes share a head: channels of a lane vector; pairs near each other or far; one vector of a lane (a head's access is
+// whole) or two.
+struct RotaryCut {
+  int vec;
+  bool near, whole;
+};
 // Most heads of a token that a group of lanes turns; backward, most lane vectors of x (and as many of its gradient) that a lane holds.
 constexpr int kRotaryHeads = 4, kRotaryBwdVecs = 4;
 struct RotarySide {  // q or k
@@ -77,8 +83,8 @@ constexpr int64_t kCachedBytes = (int64_t)224 << 20;
 #define GN_DECLARE_TOKENS(S)                                                                            \
   hipError_t launch_rms_fwd_##S(const RmsFwd &a, const RowCut &cut, int pdtype, bool quant, hipStream_t stream);   \
   hipError_t launch_rms_bwd_##S(const RmsBwd &a, const RowCut &cut, int pdtype, int blocks, void *dw, hipStream_t stream); \
-  hipError_t launch_rotary_##S(const RotaryArgs &a, int vec, bool near, bool norm, int pdtype, hipStream_t stream);         \
-  hipError_t launch_rotary_norm_bwd_##S(const RotaryArgs &a, int vec, bool near, int pdtype, int blocks, void *const (&dw)[2], hipStream_t stream);
+  hipError_t launch_rotary_##S(const RotaryArgs &a, const RotaryCut &cut, bool norm, int pdtype, hipStream_t stream);         \
+  hipError_t launch_rotary_norm_bwd_##S(const RotaryArgs &a, const RotaryCut &cut, int pdtype, int blocks, void *const (&dw)[2], hipStream_t stream);
 // Gradients of one launch; the whole table travels as a kernel argument.
 struct ClipEntry {
   const void *in;

@@ -122,7 +122,7 @@ namespace {
 // ---- rotary ----
 struct RotaryPlan {
   RotaryArgs a;
-  int vec;     // channels of a lane vector
+  RotaryCut cut;
   int blocks;  // of the backward behind a norm
   bool empty;
 };
@@ -155,17 +155,27 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   a.D = (int)c->head_dim;
   a.P = (int)last;
   const int half = a.D / 2, most = c->dtype == GN_F64 ? 2 : c->dtype == GN_F32 ? 4 : 8;
-  // The widest lane vector that divides half of a head and far pairs, or (near pairs of 16 bits, kNearWhole) a head; half of 16
-  // bytes for half-precision heads such as 40 with far pairs.
-  const bool whole = c->interleaved && (c->dtype == GN_F16 || c->dtype == GN_BF16);
-  p.vec = 1;
+  // The widest lane vector that divides what it has to; half of 16 bytes for half-precision heads such as 40 with far pairs.
+  // Whole heads (PairLane, gn_rotary.h) for 16 bits:
+  // - near pairs, always: (16384, 20 + 20, 64) 31 us, in halves 36.5; (65536, 8 + 8, 80) 59 and 71; behind a norm backward 47 and
+  //   51, 123 and 153.  Of 32 bits halves are longer and a workgroup of half as many heads costs more: (308142, 2 + 1, 96) whole
+  //   150, in halves 129; (770, 24 + 12, 40) 5.3 and 4.9.
+  // - far pairs, forward, where they fill three quarters of the lanes: (16384, 20 + 20, 64) 31.7 us, in halves 35.7; (46800,
+  //   24 + 24, 96) 149 and 183; of 160 channels, 20 of 32 lanes, (13000, 5 + 1) 18.6 and 15.4.  Behind a norm backward: 50 and 50,
+  //   (13770, 12 + 2, 80) 29 and 24.
+  const bool bits16 = c->dtype == GN_F16 || c->dtype == GN_BF16, near = c->interleaved != 0;
+  const int vecs16 = a.D / 8;
+  const bool far_whole = bits16 && !near && !(backward && norm) && a.D % 8 == 0 && a.P % 8 == 0 && 4 * vecs16 >= 3 << log2_of(vecs16);
+  const bool wide = far_whole || (bits16 && near);
+  int vec = 1;
   for (int s = most; s > 1; s >>= 1)
-    if (!(s == 2 && most != 2) && (whole ? a.D % s == 0 : half % s == 0 && (c->interleaved || a.P % s == 0))) {
-      p.vec = s;
+    if (!(s == 2 && most != 2) && (wide ? a.D : half) % s == 0 && (near || a.P % s == 0)) {
+      vec = s;
       break;
     }
-  const int vecs = whole && p.vec > 1 ? 1 : 2;
-  a.nvec = a.D / (vecs * p.vec);
+  p.cut = {vec, near, wide && vec > 1};
+  const int vecs = p.cut.whole ? 1 : 2;
+  a.nvec = a.D / (vecs * vec);
   if (a.nvec > 64) return invalid("heads of more than 128 channels must have a multiple of 8 channels, and so must their pairs");
   a.lanes_log2 = log2_of(a.nvec);
   a.lanes = 1 << a.lanes_log2;
@@ -307,7 +317,7 @@ int gnnhwc_rotary(const gnnhwc_rotary_call *c, void *stream) {
   if (const int rc = plan_rotary(c, false, p)) return rc;
   if (p.empty) return GNNHWC_OK;
   const bool norm = c->q_weight != nullptr;
-#define GN_CALL(S) launch_rotary_##S(p.a, p.vec, c->interleaved != 0, norm, (int)c->param_dtype, (hipStream_t)stream)
+#define GN_CALL(S) launch_rotary_##S(p.a, p.cut, norm, (int)c->param_dtype, (hipStream_t)stream)
   return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary");
 #undef GN_CALL
 }
@@ -324,7 +334,7 @@ int gnnhwc_rotary_bwd(const gnnhwc_rotary_call *c, void *workspace, size_t works
   const bool norm = c->q_weight != nullptr;
   if (p.empty && !norm) return GNNHWC_OK;
   if (!norm) {
-#define GN_CALL(S) launch_rotary_##S(p.a, p.vec, c->interleaved != 0, false, (int)c->dtype, (hipStream_t)stream)
+#define GN_CALL(S) launch_rotary_##S(p.a, p.cut, false, (int)c->dtype, (hipStream_t)stream)
     return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary_bwd");
 #undef GN_CALL
   }
@@ -332,7 +342,7 @@ int gnnhwc_rotary_bwd(const gnnhwc_rotary_call *c, void *workspace, size_t works
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_rotary_bwd_workspace_bytes");
   p.a.part = workspace;
   void *const dw[2] = {c->q_dweight, c->kv_heads ? c->k_dweight : nullptr};
-#define GN_CALL(S) launch_rotary_norm_bwd_##S(p.a, p.vec, c->interleaved != 0, (int)c->param_dtype, p.blocks, dw, (hipStream_t)stream)
+#define GN_CALL(S) launch_rotary_norm_bwd_##S(p.a, p.cut, (int)c->param_dtype, p.blocks, dw, (hipStream_t)stream)
   return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_rotary_bwd");
 #undef GN_CALL
 }
