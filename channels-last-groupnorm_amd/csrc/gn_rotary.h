@@ -207,6 +207,11 @@ __device__ __forceinline__ HeadWalk head_walk(const RotaryArgs &q, int group) {
   w.l = w.token - w.b * q.L;
   return w;
 }
+// Tokens that a workgroup's groups belong to: at most span, and often one less.
+__device__ __forceinline__ int tokens_of(const RotaryArgs &q, int start, int subs) {
+  const int n = div_by(start + subs - 1, q.by_groups) - div_by(start, q.by_groups) + 1;
+  return n < q.span ? n : q.span;
+}
 // q's or k's tensors, field by field: both are scalar loads of the argument block and a selection.
 struct Side {
   const void *in, *grad, *weight;
@@ -256,7 +261,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
   A sn[Lane::kPairs], cs[Lane::kPairs], w[Lane::kWidth];
   if constexpr (NORM) pl.weights((const P *)side.weight, w);
   const int first = div_by(start, q.by_groups);
-  fill_angles(q, first, q.span, table);
+  fill_angles(q, first, tokens_of(q, start, subs), table);
   __syncthreads();
   pl.angles(table + (walk.token - first) * (q.D >> 1), sn, cs);
 #pragma unroll
@@ -297,7 +302,7 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
   const HeadWalk walk = head_walk(q, works ? start + sub : start);
   const Side side = side_of(q, walk.which);
   SinCos<A> *const tables = (SinCos<A> *)lds_dyn;
-  const int first = div_by(start, q.by_groups), half = q.D >> 1;
+  const int first = div_by(start, q.by_groups), tokens = tokens_of(q, start, subs), half = q.D >> 1;
   A w[kWidth], dw[kWidth];
   pl.weights((const P *)side.weight, w);
 #pragma unroll
@@ -317,7 +322,7 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
       pl.load(grad + h * side.grad_stride[2], rd[i]);
     }
     SinCos<A> *const table = tables + turn * q.span * half;
-    fill_angles(q, first + at, q.span, table);
+    fill_angles(q, first + at, tokens, table);
     __syncthreads();
     A sn[Lane::kPairs], cs[Lane::kPairs];
     pl.angles(table + (walk.token - first) * half, sn, cs);
