@@ -96,7 +96,11 @@ int check_fwd(const void *x, const void *residual, void *sum_out, const void *y,
 
 // How a row's lane vectors are dealt to lanes: the fewest lanes (a power of two) that leave none more than three (forward of
 // float16 (65536, 2560): 223 us with three, 228 with five; bf16 in 8 bits, 128 channels a block, (16384, 2560): 54 and 61).
-RowCut rms_cut(int64_t C, int esize, int least_lanes) {
+// `whole`: rows that are not whole lines of memory in one access each, up to a wavefront, where several would write parts of
+// lines (forward, bf16 (140000, 200) with a residual 53 -> 37 us, (966103, 80) 103 -> 61; rows of whole lines lose by it,
+// (90000, 320) 20 -> 24, as do the backward, (140000, 200) 34 -> 44, whose few workgroups want more of each row on its way, and
+// 8 bits, (280000, 200) 34 -> 45).
+RowCut rms_cut(int64_t C, int esize, int least_lanes, bool whole) {
   const int vec = 16 / esize;
   RowCut c;
   c.vec = C < vec ? 1 : vec;
@@ -104,6 +108,8 @@ RowCut rms_cut(int64_t C, int esize, int least_lanes) {
   c.ragged = C % c.vec != 0;
   c.lpr = std::max(8, least_lanes);
   // (two where a workgroup is wider than 256: a third does not fit the registers of 1024 threads in the backward)
+  if (whole && C * esize % 128 != 0)
+    while (c.lpr < 64 && c.nvec > c.lpr) c.lpr <<= 1;
   while (c.lpr < 1024 && c.nvec > (c.lpr > 256 ? 2 : kRowVectors) * c.lpr) c.lpr <<= 1;
   c.nv = (int)ceil_div(c.nvec, c.lpr);
   c.lpr_log2 = log2_of(c.lpr);
@@ -254,7 +260,7 @@ int gnnhwc_rms_fwd(const void *x, const void *residual, const void *weight, void
   if (const int rc = check_eps(eps)) return rc;
   if (const int rc = check_fwd(x, residual, sum_out, y, rows)) return rc;
   if (rows == 0) return GNNHWC_OK;
-  const RowCut cut = rms_cut(C, elem_size(dtype), 8);
+  const RowCut cut = rms_cut(C, elem_size(dtype), 8, true);
   RmsFwd a = fwd_args(x, residual, weight, sum_out, y, rows, C, x_stride, residual_stride, eps, cut);
   return launch_fwd(a, cut, dtype, weight ? param_dtype : dtype, false, (hipStream_t)stream, "gnnhwc_rms_fwd");
 }
@@ -273,7 +279,7 @@ int gnnhwc_rms_fwd_quant(const void *x, const void *residual, const void *weight
     return fail(GNNHWC_ERR_INVALID_ARGUMENT, "a block of %lld channels: a power of two from 16 to 256, or 0 for whole rows", (long long)block);
   if (rows == 0) return GNNHWC_OK;
   const int lanes = by_row ? 0 : (int)block / (16 / elem_size(dtype));
-  const RowCut cut = rms_cut(C, elem_size(dtype), std::max(8, lanes));
+  const RowCut cut = rms_cut(C, elem_size(dtype), std::max(8, lanes), false);
   RmsFwd a = fwd_args(x, residual, weight, sum_out, q, rows, C, x_stride, residual_stride, eps, cut);
   a.scales = scales;
   a.block_lanes = lanes;
@@ -285,7 +291,7 @@ int gnnhwc_rms_fwd_quant(const void *x, const void *residual, const void *weight
 
 size_t gnnhwc_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype) {
   if (check_rows(rows, C, dtype, dtype)) return 0;
-  const RowCut cut = rms_cut(C, elem_size(dtype), 8);
+  const RowCut cut = rms_cut(C, elem_size(dtype), 8, false);
   return 256 + (size_t)rms_bwd_blocks(rows, cut) * (size_t)C * (dtype == GN_F64 ? 8 : 4);
 }
 
@@ -298,7 +304,7 @@ int gnnhwc_rms_bwd(const void *dy, const void *ds, const void *s, const void *we
   if (!dx && !dweight) return GNNHWC_OK;
   if (dweight && (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < gnnhwc_rms_bwd_workspace_bytes(rows, C, dtype)))
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_rms_bwd_workspace_bytes");
-  const RowCut cut = rms_cut(C, elem_size(dtype), 8);
+  const RowCut cut = rms_cut(C, elem_size(dtype), 8, false);
   RmsBwd a = {};
   a.dy = dy; a.ds = ds; a.s = s; a.w = weight;
   a.dx = dx; a.part = dweight ? workspace : nullptr;
