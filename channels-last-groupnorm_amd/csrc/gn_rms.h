@@ -300,7 +300,9 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
 // Backward: float16 (65536, 2560) with a gradient of the sum 234 us (5.7 TB/s), bf16 (16384, 1280) 34.5 (4.9).  A workgroup
 // walks over rows and keeps its share of dw in registers, in a fixed order, and leaves one partial row of dw; partial_sum_kernel
 // adds those.  r is computed again from s, whose sum of squares rides along with that of g s, so that the forward saves no
-// statistics: with G = sum g s, mean(g h) = r G / C.
+// statistics: with G = sum g s, mean(g h) = r G / C.  The second term is h (r mean(g h)), not s (r^3 G / C): r^3 leaves a float's
+// range where r and the result are well inside.  (That is one product more an element and nothing in time; g - h mean(g h) times
+// r would keep all g of the sums, and with them one workgroup per CU less.)
 template <typename T, typename P, int VEC, int NV, int THREADS, bool RAGGED, bool DS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
   using A = acc_of_t<T>;
@@ -353,9 +355,8 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
       gs += cut.has(k) ? p1 : (A)0;
     }
     row_sum2(ss, gs, q.lpr, lds, turn);
-    // r (g - h mean(g h)) = r g - s (r^3 G / C)
     const A r = row_rsqrt(ss * (A)q.inv_c + (A)q.eps);
-    const A c = -r * r * r * gs * (A)q.inv_c;
+    const A c = -(r * gs * (A)q.inv_c) * r;
     if (!live) continue;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -364,9 +365,9 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
       LV::unpack(dy[k], dv);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const A dr = dv[i] * r;
+        const A dr = dv[i] * r, h = sv[i] * r;
         dw[k][i] += dr * sv[i];
-        dx[i] = dr * w[k][i] + sv[i] * c;
+        dx[i] = dr * w[k][i] + h * c;
       }
       if constexpr (DS) {
         A u[VEC];

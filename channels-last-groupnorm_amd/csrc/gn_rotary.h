@@ -341,13 +341,13 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
       }
       if (lane >= q.nvec) ss = gt = 0;
       segment_sum2(ss, gt, q.lanes);
-      // with h = t r and mean(g h) = r gt / D:  r (g - h mean) = r g - t (r^3 gt / D)
-      const A r = row_rsqrt(ss * (A)q.inv_d + (A)q.eps), m = -r * r * r * gt * (A)q.inv_d;
+      // dt = r g - h (r mean(g h)) with mean(g h) = r gt / D, as in rms_bwd_kernel: r^3 would leave a float's range
+      const A r = row_rsqrt(ss * (A)q.inv_d + (A)q.eps), m = -(r * gt * (A)q.inv_d) * r;
 #pragma unroll
       for (int c = 0; c < kWidth; ++c) {
-        const A dr = d[c] * r;
+        const A dr = d[c] * r, h = t[c] * r;
         dw[c] += dr * t[c];
-        d[c] = dr * w[c] + t[c] * m;
+        d[c] = dr * w[c] + h * m;
       }
       if (lane < q.nvec) pl.store(out + h * side.out_stride[2], d);
     }
