@@ -182,6 +182,65 @@ def _rms_norm_backward(ctx, dy, ds):
 torch.library.register_autograd("gnop::rms_norm", _rms_norm_backward, setup_context=_rms_norm_setup_context, lib=_op_lib)
 
 
+def _wide(t):
+    """t in the type that the kernels compute in."""
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def _norm_second(d, t, weight, eps, a, b):
+    """Gradients with respect to d, t and weight of <a, dt> + <b, dw>, where dt and dw are the norm's own gradients,
+      dt = r (g - h mean(g h)),  dw = sum d h,  g = d w, h = t r;
+    a or b may be None.  The map from g to dt is symmetric, which gives the parts of d and weight; with dr / dt = -r^2 h / C,
+      -r^2 (h (mean(a g) - 3 mean(a h) mean(g h)) + a mean(g h) + g mean(a h))
+    is that of t.  Elementary operations on _wide tensors: differentiable in their turn."""
+    def mean(v):
+        return v.mean(-1, keepdim=True)
+
+    r = (mean(t * t) + eps).rsqrt()
+    h = t * r
+    of_d = of_t = of_w = None
+    if a is not None:
+        g = d if weight is None else d * weight
+        ah, gh = mean(a * h), mean(g * h)
+        back = r * (a - h * ah)
+        of_d = back if weight is None else back * weight
+        of_t = -r * r * (h * (mean(a * g) - 3 * ah * gh) + a * gh + g * ah)
+        of_w = None if weight is None else (back * d).reshape(-1, t.shape[-1]).sum(0)
+    if b is not None:
+        e = b * d
+        of_d = b * h if of_d is None else of_d + b * h
+        back = r * (e - h * mean(e * h))
+        of_t = back if of_t is None else of_t + back
+    return of_d, of_t, of_w
+
+
+def _second(d, t, weight, eps, a, b):
+    """_norm_second of tensors in any type, each result in its tensor's type and shape; None where there is none."""
+    if a is None and b is None:
+        return None, None, None
+    w = None if weight is None else _wide(weight).reshape(-1)
+    grads = _norm_second(_wide(d), _wide(t), w, eps, None if a is None else _wide(a), None if b is None else _wide(b))
+    return tuple(None if g is None else g.view(like.shape).to(like.dtype) for g, like in zip(grads, (d, t, weight)))
+
+
+def _rms_norm_bwd_setup_context(ctx, inputs, output):
+    dy, ds, s, weight, ctx.eps = inputs
+    ctx.has_ds = ds is not None
+    ctx.save_for_backward(dy, s, weight)
+    ctx.set_materialize_grads(False)
+    if weight is None:
+        ctx.mark_non_differentiable(output[1])
+
+
+def _rms_norm_bwd_backward(ctx, a, b):
+    dy, s, weight = ctx.saved_tensors
+    of_dy, of_s, of_weight = _second(dy, s, weight, ctx.eps, a, None if weight is None else b)
+    return of_dy, a if ctx.has_ds else None, of_s, of_weight, None
+
+
+torch.library.register_autograd("gnop::rms_norm_bwd", _rms_norm_bwd_backward, setup_context=_rms_norm_bwd_setup_context, lib=_op_lib)
+
+
 def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -193,8 +252,8 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, return_sum=False, channel_
     taken as it is; float32, float64, float16 or bfloat16, C up to 16384 (float64: 8192).  weight: (C,) in x's dtype, or float32
     beside half-precision data, or None.  residual: a tensor like x; the sum is rounded to x's dtype once, as an addition in
     front would, and is what is normalised.  With return_sum=True the call returns (y, s), so that s is the next residual
-    (without a residual, s is x).  Means and products are in float32 (float64).  Differentiable in x, residual and weight;
-    the gradients of s reach x and residual too."""
+    (without a residual, s is x).  Means and products are in float32 (float64).  Differentiable in x, residual and weight, as
+    often as need be (from the second derivative on in elementary operations); the gradients of s reach x and residual too."""
     if channel_dim != -1 and channel_dim != x.dim() - 1:
         last = [None if t is None else t.movedim(channel_dim, -1) for t in (x, residual)]
         out = rms_norm(last[0], weight, eps, last[1], return_sum)
@@ -437,6 +496,40 @@ def _rotary_backward(ctx, dq, dk):
 torch.library.register_autograd("gnop::rotary", _rotary_backward, setup_context=_rotary_setup_context, lib=_op_lib)
 
 
+def _rotary_bwd_setup_context(ctx, inputs, output):
+    q_grad, k_grad, q, k, positions, frequencies, ctx.sections, ctx.interleaved, q_weight, k_weight, ctx.eps = inputs
+    norm = q_weight is not None
+    ctx.norm, ctx.has_k = norm, k_grad is not None
+    # (without a norm the gradients are linear in the incoming ones, and nothing else is differentiated)
+    ctx.save_for_backward(positions, frequencies, *((q_grad, k_grad, q, k, q_weight, k_weight) if norm else ()))
+    ctx.set_materialize_grads(False)
+    absent = [t for t, there in zip(output, (True, ctx.has_k, norm, norm and ctx.has_k)) if not there]
+    ctx.mark_non_differentiable(*absent)
+
+
+def _rotary_bwd_backward(ctx, *grads):
+    positions, frequencies, *rest = ctx.saved_tensors
+    turn = (positions, frequencies, ctx.sections, ctx.interleaved, None, None, ctx.eps)
+
+    def side(i, there):
+        """Gradients with respect to the incoming gradient, the heads and the weight of q (0) or k (1)."""
+        a, b = grads[i], grads[2 + i]
+        if not there or (a is None and (b is None or not ctx.norm)):
+            return None, None, None
+        if not ctx.norm:
+            return torch.ops.gnop.rotary(a, None, *turn)[0], None, None
+        g, t, w = rest[i], rest[2 + i], rest[4 + i]
+        d = torch.ops.gnop.rotary_bwd(_wide(g), None, None, None, *turn)[0]  # behind the turn, in front of the norm
+        of_d, of_t, of_w = _second(d, t, w, ctx.eps, a, b)
+        return torch.ops.gnop.rotary(of_d, None, *turn)[0].to(g.dtype), of_t, of_w
+
+    (gq, tq, wq), (gk, tk, wk) = side(0, True), side(1, ctx.has_k)
+    return gq, gk, tq, tk, None, None, None, None, wq, wk, None
+
+
+torch.library.register_autograd("gnop::rotary_bwd", _rotary_bwd_backward, setup_context=_rotary_bwd_setup_context, lib=_op_lib)
+
+
 def rotary(q, k, positions, frequencies, sections=None, interleaved=False, q_weight=None, k_weight=None, eps=1e-6):
     """Rotary positions with one to four axes (time, height, width, ...) on q and k.  Returns (q', k'), or q' if k is None.
 
@@ -449,7 +542,8 @@ def rotary(q, k, positions, frequencies, sections=None, interleaved=False, q_wei
 
     With q_weight / k_weight, (D,) in q's dtype or float32 beside half precision, every head is first normalised over its D
     channels, t / sqrt(mean(t^2) + eps) * weight, in the same pass.  Everything in between is float32 (float64).
-    Differentiable in q, k and the weights."""
+    Differentiable in q, k and the weights, as often as need be (behind a norm from the second derivative on in elementary
+    operations)."""
     if not torch.compiler.is_compiling():
         out = _native.rotary(q, k, positions, frequencies, sections, interleaved, q_weight, k_weight, eps)
         if out is not NotImplemented:
