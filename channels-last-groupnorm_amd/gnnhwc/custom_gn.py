@@ -6,8 +6,6 @@ reference; the kernels behind the operators are the HIP ones in libgnnhwc_hip.so
 C ABI (include/gnnhwc.h) with raw device pointers and the current HIP stream.  torch only provides
 device memory (outputs, workspace) and the stream.
 """
-import collections
-import threading
 
 import torch
 import torch.nn as nn
@@ -108,30 +106,11 @@ class _on_device:
         return False
 
 
-_workspaces = collections.OrderedDict()
-_workspaces_lock = threading.Lock()
-_MAX_CACHED_WORKSPACES = 8
-
-
-def _workspace(nbytes, device, stream_ptr):
-    """Scratch memory for one call.  Calls on one stream follow each other, so they can share one buffer per
-    (device, stream), grown on demand; while the stream is recording a graph the buffer comes from the allocator
-    instead (it then belongs to the graph's own memory pool, like every other tensor of the capture).
-    The cache is shared by the caller's thread and the autograd engine's, hence the lock; it keeps the buffers of the
-    most recently used streams only, so that streams that no longer exist do not pin memory for ever (a buffer that is
-    dropped while a kernel still uses it stays valid: the caching allocator only reuses it in stream order)."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty((nbytes,), dtype=torch.uint8, device=device)
-    key = (device.index, stream_ptr)
-    with _workspaces_lock:
-        ws = _workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.empty((max(nbytes, 1 << 20),), dtype=torch.uint8, device=device)
-            _workspaces[key] = ws
-        _workspaces.move_to_end(key)
-        while len(_workspaces) > _MAX_CACHED_WORKSPACES:
-            _workspaces.popitem(last=False)
-    return ws
+def _workspace(nbytes, device):
+    """Scratch memory of one call, from the caching allocator: in stream order, and part of a graph's own pool under capture.
+    It must not be shared between calls: one that takes several launches hands results from one to the next in it, and the
+    library's functions release the interpreter lock, so that another thread may submit to the same stream in between."""
+    return torch.empty((nbytes,), dtype=torch.uint8, device=device)
 
 
 def gn_nhwc_fwd(X, weight, bias, G, eps, act_fn_option):
@@ -169,7 +148,7 @@ def _nhwc_fwd(X, weight, bias, G, eps, act_fn_option, out_dtype, opname):
         if nbytes == 0:
             raise RuntimeError(opname + ": " + _cabi.last_error())
         stream = _current_stream_ptr(X.device)
-        ws = _workspace(nbytes, X.device, stream)
+        ws = _workspace(nbytes, X.device)
         rc = lib.gnnhwc_fwd_cast(
             X_nrc.data_ptr(), w_ptr, b_ptr,
             Y.data_ptr(), means.data_ptr(), rstds.data_ptr(),
@@ -210,7 +189,7 @@ def gn_nhwc_bwd(dy, X, weight, bias, means, rstds, G, act_fn_option):
         if nbytes == 0:
             raise RuntimeError("gnop::bwd: " + _cabi.last_error())
         stream = _current_stream_ptr(X.device)
-        ws = _workspace(nbytes, X.device, stream)
+        ws = _workspace(nbytes, X.device)
         rc = lib.gnnhwc_bwd_cast(
             dy_nrc.data_ptr(), X_nrc.data_ptr(), w_ptr, b_ptr,
             means.contiguous().data_ptr(), rstds.contiguous().data_ptr(),
@@ -241,7 +220,7 @@ def gn_nchw_fwd(X, weight, bias, G, eps, act_fn_option):
         if nbytes == 0:
             raise RuntimeError("gnop::fwd_nchw: " + _cabi.last_error())
         stream = _current_stream_ptr(X.device)
-        ws = _workspace(nbytes, X.device, stream)
+        ws = _workspace(nbytes, X.device)
         rc = lib.gnnhwc_fwd_nchw(
             X.data_ptr(), w_ptr, b_ptr,
             Y.data_ptr(), means.data_ptr(), rstds.data_ptr(),
@@ -281,7 +260,7 @@ def gn_nchw_bwd(dy, X, weight, bias, means, rstds, G, act_fn_option):
         if nbytes == 0:
             raise RuntimeError("gnop::bwd_nchw: " + _cabi.last_error())
         stream = _current_stream_ptr(X.device)
-        ws = _workspace(nbytes, X.device, stream)
+        ws = _workspace(nbytes, X.device)
         rc = lib.gnnhwc_bwd_nchw(
             dy.data_ptr(), X.data_ptr(), w_ptr, b_ptr,
             means.contiguous().data_ptr(), rstds.contiguous().data_ptr(),
@@ -335,7 +314,7 @@ def gn_nhwc_fwd_add(X, residual, channel_bias, weight, bias, G, eps, act_fn_opti
         if nbytes == 0:
             raise RuntimeError("gnop::fwd_add: " + _cabi.last_error())
         stream = _current_stream_ptr(X.device)
-        ws = _workspace(nbytes, X.device, stream)
+        ws = _workspace(nbytes, X.device)
         rc = lib.gnnhwc_fwd_add(
             X_nrc.data_ptr(), res_ptr, cb_ptr, S.data_ptr() if return_sum else None,
             weight.contiguous().data_ptr(), bias.contiguous().data_ptr(),

@@ -97,7 +97,7 @@ def _rms_norm_bwd(dy, ds, s, weight, eps):
         if nbytes == 0:
             raise RuntimeError("gnop::rms_norm_bwd: " + _cabi.last_error())
         stream = _stream_args(s)
-        ws = _workspace(nbytes, s.device, stream)
+        ws = _workspace(nbytes, s.device)
         rc = lib.gnnhwc_rms_bwd(dyr.data_ptr(), _ptr(dsr), sr.data_ptr(), _ptr(w), dx.data_ptr(), dw.data_ptr() if w is not None else None,
                                 sr.shape[0], C, dyr.stride(0), 0 if dsr is None else dsr.stride(0), sr.stride(0), float(eps), dt, pdt,
                                 ws.data_ptr(), ws.numel(), stream)
@@ -444,7 +444,7 @@ def _rotary_bwd(q_grad, k_grad, q, k, positions, frequencies, sections, interlea
             nbytes = lib.gnnhwc_rotary_bwd_workspace_bytes(ctypes.byref(c))
             if nbytes == 0:
                 raise RuntimeError("gnop::rotary_bwd: " + _cabi.last_error())
-            ws = _workspace(nbytes, dev, stream)
+            ws = _workspace(nbytes, dev)
             ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
         rc = lib.gnnhwc_rotary_bwd(ctypes.byref(c), ws_ptr, ws_bytes, stream)
     _cabi.check(rc, "gnop::rotary_bwd")
@@ -656,7 +656,7 @@ def _clip_general(grads, outs, max_norm, grad_scale, eps):
     lib = _cabi.lib
     with _on_device(dev):
         stream = _current_stream_ptr(dev)
-        ws = _workspace(lib.gnnhwc_clip_workspace_bytes(n), dev, stream)
+        ws = _workspace(lib.gnnhwc_clip_workspace_bytes(n), dev)
         rc = lib.gnnhwc_clip(ins, to, sizes, types, to_types, n, float(max_norm), float(eps), float(grad_scale), total.data_ptr(),
                              _DTYPE_CODE[total.dtype], ws.data_ptr(), ws.numel(), stream)
     _cabi.check(rc, "clip_gradients")
