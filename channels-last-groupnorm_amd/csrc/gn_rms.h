@@ -136,6 +136,14 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, int lpr, uint32_t *lds) 
   return v;
 }
 
+// y / d, where inv is 1 / d rounded: a product and one correction by its remainder (Markstein), which leaves the rounded quotient
+// but for cases next to the middle of two floats.  (Against a product alone bf16 (700000, 80) 39.5 -> 42 us, (16384, 2560) the
+// same; a division 55.6 and 53.3.)
+__device__ __forceinline__ float quotient(float y, float d, float inv) {
+  const float q = y * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, d, y), inv, q);
+}
+
 // VEC values as 8-bit numbers, packed.  |v| <= q_most up to the rounding of the scale, which both conversions round down to
 // q_most.
 template <int VEC> struct Bytes {
@@ -265,7 +273,7 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
       const uint32_t b = q.block_lanes == 0 ? whole : segment_max(most[k], q.block_lanes);
       const float a = __builtin_bit_cast(float, b) / q.q_most;
       const float scale = a < 0x1p-126f ? 0x1p-126f : a;  // (a NaN stays)
-      const float inv = 1.0f / scale;
+      const float inv = 1.0f / scale, divisor = inv > 0 ? scale : 0.0f;  // (an infinite scale has no remainders: y * 0 stays)
       if (!live || !cut.has(k)) continue;
       const int j = cut.vector(k);
       if (q.block_lanes == 0) {
@@ -275,7 +283,7 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
       }
       float v[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = y[k][i] * inv;
+      for (int i = 0; i < VEC; ++i) v[i] = quotient(y[k][i], divisor, inv);
       const Bytes<VEC> p = pack_bytes<VEC>(v, q.qtype);
       uint8_t *out = (uint8_t *)q.y + row * q.C + cut.start(k);
       const int skip = cut.doubled(k);
