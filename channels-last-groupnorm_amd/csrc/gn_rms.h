@@ -40,13 +40,26 @@ template <typename LV, typename T> __device__ __forceinline__ void store_loose(T
 }
 
 template <typename T> using acc_of_t = typename acc_of<T>::type;
-// 1 / sqrt(v) within an ulp or so: the hardware's estimate and one Newton step (six instructions, where a root and a division
-// take about thirty), except where the step would meet a zero, an infinity or a subnormal.
-__device__ __forceinline__ float row_rsqrt(float v) {
-  if (v > 0x1p-100f && v < 0x1p+120f) return fast_rsqrt(v);
-  return 1.0f / __builtin_sqrtf(v);
+// y / d, where inv is 1 / d rounded: a product and one correction by its remainder (Markstein), which leaves the rounded quotient
+// but for cases next to the middle of two floats.
+__device__ __forceinline__ float quotient(float y, float d, float inv) {
+  const float q = y * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, d, y), inv, q);
 }
-__device__ __forceinline__ double row_rsqrt(double v) { return 1.0 / __builtin_sqrt(v); }
+// 1 / sqrt(ss / n + eps) of a row's sum of squares.  Whatever it is off by is off in all of the row, so that each of its steps is
+// rounded once: the mean by quotient(), the root from the hardware's estimate (an ulp) and one Newton step in the form
+// r + r (1 - v r^2) / 2, whose correction needs few bits.  About a dozen instructions, where a division, a root and a division
+// take fifty; those are left for where the step would meet a zero, an infinity or a subnormal.
+__device__ __forceinline__ float row_rstd(float ss, int n, double inv_n, double eps) {
+  const float v = quotient(ss, (float)n, (float)inv_n) + (float)eps;
+  if (v > 0x1p-100f && v < 0x1p+120f) {
+    const float r = __builtin_amdgcn_rsqf(v), t = v * r;
+    const float left = __builtin_fmaf(-t, r, 1.0f) - __builtin_fmaf(v, r, -t) * r;
+    return __builtin_fmaf(0.5f * r, left, r);
+  }
+  return 1.0f / __builtin_sqrtf(ss / (float)n + (float)eps);
+}
+__device__ __forceinline__ double row_rstd(double ss, int n, double, double eps) { return 1.0 / __builtin_sqrt(ss / n + eps); }
 
 // One lane vector's worth of VEC parameters of type P, as accumulators.
 template <typename P, int VEC, typename A> __device__ __forceinline__ void load_params(const P *w, A (&v)[VEC]) {
@@ -136,14 +149,6 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, int lpr, uint32_t *lds) 
   return v;
 }
 
-// y / d, where inv is 1 / d rounded: a product and one correction by its remainder (Markstein), which leaves the rounded quotient
-// but for cases next to the middle of two floats.  (Against a product alone bf16 (700000, 80) 39.5 -> 42 us, (16384, 2560) the
-// same; a division 55.6 and 53.3.)
-__device__ __forceinline__ float quotient(float y, float d, float inv) {
-  const float q = y * inv;
-  return __builtin_fmaf(__builtin_fmaf(-q, d, y), inv, q);
-}
-
 // VEC values as 8-bit numbers, packed.  |v| <= q_most up to the rounding of the scale, which both conversions round down to
 // q_most.
 template <int VEC> struct Bytes {
@@ -228,7 +233,7 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
     ss += cut.has(k) ? part : (A)0;
   }
   row_sum2(ss, none, q.lpr, lds, 0);
-  const A rstd = row_rsqrt(ss * (A)q.inv_c + (A)q.eps);
+  const A rstd = row_rstd(ss, q.C, q.inv_c, q.eps);
 
   if constexpr (!QUANT) {
 #pragma unroll
@@ -273,6 +278,7 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
       const uint32_t b = q.block_lanes == 0 ? whole : segment_max(most[k], q.block_lanes);
       const float a = __builtin_bit_cast(float, b) / q.q_most;
       const float scale = a < 0x1p-126f ? 0x1p-126f : a;  // (a NaN stays)
+      // (against a product with inv alone bf16 (700000, 80) 39.5 -> 42 us, (16384, 2560) the same; divisions 55.6 and 53.3)
       const float inv = 1.0f / scale, divisor = inv > 0 ? scale : 0.0f;  // (an infinite scale has no remainders: y * 0 stays)
       if (!live || !cut.has(k)) continue;
       const int j = cut.vector(k);
@@ -363,7 +369,7 @@ __global__ __launch_bounds__(THREADS) void rms_bwd_kernel(const RmsBwd q) {
       gs += cut.has(k) ? p1 : (A)0;
     }
     row_sum2(ss, gs, q.lpr, lds, turn);
-    const A r = row_rsqrt(ss * (A)q.inv_c + (A)q.eps);
+    const A r = row_rstd(ss, q.C, q.inv_c, q.eps);
     const A c = -(r * gs * (A)q.inv_c) * r;
     if (!live) continue;
 #pragma unroll

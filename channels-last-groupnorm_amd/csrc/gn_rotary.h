@@ -275,7 +275,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
 #pragma unroll
       for (int c = 0; c < Lane::kWidth; ++c) ss += v[c] * v[c];
       ss = segment_sum(lane < q.nvec ? ss : (A)0, q.lanes);
-      const A rstd = row_rsqrt(ss * (A)q.inv_d + (A)q.eps);
+      const A rstd = row_rstd(ss, q.D, q.inv_d, q.eps);
 #pragma unroll
       for (int c = 0; c < Lane::kWidth; ++c) v[c] = v[c] * rstd * w[c];
     }
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_bwd_kernel(const RotaryArg
       if (lane >= q.nvec) ss = gt = 0;
       segment_sum2(ss, gt, q.lanes);
       // dt = r g - h (r mean(g h)) with mean(g h) = r gt / D, as in rms_bwd_kernel: r^3 would leave a float's range
-      const A r = row_rsqrt(ss * (A)q.inv_d + (A)q.eps), m = -(r * gt * (A)q.inv_d) * r;
+      const A r = row_rstd(ss, q.D, q.inv_d, q.eps), m = -(r * gt * (A)q.inv_d) * r;
 #pragma unroll
       for (int c = 0; c < kWidth; ++c) {
         const A dr = d[c] * r, h = t[c] * r;
