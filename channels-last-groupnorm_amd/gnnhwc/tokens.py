@@ -667,9 +667,11 @@ def _clip_general(grads, outs, max_norm, grad_scale, eps):
     return total
 
 
-def clip_grad_norm_(parameters, max_norm, grad_scale=1.0, eps=1e-6):
-    """clip_gradients in place over the gradients of `parameters` (a parameter that is listed twice counts once); as
-    torch.nn.utils.clip_grad_norm_ with the Euclidean norm."""
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, *, grad_scale=1.0, eps=1e-6):
+    """clip_gradients in place over the gradients of `parameters` (a parameter that is listed twice counts once).  The first
+    three arguments are those of torch.nn.utils.clip_grad_norm_; the Euclidean norm is the only norm_type."""
+    if norm_type != 2:
+        raise RuntimeError("clip_grad_norm_: norm_type must be 2, got %s" % (norm_type,))
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     unique = {id(p): p for p in parameters}.values()
