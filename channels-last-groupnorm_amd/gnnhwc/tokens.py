@@ -618,18 +618,27 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
         return _clip_general(grads, outs, max_norm, grad_scale, eps)
 
 
+def _check_written(t, name):
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):  # an expanded tensor
+        raise RuntimeError("%s cannot be written: its elements share memory" % name)
+
+
 def _clip_general(grads, outs, max_norm, grad_scale, eps):
     dev = grads[0].device
     keep, back = [], []
+    changes = outs is not None or grad_scale != 1.0 or max_norm < math.inf
     for i, g in enumerate(grads):
         _check_device(g, "gradient %d" % i)
         _dtype_code(g, "gradient %d" % i)
         if g.layout != torch.strided or g.device != dev:
             raise RuntimeError("gradient %d must be a dense tensor on %s" % (i, dev))
         if outs is None:
+            if changes:
+                _check_written(g, "gradient %d" % i)
             if not _dense(g) or g.is_neg():  # a slice with gaps, or a view that only stands for negated memory: through a copy
                 c = g.resolve_neg().contiguous()
-                back.append((g, c))
+                if changes:
+                    back.append((g, c))
                 g = c
             keep.append((g, g))
             continue
@@ -638,6 +647,7 @@ def _clip_general(grads, outs, max_norm, grad_scale, eps):
         _dtype_code(o, "out %d" % i)
         if o.shape != g.shape or o.device != dev or o.layout != torch.strided:
             raise RuntimeError("out %d must have the gradient's shape %s on %s" % (i, tuple(g.shape), dev))
+        _check_written(o, "out %d" % i)
         g = g.resolve_neg()
         if not (_dense(g) and _dense(o) and not o.is_neg() and (g.stride() == o.stride() or g.is_contiguous() and o.is_contiguous())):
             g = g.contiguous()
@@ -662,7 +672,7 @@ def _clip_general(grads, outs, max_norm, grad_scale, eps):
     _cabi.check(rc, "clip_gradients")
     for t, c in back:
         t.copy_(c)
-    if outs is not None or grad_scale != 1.0 or max_norm < math.inf:
+    if changes:
         torch.autograd.graph.increment_version([t for t in (grads if outs is None else outs) if not t.is_inference()])
     return total
 
