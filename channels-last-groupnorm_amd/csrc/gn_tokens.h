@@ -72,8 +72,6 @@ struct PartialSum {
   int count, C, split, out_dtype;
 };
 
-RowCut rms_cut(int64_t C, int esize, int least_lanes);
-int rms_bwd_blocks(int64_t rows, const RowCut &cut);
 constexpr int kMostChannels = 16384;
 constexpr int kRowVectors = 3;  // most lane vectors of a row per lane, but for the longest rows
 // What the memory-side cache is counted on to hold until the next kernel.  Inputs beyond it are read past the caches: forward of

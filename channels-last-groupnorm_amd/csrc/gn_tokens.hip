@@ -92,8 +92,6 @@ int check_fwd(const void *x, const void *residual, void *sum_out, const void *y,
   return GNNHWC_OK;
 }
 
-}  // namespace
-
 // How a row's lane vectors are dealt to lanes: the fewest lanes (a power of two) that leave none more than three (forward of
 // float16 (65536, 2560): 223 us with three, 228 with five; bf16 in 8 bits, 128 channels a block, (16384, 2560): 54 and 61).
 // `whole`: rows that are not whole lines of memory in one access each, up to a wavefront, where several would write parts of
@@ -107,9 +105,9 @@ RowCut rms_cut(int64_t C, int esize, int least_lanes, bool whole) {
   c.nvec = (int)ceil_div(C, c.vec);
   c.ragged = C % c.vec != 0;
   c.lpr = std::max(8, least_lanes);
-  // (two where a workgroup is wider than 256: a third does not fit the registers of 1024 threads in the backward)
   if (whole && C * esize % 128 != 0)
     while (c.lpr < 64 && c.nvec > c.lpr) c.lpr <<= 1;
+  // (two where a workgroup is wider than 256: a third does not fit the registers of 1024 threads in the backward)
   while (c.lpr < 1024 && c.nvec > (c.lpr > 256 ? 2 : kRowVectors) * c.lpr) c.lpr <<= 1;
   c.nv = (int)ceil_div(c.nvec, c.lpr);
   c.lpr_log2 = log2_of(c.lpr);
@@ -122,8 +120,6 @@ int rms_bwd_blocks(int64_t rows, const RowCut &cut) {
   const int64_t steps = ceil_div(rows, cut.threads / cut.lpr);
   return steps == 0 ? 0 : (int)ceil_div(steps, ceil_div(steps, 2 * kNumCU));
 }
-
-namespace {
 
 // ---- rotary ----
 struct RotaryPlan {
