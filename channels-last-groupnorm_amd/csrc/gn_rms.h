@@ -7,8 +7,8 @@
 // Quantised: per block of channels (or row) a = max |y|, scale = max(a / q_most, 2^-126), q = round(y / scale).
 //
 // What bounds them is memory: a row is read once, kept packed in registers between the sum of squares and the result, and
-// written once: forward of float16 (65536, 2560) with its sum 217 us, 6.2 TB/s; bf16 (16384, 1280) 29.6 us, 5.7; in 8 bits with
-// 128 channels a block bf16 (16384, 2560) 52.5 us, 5.6; a copy of their sizes runs at 5.7.  `lpr` lanes share a row (a power of
+// written once: forward of float16 (65536, 2560) with its sum 219 us, 6.1 TB/s; bf16 (16384, 1280) 30.1 us, 5.6; in 8 bits with
+// 128 channels a block bf16 (16384, 2560) 52.9 us, 5.6; a copy of their sizes runs at 5.7.  `lpr` lanes share a row (a power of
 // two: part of a wavefront, or several wavefronts that add their sums through LDS), each with NV lane vectors, vector k of lane
 // l being k * lpr + l, so that every access of a wavefront is one run of memory.
 //
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(THREADS) void rms_fwd_kernel(const RmsFwd q) {
   }
 }
 
-// Backward: float16 (65536, 2560) with a gradient of the sum 234 us (5.7 TB/s), bf16 (16384, 1280) 34.5 (4.9).  A workgroup
+// Backward: float16 (65536, 2560) with a gradient of the sum 233 us (5.8 TB/s), bf16 (16384, 1280) 34.9 (4.8).  A workgroup
 // walks over rows and keeps its share of dw in registers, in a fixed order, and leaves one partial row of dw; partial_sum_kernel
 // adds those.  r is computed again from s, whose sum of squares rides along with that of g s, so that the forward saves no
 // statistics: with G = sum g s, mean(g h) = r G / C.  The second term is h (r mean(g h)), not s (r^3 G / C): r^3 leaves a float's

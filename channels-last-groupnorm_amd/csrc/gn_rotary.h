@@ -6,7 +6,7 @@
 //
 // Memory bounds them: q and k are read once and written once; angles come from a position and P frequencies per token and are
 // not read from tables: float16 (46800 tokens, 24 + 24 heads, 128) 192 us, 6.0 TB/s (a copy: 5.7); bf16 (16384, 20 + 20, 64)
-// with a norm 31 us, 5.4 (a copy of that size: 5.1), its backward 46, 5.4.  A group of lanes (a power of two) takes one head at
+// with a norm 31.5 us, 5.3 (a copy of that size: 5.1), its backward 47, 5.4.  A group of lanes (a power of two) takes one head at
 // a time, each lane one or two lane vectors of it; it turns every `groups`-th head of its token, so that one set of sines and
 // cosines serves several heads and neighbouring groups read neighbouring memory.
 #pragma once
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const RotaryArgs q) {
 }
 
 // Backward behind a norm: four lane vectors of q or k and four of their gradients at once (bf16 (16384, 20 + 20, 64): eight take
-// the registers of a third workgroup a CU, 59 us instead of 50 with far pairs; two take 51 instead of 47 with near ones).  A group
+// the registers of a third workgroup a CU, 64 us instead of 50 with far pairs; two take 51 instead of 47 with near ones).  A group
 // keeps its place among the heads (and so q or k) while it walks over tokens, and its share of dw in registers; a workgroup
 // leaves one partial row of 2 D values (q's, k's).
 template <typename T, typename P, int S, bool NEAR, bool WHOLE>

@@ -37,8 +37,9 @@ template <typename P, int S, bool NEAR, bool WHOLE, bool NORM> void launch_one(c
   const dim3 grid((unsigned)(((int64_t)a.tokens * a.groups + per_block - 1) / per_block));
   const size_t lds = (size_t)a.span * (a.D / 2) * sizeof(SinCos<A>);
   // Heads that no cache can hold are read past the caches where each access is whole lines of memory (float16 (46800, 24 + 24
-  // heads, 128): 203 -> 192 us; bf16 (74800, 24 + 24, 64): 161 -> 152); other halves share lines, which are then fetched twice
-  // (float32 (308142, 2 + 1, 96): 134 -> 169), as are heads that stand in for missing ones (float32 (500000, 2 + 1, 64): 132 -> 145).
+  // heads, 128): 203 -> 192 us; bf16 (74800, 24 + 24, 64): 162 -> 153); other halves share lines, which are then fetched twice
+  // (float32 (308142, 2 + 1, 96): 127 -> 167; not so heads that are whole in an access, bf16 (46800, 24 + 24, 96): 149 -> 142), as
+  // are heads that stand in for missing ones (float32 (500000, 2 + 1, 64): 128 -> 148).
   if constexpr (S * sizeof(elem_t) == 16) {
     const int heads = a.side[0].heads + a.side[1].heads;
     const int64_t bytes = (int64_t)a.tokens * heads * a.D * sizeof(elem_t);

@@ -74,8 +74,8 @@ struct PartialSum {
 
 constexpr int kMostChannels = 16384;
 constexpr int kRowVectors = 3;  // most lane vectors of a row per lane, but for the longest rows
-// What the memory-side cache is counted on to hold until the next kernel.  Inputs beyond it are read past the caches: forward of
-// float16 (65536, 2560) 229 -> 221 us, its backward 235 -> 229; but bf16 (16384, 1280), which the cache can hold, 26 -> 30.
+// What the memory-side cache is counted on to hold until the next kernel.  Inputs beyond it are read past the caches: backward of
+// float16 (65536, 2560) 239 -> 233 us, its forward 220 -> 219; but forward of bf16 (90000, 320), which the cache can hold, 17.7 -> 20.1.
 constexpr int64_t kCachedBytes = (int64_t)224 << 20;
 
 #define GN_DECLARE_TOKENS(S)                                                                            \

@@ -92,12 +92,13 @@ int check_fwd(const void *x, const void *residual, void *sum_out, const void *y,
   return GNNHWC_OK;
 }
 
-// How a row's lane vectors are dealt to lanes: the fewest lanes (a power of two) that leave none more than three (forward of
-// float16 (65536, 2560): 223 us with three, 228 with five; bf16 in 8 bits, 128 channels a block, (16384, 2560): 54 and 61).
+// How a row's lane vectors are dealt to lanes: the fewest lanes (a power of two) that leave none more than three (against five:
+// bf16 in 8 bits (280000, 200) 36 and 50 us, (16384, 2560) with 128 channels a block 53 and 55; backward of bf16 (140000, 200) 34
+// and 38; of float16 (65536, 2560) 233 and 229, its forward 219 either way).
 // `whole`: rows that are not whole lines of memory in one access each, up to a wavefront, where several would write parts of
-// lines (forward, bf16 (140000, 200) with a residual 53 -> 37 us, (966103, 80) 103 -> 61; rows of whole lines lose by it,
-// (90000, 320) 20 -> 24, as do the backward, (140000, 200) 34 -> 44, whose few workgroups want more of each row on its way, and
-// 8 bits, (280000, 200) 34 -> 45).
+// lines (forward, bf16 (140000, 200) with a residual 57 -> 39 us, (966103, 80) 102 -> 61; rows of whole lines lose by it,
+// (90000, 320) 17.7 -> 19.9, as do the backward, (140000, 200) 34 -> 46, whose few workgroups want more of each row on its way,
+// and 8 bits, (280000, 200) 36 -> 47).
 RowCut rms_cut(int64_t C, int esize, int least_lanes, bool whole) {
   const int vec = 16 / esize;
   RowCut c;
@@ -115,7 +116,8 @@ RowCut rms_cut(int64_t C, int esize, int least_lanes, bool whole) {
   return c;
 }
 // Workgroups of the backward's walk: as many as walk equally far, up to two per CU (with three or four, float16 (65536, 2560)
-// takes 251 and 274 us instead of 235, bf16 (16384, 1280) 37 and 42 instead of 38).
+// takes 240 and 262 us instead of 233; bf16 (16384, 1280) 33.5 and 37.7 instead of 34.9, (140000, 200) 31 and 32 instead of 34,
+// but each leaves a partial row to write and to add).
 int rms_bwd_blocks(int64_t rows, const RowCut &cut) {
   const int64_t steps = ceil_div(rows, cut.threads / cut.lpr);
   return steps == 0 ? 0 : (int)ceil_div(steps, ceil_div(steps, 2 * kNumCU));
@@ -159,12 +161,12 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   const int half = a.D / 2, most = c->dtype == GN_F64 ? 2 : c->dtype == GN_F32 ? 4 : 8;
   // The widest lane vector that divides what it has to; half of 16 bytes for half-precision heads such as 40 with far pairs.
   // Whole heads (PairLane, gn_rotary.h) for 16 bits:
-  // - near pairs, always: (16384, 20 + 20, 64) 31 us, in halves 36.5; (65536, 8 + 8, 80) 59 and 71; behind a norm backward 47 and
-  //   51, 123 and 153.  Of 32 bits halves are longer and a workgroup of half as many heads costs more: (308142, 2 + 1, 96) whole
-  //   150, in halves 129; (770, 24 + 12, 40) 5.3 and 4.9.
-  // - far pairs, forward, where they fill three quarters of the lanes: (16384, 20 + 20, 64) 31.7 us, in halves 35.7; (46800,
-  //   24 + 24, 96) 149 and 183; of 160 channels, 20 of 32 lanes, (13000, 5 + 1) 18.6 and 15.4.  Behind a norm backward: 50 and 50,
-  //   (13770, 12 + 2, 80) 29 and 24.
+  // - near pairs, always: (16384, 20 + 20, 64) 31 us, in halves 36; (65536, 8 + 8, 80) 59 and 72; (74800, 24 + 24, 64) 153 and
+  //   178; behind a norm backward 47 and 65, 121 and 116.  Of 32 bits halves are longer and a workgroup of half as many heads costs
+  //   more: (308142, 2 + 1, 96) whole 140, in halves 127; (770, 24 + 12, 40) 5.0 and 4.3.
+  // - far pairs, forward, where they fill three quarters of the lanes: (16384, 20 + 20, 64) 32 us, in halves 36.5; (46800,
+  //   24 + 24, 96) 149 and 183; of 160 channels, 20 of 32 lanes, (13000, 5 + 1) 15.3 and 12.5.  Behind a norm backward: 50 and 50,
+  //   (13770, 12 + 2, 80) 30 and 24.7.
   const bool bits16 = c->dtype == GN_F16 || c->dtype == GN_BF16, near = c->interleaved != 0;
   const int vecs16 = a.D / 8;
   const bool far_whole = bits16 && !near && !(backward && norm) && a.D % 8 == 0 && a.P % 8 == 0 && 4 * vecs16 >= 3 << log2_of(vecs16);
@@ -232,8 +234,8 @@ int plan_rotary(const gnnhwc_rotary_call *c, bool backward, RotaryPlan &p) {
   a.inv_d = 1.0 / a.D;
   a.sign = backward ? -1.0f : 1.0f;
   if (backward && norm) {
-    // A walk of whole sets of groups, alike in length: at most three workgroups per CU (a few more than that leave some CUs with
-    // four: 151 us instead of 123 for float16 (65536, 8 + 8, 80)), or four where that spares the second turn.
+    // A walk of whole sets of groups, alike in length: at most three workgroups per CU (with four bf16 (16384, 20 + 20, 64) takes
+    // 59 us instead of 47, float16 (65536, 8 + 8, 80) 132 instead of 121), or four where that spares the second turn.
     const int64_t steps = std::max<int64_t>(1, 3 * kNumCU * subs / a.groups);
     const int64_t turns = tokens <= steps + steps / 3 ? 1 : ceil_div(tokens, steps);
     a.token_step = (int)ceil_div(tokens, turns);

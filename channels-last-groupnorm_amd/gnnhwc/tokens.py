@@ -5,7 +5,8 @@ counterpart to any of them.
 
 The kernels are those of include/gnnhwc_tokens.h in libgnnhwc_hip.so.  Ordinary eager calls run in native code
 (csrc/gn_tokens_torch.cpp); what that declines -- tracing, subclasses, tensors in other layouts, and every error -- comes
-here, through the ``gnop::`` operators, which carry meta kernels and autograd formulas.
+here, through the ``gnop::`` operators, which carry meta kernels and autograd formulas (``clip_gradients``, which has no derivative
+and works on lists, has none).
 """
 import ctypes
 import math
@@ -535,10 +536,10 @@ def rotary(q, k, positions, frequencies, sections=None, interleaved=False, q_wei
 
     q: (B, L, heads, D), k: (B, L, kv_heads, D) or None, with any strides as long as a head's channels are contiguous (slices of
     one packed projection are read where they are); D even, up to 256.  positions: (L, axes) or (B, L, axes), int32, int64 or
-    float32, whole numbers within 32 bits and exact to 2^24 (with one axis also (L,) or (B, L)).  frequencies: float32, one for each turning pair, see rotary_frequencies;
-    sections: how many of them belong to each axis, in order (None: all to one axis).  Pair j of a head is its channels
-    (2 j, 2 j + 1) if `interleaved`, else (j, j + P), P = sum(sections); it is turned by positions[axis] * frequencies[j].
-    Channels behind the 2 P first stay as they are.
+    float32, whole numbers within 32 bits and exact to 2^24 (with one axis also (L,) or (B, L)).  frequencies: float32, one for
+    each turning pair, see rotary_frequencies; sections: how many of them belong to each axis, in order (None: all to one axis).
+    Pair j of a head is its channels (2 j, 2 j + 1) if `interleaved`, else (j, j + P), P = sum(sections); it is turned by
+    positions[axis] * frequencies[j].  Channels behind the 2 P first stay as they are.
 
     With q_weight / k_weight, (D,) in q's dtype or float32 beside half precision, every head is first normalised over its D
     channels, t / sqrt(mean(t^2) + eps) * weight, in the same pass.  Everything in between is float32 (float64).
@@ -603,8 +604,9 @@ def clip_gradients(grads, max_norm, out=None, grad_scale=1.0, eps=1e-6):
     grads: tensors on one device, any floating types and dense layouts (channels-last included), mixed.  out=None: in place;
     else tensors like the gradients, in any floating types, that receive the results (e.g. float32 ones of half-precision
     gradients).  grad_scale: the reciprocal of a loss scale.  max_norm=math.inf computes the norm only (unless out or
-    grad_scale ask for more).  A norm that is NaN or infinite gives NaN, as the formula does.  Squares are summed in float64,
-    in a fixed order; the norm is float32 (float64 if all gradients are)."""
+    grad_scale ask for more).  As the formula has it, a norm that is NaN gives NaN throughout, and an infinite one zeros for what
+    is finite and NaN for what is not.  Squares are summed in float64, in a fixed order; the norm is float32 (float64 if all
+    gradients are).  An ordinary function on lists, not an operator of torch.library: it is called outside compiled graphs."""
     grads = list(grads)
     outs = None if out is None else list(out)
     if outs is not None and len(outs) != len(grads):

@@ -56,8 +56,9 @@ class Block(nn.Module):
         return self.down(F.silu(self.up(n))), residual
 
     def serve(self, h, residual, positions):
-        """The same with both norms leaving in 8 bits, a scale per token: the products take 8-bit values, and the scales, one
-        for each row of a product, are applied to its result."""
+        """The same with both norms leaving in 8 bits, a scale per token, which is one for each row of a product and is applied
+        to its result.  (The weights here stay in bfloat16, and the 8-bit values are widened in front of the product; a serving
+        program hands them to an 8-bit one as they are.)"""
         def product(q, scales, linear):
             return (F.linear(q.to(linear.weight.dtype), linear.weight) * scales).to(linear.weight.dtype)
 
