@@ -1,0 +1,172 @@
+// C ABI of the attention (declared in include/gnnhwc_tokens.h): argument checks and launch planning.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "gn_error.h"
+#include "gn_window_args.h"
+
+namespace gn {
+namespace {
+
+constexpr int64_t kMostTokens = (int64_t)1 << 30;
+constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
+
+int invalid(const char *what) { return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s", what); }
+int launched(hipError_t e, const char *what) {
+  return e == hipSuccess ? GNNHWC_OK : fail(GNNHWC_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
+
+int put_rows(HeadRows &r, const void *base, const int64_t (&stride)[3], int64_t batch, int64_t tokens, int64_t heads, int64_t es, const char *name) {
+  r = {};
+  if (batch == 0 || tokens == 0) return GNNHWC_OK;
+  if (!base) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s is null", name);
+  const int64_t size[3] = {batch, tokens, heads};
+  int64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    const int64_t s = size[i] == 1 ? 0 : stride[i];
+    if (s < 0 || s > ((int64_t)1 << 56) / size[i]) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s: stride out of range", name);
+    bytes[i] = s * es;
+    if (bytes[i] % 16) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s: its strides must be whole multiples of 16 bytes", name);
+  }
+  if ((uintptr_t)base % 16) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s must be aligned to 16 bytes", name);
+  if (bytes[1] > 0x7fffffff) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s: a token's stride must be below 2^31 bytes", name);
+  r.base = base;
+  r.batch_bytes = bytes[0];
+  r.token_bytes = (int)bytes[1];
+  r.head_bytes = bytes[2];
+  return GNNHWC_OK;
+}
+
+struct WindowPlan {
+  WindowArgs a, kv;  // queries' tiles, keys' tiles
+  bool empty;
+  size_t delta, largest, part_k, part_v, bytes;  // backward's workspace
+};
+
+int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
+  if (!c) return invalid("null call");
+  const int64_t es = c->dtype == GN_F32 ? 4 : c->dtype == GN_F16 || c->dtype == GN_BF16 ? 2 : 0;
+  if (!es) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "dtype code %lld: attention takes f32, f16 or bf16", (long long)c->dtype);
+  if (c->batch < 0 || c->tokens < 0 || c->keys < 0) return invalid("batch, tokens and keys must not be negative");
+  if (c->tokens > kMostTokens || c->keys > kMostTokens || c->batch > kMostTokens) return invalid("batch, tokens or keys out of range: at most 2^30");
+  if (c->heads < 1 || c->kv_heads < 1 || c->heads > 65535 || c->heads % c->kv_heads) return invalid("heads must be 1 to 65535 and a multiple of kv_heads");
+  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8) return invalid("head_dim must be a multiple of 8 from 8 to 256");
+  if (c->window < -1 || c->sinks < 0) return invalid("window must be -1 or more, and sinks not negative");
+  if (c->length_type != 0 && c->length_type != 1) return invalid("length_type must be 0 (int32) or 1 (int64)");
+  if (!(c->scale > 0 && c->scale < INFINITY)) return invalid("scale must be positive and finite");
+  if (!c->at_end && c->tokens > c->keys) return invalid("more queries than keys: the queries are the last of the keys' tokens");
+  if (backward && c->at_end) return invalid("attention against a cache has no backward");
+  p = {};
+  WindowArgs &a = p.a;
+  const int64_t rows = c->heads, kv = c->kv_heads;
+  if (const int rc = put_rows(a.q, c->q, c->q_stride, c->batch, c->tokens, rows, es, "q")) return rc;
+  if (const int rc = put_rows(a.k, c->k, c->k_stride, c->batch, c->keys, kv, es, "k")) return rc;
+  if (const int rc = put_rows(a.v, c->v, c->v_stride, c->batch, c->keys, kv, es, "v")) return rc;
+  if (const int rc = put_rows(a.out, c->out, c->out_stride, c->batch, c->tokens, rows, es, "out")) return rc;
+  if (backward) {
+    if (const int rc = put_rows(a.dout, c->out_grad, c->out_grad_stride, c->batch, c->tokens, rows, es, "out_grad")) return rc;
+    if (const int rc = put_rows(a.dq, c->q_grad, c->q_grad_stride, c->batch, c->tokens, rows, es, "q_grad")) return rc;
+    if (const int rc = put_rows(a.dk, c->k_grad, c->k_grad_stride, c->batch, c->keys, kv, es, "k_grad")) return rc;
+    if (const int rc = put_rows(a.dv, c->v_grad, c->v_grad_stride, c->batch, c->keys, kv, es, "v_grad")) return rc;
+    if (c->batch && c->tokens && !c->lse) return invalid("lse is null");
+  }
+  a.lse = c->lse;
+  a.lengths = c->lengths;
+  a.length_type = (int)c->length_type;
+  a.at_end = c->at_end != 0;
+  a.B = (int)c->batch; a.L = (int)c->tokens; a.S = (int)c->keys; a.H = (int)c->heads; a.K = (int)c->kv_heads; a.D = (int)c->head_dim;
+  a.group = a.H / a.K;
+  a.causal = c->causal != 0;
+  a.left = (int)(c->window < 0 ? kMostTokens : std::min(c->window, kMostTokens));
+  a.right = a.causal ? 0 : a.left;
+  a.sinks = c->window < 0 ? 0 : (int)std::min(c->sinks, kMostTokens);  // (without a bound all are seen)
+  a.scale = (float)c->scale;
+  a.scale_log2 = (float)(c->scale * 1.4426950408889634);
+  if (!(a.scale > 0 && a.scale_log2 < INFINITY)) return invalid("scale must be positive and finite");
+  a.tiles = (int)ceil_div(a.L, kQueries);
+  const int64_t items = (int64_t)a.tiles * a.H * a.B;
+  if (items > kMostItems || (int64_t)a.H * a.B > kMostItems) return invalid("too many tokens and heads for one call");
+  a.items = (int)items;
+  p.empty = items == 0;
+  if (!backward) return GNNHWC_OK;
+
+  // Workgroups of dk and dv.  A key that all queries see (a sink) has many times the others' work, and a short batch has fewer tiles
+  // than the device has room for: several workgroups then share a tile's queries.
+  p.kv = a;
+  WindowArgs &w = p.kv;
+  w.tiles = (int)ceil_div(a.S, kQueries);
+  w.sink_tiles = (int)std::min<int64_t>(w.tiles, ceil_div(a.sinks, kQueries));
+  const int64_t step = es == 2 ? 64 : 32, all = ceil_div(a.L, step) * a.group;  // queries that a step takes, steps of a sink's tile
+  const int64_t reach = std::min<int64_t>((int64_t)a.left + a.right + kQueries, a.L);
+  const int64_t usual = std::min(all, (ceil_div(reach, step) + 1) * a.group);
+  const int64_t heads = (int64_t)a.B * a.K, work = heads * (w.sink_tiles * all + (w.tiles - w.sink_tiles) * usual);
+  const int64_t most = std::max<int64_t>(4, work / (8 * kNumCU));  // steps of a workgroup: a quarter of what is for each of two per CU
+  w.shares = (int)std::clamp<int64_t>(ceil_div(usual, most), 1, 256);
+  w.sink_shares = w.sink_tiles ? (int)std::clamp<int64_t>(ceil_div(all, most), 1, 256) : 1;
+  const int64_t per = (int64_t)w.sink_tiles * w.sink_shares + (int64_t)(w.tiles - w.sink_tiles) * w.shares;
+  if (per * heads > kMostItems) return invalid("too many tokens and heads for one call");
+  w.items = (int)(per * heads);
+  w.parts = (int)((w.sink_shares > 1 ? (int64_t)w.sink_tiles * w.sink_shares : 0) + (w.shares > 1 ? (int64_t)(w.tiles - w.sink_tiles) * w.shares : 0));
+  const size_t lse = round_up((size_t)a.B * a.H * a.L * sizeof(float)), part = round_up((size_t)w.parts * heads * kQueries * a.D * sizeof(float));
+  p.delta = 0;
+  p.largest = lse;
+  p.part_k = p.largest + (c->dtype == GN_F16 ? lse : 0);
+  p.part_v = p.part_k + part;
+  p.bytes = 256 + p.part_v + part;
+  return GNNHWC_OK;
+}
+
+#define GN_BY_TYPE(dtype, call) ((dtype) == GN_F32 ? call(f32) : (dtype) == GN_F16 ? call(f16) : call(bf16))
+
+}  // namespace
+}  // namespace gn
+
+using namespace gn;
+
+extern "C" {
+
+size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *c) {
+  WindowPlan p;
+  if (plan_window(c, false, p)) return 0;
+  return 256;
+}
+
+int gnnhwc_window(const gnnhwc_window_call *c, void *workspace, size_t workspace_bytes, void *stream) {
+  WindowPlan p;
+  if (const int rc = plan_window(c, false, p)) return rc;
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < 256)
+    return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_workspace_bytes");
+  if (p.empty) return GNNHWC_OK;
+#define GN_CALL(S) launch_window_forward_##S(p.a, (hipStream_t)stream)
+  return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window");
+#undef GN_CALL
+}
+
+size_t gnnhwc_window_bwd_workspace_bytes(const gnnhwc_window_call *c) {
+  WindowPlan p;
+  if (plan_window(c, true, p)) return 0;
+  return p.bytes;
+}
+
+int gnnhwc_window_bwd(const gnnhwc_window_call *c, void *workspace, size_t workspace_bytes, void *stream) {
+  WindowPlan p;
+  if (const int rc = plan_window(c, true, p)) return rc;
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes)
+    return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_bwd_workspace_bytes");
+  for (WindowArgs *a : {&p.a, &p.kv}) {
+    a->delta = (float *)((char *)workspace + p.delta);
+    a->largest = (float *)((char *)workspace + p.largest);
+    a->part_k = (float *)((char *)workspace + p.part_k);
+    a->part_v = (float *)((char *)workspace + p.part_v);
+  }
+  if (p.a.items == 0 && p.kv.items == 0) return GNNHWC_OK;
+#define GN_CALL(S) launch_window_backward_##S(p.a, p.kv, (hipStream_t)stream)
+  return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window_bwd");
+#undef GN_CALL
+}
+
+}  // extern "C"

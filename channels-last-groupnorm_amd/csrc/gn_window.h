@@ -1,0 +1,896 @@
+// Softmax attention in which a token sees a window around it and a few first tokens (sinks): forward and backward.
+//
+//   s[i][j] = scale q[i] . k[j],   P[i][.] = softmax of s[i][.] over the tokens that i sees,   o[i] = sum_j P[i][j] v[j]
+// backward, with delta[i] = do[i] . o[i] and dS[i][j] = P[i][j] (do[i] . v[j] - delta[i]):
+//   dq[i] = scale sum_j dS[i][j] k[j],   dk[j] = scale sum_i dS[i][j] q[i],   dv[j] = sum_i P[i][j] do[i]
+//
+// Every product runs on matrix instructions of 32 x 32 x 16 whose result has one token of one side per lane, so that no value
+// of a score tile changes lanes: S^T = K Q^T leaves a query in each lane's column, with 16 of 32 keys, and the second product
+// takes them as its B operand where they are, for the order of its 16 summands is free as long as both operands have the same:
+// summand i of half h is row 8 (i / 4) + 4 h + i % 4, which is also what a transposing read of two times four rows delivers.
+// The running maximum and sum of the softmax then belong to a lane.
+//
+// Tiles of the other side are copied from memory into shared memory without passing through registers, two deep: the next one
+// travels while this one is multiplied.  A row of a tile is cut into chunks of 16 bytes whose order depends on the row
+// (chunk_of), so that rows read side by side lie in different banks.
+#pragma once
+#include "gn_device.h"
+#include "gn_window_args.h"
+
+namespace gn {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+
+// Eight elements of a lane: an operand's share of 16 summands.
+template <typename T> struct Operand;
+template <> struct Operand<bf16_t> {
+  typedef bf16x8_t type;
+  static __device__ __forceinline__ f32x16_t product(type a, type b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Operand<f16_t> {
+  typedef f16x8_t type;
+  static __device__ __forceinline__ f32x16_t product(type a, type b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Operand<float> {  // eight products of two summands each
+  typedef f32x8_t type;
+  static __device__ __forceinline__ f32x16_t product(type a, type b, f32x16_t c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+template <typename T> using operand_t = typename Operand<T>::type;
+
+// Values 8 t .. 8 t + 7 of a lane's column, rounded to T once: what the products' results cost beside float32 operands, half a
+// unit in the last place of each summand, like the operands that come from memory.
+template <typename T> __device__ __forceinline__ operand_t<T> operand_of(const f32x16_t &v, int t) {
+  if constexpr (sizeof(T) == 4) {
+    f32x8_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = v[8 * t + i];
+    return r;
+  } else if constexpr (__is_same(T, bf16_t)) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack_bf16x2(v[8 * t + 2 * i], v[8 * t + 2 * i + 1]);
+    return __builtin_bit_cast(bf16x8_t, r);
+  } else {
+    f16x8_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (_Float16)v[8 * t + i];
+    return r;
+  }
+}
+__device__ __forceinline__ f32x16_t zeros16() {
+  f32x16_t v;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+  return v;
+}
+// Row of a result tile that register r of a lane in half h holds.
+__device__ __forceinline__ constexpr int row_of(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
+
+template <typename T> __device__ __forceinline__ float to_float(const T *p) {
+  float v[1];
+  LaneVec<T, 1>::unpack(LaneVec<T, 1>::load(p), v);
+  return v[0];
+}
+
+// ---- tiles in shared memory ----
+template <typename T, int DP> struct Tile {
+  static constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
+  static constexpr int kChunks = DP * (int)sizeof(T) / 16;  // of a row
+  static constexpr int kBytes = kRows * kChunks * 16;
+  static constexpr int kCopies = kRows * kChunks / kBlock;  // chunks that each thread of a workgroup copies
+  static_assert(kRows * kChunks % kBlock == 0 && kChunks % 4 == 0, "a tile is copied by whole workgroups");
+
+  // Place of chunk c in its row: four neighbouring rows lie in different quarters of the 64 banks, which suits the transposing
+  // reads of four rows, and sixteen in different places, which suits the reads of a chunk of many rows.
+  static __device__ __forceinline__ int chunk_of(int row, int c) {
+    if constexpr (kChunks % 16 == 0) return c ^ ((row & 3) << 2 | (row >> 2 & 3));
+    else if constexpr (kChunks % 8 == 0) return c ^ ((row >> 1 & 1) << 2 | (row >> 2 & 3));
+    else return c ^ (row >> 2 & 3);
+  }
+  // Operand whose rows are the tile's, summands 16 s + 8 h ..
+  static __device__ __forceinline__ operand_t<T> rows(const char *tile, int first, int s, int lane) {
+    const int row = first + (lane & 31), h = lane >> 5;
+    const char *at = tile + row * (kChunks * 16);
+    if constexpr (sizeof(T) == 2) {
+      return *(const operand_t<T> *)(at + chunk_of(row, 2 * s + h) * 16);
+    } else {
+      const f32x4 a = *(const f32x4 *)(at + chunk_of(row, 4 * s + 2 * h) * 16), b = *(const f32x4 *)(at + chunk_of(row, 4 * s + 2 * h + 1) * 16);
+      return f32x8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+  // Operand whose rows are the channels 32 c .., its summands the tile's rows first .. first + 15 in a result's order.
+  static __device__ __forceinline__ operand_t<T> columns(char *tile, int first, int c, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      // a group of 16 lanes reads four rows of 16 channels, four to a lane, and each lane is left with a channel
+      const int m = lane & 15, row = first + 4 * h + (m >> 2), chunk = 4 * c + (lane >> 4 & 1) * 2 + (m >> 1 & 1), part = (m & 1) * 8;
+      typedef __attribute__((address_space(3))) s16x4_t lds4;
+      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + row * (kChunks * 16) + chunk_of(row, chunk) * 16 + part));
+      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + (row + 8) * (kChunks * 16) + chunk_of(row + 8, chunk) * 16 + part));
+      return __builtin_bit_cast(operand_t<T>, s16x8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    } else {
+      f32x8_t r;
+      const int d = 32 * c + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = first + row_of(i, h);
+        r[i] = *(const float *)(tile + row * (kChunks * 16) + chunk_of(row, d >> 2) * 16 + (d & 3) * 4);
+      }
+      return r;
+    }
+  }
+};
+
+// Each lane's BYTES from memory into shared memory, the lanes' behind each other from `to` on, which is the same for all of them.
+// (The compiler would have every transposing read wait for all copies that are on their way, other buffers' too: it is not told
+// of these.  Nothing is written to a register but m0, which nothing else here uses; tiles_turn waits.)
+template <int BYTES> __device__ __forceinline__ void copy_to_lds(const void *from, void *to) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)to);
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "memory");
+}
+
+// Copies tiles of rows into shared memory.  Rows past `last` and chunks past the head are other rows and chunks of the same
+// tensor (memory that is there, and values whose products are left out).
+template <typename T, int DP> struct TileCopy {
+  using G = Tile<T, DP>;
+  int row[G::kCopies], byte[G::kCopies];
+  __device__ __forceinline__ void init(int D) {
+#pragma unroll
+    for (int i = 0; i < G::kCopies; ++i) {
+      const int slot = i * kBlock + (int)threadIdx.x;
+      row[i] = slot / G::kChunks;
+      const int c = G::chunk_of(row[i], slot % G::kChunks) * 16;  // (its own inverse)
+      byte[i] = c < D * (int)sizeof(T) ? c : 0;
+    }
+  }
+  __device__ __forceinline__ void issue(const char *base, int stride, int first, int last, char *tile) const {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < G::kCopies; ++i) {
+      int r = first + row[i];
+      r = r < last ? r : last;
+      const char *from = base + (int64_t)r * stride + byte[i];
+      copy_to_lds<16>(from, tile + (i * kBlock + wave * 64) * 16);
+    }
+  }
+};
+// All of this workgroup's copies have arrived and all of its reads of shared memory are done.
+__device__ __forceinline__ void tiles_turn() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// ---- which tokens see which ----
+// A sample's tokens: keys 0 .. n - 1; query i stands at place i + off, those with first <= i < last stand among the keys.
+struct Sample {
+  int n, off, first, last;
+};
+__device__ __forceinline__ Sample sample_of(const WindowArgs &a, int b) {
+  Sample s;
+  s.n = a.S;
+  if (a.lengths) {
+    const int64_t n = a.length_type ? load_global<int64_t>((const int64_t *)a.lengths + b) : (int64_t)load_global<int>((const int *)a.lengths + b);
+    s.n = n < 0 ? 0 : n < a.S ? (int)n : a.S;
+  }
+  s.off = (a.at_end ? s.n : a.S) - a.L;
+  s.first = s.off < 0 ? -s.off : 0;
+  s.last = s.n - s.off < a.L ? s.n - s.off : a.L;
+  return s;
+}
+// What a query sees: keys low .. low + count - 1, and keys below `sinks`.
+struct Sight {
+  int low, count, sinks;
+  __device__ __forceinline__ bool sees(int j) const { return (unsigned)(j - low) < (unsigned)count || j < sinks; }
+};
+__device__ __forceinline__ Sight sight_of(const WindowArgs &a, const Sample &s, int i) {
+  Sight g = {0, 0, 0};
+  if (i >= s.first && i < s.last) {
+    const int p = i + s.off, high = p + a.right < s.n ? p + a.right : s.n - 1;
+    g.low = p > a.left ? p - a.left : 0;
+    g.count = high - g.low + 1;
+    g.sinks = a.sinks < s.n ? a.sinks : s.n;
+    if (a.causal && p + 1 < g.sinks) g.sinks = p + 1;
+  }
+  return g;
+}
+// The places from which a key is seen: from, .. from + count - 1 (the queries that are there).
+struct Seen {
+  int from, count;
+};
+__device__ __forceinline__ Seen seen_of(const WindowArgs &a, const Sample &s, int j) {
+  Seen g = {0, 0};
+  if (j < s.n && s.last > s.first) {
+    int lo = j - a.right, hi = j + a.left;
+    if (j < a.sinks) {
+      if (!a.causal) lo = 0;
+      hi = s.n - 1;
+    }
+    const int least = s.first + s.off, most = s.last - 1 + s.off;
+    lo = lo > least ? lo : least;
+    hi = hi < most ? hi : most;
+    g.from = lo;
+    g.count = hi < lo ? 0 : hi - lo + 1;
+  }
+  return g;
+}
+// Tiles of `rows` keys that a workgroup with queries at places low .. high has to visit: those of the sinks, then the window's.
+struct Walk {
+  int sinks, first, last;  // tiles of the sinks; the window's tiles behind them: first .. last
+  __device__ __forceinline__ int start() const { return sinks > 0 ? 0 : first; }
+  __device__ __forceinline__ int next(int t) const { return t + 1 == sinks ? first : t + 1; }
+  __device__ __forceinline__ bool more(int t) const { return t < sinks || t <= last; }
+};
+__device__ __forceinline__ Walk walk_of(const WindowArgs &a, const Sample &s, int low, int high, int rows) {
+  Walk w;
+  int sinks = a.sinks < s.n ? a.sinks : s.n;
+  if (a.causal && high + 1 < sinks) sinks = high + 1;
+  w.sinks = (sinks + rows - 1) / rows;
+  const int from = low > a.left ? low - a.left : 0, to = high + a.right < s.n ? high + a.right : s.n - 1;
+  w.first = from / rows;
+  if (w.first < w.sinks) w.first = w.sinks;
+  w.last = to / rows;
+  return w;
+}
+
+// Workgroups are dealt to the eight dies in turn, each with a cache of its own: neighbours in the work's order go to one die.
+__device__ __forceinline__ int work_item(int items) {
+  const int id = blockIdx.x, share = (items + 7) >> 3;
+  return (id & 7) * share + (id >> 3);  // (items and beyond: nothing to do)
+}
+
+// ---- rows by their formulas, for results that are not finite ----
+// A tile's products reach over all of its rows: what a token does not see has the weight 0 there, and 0 times an infinity or a NaN
+// of such a token is NaN.  A row that comes out infinite or NaN is therefore computed again over the pairs that see each other
+// alone, by one wavefront, in float32.  (Rows that have to be so, as in a training that has diverged, take this path too.)
+template <typename T> __device__ __forceinline__ float dot(const T *a, const T *b, int D) {
+  float s = 0.0f;
+#pragma unroll 4
+  for (int d = 0; d < D; ++d) s = __builtin_fmaf(to_float(a + d), to_float(b + d), s);
+  return s;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+// Calls f(j0, j) for the keys that a query sees, 64 at a time: j of this lane, or -1.
+template <typename F> __device__ __forceinline__ void for_keys(const Sight &g, F &&f) {
+  const int lane = threadIdx.x & 63;
+  const int sinks = g.count > 0 && g.low < g.sinks ? g.low : g.sinks;  // (those of the window once)
+  for (int j0 = 0; j0 < sinks; j0 += 64) f(j0, j0 + lane < sinks ? j0 + lane : -1);
+  for (int j0 = g.low; j0 < g.low + g.count; j0 += 64) f(j0, j0 + lane < g.low + g.count ? j0 + lane : -1);
+  if (g.count > 0 && g.low + g.count < g.sinks)
+    for (int j0 = g.low + g.count; j0 < g.sinks; j0 += 64) f(j0, j0 + lane < g.sinks ? j0 + lane : -1);
+}
+template <typename T> __device__ void row_again(const WindowArgs &a, const Sample &s, int b, int h, int i) {
+  const int lane = threadIdx.x & 63, kh = h / a.group;
+  const Sight g = sight_of(a, s, i);
+  const T *q = (const T *)a.q.row(b, i, h);
+  float most = -INFINITY, nan = 0.0f;
+  for_keys(g, [&](int, int j) {
+    if (j >= 0) {
+      const float v = dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2;
+      most = fmaxf(most, v);
+      nan += v == v ? 0.0f : v;  // (a maximum loses it)
+    }
+  });
+  most = wave_max(most);
+  most = most == -INFINITY ? 0.0f : most;
+  float sum = nan;
+  for_keys(g, [&](int, int j) {
+    if (j >= 0) sum += __builtin_amdgcn_exp2f(dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2 - most);
+  });
+  sum = wave_sum(sum);
+  float o[4] = {};
+  for_keys(g, [&](int j0, int j) {
+    const float p = j >= 0 ? __builtin_amdgcn_exp2f(dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2 - most) / sum : 0.0f;
+    for (int u = 0; u < 64; ++u) {
+      const int ju = __shfl(j, u);
+      const float pu = __shfl(p, u);
+      if (ju < 0) break;
+      const T *v = (const T *)a.v.row(b, ju, kh);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (x * 64 + lane < a.D) o[x] = __builtin_fmaf(pu, to_float(v + x * 64 + lane), o[x]);
+    }
+  });
+  T *to = (T *)a.out.row(b, i, h);
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (x * 64 + lane < a.D) {
+      const float t[1] = {o[x]};
+      LaneVec<T, 1>::store(to + x * 64 + lane, LaneVec<T, 1>::pack(t));
+    }
+  if (a.lse && lane == 0) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, most + __builtin_amdgcn_logf(sum));
+}
+// dq of one row.
+template <typename T> __device__ void dq_again(const WindowArgs &a, const Sample &s, int b, int h, int i, float lse, float delta) {
+  const int lane = threadIdx.x & 63, kh = h / a.group;
+  const T *q = (const T *)a.q.row(b, i, h), *g = (const T *)a.dout.row(b, i, h);
+  float acc[4] = {};
+  for_keys(sight_of(a, s, i), [&](int, int j) {
+    float ds = 0.0f;
+    if (j >= 0) {
+      const float p = __builtin_amdgcn_exp2f(dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2 - lse);
+      ds = p * (dot(g, (const T *)a.v.row(b, j, kh), a.D) - delta);
+    }
+    for (int u = 0; u < 64; ++u) {
+      const int ju = __shfl(j, u);
+      const float du = __shfl(ds, u);
+      if (ju < 0) break;
+      const T *k = (const T *)a.k.row(b, ju, kh);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (x * 64 + lane < a.D) acc[x] = __builtin_fmaf(du, to_float(k + x * 64 + lane), acc[x]);
+    }
+  });
+  T *to = (T *)a.dq.row(b, i, h);
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (x * 64 + lane < a.D) {
+      const float t[1] = {acc[x] * a.scale};
+      LaneVec<T, 1>::store(to + x * 64 + lane, LaneVec<T, 1>::pack(t));
+    }
+}
+// dk or dv of one row.
+template <typename T> __device__ void dkv_again(const WindowArgs &a, const Sample &s, int b, int kh, int j, bool of_k) {
+  const int lane = threadIdx.x & 63;
+  const T *k = (const T *)a.k.row(b, j, kh), *v = (const T *)a.v.row(b, j, kh);
+  const Seen w = seen_of(a, s, j);
+  float acc[4] = {};
+  for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
+    const int64_t rows = ((int64_t)b * a.H + h) * a.L;
+    for (int i0 = 0; i0 < w.count; i0 += 64) {
+      const int i = i0 + lane < w.count ? w.from + i0 + lane - s.off : -1;
+      float t = 0.0f;
+      if (i >= 0) {
+        t = __builtin_amdgcn_exp2f(dot((const T *)a.q.row(b, i, h), k, a.D) * a.scale_log2 - load_global<float>(a.lse + rows + i));
+        if (of_k) t *= dot((const T *)a.dout.row(b, i, h), v, a.D) - load_global<float>(a.delta + rows + i);
+      }
+      for (int u = 0; u < 64; ++u) {
+        const int iu = __shfl(i, u);
+        const float tu = __shfl(t, u);
+        if (iu < 0) break;
+        const T *r = of_k ? (const T *)a.q.row(b, iu, h) : (const T *)a.dout.row(b, iu, h);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (x * 64 + lane < a.D) acc[x] = __builtin_fmaf(tu, to_float(r + x * 64 + lane), acc[x]);
+      }
+    }
+  }
+  T *to = (T *)(of_k ? a.dk.row(b, j, kh) : a.dv.row(b, j, kh));
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (x * 64 + lane < a.D) {
+      const float t[1] = {of_k ? acc[x] * a.scale : acc[x]};
+      LaneVec<T, 1>::store(to + x * 64 + lane, LaneVec<T, 1>::pack(t));
+    }
+}
+
+// ---- a lane's token of the side that stays in registers ----
+// Operands of one token per lane: channels 16 s + 8 h ..; zeros past the head.
+template <typename T, int DP> __device__ __forceinline__ void load_token(const T *p, int D, operand_t<T> (&f)[DP / 16]) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int d = 16 * s + 8 * h;
+    operand_t<T> z = {};
+    if (d < D) {
+      if constexpr (sizeof(T) == 2) {
+        z = load_global<operand_t<T>>(p + d);
+      } else {
+        const f32x4 x = load_global<f32x4>(p + d), y = load_global<f32x4>(p + d + 4);
+        z = f32x8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      }
+    }
+    f[s] = z;
+  }
+}
+// Channels of one token per lane from a transposed result, times `factor`, rounded once.
+template <typename T, int DP> __device__ __forceinline__ void store_token(T *p, int D, const f32x16_t (&acc)[DP / 32], float factor) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * c + row_of(r, h);
+      if (d < D) {
+        const float t[4] = {acc[c][r] * factor, acc[c][r + 1] * factor, acc[c][r + 2] * factor, acc[c][r + 3] * factor};
+        using LV = LaneVec<T, 4>;
+        LV::store(p + d, LV::pack(t));
+      }
+    }
+}
+template <int N> __device__ __forceinline__ bool any_not_finite(const f32x16_t (&acc)[N]) {
+  float t = 0.0f;
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t = __builtin_fmaf(acc[c][r], 0.0f, t);
+  return !(t == 0.0f);
+}
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+__device__ __forceinline__ bool either_half(bool v) {
+  const uint64_t m = __ballot(v);
+  return ((m | m >> 32 | m << 32) >> (threadIdx.x & 63)) & 1;
+}
+
+// ---- forward ----
+// The exponentials' reference is raised only when a score passes it by this much (in powers of two): the sums stay far inside a
+// float's range, weights below 2^8 inside a float16's, and most tiles leave the accumulators alone.
+constexpr float kRaise = 8.0f;
+
+template <typename T, int DP> struct ForwardState {
+  operand_t<T> q[DP / 16];
+  f32x16_t o[DP / 32];
+  float reference, sum;  // of the lane's half of the keys; in powers of two
+  Sight sight;
+};
+
+// 32 keys against the wavefront's 32 queries: scores, then weights in their place.
+template <typename T, int DP> __device__ __forceinline__ void forward_tile(ForwardState<T, DP> &st, const char *kt, char *vt, int first, int j0, float c) {
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const Sight &g = st.sight;
+  const int left = j0 - g.low;
+  const bool inside = (left >= 0 && left + 31 < g.count) || j0 + 31 < g.sinks;
+  const bool touches = (left + 31 >= 0 && left < g.count) || j0 < g.sinks;
+  if (!__any(touches)) return;
+  f32x16_t s = zeros16();
+#pragma unroll
+  for (int x = 0; x < DP / 16; ++x) s = Operand<T>::product(Tile<T, DP>::rows(kt, first, x, lane), st.q[x], s);
+  if (!__all(inside)) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (!g.sees(j0 + row_of(r, h))) s[r] = -INFINITY;
+  }
+  float most = s[0];
+#pragma unroll
+  for (int r = 1; r < 16; ++r) most = fmaxf(most, s[r]);
+  if (__any(most * c > st.reference + kRaise)) {
+    most = fmaxf(most, other_half(most)) * c;
+    const float reference = fmaxf(most, st.reference);
+    const float factor = reference == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.reference - reference);
+    st.reference = reference;
+    st.sum *= factor;
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.o[x][r] *= factor;
+  }
+  const float ref = st.reference == -INFINITY ? 0.0f : st.reference;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ref));
+    st.sum += s[r];
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const operand_t<T> p = operand_of<T>(s, t);
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) st.o[x] = Operand<T>::product(Tile<T, DP>::columns(vt, first + 16 * t, x, lane), p, st.o[x]);
+  }
+}
+
+// A workgroup: 128 queries of one head, 32 a wavefront.
+template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
+  using G = Tile<T, DP>;
+  __shared__ __attribute__((aligned(16))) char keys[2][G::kBytes], values[2][G::kBytes];
+  const int item = work_item(a.items);
+  if (item >= a.items) return;
+  // (the heads of a group are neighbours, then the tiles of queries, the last ones, which see most, first)
+  const int g = item % a.group, rest = item / a.group, tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
+  const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
+  const Sample s = sample_of(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = tile * kQueries + wave * 32 + (lane & 31);
+  ForwardState<T, DP> st;
+  st.sight = sight_of(a, s, i);
+  st.reference = -INFINITY;
+  st.sum = 0.0f;
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x) st.o[x] = zeros16();
+  const int from = tile * kQueries > s.first ? tile * kQueries : s.first, to = (tile + 1) * kQueries < s.last ? (tile + 1) * kQueries : s.last;
+  if (from < to) {
+    const int ic = i < from ? from : i < to ? i : to - 1;
+    load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
+    const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows);
+    TileCopy<T, DP> copy;
+    copy.init(a.D);
+    const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
+    int t = w.start();
+    if (w.more(t)) {
+      copy.issue(kb, a.k.token_bytes, t * G::kRows, s.n - 1, keys[0]);
+      copy.issue(vb, a.v.token_bytes, t * G::kRows, s.n - 1, values[0]);
+    }
+    auto turn = [&](auto buffer) {
+      constexpr int B = decltype(buffer)::value;
+      tiles_turn();
+      const int next = w.next(t);
+      if (w.more(next)) {
+        copy.issue(kb, a.k.token_bytes, next * G::kRows, s.n - 1, keys[1 - B]);
+        copy.issue(vb, a.v.token_bytes, next * G::kRows, s.n - 1, values[1 - B]);
+      }
+#pragma unroll
+      for (int f = 0; f < G::kRows; f += 32) forward_tile<T, DP>(st, keys[B], values[B], f, t * G::kRows + f, a.scale_log2);
+      t = next;
+    };
+    while (w.more(t)) {
+      turn(std::integral_constant<int, 0>());
+      if (!w.more(t)) break;
+      turn(std::integral_constant<int, 1>());
+    }
+  }
+  const float sum = st.sum + other_half(st.sum);
+  const bool nothing = st.reference == -INFINITY && sum == 0.0f;  // (of no key seen, or scores of -inf alone: the latter is computed again)
+  const float factor = nothing ? 0.0f : 1.0f / sum;
+  const bool there = i < a.L, seeing = st.sight.count > 0 || st.sight.sinks > 0;
+  bool again = any_not_finite(st.o) || !(factor < INFINITY) || nothing;
+  again = either_half(again) && seeing;
+  if (there) {
+    store_token<T, DP>((T *)a.out.row(b, i, h), a.D, st.o, factor);
+    if (a.lse && lane < 32) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, nothing ? INFINITY : st.reference + __builtin_amdgcn_logf(sum));
+  }
+  uint64_t rows = __ballot(again && there) & 0xffffffffu;
+  while (rows) {
+    const int r = __builtin_ctzll(rows);
+    rows &= rows - 1;
+    row_again<T>(a, s, b, h, tile * kQueries + wave * 32 + r);
+  }
+}
+
+// ---- backward: dq ----
+// delta and the largest |do| of a row go to the workspace for the other kernel.
+// float16 holds 2^-24 to 65504: weights and dS are kept in its middle by powers of two, weights as 2^12 P, dS relative to the
+// largest |do| (of a row, or of the rows that a workgroup visits), whatever scale a loss has been given.
+constexpr float kWeightBits = 12.0f, kGradBits = 5.0f;
+template <typename T> __device__ __forceinline__ float gradient_unit(float most) {  // a power of two near 1 / most
+  if constexpr (!__is_same(T, f16_t)) return 1.0f;
+  else return most > 0.0f && most < INFINITY ? __builtin_amdgcn_ldexpf(1.0f, -__builtin_amdgcn_frexp_expf(most)) : 1.0f;
+}
+
+template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && sizeof(T) == 2 ? 2 : 1) void window_dq_kernel(const WindowArgs a) {
+  using G = Tile<T, DP>;
+  __shared__ __attribute__((aligned(16))) char keys[2][G::kBytes], values[2][G::kBytes];
+  const int item = work_item(a.items);
+  if (item >= a.items) return;
+  const int g = item % a.group, rest = item / a.group, tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
+  const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
+  const Sample s = sample_of(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, i = tile * kQueries + wave * 32 + (lane & 31);
+  const Sight sight = sight_of(a, s, i);
+  const int64_t row = ((int64_t)b * a.H + h) * a.L + i;
+  f32x16_t acc[DP / 32];
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x) acc[x] = zeros16();
+  float lse = INFINITY, delta = 0.0f, unit = 1.0f;
+  const int from = tile * kQueries > s.first ? tile * kQueries : s.first, to = (tile + 1) * kQueries < s.last ? (tile + 1) * kQueries : s.last;
+  if (from < to) {
+    const int ic = i < from ? from : i < to ? i : to - 1;
+    operand_t<T> q[DP / 16], dout[DP / 16];
+    load_token<T, DP>((const T *)a.dout.row(b, ic, h), a.D, dout);
+    {
+      load_token<T, DP>((const T *)a.out.row(b, ic, h), a.D, q);  // (o, for delta; q's place)
+      float most = 0.0f;
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          delta = __builtin_fmaf((float)dout[x][e], (float)q[x][e], delta);
+          most = fmaxf(most, fabsf((float)dout[x][e]));
+        }
+      delta += other_half(delta);
+      most = fmaxf(most, other_half(most));
+      unit = gradient_unit<T>(most);
+      if (i >= from && i < to && lane < 32) {
+        store_global<float>(a.delta + row, delta);
+        if constexpr (__is_same(T, f16_t)) store_global<float>(a.largest + row, most);
+      }
+    }
+    load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, q);
+    if (i >= from && i < to) lse = load_global<float>(a.lse + row);
+    const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows);
+    TileCopy<T, DP> copy;
+    copy.init(a.D);
+    const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
+    // P 2^bits (dP - delta) unit: one exponential and one fused step per element
+    const float bits = __is_same(T, f16_t) ? kGradBits : 0.0f, lift = bits - lse, lowered = -delta * unit;
+    int t = w.start();
+    if (w.more(t)) {
+      copy.issue(kb, a.k.token_bytes, t * G::kRows, s.n - 1, keys[0]);
+      copy.issue(vb, a.v.token_bytes, t * G::kRows, s.n - 1, values[0]);
+    }
+    auto turn = [&](auto buffer) {
+      constexpr int B = decltype(buffer)::value;
+      tiles_turn();
+      const int next = w.next(t);
+      if (w.more(next)) {
+        copy.issue(kb, a.k.token_bytes, next * G::kRows, s.n - 1, keys[1 - B]);
+        copy.issue(vb, a.v.token_bytes, next * G::kRows, s.n - 1, values[1 - B]);
+      }
+#pragma unroll
+      for (int f = 0; f < G::kRows; f += 32) {
+        const int j0 = t * G::kRows + f, left = j0 - sight.low;
+        const bool inside = (left >= 0 && left + 31 < sight.count) || j0 + 31 < sight.sinks;
+        const bool touches = (left + 31 >= 0 && left < sight.count) || j0 < sight.sinks;
+        if (!__any(touches)) continue;
+        f32x16_t p = zeros16(), dp = zeros16();
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+          p = Operand<T>::product(G::rows(keys[B], f, x, lane), q[x], p);
+          dp = Operand<T>::product(G::rows(values[B], f, x, lane), dout[x], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, lift)) * __builtin_fmaf(dp[r], unit, lowered);
+        if (!__all(inside)) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!sight.sees(j0 + row_of(r, half))) p[r] = 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const operand_t<T> ds = operand_of<T>(p, u);
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x) acc[x] = Operand<T>::product(G::columns(keys[B], f + 16 * u, x, lane), ds, acc[x]);
+        }
+      }
+      t = next;
+    };
+    while (w.more(t)) {
+      turn(std::integral_constant<int, 0>());
+      if (!w.more(t)) break;
+      turn(std::integral_constant<int, 1>());
+    }
+  }
+  const bool there = i < a.L, seeing = sight.count > 0 || sight.sinks > 0;
+  bool again = any_not_finite(acc);
+  again = either_half(again) && seeing && there;
+  if (there) {
+    const float factor = a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f);
+    store_token<T, DP>((T *)a.dq.row(b, i, h), a.D, acc, seeing ? factor : 0.0f);
+  }
+  uint64_t rows = __ballot(again) & 0xffffffffu;
+  while (rows) {
+    const int r = __builtin_ctzll(rows);
+    rows &= rows - 1;
+    dq_again<T>(a, s, b, h, tile * kQueries + wave * 32 + r, __shfl(lse, r), __shfl(delta, r));
+  }
+}
+static_assert(kGradBits == 5.0f, "the factors of 1 / 32 undo it");
+
+// ---- backward: dk and dv ----
+// Where the workgroup `at` of a head leaves its sums: those of tiles that several share have a place.
+__device__ __forceinline__ int64_t part_slot(const WindowArgs &a, int bk, int at) {
+  const int sink_items = a.sink_tiles * a.sink_shares;
+  return (int64_t)bk * a.parts + (at < sink_items || a.sink_shares > 1 ? at : at - sink_items);
+}
+// A workgroup: 128 keys of one head, 32 a wavefront, against a share of the queries that see any of them, of all heads of the
+// group.  PARTS: 1 dv, 2 dk, 3 both (heads of more than 128 channels do not fit the registers at once).  Where several workgroups
+// share a tile's queries, each leaves float32 sums, which window_sum_kernel adds in their order.
+template <typename T, int DP, int PARTS>
+__global__ __launch_bounds__(kBlock, DP <= 96 && sizeof(T) == 2 ? 2 : 1) void window_dkv_kernel(const WindowArgs a) {
+  using G = Tile<T, DP>;
+  constexpr bool kDv = PARTS & 1, kDk = PARTS & 2;
+  __shared__ __attribute__((aligned(16))) char queries[2][G::kBytes], grads[2][G::kBytes];
+  __shared__ __attribute__((aligned(16))) float lses[2][64], deltas[2][64];
+  __shared__ float reduce[4];
+  const int item = work_item(a.items);
+  if (item >= a.items) return;
+  // first the shares of the sinks' tiles, then the others
+  const int sink_items = a.sink_tiles * a.sink_shares, per = sink_items + (a.tiles - a.sink_tiles) * a.shares;
+  const int bk = item / per, at = item % per, b = bk / a.K, kh = bk % a.K;
+  int tile, share, shares;
+  if (at < sink_items) {
+    shares = a.sink_shares;
+    tile = at / shares;
+    share = at % shares;
+  } else {
+    shares = a.shares;
+    tile = a.sink_tiles + (at - sink_items) / shares;
+    share = (at - sink_items) % shares;
+  }
+  const Sample s = sample_of(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, j = tile * kQueries + wave * 32 + (lane & 31);
+  const Seen seen = seen_of(a, s, j);
+  f32x16_t dk[kDk ? DP / 32 : 1], dv[kDv ? DP / 32 : 1];
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x) {
+    if constexpr (kDk) dk[x] = zeros16();
+    if constexpr (kDv) dv[x] = zeros16();
+  }
+  float unit = 1.0f;
+  // the queries that see any key of the tile: those of its first key, of its last, and what is between
+  const int top = (tile + 1) * kQueries < s.n ? (tile + 1) * kQueries : s.n;
+  int from = 0, to = -1;
+  if (tile * kQueries < top && s.first < s.last) {
+    const int j0 = tile * kQueries, least = s.first + s.off, most = s.last - 1 + s.off;
+    from = j0 > a.right ? j0 - a.right : 0;
+    to = top - 1 + a.left;
+    if (j0 < a.sinks) {
+      if (!a.causal) from = 0;
+      to = s.n - 1;
+    }
+    from = (from > least ? from : least) - s.off;
+    to = (to < most ? to : most) - s.off;
+  }
+  if (from <= to) {
+    const int first = from / G::kRows, tiles = to / G::kRows - first + 1, steps = tiles * a.group;
+    const int begin = (int)((int64_t)steps * share / shares), end = (int)((int64_t)steps * (share + 1) / shares);
+    if constexpr (__is_same(T, f16_t)) {
+      float most = 0.0f;
+      for (int st = begin; st < end; ++st) {
+        const int64_t rows = ((int64_t)b * a.H + kh * a.group + st / tiles) * a.L;
+        const int i = (first + st % tiles) * G::kRows + (int)(threadIdx.x & 63);
+        if (wave == (st & 3) && i >= from && i <= to) most = fmaxf(most, load_global<float>(a.largest + rows + i));
+      }
+      most = wave_max(most);
+      if (lane == 0) reduce[wave] = most;
+      __syncthreads();
+      most = fmaxf(fmaxf(reduce[0], reduce[1]), fmaxf(reduce[2], reduce[3]));
+      unit = gradient_unit<T>(most);
+    }
+    operand_t<T> k[DP / 16], v[kDk ? DP / 16 : 1];
+    const int jc = j < s.n ? j : s.n - 1;
+    load_token<T, DP>((const T *)a.k.row(b, jc, kh), a.D, k);
+    if constexpr (kDk) load_token<T, DP>((const T *)a.v.row(b, jc, kh), a.D, v);
+    TileCopy<T, DP> copy;
+    copy.init(a.D);
+    auto issue = [&](int st, char *qt, char *gt, float *lt, float *dt) {
+      const int h = kh * a.group + st / tiles, i0 = (first + st % tiles) * G::kRows;
+      copy.issue((const char *)a.q.row(b, 0, h), a.q.token_bytes, i0, to, qt);
+      copy.issue((const char *)a.dout.row(b, 0, h), a.dout.token_bytes, i0, to, gt);
+      int i = i0 + lane;
+      i = i < to ? i : to;
+      const int64_t row = ((int64_t)b * a.H + h) * a.L + i;
+      if (wave == 0) copy_to_lds<4>(a.lse + row, lt);
+      if (kDk && wave == 1) copy_to_lds<4>(a.delta + row, dt);
+    };
+    const float bits = __is_same(T, f16_t) ? kWeightBits : 0.0f;
+    const float lowering = __is_same(T, f16_t) ? unit * (1.0f / 128.0f) : 1.0f;  // 2^(kGradBits - kWeightBits)
+    int st = begin;
+    if (st < end) issue(st, queries[0], grads[0], lses[0], deltas[0]);
+    auto turn = [&](auto buffer) {
+      constexpr int B = decltype(buffer)::value;
+      tiles_turn();
+      if (st + 1 < end) issue(st + 1, queries[1 - B], grads[1 - B], lses[1 - B], deltas[1 - B]);
+#pragma unroll
+      for (int f = 0; f < G::kRows; f += 32) {
+        const int p0 = (first + st % tiles) * G::kRows + f + s.off, left = p0 - seen.from;
+        const bool inside = left >= 0 && left + 31 < seen.count, touches = left + 31 >= 0 && left < seen.count;
+        if (!__any(touches)) continue;
+        f32x16_t p = zeros16(), dp = zeros16();
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+          p = Operand<T>::product(G::rows(queries[B], f, x, lane), k[x], p);
+          if constexpr (kDk) dp = Operand<T>::product(G::rows(grads[B], f, x, lane), v[x], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const f32x4 l4 = *(const f32x4 *)&lses[B][f + row_of(r, half)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r + e], a.scale_log2, bits - l4[e]));
+        }
+        const bool whole = __all(inside);
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if ((unsigned)(left + row_of(r, half)) >= (unsigned)seen.count) p[r] = 0.0f;
+        }
+        if constexpr (kDv) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const operand_t<T> w = operand_of<T>(p, u);
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x) dv[x] = Operand<T>::product(G::columns(grads[B], f + 16 * u, x, lane), w, dv[x]);
+          }
+        }
+        if constexpr (kDk) {
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            const f32x4 d4 = *(const f32x4 *)&deltas[B][f + row_of(r, half)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[r + e] *= __builtin_fmaf(dp[r + e], lowering, -d4[e] * lowering);
+          }
+          if (!whole) {  // (a zero weight times an infinite gradient)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if ((unsigned)(left + row_of(r, half)) >= (unsigned)seen.count) p[r] = 0.0f;
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const operand_t<T> ds = operand_of<T>(p, u);
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x) dk[x] = Operand<T>::product(G::columns(queries[B], f + 16 * u, x, lane), ds, dk[x]);
+          }
+        }
+      }
+      ++st;
+    };
+    while (st < end) {
+      turn(std::integral_constant<int, 0>());
+      if (st >= end) break;
+      turn(std::integral_constant<int, 1>());
+    }
+  }
+  const bool there = j < a.S;
+  const float v_factor = __is_same(T, f16_t) ? 1.0f / 4096.0f : 1.0f, k_factor = a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f);
+  if (shares > 1) {
+    // (rows of D floats, the shares of a tile behind each other)
+    const int64_t slot = part_slot(a, bk, at) * kQueries + wave * 32 + (lane & 31);
+    if constexpr (kDk) store_token<float, DP>(a.part_k + slot * a.D, a.D, dk, k_factor);
+    if constexpr (kDv) store_token<float, DP>(a.part_v + slot * a.D, a.D, dv, v_factor);
+    return;
+  }
+  if (there) {
+    if constexpr (kDk) store_token<T, DP>((T *)a.dk.row(b, j, kh), a.D, dk, k_factor);
+    if constexpr (kDv) store_token<T, DP>((T *)a.dv.row(b, j, kh), a.D, dv, v_factor);
+  }
+  bool bad_k = false, bad_v = false;
+  if constexpr (kDk) bad_k = any_not_finite(dk);
+  if constexpr (kDv) bad_v = any_not_finite(dv);
+  const bool counts = there && seen.count > 0;
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const bool bad = part ? bad_k : bad_v;
+    uint64_t rows = __ballot(either_half(bad) && counts) & 0xffffffffu;
+    while (rows) {
+      const int r = __builtin_ctzll(rows);
+      rows &= rows - 1;
+      dkv_again<T>(a, s, b, kh, tile * kQueries + wave * 32 + r, part == 1);
+    }
+  }
+}
+static_assert(kWeightBits == 12.0f, "the factors of 1 / 4096 and 1 / 128 undo it");
+
+// The shares' sums: a wavefront per row.
+template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kernel(const WindowArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  // rows of the tiles that were shared: the sinks', or all
+  const int shared_tiles = a.shares > 1 ? a.tiles : a.sink_tiles, skipped = a.sink_shares > 1 ? 0 : a.sink_tiles;
+  const int rows = (shared_tiles - skipped) * kQueries;
+  const int bk = (int)(id / rows), r = (int)(id % rows);
+  const int tile = skipped + r / kQueries, j = tile * kQueries + r % kQueries, b = bk / a.K, kh = bk % a.K;
+  if (bk >= a.B * a.K || j >= a.S) return;
+  const int shares = tile < a.sink_tiles ? a.sink_shares : a.shares;
+  const int first = tile < a.sink_tiles ? tile * a.sink_shares : a.sink_tiles * a.sink_shares + (tile - a.sink_tiles) * a.shares;
+  const int64_t slot = part_slot(a, bk, first) * kQueries + r % kQueries;
+  const Sample s = sample_of(a, b);
+  const Seen seen = seen_of(a, s, j);
+  float k[4] = {}, v[4] = {}, bad_k = 0.0f, bad_v = 0.0f;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int d = x * 64 + lane;
+    if (d < a.D) {
+      for (int n = 0; n < shares; ++n) {
+        const int64_t e = (slot + (int64_t)n * kQueries) * a.D + d;
+        k[x] += load_global<float>(a.part_k + e);
+        v[x] += load_global<float>(a.part_v + e);
+      }
+      bad_k = __builtin_fmaf(k[x], 0.0f, bad_k);
+      bad_v = __builtin_fmaf(v[x], 0.0f, bad_v);
+      const float tk[1] = {k[x]}, tv[1] = {v[x]};
+      LaneVec<T, 1>::store((T *)a.dk.row(b, j, kh) + d, LaneVec<T, 1>::pack(tk));
+      LaneVec<T, 1>::store((T *)a.dv.row(b, j, kh) + d, LaneVec<T, 1>::pack(tv));
+    }
+  }
+  if (seen.count > 0) {
+    if (__any(!(bad_v == 0.0f))) dkv_again<T>(a, s, b, kh, j, false);
+    if (__any(!(bad_k == 0.0f))) dkv_again<T>(a, s, b, kh, j, true);
+  }
+}
+
+}  // namespace gn

@@ -1,0 +1,44 @@
+// Host-side interface of the attention kernels: argument block and launchers (gn_window.hip, compiled once per element type;
+// the C ABI is in gn_attention.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+#include "../../include/gnnhwc_tokens.h"
+#include "gn_plan.h"
+
+namespace gn {
+
+constexpr int kQueries = 128;  // tokens of a workgroup's tile: 32 a wavefront
+
+// Rows of heads: strides in bytes.
+struct HeadRows {
+  const void *base;
+  int64_t batch_bytes, head_bytes;
+  int token_bytes;
+  __host__ __device__ __forceinline__ char *row(int b, int i, int h) const {
+    return (char *)const_cast<void *>(base) + (int64_t)b * batch_bytes + (int64_t)i * token_bytes + (int64_t)h * head_bytes;
+  }
+};
+struct WindowArgs {
+  HeadRows q, k, v, out, dout, dq, dk, dv;
+  float *lse, *delta, *largest, *part_k, *part_v;
+  const void *lengths;
+  int length_type, at_end;  // at_end: the queries are the last of a sample's own tokens, not of all S
+  int B, L, S, H, K, D, group;
+  int left, right, sinks, causal;
+  int tiles, items;                        // tiles of a head, workgroups with work
+  int sink_tiles, sink_shares, shares;     // dk / dv: tiles that hold sinks; workgroups that share a tile of those, of the others
+  int parts;                               // ... and of a head, those that leave sums for window_sum_kernel
+  float scale, scale_log2;
+};
+
+#define GN_DECLARE_WINDOW(S)                                                            \
+  hipError_t launch_window_forward_##S(const WindowArgs &a, hipStream_t stream);        \
+  hipError_t launch_window_backward_##S(const WindowArgs &a, const WindowArgs &kv, hipStream_t stream);
+GN_DECLARE_WINDOW(f32)
+GN_DECLARE_WINDOW(f16)
+GN_DECLARE_WINDOW(bf16)
+#undef GN_DECLARE_WINDOW
+
+}  // namespace gn

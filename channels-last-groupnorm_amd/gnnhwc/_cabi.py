@@ -54,6 +54,10 @@ SYMBOLS = (
     "gnnhwc_rotary_bwd",
     "gnnhwc_clip_workspace_bytes",
     "gnnhwc_clip",
+    "gnnhwc_window_workspace_bytes",
+    "gnnhwc_window",
+    "gnnhwc_window_bwd_workspace_bytes",
+    "gnnhwc_window_bwd",
 )
 
 
@@ -68,6 +72,18 @@ class RotaryCall(ctypes.Structure):
            ("position_stride", ctypes.c_int64 * 2), ("position_type", ctypes.c_int64)]
         + [(n, ctypes.c_void_p) for n in ("frequencies", "q_weight", "k_weight", "q_dweight", "k_dweight")]
         + [("eps", ctypes.c_double), ("dtype", ctypes.c_int64), ("param_dtype", ctypes.c_int64)]
+    )
+
+
+class WindowCall(ctypes.Structure):
+    """gnnhwc_window_call of include/gnnhwc_tokens.h."""
+
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "out_grad", "q_grad", "k_grad", "v_grad")]
+        + [(n + "_stride", ctypes.c_int64 * 3) for n in ("q", "k", "v", "out", "out_grad", "q_grad", "k_grad", "v_grad")]
+        + [(n, ctypes.c_int64) for n in ("batch", "tokens", "keys", "heads", "kv_heads", "head_dim", "window", "sinks", "causal")]
+        + [("lengths", ctypes.c_void_p), ("length_type", ctypes.c_int64), ("at_end", ctypes.c_int64), ("scale", ctypes.c_double),
+           ("dtype", ctypes.c_int64)]
     )
 
 
@@ -151,6 +167,12 @@ def _load():
     lib.gnnhwc_clip_workspace_bytes.restype = sz
     lib.gnnhwc_clip.argtypes = [vp, vp, vp, vp, vp, i64, dbl, dbl, dbl, vp, ci, vp, sz, vp]
     lib.gnnhwc_clip.restype = ci
+    window = ctypes.POINTER(WindowCall)
+    for name in ("gnnhwc_window", "gnnhwc_window_bwd"):
+        getattr(lib, name + "_workspace_bytes").argtypes = [window]
+        getattr(lib, name + "_workspace_bytes").restype = sz
+        getattr(lib, name).argtypes = [window, vp, sz, vp]
+        getattr(lib, name).restype = ci
     lib.gnnhwc_kernel_kind_name.argtypes = [ci]
     lib.gnnhwc_kernel_kind_name.restype = ctypes.c_char_p
     return lib

@@ -7,6 +7,8 @@
  *                      results in 8 bits with scales
  *   gnnhwc_rotary*     rotary positions with several axes on q and k, optionally behind a norm of each head
  *   gnnhwc_clip        the norm over many gradients and their clipping
+ *   gnnhwc_window_*    softmax attention in which a token sees a window around it and a few first tokens, forward, backward, and
+ *                      of the newest tokens against what a cache holds
  *
  * Conventions are those of gnnhwc.h: device pointers on the current device, asynchronous on `stream`, no synchronisation, no
  * allocation, a caller-provided workspace whose contents on entry are ignored (8-byte aligned is enough here), GNNHWC_OK or
@@ -120,6 +122,47 @@ size_t gnnhwc_clip_workspace_bytes(int64_t count);
 int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const int *dtype, const int *out_dtype,
                 int64_t count, double max_norm, double eps, double grad_scale, void *total, int total_dtype,
                 void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Softmax attention of `heads` query heads over `kv_heads` key heads (a divisor; head h goes with key head h / (heads / kv_heads)):
+ *   s_ij = scale q_i . k_j,   out_i = sum_j softmax_j(s_ij) v_j   over the keys j that query i sees.
+ * A sample has n keys: `keys`, or its entry of `lengths` (clamped to 0 .. keys).  Query i stands at place p = i + keys - tokens,
+ * or with `at_end` at i + n - tokens: the queries are the newest of the sample's own tokens.  It sees key j < n if
+ * |p - j| <= window or j < sinks, and, if `causal`, j <= p.  A query whose p is not among 0 .. n - 1, or that sees nothing, gets
+ * zeros; what lies behind n in k and v is not read, in q and out_grad has no effect, and gets zeros for gradients.  An infinity or a NaN reaches
+ * only the tokens that see it.
+ * Scores, softmax and sums are in float32; softmax weights (and in the backward their derivatives) are rounded to dtype
+ * once, as operands of the second product.  dtype: F32, F16 or BF16.
+ *   lse      : float (batch, heads, tokens): log2 of the softmax's sum, infinite for a query that sees nothing.  Written by the
+ *              forward unless NULL, read by the backward.
+ *   strides  : of batch, token and head in elements, each a whole multiple of 16 bytes (but for dimensions of size 1), as are the
+ *              addresses; a token's below 2^31 bytes.  Channels of a head are contiguous.
+ * Backward (not with at_end): reads q, k, v, out, out_grad and lse, writes q_grad, k_grad and v_grad.
+ * Outputs must not overlap inputs or each other.
+ */
+typedef struct gnnhwc_window_call {
+  const void *q, *k, *v;        /* (batch, tokens, heads, head_dim), (batch, keys, kv_heads, head_dim) twice */
+  void *out;                    /* like q; read by the backward */
+  float *lse;
+  const void *out_grad;
+  void *q_grad, *k_grad, *v_grad;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  int64_t out_grad_stride[3], q_grad_stride[3], k_grad_stride[3], v_grad_stride[3];
+  int64_t batch, tokens, keys, heads, kv_heads;
+  int64_t head_dim;             /* a multiple of 8, to 256 */
+  int64_t window;               /* -1: no bound */
+  int64_t sinks, causal;
+  const void *lengths;          /* batch values, or NULL */
+  int64_t length_type;          /* 0 int32, 1 int64 */
+  int64_t at_end;
+  double scale;                 /* positive */
+  int64_t dtype;
+} gnnhwc_window_call;
+
+size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *call);
+int gnnhwc_window(const gnnhwc_window_call *call, void *workspace, size_t workspace_bytes, void *stream);
+size_t gnnhwc_window_bwd_workspace_bytes(const gnnhwc_window_call *call);
+int gnnhwc_window_bwd(const gnnhwc_window_call *call, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

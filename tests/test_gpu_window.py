@@ -1,0 +1,189 @@
+"""GPU tests of window_attention against its formula in float64 (tests/window_refs.py has the bounds and where they come from)."""
+import math
+
+import pytest
+import torch
+
+from gnnhwc import window_attention
+from tests import window_refs as ref
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def normal(shape, dtype, device, seed, scale=1.0):
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    return (scale * torch.randn(shape, generator=g)).to(dtype).to(device)
+
+
+def run(dtype, device, B, L, S, H, K, D, window, sinks, causal, lengths=None, scale=None, seed=0, gain=1.0):
+    print("window_attention", dtype, B, L, S, H, K, D, window, sinks, causal, lengths, flush=True)
+    q, k, v = (normal((B, n, h, D), dtype, device, seed + i, g).requires_grad_(True)
+               for i, (n, h, g) in enumerate(((L, H, 1.5), (S, K, 1.0), (S, K, 1.0))))
+    dout = normal((B, L, H, D), dtype, device, seed + 3, gain)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=device)
+    out = window_attention(q, k, v, window, sinks, causal, n, scale)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, [q, k, v], dout)), out=out)
+    seen = ref.sees(B, L, S, window, sinks, causal, n, False, device)
+    want = ref.attention(q, k, v, seen, D ** -0.5 if scale is None else scale, dout)
+    for name in ("out", "dq", "dk", "dv"):
+        ref.check(got[name], want[name], "%s %s" % (name, dtype))
+    return q, k, v, dout, n, got
+
+
+# lengths around a tile's 32, 64 and 128 tokens, windows that end inside and at tiles, sinks inside and past the window
+SHAPES = [
+    (1, 1, 1, 1, 1, 8, None, 0, False), (2, 2, 2, 2, 1, 16, 0, 0, False), (1, 31, 31, 2, 2, 64, 3, 1, True), (2, 32, 32, 4, 2, 40, None, 0, True),
+    (1, 33, 33, 3, 1, 96, 5, 2, False), (1, 63, 64, 2, 1, 128, 16, 0, False), (2, 64, 64, 1, 1, 72, 64, 4, True), (1, 65, 130, 2, 2, 64, 40, 7, True),
+    (3, 127, 127, 2, 1, 24, 1, 0, False), (1, 128, 128, 6, 2, 128, 31, 33, False), (1, 129, 129, 2, 2, 80, None, 5, False),
+    (2, 200, 333, 4, 1, 64, 70, 65, False), (1, 257, 257, 2, 1, 64, 128, 1, True), (1, 300, 300, 5, 5, 128, 37, 300, True),
+    (1, 515, 515, 2, 1, 96, 100, 129, False), (2, 640, 640, 2, 2, 64, 63, 16, False), (1, 1030, 1030, 4, 2, 64, 200, 4, True),
+    (1, 700, 1500, 2, 1, 128, None, 0, True), (1, 130, 130, 2, 1, 160, 33, 3, False), (1, 200, 200, 2, 2, 256, None, 0, True),
+    (1, 70, 70, 1, 1, 248, 20, 2, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_backward(shape, dtype, device):
+    run(dtype, device, *shape)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [1, 4, 10, 66, 130])
+def test_heads_that_no_lane_vector_divides(D, dtype, device):
+    run(dtype, device, 2, 70, 70, 2, 1, D, 9, 2, False)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths", [[150, 0, 1], [64, 33, 149], [200, -5, 150]])
+@pytest.mark.parametrize("causal", [False, True])
+def test_padded_batches(lengths, causal, dtype, device):
+    """Padding holds NaN: it reaches nobody, and gets zeros."""
+    B, L, H, K, D = 3, 150, 4, 2, 64
+    q, k, v, dout = (normal((B, L, h, D), dtype, device, i) for i, h in enumerate((H, K, K, H)))
+    n = torch.tensor(lengths, device=device)
+    seen = ref.sees(B, L, L, 21, 3, causal, n, False, device)
+    want = ref.attention(q, k, v, seen, 0.2, dout)
+    for t in (q, k, v, dout):
+        for b, m in enumerate(lengths):
+            t[b, max(0, m):] = math.nan
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = window_attention(q, k, v, 21, 3, causal, n, 0.2)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, [q, k, v], dout)), out=out)
+    for name in ("out", "dq", "dk", "dv"):
+        ref.check(got[name], want[name], name)
+        for b, m in enumerate(lengths):
+            assert not got[name][b, max(0, m):].any(), name
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("causal", [False, True])
+def test_values_that_are_not_finite_reach_those_that_see_them(bad, causal, dtype, device):
+    """One token of q, k, v or the gradient is NaN or infinite: what does not see it is as without it."""
+    B, L, H, K, D, window, sinks, at = 1, 200, 2, 1, 64, 20, 3, 100
+    seen = ref.sees(B, L, L, window, sinks, causal, None, False, device)[0]
+    tensors = [normal((B, L, h, D), dtype, device, i) for i, h in enumerate((H, K, K, H))]
+    want = ref.attention(*tensors[:3], seen.unsqueeze(0), D ** -0.5, tensors[3])
+    by_key = seen[:, at]                         # queries that see the token
+    by_query = seen[at]                          # keys that the token sees
+    near = (seen[by_key].any(0))                 # keys that a query which sees it sees, too
+    alone = torch.arange(L, device=device) == at
+    touched = {  # tensor: rows of out, dq, dk, dv that may change
+        "q": (alone, alone, by_query, by_query), "k": (by_key, by_key, near | alone, near | alone), "v": (by_key, by_key, near | alone, alone),
+        "dout": (torch.zeros_like(alone), alone, by_query, by_query)}
+    for i, which in enumerate(("q", "k", "v", "dout")):
+        print(which, bad, causal, dtype, flush=True)
+        changed = [t.clone() for t in tensors]
+        changed[i][:, at, :, 5] = bad
+        q, k, v = (t.requires_grad_(True) for t in changed[:3])
+        out = window_attention(q, k, v, window, sinks, causal)
+        got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, [q, k, v], changed[3])), out=out)
+        for name, rows in zip(("out", "dq", "dk", "dv"), touched[which]):
+            ref.check(got[name][:, ~rows], tuple(t[:, ~rows] for t in want[name]), "%s with %s in %s" % (name, bad, which))
+        if which == "v":
+            assert not torch.isfinite(got["out"][:, by_key, :, 5]).any()
+
+
+@pytest.mark.parametrize("gain", [2.0 ** -20, 2.0 ** 12])
+def test_gradients_of_any_scale_in_half_precision(gain, device):
+    """float16 gradients of a scaled or an averaged loss: dS is held relative to the largest."""
+    q, k, v, dout, n, got = run(F16, device, 1, 300, 300, 2, 1, 64, None, 0, False, gain=gain, seed=5)
+    assert all(torch.isfinite(t).all() for t in got.values())
+
+
+def test_layouts(device):
+    """Slices of a packed projection, expanded, transposed and misaligned tensors give what their contiguous copies give."""
+    B, L, H, K, D = 2, 100, 4, 2, 64
+    qkv = normal((B, L, (H + 2 * K) * D), BF16, device, 1)
+    q, k, v = (t.unflatten(-1, (-1, D)) for t in qkv.split([H * D, K * D, K * D], dim=-1))
+    want = window_attention(q.contiguous(), k.contiguous(), v.contiguous(), 10, 2, True)
+    assert torch.equal(window_attention(q, k, v, 10, 2, True), want)
+    by_heads = tuple(t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v))
+    assert torch.equal(window_attention(*by_heads, 10, 2, True), want)
+    wide = tuple(torch.zeros((B, L, t.shape[2], D + 3), dtype=BF16, device=device) for t in (q, k, v))
+    odd = tuple(w[..., 1:1 + D] for w in wide)
+    for o, t in zip(odd, (q, k, v)):
+        o.copy_(t)
+    assert torch.equal(window_attention(*odd, 10, 2, True), want)
+    apart = tuple(torch.empty(t.shape[:-1] + (2 * D,), dtype=BF16, device=device)[..., ::2] for t in (q, k, v))
+    for o, t in zip(apart, (q, k, v)):
+        o.copy_(t)
+    assert torch.equal(window_attention(*apart, 10, 2, True), want)
+    one = k[:, :1].expand(B, L, K, D)
+    assert torch.equal(window_attention(q, one, one, 10, 2, True), window_attention(q, one.contiguous(), one.contiguous(), 10, 2, True))
+    # gradients through the slices, and an expanded gradient
+    qkv.requires_grad_(True)
+    q, k, v = (t.unflatten(-1, (-1, D)) for t in qkv.split([H * D, K * D, K * D], dim=-1))
+    g, = torch.autograd.grad(window_attention(q, k, v, 10, 2, True).sum(), qkv)
+    parts = [t.detach().contiguous().requires_grad_(True) for t in (q, k, v)]
+    each = torch.autograd.grad(window_attention(*parts, 10, 2, True), parts, torch.ones((B, L, H, D), dtype=BF16, device=device))
+    assert torch.equal(g, torch.cat([t.flatten(2) for t in each], dim=-1))
+
+
+def test_results_are_reproducible(device):
+    q, k, v, dout, n, first = run(BF16, device, 2, 400, 400, 4, 2, 64, 50, 5, False)
+    for _ in range(3):
+        out = window_attention(q, k, v, 50, 5, False, n)
+        again = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, [q, k, v], dout)), out=out)
+        assert all(torch.equal(first[name], again[name]) for name in first)
+
+
+def test_gradients_against_differences(device):
+    """Central differences of a float32 call along random directions: the difference of f over h = 2^-6 is off by h^2 f''' / 6
+    (about 2e-4 of |f'| here, where third derivatives are of f's size) and by 2 n u |f| / h of the sums."""
+    q, k, v = (normal((1, 40, h, 16), F32, device, i) for i, h in enumerate((2, 1, 1)))
+    dout = normal((1, 40, 2, 16), F32, device, 9).double()
+
+    def f(*t):
+        return float((window_attention(*t, 6, 2, False).double() * dout).sum())
+
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(window_attention(*leaves, 6, 2, False), leaves, dout.float())
+    h = 2.0 ** -6
+    for i in range(3):
+        d = normal(leaves[i].shape, F32, device, 20 + i)
+        d = d / d.norm()
+        up, down = [[t + s * h * d if j == i else t for j, t in enumerate((q, k, v))] for s in (1, -1)]
+        assert abs((f(*up) - f(*down)) / (2 * h) - float((grads[i].double() * d).sum())) < 2e-3 * float(grads[i].norm())
+
+
+def test_empty_batches(device):
+    for B, L, S in ((0, 5, 5), (2, 0, 0), (2, 0, 7)):
+        q, k, v = (torch.zeros((B, n, 2, 64), dtype=BF16, device=device, requires_grad=True) for n in (L, S, S))
+        out = window_attention(q, k, v, 4)
+        assert out.shape == q.shape
+        dq, dk, dv = torch.autograd.grad(out, [q, k, v], torch.zeros_like(out))
+        assert dq.shape == q.shape and dk.shape == k.shape and not dk.any() and not dv.any()
+
+
+def test_the_operator(device):
+    q, k, v = (normal((1, 20, h, 16), F32, device, i).requires_grad_(True) for i, h in enumerate((2, 1, 1)))
+    n = torch.tensor([18], device=device)
+    torch.library.opcheck(torch.ops.gnop.window_attention, (q, k, v, n, 4, 1, True, False, 0.25, True), test_utils=("test_schema", "test_faketensor"))
+    with pytest.raises(RuntimeError, match="once only"):
+        out = window_attention(q, k, v, 4)
+        g, = torch.autograd.grad(out.sum(), q, create_graph=True)
+        g.sum().backward()
