@@ -27,6 +27,11 @@ struct Entry {
   decltype(&gnnhwc_rotary_bwd) rotary_bwd;
   decltype(&gnnhwc_clip_workspace_bytes) clip_workspace_bytes;
   decltype(&gnnhwc_clip) clip;
+  decltype(&gnnhwc_window_workspace_bytes) window_workspace_bytes;
+  decltype(&gnnhwc_window) window;
+  decltype(&gnnhwc_window_bwd_workspace_bytes) window_bwd_workspace_bytes;
+  decltype(&gnnhwc_window_bwd) window_bwd;
+  decltype(&gnnhwc_dropout) dropout;
 } abi = {};
 
 void check(int rc, const char *what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, "): ", abi.last_error()); }
@@ -530,6 +535,244 @@ PyObject *clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- attention ----
+// Whether the kernels read t where it is: (B, tokens, heads, D) with contiguous channels, rows whole 16 bytes apart.
+bool rows16(const Tensor &t, const c10::Device &device, at::ScalarType type) {
+  if (!plain(t, device) || t.dim() != 4 || t.scalar_type() != type || t.numel() == 0 || t.stride(3) != 1 || (uintptr_t)t.data_ptr() % 16) return false;
+  const int64_t each = 16 / t.element_size();
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) != 1 && t.stride(i) % each) return false;
+  return t.size(1) == 1 || t.stride(1) * t.element_size() < (int64_t)1 << 31;
+}
+bool window_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lengths, gnnhwc_window_call &c) {
+  const c10::Device device = q.device();
+  const at::ScalarType type = q.scalar_type();
+  const int code = code_of(type);
+  if (code < 0 || code == GNNHWC_F64 || !rows16(q, device, type) || !rows16(k, device, type) || !rows16(v, device, type)) return false;
+  if (k.size(0) != q.size(0) || k.size(3) != q.size(3) || v.sizes() != k.sizes() || q.size(2) % k.size(2) || q.size(3) % 8 || q.size(3) > 256) return false;
+  if (lengths.defined()) {
+    if (!plain(lengths, device) || lengths.dim() != 1 || lengths.size(0) != q.size(0) || !lengths.is_contiguous()) return false;
+    if (lengths.scalar_type() != at::kInt && lengths.scalar_type() != at::kLong) return false;
+    c.lengths = lengths.data_ptr();
+    c.length_type = lengths.scalar_type() == at::kLong;
+  }
+  c.q = q.data_ptr();
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  put_strides(q, c.q_stride);
+  put_strides(k, c.k_stride);
+  put_strides(v, c.v_stride);
+  c.batch = q.size(0);
+  c.tokens = q.size(1);
+  c.keys = k.size(1);
+  c.heads = q.size(2);
+  c.kv_heads = k.size(2);
+  c.head_dim = q.size(3);
+  c.dtype = code;
+  return true;
+}
+void run_window(const Tensor &q, gnnhwc_window_call &c, bool want_lse, Tensor &out, Tensor &lse) {
+  const c10::DeviceGuard guard(q.device());
+  const at::AutoDispatchBelowADInplaceOrView below;
+  const OperatorRange range("gnop::window_attention");
+  out = fresh(q.sizes(), q.scalar_type(), q);
+  c.out = out.data_ptr();
+  put_strides(out, c.out_stride);
+  if (want_lse) {
+    lse = fresh({q.size(0), q.size(2), q.size(1)}, at::kFloat, q);
+    c.lse = (float *)lse.data_ptr();
+  }
+  const size_t bytes = abi.window_workspace_bytes(&c);
+  const Tensor ws = workspace(bytes, q, "gnop::window_attention");
+  check(abi.window(&c, ws.data_ptr(), bytes, stream_of(q)), "gnop::window_attention");
+}
+
+struct WindowNode : public torch::autograd::Function<WindowNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v,
+                                                const optional<Tensor> &lengths, gnnhwc_window_call *c) {
+    Tensor out, lse;
+    run_window(q, *c, true, out, lse);
+    ctx->save_for_backward({q, k, v, out, lse, defined(lengths)});
+    ctx->saved_data["window"] = c->window;
+    ctx->saved_data["sinks"] = c->sinks;
+    ctx->saved_data["causal"] = (bool)c->causal;
+    ctx->saved_data["scale"] = c->scale;
+    return {out};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor q = saved[0], k = saved[1], v = saved[2], out = saved[3], lse = saved[4], lengths = saved[5], dout = grads[0];
+    const c10::Device device = dout.device();
+    gnnhwc_window_call c = {};
+    c.window = ctx->saved_data["window"].toInt();
+    c.sinks = ctx->saved_data["sinks"].toInt();
+    c.causal = ctx->saved_data["causal"].toBool();
+    c.scale = ctx->saved_data["scale"].toDouble();
+    Tensor dq, dk, dv;
+    // (as for the norm: whatever is not plain goes through the operator)
+    if (at::GradMode::is_enabled() || !ordinary_dispatch() || !plain(q, device) || !window_call(q, k, v, lengths, c) ||
+        !rows16(dout, device, q.scalar_type()) || dout.sizes() != q.sizes() || !rows16(out, device, q.scalar_type()) || out.sizes() != q.sizes() ||
+        !plain(lse, device) || !lse.is_contiguous() || lse.scalar_type() != at::kFloat || lse.numel() != q.size(0) * q.size(1) * q.size(2)) {
+      using Signature = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                                           const optional<Tensor> &, int64_t, int64_t, bool, double);
+      const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnop::window_attention_bwd", "").typed<Signature>();
+      std::tie(dq, dk, dv) = op.call(dout, q, k, v, out, lse, lengths.defined() ? optional<Tensor>(lengths) : std::nullopt, c.window, c.sinks, c.causal, c.scale);
+    } else {
+      const c10::DeviceGuard guard(device);
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const OperatorRange range("gnop::window_attention_bwd");
+      dq = fresh(q.sizes(), q.scalar_type(), q);
+      dk = fresh(k.sizes(), k.scalar_type(), k);
+      dv = fresh(v.sizes(), v.scalar_type(), v);
+      c.out = out.data_ptr();
+      c.lse = (float *)lse.data_ptr();
+      c.out_grad = dout.data_ptr();
+      c.q_grad = dq.data_ptr();
+      c.k_grad = dk.data_ptr();
+      c.v_grad = dv.data_ptr();
+      put_strides(out, c.out_stride);
+      put_strides(dout, c.out_grad_stride);
+      put_strides(dq, c.q_grad_stride);
+      put_strides(dk, c.k_grad_stride);
+      put_strides(dv, c.v_grad_stride);
+      const size_t bytes = abi.window_bwd_workspace_bytes(&c);
+      const Tensor ws = workspace(bytes, q, "gnop::window_attention_bwd");
+      check(abi.window_bwd(&c, ws.data_ptr(), bytes, stream_of(q)), "gnop::window_attention_bwd");
+    }
+    return {dq, dk, dv, Tensor(), Tensor()};
+  }
+};
+
+// A Python integer that is exactly one and not negative, or false.
+bool whole_number(PyObject *o, int64_t &v) {
+  if (!PyLong_CheckExact(o)) return false;
+  v = PyLong_AsLongLong(o);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return v >= 0;
+}
+
+// window_attention(q, k, v, lengths, window or None, sinks, causal, at_end, scale or None) -> out or NotImplemented
+PyObject *window_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(nargs == 9, "window_attention takes 9 arguments");
+  optional<Tensor> q_, k_, v_, lengths_;
+  if (!tensor_or_none(args[0], q_) || !q_.has_value() || !ordinary_thread() || !tensor_or_none(args[1], k_) || !k_.has_value() ||
+      !tensor_or_none(args[2], v_) || !v_.has_value() || !tensor_or_none(args[3], lengths_) || !PyBool_Check(args[6]) || !PyBool_Check(args[7]))
+    return decline();
+  const Tensor q = *q_, k = *k_, v = *v_, lengths = defined(lengths_);
+  gnnhwc_window_call c = {};
+  c.window = -1;
+  if (args[4] != Py_None && !whole_number(args[4], c.window)) return decline();
+  if (!whole_number(args[5], c.sinks) || !window_call(q, k, v, lengths, c)) return decline();
+  c.causal = args[6] == Py_True;
+  c.at_end = args[7] == Py_True;
+  c.scale = 1.0 / std::sqrt((double)c.head_dim);
+  if (args[8] != Py_None) {
+    if (!PyFloat_CheckExact(args[8])) return decline();
+    c.scale = PyFloat_AS_DOUBLE(args[8]);
+  }
+  const bool differentiates = wants_grad({q, k, v});
+  // (sizes that the library may refuse: the general form says why)
+  if (!(c.scale > 1e-30 && c.scale < 1e30) || (!c.at_end && c.tokens > c.keys) || (c.at_end && differentiates) || c.keys > (1 << 30) || c.tokens > (1 << 30) ||
+      c.heads > 65535 || c.batch * c.heads * (c.tokens / 128 + 1) > 1 << 22)
+    return decline();
+  Tensor out, lse;
+  {
+    const WithoutGil released;
+    if (differentiates) out = WindowNode::apply(q, k, v, lengths_, &c)[0];
+    else run_window(q, c, false, out, lse);
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- dropout ----
+struct DropoutCall {
+  double p = 0;
+  uint64_t seed = 0, offset = 0;
+  Tensor seed_at;  // possibly undefined
+};
+Tensor run_dropout(const Tensor &x, const Tensor &residual, const DropoutCall &c) {
+  const c10::DeviceGuard guard(x.device());
+  const at::AutoDispatchBelowADInplaceOrView below;
+  const OperatorRange range("gnop::dropout");
+  Tensor y = fresh(x.sizes(), x.scalar_type(), x);
+  check(abi.dropout(x.data_ptr(), ptr(residual), y.data_ptr(), x.numel(), c.p, c.seed, (const int64_t *)ptr(c.seed_at), c.offset,
+                    code_of(x.scalar_type()), stream_of(x)),
+        "gnop::dropout");
+  return y;
+}
+struct DropoutNode : public torch::autograd::Function<DropoutNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const optional<Tensor> &residual,
+                                                const DropoutCall *c) {
+    ctx->save_for_backward({c->seed_at});
+    ctx->saved_data["p"] = c->p;
+    ctx->saved_data["seed"] = (int64_t)c->seed;
+    ctx->saved_data["offset"] = (int64_t)c->offset;
+    ctx->saved_data["residual"] = residual.has_value();
+    return {run_dropout(x, defined(residual), *c)};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    const Tensor dy = grads[0];
+    const bool residual = ctx->saved_data["residual"].toBool();
+    DropoutCall c;
+    c.p = ctx->saved_data["p"].toDouble();
+    c.seed = (uint64_t)ctx->saved_data["seed"].toInt();
+    c.offset = (uint64_t)ctx->saved_data["offset"].toInt();
+    c.seed_at = ctx->get_saved_variables()[0];
+    Tensor dx;
+    if (ctx->needs_input_grad(0)) {
+      if (at::GradMode::is_enabled() || !ordinary_dispatch() || !plain(dy, dy.device()) || !dy.is_contiguous() || dy.numel() == 0 ||
+          code_of(dy.scalar_type()) < 0) {
+        using Signature = Tensor(const Tensor &, const optional<Tensor> &, double, int64_t, const optional<Tensor> &, int64_t);
+        const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnop::dropout", "").typed<Signature>();
+        dx = op.call(dy, std::nullopt, c.p, (int64_t)c.seed, c.seed_at.defined() ? optional<Tensor>(c.seed_at) : std::nullopt, (int64_t)c.offset);
+      } else {
+        dx = run_dropout(dy, Tensor(), c);
+      }
+    }
+    return {dx, residual ? dy : Tensor(), Tensor()};
+  }
+};
+
+// dropout(x, residual, p, seed (integer of 64 bits or tensor), offset) -> y or NotImplemented
+PyObject *dropout(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(nargs == 5, "dropout takes 5 arguments");
+  optional<Tensor> x_, residual_;
+  DropoutCall c;
+  if (!tensor_or_none(args[0], x_) || !x_.has_value() || !ordinary_thread() || !tensor_or_none(args[1], residual_) || !PyFloat_CheckExact(args[2]))
+    return decline();
+  const Tensor x = *x_, residual = defined(residual_);
+  const auto fits = [&](const Tensor &t) {
+    return plain(t, x.device()) && t.is_contiguous() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes();
+  };
+  if (code_of(x.scalar_type()) < 0 || !fits(x) || x.numel() == 0 || x.numel() > (int64_t)1 << 34 || (residual.defined() && !fits(residual))) return decline();
+  c.p = PyFloat_AS_DOUBLE(args[2]);
+  int64_t seed = 0, offset = 0;
+  if (!(c.p >= 0 && c.p <= 1) || !whole_number(args[4], offset)) return decline();
+  if (!whole_number(args[3], seed)) {
+    optional<Tensor> seed_at;
+    if (args[3] == Py_None || !tensor_or_none(args[3], seed_at)) return decline();
+    if (!plain(*seed_at, x.device()) || seed_at->scalar_type() != at::kLong || seed_at->numel() != 1) return decline();
+    c.seed_at = *seed_at;
+    seed = 0;
+  }
+  c.seed = (uint64_t)seed;
+  c.offset = (uint64_t)offset;
+  Tensor y;
+  {
+    const WithoutGil released;
+    if (wants_grad({x, residual})) y = DropoutNode::apply(x, residual_, &c)[0];
+    else y = run_dropout(x, residual, c);
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind_tokens(address, ...): the C ABI's functions in the order of Entry.
 PyObject *bind_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   void **slot = reinterpret_cast<void **>(&abi);
@@ -557,6 +800,9 @@ PyMethodDef methods[] = {
      "rotary(q, k, positions, frequencies, sections, interleaved, q_weight, k_weight, eps) -> q', (q', k') or NotImplemented"},
     {"clip_gradients", (PyCFunction)(void (*)(void))clip_gradients, METH_FASTCALL,
      "clip_gradients(grads, max_norm, out, grad_scale, eps) -> total or NotImplemented"},
+    {"window_attention", (PyCFunction)(void (*)(void))window_attention, METH_FASTCALL,
+     "window_attention(q, k, v, lengths, window, sinks, causal, at_end, scale) -> out or NotImplemented"},
+    {"dropout", (PyCFunction)(void (*)(void))dropout, METH_FASTCALL, "dropout(x, residual, p, seed, offset) -> y or NotImplemented"},
     {"bind_tokens", (PyCFunction)(void (*)(void))bind_tokens, METH_FASTCALL, "bind_tokens(*addresses): the C ABI's entry points"},
     {nullptr, nullptr, 0, nullptr}};
 

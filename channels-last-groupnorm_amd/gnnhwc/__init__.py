@@ -4,3 +4,4 @@ from .custom_gn import GN_NCHW_Func  # noqa: F401  (channels-first input; the re
 # operators for token streams (no counterparts in the reference)
 from .tokens import RMSNorm, Rotary, clip_grad_norm_, clip_gradients, rms_norm, rms_norm_quant, rotary, rotary_frequencies  # noqa: F401
 from .attention import window_attention, window_attention_cached  # noqa: F401
+from .dropout import Dropout, dropout  # noqa: F401

@@ -58,6 +58,7 @@ SYMBOLS = (
     "gnnhwc_window",
     "gnnhwc_window_bwd_workspace_bytes",
     "gnnhwc_window_bwd",
+    "gnnhwc_dropout",
 )
 
 
@@ -173,6 +174,8 @@ def _load():
         getattr(lib, name + "_workspace_bytes").restype = sz
         getattr(lib, name).argtypes = [window, vp, sz, vp]
         getattr(lib, name).restype = ci
+    lib.gnnhwc_dropout.argtypes = [vp, vp, vp, i64, dbl, ctypes.c_uint64, vp, ctypes.c_uint64, ci, vp]
+    lib.gnnhwc_dropout.restype = ci
     lib.gnnhwc_kernel_kind_name.argtypes = [ci]
     lib.gnnhwc_kernel_kind_name.restype = ctypes.c_char_p
     return lib
@@ -188,7 +191,8 @@ NATIVE_ENTRY_POINTS = ("last_error", "fwd_workspace_bytes", "bwd_workspace_bytes
                        "fwd_add", "fwd_nchw", "bwd_nchw")
 _native.bind(*[ctypes.cast(getattr(lib, "gnnhwc_" + name), ctypes.c_void_p).value for name in NATIVE_ENTRY_POINTS])
 TOKEN_ENTRY_POINTS = ("last_error", "rms_fwd", "rms_fwd_quant", "rms_bwd_workspace_bytes", "rms_bwd", "rotary", "rotary_bwd_workspace_bytes",
-                      "rotary_bwd", "clip_workspace_bytes", "clip")
+                      "rotary_bwd", "clip_workspace_bytes", "clip", "window_workspace_bytes", "window", "window_bwd_workspace_bytes", "window_bwd",
+                      "dropout")
 _native.bind_tokens(*[ctypes.cast(getattr(lib, "gnnhwc_" + name), ctypes.c_void_p).value for name in TOKEN_ENTRY_POINTS])
 
 

@@ -12,7 +12,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import _cabi
+from . import _cabi, _native
 from .custom_gn import _check_device, _current_stream_ptr, _DTYPE_CODE, _on_device, _op_lib, _workspace
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -202,6 +202,10 @@ def window_attention(q, k, v, window=None, sinks=0, causal=False, lengths=None, 
     throughout.  An infinity or a NaN in a token reaches only those that see it.  Slices of one packed projection are read where
     they are; rows that are not whole 16 bytes apart are copied first.  Differentiable once in q, k and v; results and gradients
     are the same bit for bit on every run."""
+    if not torch.compiler.is_compiling():
+        out = _native.window_attention(q, k, v, lengths, window, sinks, causal, False, scale)
+        if out is not NotImplemented:
+            return out
     return _attend(q, k, v, lengths, window, sinks, causal, False, scale)
 
 
@@ -211,4 +215,8 @@ def window_attention_cached(q, k_cache, v_cache, lengths, window=None, sinks=0, 
     q: (B, T, heads, D), k_cache, v_cache: (B, S, kv_heads, D) with room for S tokens, lengths: (B,) int32 or int64, tokens of each
     request that its cache holds (clamped to 0 .. S), the T of q, which are the last of them, included.  What a cache holds behind
     its length has no effect.  A request shorter than T has zeros in front.  It has no derivative."""
+    if not torch.compiler.is_compiling():
+        out = _native.window_attention(q, k_cache, v_cache, lengths, window, sinks, True, True, scale)
+        if out is not NotImplemented:
+            return out
     return _attend(q, k_cache, v_cache, lengths, window, sinks, True, True, scale)

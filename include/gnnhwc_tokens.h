@@ -9,6 +9,7 @@
  *   gnnhwc_clip        the norm over many gradients and their clipping
  *   gnnhwc_window_*    softmax attention in which a token sees a window around it and a few first tokens, forward, backward, and
  *                      of the newest tokens against what a cache holds
+ *   gnnhwc_dropout     dropout from a counter-based generator, with the residual's addition
  *
  * Conventions are those of gnnhwc.h: device pointers on the current device, asynchronous on `stream`, no synchronisation, no
  * allocation, a caller-provided workspace whose contents on entry are ignored (8-byte aligned is enough here), GNNHWC_OK or
@@ -163,6 +164,18 @@ size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *call);
 int gnnhwc_window(const gnnhwc_window_call *call, void *workspace, size_t workspace_bytes, void *stream);
 size_t gnnhwc_window_bwd_workspace_bytes(const gnnhwc_window_call *call);
 int gnnhwc_window_bwd(const gnnhwc_window_call *call, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Dropout:  y[e] = (kept ? x[e] / (1 - p') : 0) + residual[e],  rounded once, for e in 0 .. n - 1.
+ * p' is p in whole multiples of 2^-16, rounded to nearest.  Element e is kept if its 16 random bits are at least 65536 p': they are
+ * half e % 2 (the lower first) of word (e / 2) % 4 of Philox 4x32 with 7 rounds, whose counter is (e / 8, offset), both 64 bits, the
+ * lower word first, and whose key is the seed.  The same seed and offset give the same bits: the backward is this call on the gradient, without a
+ * residual.  What is dropped has no effect, an infinity or a NaN neither.
+ *   residual : NULL for none.    y : may be x, or residual.
+ *   seed_at  : device memory that holds the seed when the kernel runs (so that a captured graph's replays differ), or NULL.
+ */
+int gnnhwc_dropout(const void *x, const void *residual, void *y, int64_t n, double p, uint64_t seed, const int64_t *seed_at,
+                   uint64_t offset, int dtype, void *stream);
 
 #ifdef __cplusplus
 }
