@@ -11,6 +11,7 @@ namespace gn {
 namespace {
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;
+constexpr int64_t kFewRows = 128, kFewItems = 512, kFewSteps = 8;
 constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
 
 int invalid(const char *what) { return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s", what); }
@@ -43,7 +44,8 @@ int put_rows(HeadRows &r, const void *base, const int64_t (&stride)[3], int64_t 
 
 struct WindowPlan {
   WindowArgs a, kv;  // queries' tiles, keys' tiles
-  bool empty;
+  bool empty, few;  // few: 32 rows of a key head at a time, see window_few_kernel
+  size_t join;      // forward's workspace: references and sums first
   size_t delta, largest, part_k, part_v, bytes;  // backward's workspace
 };
 
@@ -92,7 +94,24 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   if (items > kMostItems || (int64_t)a.H * a.B > kMostItems) return invalid("too many tokens and heads for one call");
   a.items = (int)items;
   p.empty = items == 0;
-  if (!backward) return GNNHWC_OK;
+  if (!backward) {
+    const int64_t few_rows = (int64_t)a.L * a.group;
+    p.few = few_rows <= kFewRows;
+    p.bytes = 256;
+    if (p.few && !p.empty) {
+      a.tiles = (int)ceil_div(few_rows, 32);
+      const int64_t heads = (int64_t)a.B * a.K * a.tiles;
+      // keys that a tile's rows see at most, in tiles of 32; a share is four or more of them
+      const int64_t seen = std::min<int64_t>(a.S, (int64_t)a.left + a.right + a.L + a.sinks + 64), steps = ceil_div(seen, 32);
+      a.splits = (int)std::clamp<int64_t>(ceil_div(kFewItems, heads), 1, std::min<int64_t>(64, std::max<int64_t>(1, steps / kFewSteps)));
+      a.items = (int)(heads * a.splits);
+      if (a.splits > 1) {
+        p.join = round_up((size_t)a.items * 32 * 2 * sizeof(float));
+        p.bytes += p.join + (size_t)a.items * 32 * a.D * sizeof(float);
+      }
+    }
+    return GNNHWC_OK;
+  }
 
   // Workgroups of dk and dv.  A key that all queries see (a sink) has many times the others' work, and a short batch has fewer tiles
   // than the device has room for: several workgroups then share a tile's queries.
@@ -132,15 +151,22 @@ extern "C" {
 size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *c) {
   WindowPlan p;
   if (plan_window(c, false, p)) return 0;
-  return 256;
+  return p.bytes;
 }
 
 int gnnhwc_window(const gnnhwc_window_call *c, void *workspace, size_t workspace_bytes, void *stream) {
   WindowPlan p;
   if (const int rc = plan_window(c, false, p)) return rc;
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < 256)
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes)
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_workspace_bytes");
   if (p.empty) return GNNHWC_OK;
+  if (p.few) {
+    p.a.part_k = (float *)workspace;
+    p.a.part_v = (float *)((char *)workspace + p.join);
+#define GN_CALL(S) launch_window_few_##S(p.a, (hipStream_t)stream)
+    return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window");
+#undef GN_CALL
+  }
 #define GN_CALL(S) launch_window_forward_##S(p.a, (hipStream_t)stream)
   return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window");
 #undef GN_CALL

@@ -551,6 +551,180 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2
   }
 }
 
+// ---- forward of few queries: the newest tokens of requests ----
+// Rows (tokens times the heads of a group) fill one tile of 32, and the keys are what takes time: a workgroup is as many wavefronts
+// as have room for two tiles of 32 keys and values each, every one walks keys of its own, and what they found is joined at the end.
+// No barrier on the way: a wavefront waits for its own copies only.  Where there are fewer heads than the device has room for,
+// several workgroups share a head's keys (splits) and window_join_kernel joins them.
+template <typename T, int DP> struct Few {
+  static constexpr int kStage = 2 * 32 * DP * (int)sizeof(T);  // bytes of a tile of keys and one of values
+  static constexpr int kMost = 131072 / (2 * kStage);
+  static constexpr int kWaves = kMost >= 8 ? 8 : kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
+  static constexpr int kCopies = Tile<T, DP>::kChunks / 2;  // of a wavefront, for each of the two tiles
+  static constexpr int kPitch = DP + 4;                     // floats of a row while results are joined
+  static_assert(32 * kPitch * 4 <= 2 * kStage, "a wavefront's results fit its tiles");
+};
+template <int COPIES> __device__ __forceinline__ void wait_for_copies(bool newest_too) {
+  if (newest_too) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES < 63 ? COPIES : 63) : "memory");
+}
+
+// Weight and result of a row that is joined of parts: (reference, sum).
+__device__ __forceinline__ float part_weight(float reference, float most) { return most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(reference - most); }
+
+template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void window_few_kernel(const WindowArgs a) {
+  using G = Tile<T, DP>;
+  using W = Few<T, DP>;
+  constexpr int kWaves = W::kWaves;
+  __shared__ __attribute__((aligned(16))) char tiles[kWaves][2][W::kStage];
+  __shared__ float references[kWaves][32], sums[kWaves][32];
+  __shared__ int bad[32];
+  const int item = work_item(a.items);
+  if (item >= a.items) return;
+  const int split = item % a.splits, rest = item / a.splits, block = rest % a.tiles, bk = rest / a.tiles;
+  const int b = bk / a.K, kh = bk % a.K;
+  const Sample s = sample_of(a, b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int rows = a.L * a.group, row = block * 32 + (lane & 31), i = row < rows ? row / a.group : a.L, h = kh * a.group + row % a.group;
+  ForwardState<T, DP> st;
+  st.sight = sight_of(a, s, i);
+  st.reference = -INFINITY;
+  st.sum = 0.0f;
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x) st.o[x] = zeros16();
+  int from = block * 32 / a.group, to = (block * 32 + 31) / a.group + 1;
+  from = from > s.first ? from : s.first;
+  to = to < s.last ? to : s.last;
+  if (from < to) {
+    const int ic = i < from ? from : i < to ? i : to - 1;
+    load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
+    const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, 32);
+    const int window = w.last >= w.first ? w.last - w.first + 1 : 0, steps = w.sinks + window;
+    const int begin = (int)((int64_t)steps * split / a.splits), end = (int)((int64_t)steps * (split + 1) / a.splits);
+    const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
+    auto tile_at = [&](int u) { return u < w.sinks ? u : w.first + (u - w.sinks); };
+    auto issue = [&](int u, char *to_tile) {
+      const int first = tile_at(u) * 32;
+#pragma unroll
+      for (int n = 0; n < W::kCopies; ++n) {
+        const int slot = n * 64 + lane, r = slot / G::kChunks;
+        int c = G::chunk_of(r, slot % G::kChunks) * 16;
+        c = c < a.D * (int)sizeof(T) ? c : 0;
+        const int j = first + r < s.n ? first + r : s.n - 1;
+        copy_to_lds<16>(kb + (int64_t)j * a.k.token_bytes + c, to_tile + n * 1024);
+        copy_to_lds<16>(vb + (int64_t)j * a.v.token_bytes + c, to_tile + W::kStage / 2 + n * 1024);
+      }
+    };
+    int u = begin + wave;
+    if (u < end) issue(u, tiles[wave][0]);
+    int turn = 0;
+    for (; u < end; u += kWaves) {
+      char *tile = tiles[wave][turn];
+      turn ^= 1;
+      const bool more = u + kWaves < end;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (reads of the tile that is now overwritten)
+      if (more) issue(u + kWaves, tiles[wave][turn]);
+      wait_for_copies<2 * W::kCopies>(!more);
+      forward_tile<T, DP>(st, tile, tile + W::kStage / 2, 0, tile_at(u) * 32, a.scale_log2);
+    }
+  }
+  // join the wavefronts
+  st.sum += other_half(st.sum);
+  if (lane < 32) {
+    references[wave][lane] = st.reference;
+    sums[wave][lane] = st.sum;
+    if (wave == 0) bad[lane] = 0;
+  }
+  __syncthreads();
+  float most = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int n = 0; n < kWaves; ++n) most = fmaxf(most, references[n][lane & 31]);
+#pragma unroll
+  for (int n = 0; n < kWaves; ++n) sum += sums[n][lane & 31] * part_weight(references[n][lane & 31], most);
+  const float weight = part_weight(st.reference, most);
+  float *mine = (float *)tiles[wave];
+  const int half = lane >> 5;
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *(f32x4 *)(mine + (lane & 31) * W::kPitch + 32 * x + row_of(r, half)) =
+          f32x4{st.o[x][r] * weight, st.o[x][r + 1] * weight, st.o[x][r + 2] * weight, st.o[x][r + 3] * weight};
+  __syncthreads();  // (also: all have read references and sums)
+  if (wave == 0 && lane < 32) {
+    references[0][lane] = most;
+    sums[0][lane] = sum;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 32 * DP / 4; e += 64 * kWaves) {
+    const int r = e / (DP / 4), d = e % (DP / 4) * 4, rr = block * 32 + r;
+    if (rr >= rows || d >= a.D) continue;
+    f32x4 v = *(const f32x4 *)((const float *)tiles[0] + r * W::kPitch + d);
+#pragma unroll
+    for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)tiles[n] + r * W::kPitch + d);
+    if (a.splits > 1) {
+      store_global<f32x4>(a.part_v + ((int64_t)item * 32 + r) * a.D + d, v);
+      continue;
+    }
+    const float total = sums[0][r], factor = total > 0.0f ? 1.0f / total : 0.0f;
+    const float t[4] = {v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor};
+    if (!(v[0] * 0.0f + v[1] * 0.0f + v[2] * 0.0f + v[3] * 0.0f + factor * 0.0f == 0.0f) || !(total > 0.0f)) bad[r] = 1;
+    using LV = LaneVec<T, 4>;
+    LV::store((T *)a.out.row(b, rr / a.group, kh * a.group + rr % a.group) + d, LV::pack(t));
+  }
+  if (a.splits > 1) {
+    if (threadIdx.x < 32) {
+      float *p = a.part_k + ((int64_t)item * 32 + threadIdx.x) * 2;
+      store_global<float>(p, references[0][threadIdx.x]);
+      store_global<float>(p + 1, sums[0][threadIdx.x]);
+    }
+    return;
+  }
+  __syncthreads();
+  for (int r = wave; r < 32; r += kWaves) {
+    const int rr = block * 32 + r;
+    if (rr >= rows) break;
+    const int ir = rr / a.group, hr = kh * a.group + rr % a.group;
+    const Sight g = sight_of(a, s, ir);
+    if (a.lse && lane == 0)
+      store_global<float>(a.lse + ((int64_t)b * a.H + hr) * a.L + ir, sums[0][r] > 0.0f ? references[0][r] + __builtin_amdgcn_logf(sums[0][r]) : INFINITY);
+    if (bad[r] && (g.count > 0 || g.sinks > 0)) row_again<T>(a, s, b, hr, ir);
+  }
+}
+
+// Rows that several workgroups share: a wavefront each.
+template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kernel(const WindowArgs a) {
+  const int lane = threadIdx.x & 63, rows = a.L * a.group;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t bk64 = id / rows;
+  if (bk64 >= (int64_t)a.B * a.K) return;
+  const int bk = (int)bk64, row = (int)(id % rows), b = bk / a.K, kh = bk % a.K, i = row / a.group, h = kh * a.group + row % a.group;
+  const int64_t slot = (((int64_t)bk * a.tiles + row / 32) * a.splits) * 32 + row % 32;
+  // (a lane holds a split's reference and sum: at most 64 splits)
+  const float reference = lane < a.splits ? load_global<float>(a.part_k + (slot + lane * 32) * 2) : -INFINITY;
+  const float part = lane < a.splits ? load_global<float>(a.part_k + (slot + lane * 32) * 2 + 1) : 0.0f;
+  const float most = wave_max(reference), weight = part_weight(reference, most), sum = wave_sum(part * weight);
+  float o[4] = {}, bad = 0.0f;
+  for (int n = 0; n < a.splits; ++n) {
+    const float w = __shfl(weight, n);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (x * 64 + lane < a.D) o[x] = __builtin_fmaf(w, load_global<float>(a.part_v + (slot + (int64_t)n * 32) * a.D + x * 64 + lane), o[x]);
+  }
+  const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (x * 64 + lane < a.D) {
+      bad = __builtin_fmaf(o[x] * factor, 0.0f, bad);
+      const float t[1] = {o[x] * factor};
+      LaneVec<T, 1>::store((T *)a.out.row(b, i, h) + x * 64 + lane, LaneVec<T, 1>::pack(t));
+    }
+  if (a.lse && lane == 0) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, sum > 0.0f ? most + __builtin_amdgcn_logf(sum) : INFINITY);
+  const Sample s = sample_of(a, b);
+  const Sight g = sight_of(a, s, i);
+  if ((__any(!(bad == 0.0f)) || !(sum > 0.0f)) && (g.count > 0 || g.sinks > 0)) row_again<T>(a, s, b, h, i);
+}
+
 // ---- backward: dq ----
 // delta and the largest |do| of a row go to the workspace for the other kernel.
 // float16 holds 2^-24 to 65504: weights and dS are kept in its middle by powers of two, weights as 2^12 P, dS relative to the

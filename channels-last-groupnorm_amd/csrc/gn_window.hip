@@ -40,6 +40,18 @@ hipError_t GN_CAT(launch_window_forward_, GN_SUFFIX)(const WindowArgs &a, hipStr
   return hipGetLastError();
 }
 
+hipError_t GN_CAT(launch_window_few_, GN_SUFFIX)(const WindowArgs &a, hipStream_t stream) {
+  with_width(a.D, [&](auto w) {
+    constexpr int DP = decltype(w)::value;
+    hipLaunchKernelGGL((window_few_kernel<elem_t, DP>), grid_of(a.items), dim3(64 * Few<elem_t, DP>::kWaves), 0, stream, a);
+  });
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.B * a.H * a.L;
+    hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)((rows + 3) / 4)), dim3(kBlock), 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
 hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const WindowArgs &kv, hipStream_t stream) {
   with_width(a.D, [&](auto w) {
     constexpr int DP = decltype(w)::value;

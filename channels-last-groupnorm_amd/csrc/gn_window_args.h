@@ -29,12 +29,14 @@ struct WindowArgs {
   int left, right, sinks, causal;
   int tiles, items;                        // tiles of a head, workgroups with work
   int sink_tiles, sink_shares, shares;     // dk / dv: tiles that hold sinks; workgroups that share a tile of those, of the others
+  int splits;                              // few queries: workgroups that share a head's keys
   int parts;                               // ... and of a head, those that leave sums for window_sum_kernel
   float scale, scale_log2;
 };
 
 #define GN_DECLARE_WINDOW(S)                                                            \
   hipError_t launch_window_forward_##S(const WindowArgs &a, hipStream_t stream);        \
+  hipError_t launch_window_few_##S(const WindowArgs &a, hipStream_t stream);            \
   hipError_t launch_window_backward_##S(const WindowArgs &a, const WindowArgs &kv, hipStream_t stream);
 GN_DECLARE_WINDOW(f32)
 GN_DECLARE_WINDOW(f16)
