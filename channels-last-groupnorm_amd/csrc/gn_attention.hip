@@ -34,7 +34,7 @@ int put_rows(HeadRows &r, const void *base, const int64_t (&stride)[3], int64_t 
     if (bytes[i] % 16) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s: its strides must be whole multiples of 16 bytes", name);
   }
   if ((uintptr_t)base % 16) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s must be aligned to 16 bytes", name);
-  if (bytes[1] > 0x7fffffff) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s: a token's stride must be below 2^31 bytes", name);
+  if (bytes[1] >= (int64_t)1 << 25) return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s: a token's stride must be below 2^25 bytes", name);
   r.base = base;
   r.batch_bytes = bytes[0];
   r.token_bytes = (int)bytes[1];

@@ -542,7 +542,7 @@ bool rows16(const Tensor &t, const c10::Device &device, at::ScalarType type) {
   const int64_t each = 16 / t.element_size();
   for (int i = 0; i < 3; ++i)
     if (t.size(i) != 1 && t.stride(i) % each) return false;
-  return t.size(1) == 1 || t.stride(1) * t.element_size() < (int64_t)1 << 31;
+  return t.size(1) == 1 || t.stride(1) * t.element_size() < (int64_t)1 << 25;
 }
 bool window_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lengths, gnnhwc_window_call &c) {
   const c10::Device device = q.device();

@@ -14,6 +14,7 @@
 // travels while this one is multiplied.  A row of a tile is cut into chunks of 16 bytes whose order depends on the row
 // (chunk_of), so that rows read side by side lie in different banks.
 #pragma once
+#include <type_traits>
 #include "gn_device.h"
 #include "gn_window_args.h"
 
@@ -86,8 +87,6 @@ template <typename T, int DP> struct Tile {
   static constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
   static constexpr int kChunks = DP * (int)sizeof(T) / 16;  // of a row
   static constexpr int kBytes = kRows * kChunks * 16;
-  static constexpr int kCopies = kRows * kChunks / kBlock;  // chunks that each thread of a workgroup copies
-  static_assert(kRows * kChunks % kBlock == 0 && kChunks % 4 == 0, "a tile is copied by whole workgroups");
 
   // Place of chunk c in its row: four neighbouring rows lie in different quarters of the 64 banks, which suits the transposing
   // reads of four rows, and sixteen in different places, which suits the reads of a chunk of many rows.
@@ -96,73 +95,116 @@ template <typename T, int DP> struct Tile {
     else if constexpr (kChunks % 8 == 0) return c ^ ((row >> 1 & 1) << 2 | (row >> 2 & 3));
     else return c ^ (row >> 2 & 3);
   }
-  // Operand whose rows are the tile's, summands 16 s + 8 h ..
-  static __device__ __forceinline__ operand_t<T> rows(const char *tile, int first, int s, int lane) {
-    const int row = first + (lane & 31), h = lane >> 5;
-    const char *at = tile + row * (kChunks * 16);
+};
+
+// Where a lane finds its operands in a tile, the same for every tile and every 32 (columns: 16) rows of it: offsets that a constant
+// is added to.  (The bits that a chunk's number and the row's pattern have are xor-ed: each step of channels costs a register, not
+// an addition.)
+template <typename T, int DP> struct LaneOffsets {
+  using G = Tile<T, DP>;
+  static constexpr int kRowBytes = G::kChunks * 16;
+  int rows[sizeof(T) == 2 ? 1 : 2][DP / 16], columns[DP / 32][sizeof(T) == 2 ? 2 : 8];
+  __device__ __forceinline__ void init() {
+    const int lane = threadIdx.x & 63, h = lane >> 5, row = lane & 31;
+#pragma unroll
+    for (int x = 0; x < DP / 16; ++x) {
+      if constexpr (sizeof(T) == 2) {
+        rows[0][x] = row * kRowBytes + G::chunk_of(row, 2 * x + h) * 16;
+      } else {
+        rows[0][x] = row * kRowBytes + G::chunk_of(row, 4 * x + 2 * h) * 16;
+        rows[1][x] = row * kRowBytes + G::chunk_of(row, 4 * x + 2 * h + 1) * 16;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) {
+      if constexpr (sizeof(T) == 2) {
+        // a group of 16 lanes reads four rows of 16 channels, four to a lane, and each lane is left with a channel
+        const int m = lane & 15, r = 4 * h + (m >> 2), chunk = 4 * x + (lane >> 4 & 1) * 2 + (m >> 1 & 1);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) columns[x][i] = (r + 8 * i) * kRowBytes + G::chunk_of(r + 8 * i, chunk) * 16 + (m & 1) * 8;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) columns[x][i] = row_of(i, h) * kRowBytes + G::chunk_of(row_of(i, h), (32 * x + row) >> 2) * 16 + (row & 3) * 4;
+      }
+    }
+  }
+  // Operand whose rows are the tile's rows FIRST .. FIRST + 31 (a multiple of 32), summands 16 x + 8 h ..
+  template <int FIRST> __device__ __forceinline__ operand_t<T> of_rows(const char *tile, int x) const {
     if constexpr (sizeof(T) == 2) {
-      return *(const operand_t<T> *)(at + chunk_of(row, 2 * s + h) * 16);
+      return *(const operand_t<T> *)(tile + rows[0][x] + FIRST * kRowBytes);
     } else {
-      const f32x4 a = *(const f32x4 *)(at + chunk_of(row, 4 * s + 2 * h) * 16), b = *(const f32x4 *)(at + chunk_of(row, 4 * s + 2 * h + 1) * 16);
+      const f32x4 a = *(const f32x4 *)(tile + rows[0][x] + FIRST * kRowBytes), b = *(const f32x4 *)(tile + rows[1][x] + FIRST * kRowBytes);
       return f32x8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
-  // Operand whose rows are the channels 32 c .., its summands the tile's rows first .. first + 15 in a result's order.
-  static __device__ __forceinline__ operand_t<T> columns(char *tile, int first, int c, int lane) {
-    const int h = lane >> 5;
+  // Operand whose rows are the channels 32 x .., its summands the tile's rows FIRST .. FIRST + 15 in a result's order.
+  template <int FIRST> __device__ __forceinline__ operand_t<T> of_columns(char *tile, int x) const {
     if constexpr (sizeof(T) == 2) {
-      // a group of 16 lanes reads four rows of 16 channels, four to a lane, and each lane is left with a channel
-      const int m = lane & 15, row = first + 4 * h + (m >> 2), chunk = 4 * c + (lane >> 4 & 1) * 2 + (m >> 1 & 1), part = (m & 1) * 8;
       typedef __attribute__((address_space(3))) s16x4_t lds4;
-      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + row * (kChunks * 16) + chunk_of(row, chunk) * 16 + part));
-      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + (row + 8) * (kChunks * 16) + chunk_of(row + 8, chunk) * 16 + part));
+      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + columns[x][0] + FIRST * kRowBytes));
+      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + columns[x][1] + FIRST * kRowBytes));
       return __builtin_bit_cast(operand_t<T>, s16x8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     } else {
       f32x8_t r;
-      const int d = 32 * c + (lane & 31);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = first + row_of(i, h);
-        r[i] = *(const float *)(tile + row * (kChunks * 16) + chunk_of(row, d >> 2) * 16 + (d & 3) * 4);
-      }
+      for (int i = 0; i < 8; ++i) r[i] = *(const float *)(tile + columns[x][i] + FIRST * kRowBytes);
       return r;
     }
   }
 };
 
-// Each lane's BYTES from memory into shared memory, the lanes' behind each other from `to` on, which is the same for all of them.
-// (The compiler would have every transposing read wait for all copies that are on their way, other buffers' too: it is not told
-// of these.  Nothing is written to a register but m0, which nothing else here uses; tiles_turn waits.)
-template <int BYTES> __device__ __forceinline__ void copy_to_lds(const void *from, void *to) {
-  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)to);
+// Each lane's BYTES from memory (base + offset) into shared memory, the lanes' behind each other from `to` on; base and `to` are the same
+// for all of them.  (The compiler would have every transposing read wait for all copies that are on their way, other buffers'
+// too: it is not told of these.  Nothing is written to a register but m0, which nothing else here uses; tiles_turn waits.)
+template <int BYTES> __device__ __forceinline__ void copy_to_lds(const char *base, unsigned offset, unsigned to) {
   if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(offset), "s"(to), "s"(base) : "memory");
   else
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, %2" ::"v"(offset), "s"(to), "s"(base) : "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const void *p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)p; }
+template <typename P> __device__ __forceinline__ P *uniform(P *p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (P *)((uint64_t)hi << 32 | lo);
 }
 
-// Copies tiles of rows into shared memory.  Rows past `last` and chunks past the head are other rows and chunks of the same
-// tensor (memory that is there, and values whose products are left out).
-template <typename T, int DP> struct TileCopy {
+// Copies tiles of ROWS rows into shared memory, by LANES lanes.  Rows past `last` and chunks past the head are other rows and chunks
+// of the same tensor (memory that is there, and values whose products are left out).
+template <typename T, int DP, int ROWS, int LANES> struct TileCopy {
   using G = Tile<T, DP>;
-  int row[G::kCopies], byte[G::kCopies];
-  __device__ __forceinline__ void init(int D) {
+  static constexpr int kCopies = ROWS * G::kChunks / LANES;
+  static_assert(ROWS * G::kChunks % LANES == 0, "a tile is whole copies");
+  unsigned offset[kCopies];
+  int stride;
+  // row and chunk of copy i of this lane; `lane` may hide that they are constants
+  static __device__ __forceinline__ int row_at(int i, int lane) { return (i * LANES + lane) / G::kChunks; }
+  static __device__ __forceinline__ int byte_at(int i, int lane, int D) {
+    const int slot = i * LANES + lane, c = G::chunk_of(slot / G::kChunks, slot % G::kChunks) * 16;  // (its own inverse)
+    return c < D * (int)sizeof(T) ? c : 0;
+  }
+  __device__ __forceinline__ void init(int D, int token_bytes) {
+    stride = token_bytes;
 #pragma unroll
-    for (int i = 0; i < G::kCopies; ++i) {
-      const int slot = i * kBlock + (int)threadIdx.x;
-      row[i] = slot / G::kChunks;
-      const int c = G::chunk_of(row[i], slot % G::kChunks) * 16;  // (its own inverse)
-      byte[i] = c < D * (int)sizeof(T) ? c : 0;
+    for (int i = 0; i < kCopies; ++i) {
+      const int lane = threadIdx.x % LANES;
+      offset[i] = (unsigned)row_at(i, lane) * (unsigned)stride + byte_at(i, lane, D);
     }
   }
-  __device__ __forceinline__ void issue(const char *base, int stride, int first, int last, char *tile) const {
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // `to`: where the tile goes, plus 1024 times the wavefront's number among those that copy it
+  __device__ __forceinline__ void issue(const char *base, int first, int last, unsigned to, int D) const {
+    const char *from = uniform(base + (int64_t)first * stride);
+    if (first + ROWS - 1 <= last) {
 #pragma unroll
-    for (int i = 0; i < G::kCopies; ++i) {
-      int r = first + row[i];
-      r = r < last ? r : last;
-      const char *from = base + (int64_t)r * stride + byte[i];
-      copy_to_lds<16>(from, tile + (i * kBlock + wave * 64) * 16);
+      for (int i = 0; i < kCopies; ++i) copy_to_lds<16>(from, offset[i], to + i * LANES * 16);
+    } else {
+      int lane = threadIdx.x % LANES, left = last - first;
+      pin(lane);  // (so that nothing of this lies in registers all along)
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int r = row_at(i, lane);
+        copy_to_lds<16>(from, (unsigned)(r < left ? r : left) * (unsigned)stride + byte_at(i, lane, D), to + i * LANES * 16);
+      }
     }
   }
 };
@@ -359,7 +401,7 @@ template <typename T> __device__ void dkv_again(const WindowArgs &a, const Sampl
       float t = 0.0f;
       if (i >= 0) {
         t = __builtin_amdgcn_exp2f(dot((const T *)a.q.row(b, i, h), k, a.D) * a.scale_log2 - load_global<float>(a.lse + rows + i));
-        if (of_k) t *= dot((const T *)a.dout.row(b, i, h), v, a.D) - load_global<float>(a.delta + rows + i);
+        if (of_k) t *= dot((const T *)a.dout.row(b, i, h), v, a.D) + load_global<float>(a.delta + rows + i);
       }
       for (int u = 0; u < 64; ++u) {
         const int iu = __shfl(i, u);
@@ -400,6 +442,11 @@ template <typename T, int DP> __device__ __forceinline__ void load_token(const T
     f[s] = z;
   }
 }
+// Waits for them here: a wait in the loop would be one for all copies on their way, too.
+template <typename O, int N> __device__ __forceinline__ void settle(O (&f)[N]) {
+#pragma unroll
+  for (int x = 0; x < N; ++x) pin(f[x]);
+}
 // Channels of one token per lane from a transposed result, times `factor`, rounded once.
 template <typename T, int DP> __device__ __forceinline__ void store_token(T *p, int D, const f32x16_t (&acc)[DP / 32], float factor) {
   const int h = (threadIdx.x & 63) >> 5;
@@ -437,68 +484,84 @@ constexpr float kRaise = 8.0f;
 template <typename T, int DP> struct ForwardState {
   operand_t<T> q[DP / 16];
   f32x16_t o[DP / 32];
-  float reference, sum;  // of the lane's half of the keys; in powers of two
+  float reference, subtract, sum;  // (sum: of the lane's half of the keys) in powers of two; subtract: the reference, or 0 while there is none
   Sight sight;
 };
 
-// 32 keys against the wavefront's 32 queries: scores, then weights in their place.
-template <typename T, int DP> __device__ __forceinline__ void forward_tile(ForwardState<T, DP> &st, const char *kt, char *vt, int first, int j0, float c) {
-  const int lane = threadIdx.x & 63, h = lane >> 5;
+// 32 N keys against the wavefront's 32 queries: scores, then weights in their place, then their products with the values.
+template <typename T, int DP, int N, typename ST> __device__ __forceinline__ void forward_tile(ST &st, const LaneOffsets<T, DP> &at, const char *kt, char *vt, int j0, float c) {
+  const int h = (threadIdx.x & 63) >> 5;
   const Sight &g = st.sight;
   const int left = j0 - g.low;
-  const bool inside = (left >= 0 && left + 31 < g.count) || j0 + 31 < g.sinks;
-  const bool touches = (left + 31 >= 0 && left < g.count) || j0 < g.sinks;
-  if (!__any(touches)) return;
-  f32x16_t s = zeros16();
+  const bool inside = (left >= 0 && left + 32 * N <= g.count) || j0 + 32 * N <= g.sinks;
+  if (!__all(inside) && !__any((left + 32 * N > 0 && left < g.count) || j0 < g.sinks)) return;
+  f32x16_t s[N];
 #pragma unroll
-  for (int x = 0; x < DP / 16; ++x) s = Operand<T>::product(Tile<T, DP>::rows(kt, first, x, lane), st.q[x], s);
-  if (!__all(inside)) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (!g.sees(j0 + row_of(r, h))) s[r] = -INFINITY;
+  for (int x = 0; x < DP / 16; ++x) {
+    s[0] = Operand<T>::product(at.template of_rows<0>(kt, x), st.q[x], x ? s[0] : zeros16());
+    if constexpr (N == 2) s[N - 1] = Operand<T>::product(at.template of_rows<32>(kt, x), st.q[x], x ? s[N - 1] : zeros16());
   }
-  float most = s[0];
+  if (!__all(inside)) {
+    int first = j0;
+    pin(first);  // (so that the comparisons stay here)
 #pragma unroll
-  for (int r = 1; r < 16; ++r) most = fmaxf(most, s[r]);
+    for (int f = 0; f < N; ++f)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (!g.sees(first + 32 * f + row_of(r, h))) s[f][r] = -INFINITY;
+  }
+  float most = s[0][0];
+#pragma unroll
+  for (int f = 0; f < N; ++f)
+#pragma unroll
+    for (int r = f ? 0 : 1; r < 16; ++r) most = fmaxf(most, s[f][r]);
   if (__any(most * c > st.reference + kRaise)) {
     most = fmaxf(most, other_half(most)) * c;
     const float reference = fmaxf(most, st.reference);
     const float factor = reference == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.reference - reference);
     st.reference = reference;
+    st.subtract = reference == -INFINITY ? 0.0f : reference;
     st.sum *= factor;
 #pragma unroll
     for (int x = 0; x < DP / 32; ++x)
 #pragma unroll
       for (int r = 0; r < 16; ++r) st.o[x][r] *= factor;
   }
-  const float ref = st.reference == -INFINITY ? 0.0f : st.reference;
+  auto part = [&](auto unit) {  // 16 keys
+    constexpr int u = decltype(unit)::value;
+    f32x16_t &p = s[u / 2];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ref));
-    st.sum += s[r];
-  }
+    for (int r = 8 * (u % 2); r < 8 * (u % 2) + 8; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], c, -st.subtract));
+      st.sum += p[r];
+    }
+    const operand_t<T> w = operand_of<T>(p, u % 2);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const operand_t<T> p = operand_of<T>(s, t);
-#pragma unroll
-    for (int x = 0; x < DP / 32; ++x) st.o[x] = Operand<T>::product(Tile<T, DP>::columns(vt, first + 16 * t, x, lane), p, st.o[x]);
+    for (int x = 0; x < DP / 32; ++x) st.o[x] = Operand<T>::product(at.template of_columns<16 * u>(vt, x), w, st.o[x]);
+  };
+  part(std::integral_constant<int, 0>());
+  part(std::integral_constant<int, 1>());
+  if constexpr (N == 2) {
+    part(std::integral_constant<int, 2>());
+    part(std::integral_constant<int, 3>());
   }
 }
 
 // A workgroup: 128 queries of one head, 32 a wavefront.
 template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
-  __shared__ __attribute__((aligned(16))) char keys[2][G::kBytes], values[2][G::kBytes];
+  __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a.items);
   if (item >= a.items) return;
   // (the heads of a group are neighbours, then the tiles of queries, the last ones, which see most, first)
   const int g = item % a.group, rest = item / a.group, tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
   const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
   const Sample s = sample_of(a, b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = tile * kQueries + wave * 32 + (lane & 31);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = tile * kQueries + wave * 32 + (lane & 31);
   ForwardState<T, DP> st;
   st.sight = sight_of(a, s, i);
   st.reference = -INFINITY;
+  st.subtract = 0.0f;
   st.sum = 0.0f;
 #pragma unroll
   for (int x = 0; x < DP / 32; ++x) st.o[x] = zeros16();
@@ -507,24 +570,28 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2
     const int ic = i < from ? from : i < to ? i : to - 1;
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
     const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows);
-    TileCopy<T, DP> copy;
-    copy.init(a.D);
+    TileCopy<T, DP, G::kRows, kBlock> ck, cv;
+    ck.init(a.D, a.k.token_bytes);
+    cv.init(a.D, a.v.token_bytes);
+    LaneOffsets<T, DP> at;
+    at.init();
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
+    const unsigned lds = lds_address(tiles) + wave * 1024;
+    settle(st.q);
     int t = w.start();
     if (w.more(t)) {
-      copy.issue(kb, a.k.token_bytes, t * G::kRows, s.n - 1, keys[0]);
-      copy.issue(vb, a.v.token_bytes, t * G::kRows, s.n - 1, values[0]);
+      ck.issue(kb, t * G::kRows, s.n - 1, lds, a.D);
+      cv.issue(vb, t * G::kRows, s.n - 1, lds + G::kBytes, a.D);
     }
     auto turn = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
       const int next = w.next(t);
       if (w.more(next)) {
-        copy.issue(kb, a.k.token_bytes, next * G::kRows, s.n - 1, keys[1 - B]);
-        copy.issue(vb, a.v.token_bytes, next * G::kRows, s.n - 1, values[1 - B]);
+        ck.issue(kb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes, a.D);
+        cv.issue(vb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes + G::kBytes, a.D);
       }
-#pragma unroll
-      for (int f = 0; f < G::kRows; f += 32) forward_tile<T, DP>(st, keys[B], values[B], f, t * G::kRows + f, a.scale_log2);
+      forward_tile<T, DP, G::kRows / 32>(st, at, tiles + B * 2 * G::kBytes, tiles + B * 2 * G::kBytes + G::kBytes, t * G::kRows, a.scale_log2);
       t = next;
     };
     while (w.more(t)) {
@@ -560,7 +627,6 @@ template <typename T, int DP> struct Few {
   static constexpr int kStage = 2 * 32 * DP * (int)sizeof(T);  // bytes of a tile of keys and one of values
   static constexpr int kMost = 131072 / (2 * kStage);
   static constexpr int kWaves = kMost >= 8 ? 8 : kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
-  static constexpr int kCopies = Tile<T, DP>::kChunks / 2;  // of a wavefront, for each of the two tiles
   static constexpr int kPitch = DP + 4;                     // floats of a row while results are joined
   static_assert(32 * kPitch * 4 <= 2 * kStage, "a wavefront's results fit its tiles");
 };
@@ -573,10 +639,9 @@ template <int COPIES> __device__ __forceinline__ void wait_for_copies(bool newes
 __device__ __forceinline__ float part_weight(float reference, float most) { return most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(reference - most); }
 
 template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void window_few_kernel(const WindowArgs a) {
-  using G = Tile<T, DP>;
   using W = Few<T, DP>;
   constexpr int kWaves = W::kWaves;
-  __shared__ __attribute__((aligned(16))) char tiles[kWaves][2][W::kStage];
+  __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * W::kStage];
   __shared__ float references[kWaves][32], sums[kWaves][32];
   __shared__ int bad[32];
   const int item = work_item(a.items);
@@ -589,6 +654,7 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   ForwardState<T, DP> st;
   st.sight = sight_of(a, s, i);
   st.reference = -INFINITY;
+  st.subtract = 0.0f;
   st.sum = 0.0f;
 #pragma unroll
   for (int x = 0; x < DP / 32; ++x) st.o[x] = zeros16();
@@ -603,29 +669,29 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
     const int begin = (int)((int64_t)steps * split / a.splits), end = (int)((int64_t)steps * (split + 1) / a.splits);
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
     auto tile_at = [&](int u) { return u < w.sinks ? u : w.first + (u - w.sinks); };
-    auto issue = [&](int u, char *to_tile) {
+    using Copy = TileCopy<T, DP, 32, 64>;
+    Copy ck, cv;
+    ck.init(a.D, a.k.token_bytes);
+    cv.init(a.D, a.v.token_bytes);
+    LaneOffsets<T, DP> at;
+    at.init();
+    const unsigned lds = lds_address(tiles) + wave * 2 * W::kStage;
+    settle(st.q);
+    auto issue = [&](int u, int buffer) {
       const int first = tile_at(u) * 32;
-#pragma unroll
-      for (int n = 0; n < W::kCopies; ++n) {
-        const int slot = n * 64 + lane, r = slot / G::kChunks;
-        int c = G::chunk_of(r, slot % G::kChunks) * 16;
-        c = c < a.D * (int)sizeof(T) ? c : 0;
-        const int j = first + r < s.n ? first + r : s.n - 1;
-        copy_to_lds<16>(kb + (int64_t)j * a.k.token_bytes + c, to_tile + n * 1024);
-        copy_to_lds<16>(vb + (int64_t)j * a.v.token_bytes + c, to_tile + W::kStage / 2 + n * 1024);
-      }
+      ck.issue(kb, first, s.n - 1, lds + buffer * W::kStage, a.D);
+      cv.issue(vb, first, s.n - 1, lds + buffer * W::kStage + W::kStage / 2, a.D);
     };
-    int u = begin + wave;
-    if (u < end) issue(u, tiles[wave][0]);
-    int turn = 0;
+    int u = begin + wave, turn = 0;
+    if (u < end) issue(u, 0);
     for (; u < end; u += kWaves) {
-      char *tile = tiles[wave][turn];
+      char *tile = tiles + (wave * 2 + turn) * W::kStage;
       turn ^= 1;
       const bool more = u + kWaves < end;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (reads of the tile that is now overwritten)
-      if (more) issue(u + kWaves, tiles[wave][turn]);
-      wait_for_copies<2 * W::kCopies>(!more);
-      forward_tile<T, DP>(st, tile, tile + W::kStage / 2, 0, tile_at(u) * 32, a.scale_log2);
+      if (more) issue(u + kWaves, turn);
+      wait_for_copies<2 * Copy::kCopies>(!more);
+      forward_tile<T, DP, 1>(st, at, tile, tile + W::kStage / 2, tile_at(u) * 32, a.scale_log2);
     }
   }
   // join the wavefronts
@@ -642,7 +708,7 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
 #pragma unroll
   for (int n = 0; n < kWaves; ++n) sum += sums[n][lane & 31] * part_weight(references[n][lane & 31], most);
   const float weight = part_weight(st.reference, most);
-  float *mine = (float *)tiles[wave];
+  float *mine = (float *)(tiles + wave * 2 * W::kStage);
   const int half = lane >> 5;
 #pragma unroll
   for (int x = 0; x < DP / 32; ++x)
@@ -659,9 +725,9 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   for (int e = threadIdx.x; e < 32 * DP / 4; e += 64 * kWaves) {
     const int r = e / (DP / 4), d = e % (DP / 4) * 4, rr = block * 32 + r;
     if (rr >= rows || d >= a.D) continue;
-    f32x4 v = *(const f32x4 *)((const float *)tiles[0] + r * W::kPitch + d);
+    f32x4 v = *(const f32x4 *)((const float *)tiles + r * W::kPitch + d);
 #pragma unroll
-    for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)tiles[n] + r * W::kPitch + d);
+    for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)(tiles + n * 2 * W::kStage) + r * W::kPitch + d);
     if (a.splits > 1) {
       store_global<f32x4>(a.part_v + ((int64_t)item * 32 + r) * a.D + d, v);
       continue;
@@ -726,7 +792,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
 }
 
 // ---- backward: dq ----
-// delta and the largest |do| of a row go to the workspace for the other kernel.
+// -delta and the largest |do| of a row go to the workspace for the other kernel.
 // float16 holds 2^-24 to 65504: weights and dS are kept in its middle by powers of two, weights as 2^12 P, dS relative to the
 // largest |do| (of a row, or of the rows that a workgroup visits), whatever scale a loss has been given.
 constexpr float kWeightBits = 12.0f, kGradBits = 5.0f;
@@ -737,13 +803,13 @@ template <typename T> __device__ __forceinline__ float gradient_unit(float most)
 
 template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && sizeof(T) == 2 ? 2 : 1) void window_dq_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
-  __shared__ __attribute__((aligned(16))) char keys[2][G::kBytes], values[2][G::kBytes];
+  __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a.items);
   if (item >= a.items) return;
   const int g = item % a.group, rest = item / a.group, tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
   const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
   const Sample s = sample_of(a, b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, i = tile * kQueries + wave * 32 + (lane & 31);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, i = tile * kQueries + wave * 32 + (lane & 31);
   const Sight sight = sight_of(a, s, i);
   const int64_t row = ((int64_t)b * a.H + h) * a.L + i;
   f32x16_t acc[DP / 32];
@@ -769,58 +835,73 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
       most = fmaxf(most, other_half(most));
       unit = gradient_unit<T>(most);
       if (i >= from && i < to && lane < 32) {
-        store_global<float>(a.delta + row, delta);
+        store_global<float>(a.delta + row, -delta);
         if constexpr (__is_same(T, f16_t)) store_global<float>(a.largest + row, most);
       }
     }
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, q);
     if (i >= from && i < to) lse = load_global<float>(a.lse + row);
     const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows);
-    TileCopy<T, DP> copy;
-    copy.init(a.D);
+    TileCopy<T, DP, G::kRows, kBlock> ck, cv;
+    ck.init(a.D, a.k.token_bytes);
+    cv.init(a.D, a.v.token_bytes);
+    LaneOffsets<T, DP> at;
+    at.init();
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
-    // P 2^bits (dP - delta) unit: one exponential and one fused step per element
-    const float bits = __is_same(T, f16_t) ? kGradBits : 0.0f, lift = bits - lse, lowered = -delta * unit;
+    const unsigned lds = lds_address(tiles) + wave * 1024;
+    // P 2^bits (dP - delta) unit: the product starts from -delta
+    const float bits = __is_same(T, f16_t) ? kGradBits : 0.0f;
+    float lift = bits - lse;
+    if constexpr (__is_same(T, f16_t)) lift += (float)__builtin_amdgcn_frexp_expf(unit) - 1.0f;  // (unit is 2^(its exponent - 1))
+    f32x16_t start;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) start[r] = -delta;
+    settle(q);
+    settle(dout);
+    pin(lift);
     int t = w.start();
     if (w.more(t)) {
-      copy.issue(kb, a.k.token_bytes, t * G::kRows, s.n - 1, keys[0]);
-      copy.issue(vb, a.v.token_bytes, t * G::kRows, s.n - 1, values[0]);
+      ck.issue(kb, t * G::kRows, s.n - 1, lds, a.D);
+      cv.issue(vb, t * G::kRows, s.n - 1, lds + G::kBytes, a.D);
     }
     auto turn = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
       const int next = w.next(t);
       if (w.more(next)) {
-        copy.issue(kb, a.k.token_bytes, next * G::kRows, s.n - 1, keys[1 - B]);
-        copy.issue(vb, a.v.token_bytes, next * G::kRows, s.n - 1, values[1 - B]);
+        ck.issue(kb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes, a.D);
+        cv.issue(vb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes + G::kBytes, a.D);
       }
-#pragma unroll
-      for (int f = 0; f < G::kRows; f += 32) {
+      char *kt = tiles + B * 2 * G::kBytes, *vt = kt + G::kBytes;
+      auto part = [&](auto first) {
+        constexpr int f = decltype(first)::value;
         const int j0 = t * G::kRows + f, left = j0 - sight.low;
-        const bool inside = (left >= 0 && left + 31 < sight.count) || j0 + 31 < sight.sinks;
-        const bool touches = (left + 31 >= 0 && left < sight.count) || j0 < sight.sinks;
-        if (!__any(touches)) continue;
-        f32x16_t p = zeros16(), dp = zeros16();
+        const bool inside = (left >= 0 && left + 32 <= sight.count) || j0 + 32 <= sight.sinks;
+        const bool whole = __all(inside);
+        if (!whole && !__any((left + 32 > 0 && left < sight.count) || j0 < sight.sinks)) return;
+        f32x16_t p, dp;
 #pragma unroll
         for (int x = 0; x < DP / 16; ++x) {
-          p = Operand<T>::product(G::rows(keys[B], f, x, lane), q[x], p);
-          dp = Operand<T>::product(G::rows(values[B], f, x, lane), dout[x], dp);
+          p = Operand<T>::product(at.template of_rows<f>(kt, x), q[x], x ? p : zeros16());
+          dp = Operand<T>::product(at.template of_rows<f>(vt, x), dout[x], x ? dp : start);
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, lift)) * __builtin_fmaf(dp[r], unit, lowered);
-        if (!__all(inside)) {
+        for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_log2, lift)) * dp[r];
+        if (!whole) {
+          int from_here = j0;
+          pin(from_here);  // (so that the comparisons stay here)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (!sight.sees(j0 + row_of(r, half))) p[r] = 0.0f;
+            if (!sight.sees(from_here + row_of(r, half))) p[r] = 0.0f;
         }
+        const operand_t<T> ds0 = operand_of<T>(p, 0), ds1 = operand_of<T>(p, 1);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const operand_t<T> ds = operand_of<T>(p, u);
+        for (int x = 0; x < DP / 32; ++x) acc[x] = Operand<T>::product(at.template of_columns<f>(kt, x), ds0, acc[x]);
 #pragma unroll
-          for (int x = 0; x < DP / 32; ++x) acc[x] = Operand<T>::product(G::columns(keys[B], f + 16 * u, x, lane), ds, acc[x]);
-        }
-      }
+        for (int x = 0; x < DP / 32; ++x) acc[x] = Operand<T>::product(at.template of_columns<f + 16>(kt, x), ds1, acc[x]);
+      };
+      part(std::integral_constant<int, 0>());
+      if constexpr (G::kRows == 64) part(std::integral_constant<int, 32>());
       t = next;
     };
     while (w.more(t)) {
@@ -858,8 +939,8 @@ template <typename T, int DP, int PARTS>
 __global__ __launch_bounds__(kBlock, DP <= 96 && sizeof(T) == 2 ? 2 : 1) void window_dkv_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   constexpr bool kDv = PARTS & 1, kDk = PARTS & 2;
-  __shared__ __attribute__((aligned(16))) char queries[2][G::kBytes], grads[2][G::kBytes];
-  __shared__ __attribute__((aligned(16))) float lses[2][64], deltas[2][64];
+  __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // queries and gradients, two deep
+  __shared__ __attribute__((aligned(16))) float lses[2 * 64], deltas[2 * 64];
   __shared__ float reduce[4];
   const int item = work_item(a.items);
   if (item >= a.items) return;
@@ -877,7 +958,7 @@ __global__ __launch_bounds__(kBlock, DP <= 96 && sizeof(T) == 2 ? 2 : 1) void wi
     share = (at - sink_items) % shares;
   }
   const Sample s = sample_of(a, b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, j = tile * kQueries + wave * 32 + (lane & 31);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, j = tile * kQueries + wave * 32 + (lane & 31);
   const Seen seen = seen_of(a, s, j);
   f32x16_t dk[kDk ? DP / 32 : 1], dv[kDv ? DP / 32 : 1];
 #pragma unroll
@@ -901,13 +982,13 @@ __global__ __launch_bounds__(kBlock, DP <= 96 && sizeof(T) == 2 ? 2 : 1) void wi
     to = (to < most ? to : most) - s.off;
   }
   if (from <= to) {
-    const int first = from / G::kRows, tiles = to / G::kRows - first + 1, steps = tiles * a.group;
+    const int first = from / G::kRows, tiles_of = to / G::kRows - first + 1, steps = tiles_of * a.group;
     const int begin = (int)((int64_t)steps * share / shares), end = (int)((int64_t)steps * (share + 1) / shares);
     if constexpr (__is_same(T, f16_t)) {
       float most = 0.0f;
       for (int st = begin; st < end; ++st) {
-        const int64_t rows = ((int64_t)b * a.H + kh * a.group + st / tiles) * a.L;
-        const int i = (first + st % tiles) * G::kRows + (int)(threadIdx.x & 63);
+        const int64_t rows = ((int64_t)b * a.H + kh * a.group + st / tiles_of) * a.L;
+        const int i = (first + st % tiles_of) * G::kRows + (int)(threadIdx.x & 63);
         if (wave == (st & 3) && i >= from && i <= to) most = fmaxf(most, load_global<float>(a.largest + rows + i));
       }
       most = wave_max(most);
@@ -920,82 +1001,113 @@ __global__ __launch_bounds__(kBlock, DP <= 96 && sizeof(T) == 2 ? 2 : 1) void wi
     const int jc = j < s.n ? j : s.n - 1;
     load_token<T, DP>((const T *)a.k.row(b, jc, kh), a.D, k);
     if constexpr (kDk) load_token<T, DP>((const T *)a.v.row(b, jc, kh), a.D, v);
-    TileCopy<T, DP> copy;
-    copy.init(a.D);
-    auto issue = [&](int st, char *qt, char *gt, float *lt, float *dt) {
-      const int h = kh * a.group + st / tiles, i0 = (first + st % tiles) * G::kRows;
-      copy.issue((const char *)a.q.row(b, 0, h), a.q.token_bytes, i0, to, qt);
-      copy.issue((const char *)a.dout.row(b, 0, h), a.dout.token_bytes, i0, to, gt);
-      int i = i0 + lane;
-      i = i < to ? i : to;
-      const int64_t row = ((int64_t)b * a.H + h) * a.L + i;
-      if (wave == 0) copy_to_lds<4>(a.lse + row, lt);
-      if (kDk && wave == 1) copy_to_lds<4>(a.delta + row, dt);
+    TileCopy<T, DP, G::kRows, kBlock> cq, cg;
+    cq.init(a.D, a.q.token_bytes);
+    cg.init(a.D, a.dout.token_bytes);
+    LaneOffsets<T, DP> at;
+    at.init();
+    const unsigned lds = lds_address(tiles) + wave * 1024, lds_lse = lds_address(lses), lds_delta = lds_address(deltas);
+    settle(k);
+    if constexpr (kDk) settle(v);
+    // step: a head of the group, a tile of queries
+    struct Step {
+      int g, t;
     };
-    const float bits = __is_same(T, f16_t) ? kWeightBits : 0.0f;
+    auto advance = [&](Step w) {
+      ++w.t;
+      if (w.t == tiles_of) {
+        w.t = 0;
+        ++w.g;
+      }
+      return w;
+    };
+    auto issue = [&](Step w, int buffer) {
+      const int h = kh * a.group + w.g, i0 = (first + w.t) * G::kRows;
+      cq.issue((const char *)a.q.row(b, 0, h), i0, to, lds + buffer * 2 * G::kBytes, a.D);
+      cg.issue((const char *)a.dout.row(b, 0, h), i0, to, lds + buffer * 2 * G::kBytes + G::kBytes, a.D);
+      if (wave < (kDk ? 2 : 1)) {
+        const int r = lane < to - i0 ? lane : to - i0;
+        const char *from = (const char *)((wave ? a.delta : a.lse) + ((int64_t)b * a.H + h) * a.L + i0);
+        copy_to_lds<4>(uniform(from), (unsigned)r * 4, (wave ? lds_delta : lds_lse) + buffer * 256);
+      }
+    };
     const float lowering = __is_same(T, f16_t) ? unit * (1.0f / 128.0f) : 1.0f;  // 2^(kGradBits - kWeightBits)
-    int st = begin;
-    if (st < end) issue(st, queries[0], grads[0], lses[0], deltas[0]);
+    int left_over = end - begin;
+    Step step = {begin / tiles_of, begin % tiles_of};
+    if (left_over > 0) issue(step, 0);
     auto turn = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
-      if (st + 1 < end) issue(st + 1, queries[1 - B], grads[1 - B], lses[1 - B], deltas[1 - B]);
+      const Step next = advance(step);
+      if (--left_over > 0) issue(next, 1 - B);
+      char *qt = tiles + B * 2 * G::kBytes, *gt = qt + G::kBytes;
+      auto part = [&](auto first_row) {
+        constexpr int f = decltype(first_row)::value;
+        const int left = (first + step.t) * G::kRows + f + s.off - seen.from;
+        const bool inside = left >= 0 && left + 32 <= seen.count, whole = __all(inside);
+        if (!whole && !__any(left + 32 > 0 && left < seen.count)) return;
+        f32x16_t p, dp;
+        if constexpr (kDk) {
 #pragma unroll
-      for (int f = 0; f < G::kRows; f += 32) {
-        const int p0 = (first + st % tiles) * G::kRows + f + s.off, left = p0 - seen.from;
-        const bool inside = left >= 0 && left + 31 < seen.count, touches = left + 31 >= 0 && left < seen.count;
-        if (!__any(touches)) continue;
-        f32x16_t p = zeros16(), dp = zeros16();
+          for (int r = 0; r < 16; r += 4) {  // (the product starts from -delta)
+            const f32x4 d4 = *(const f32x4 *)&deltas[B * 64 + f + row_of(r, half)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[r + e] = d4[e];
+          }
+        }
 #pragma unroll
         for (int x = 0; x < DP / 16; ++x) {
-          p = Operand<T>::product(G::rows(queries[B], f, x, lane), k[x], p);
-          if constexpr (kDk) dp = Operand<T>::product(G::rows(grads[B], f, x, lane), v[x], dp);
+          p = Operand<T>::product(at.template of_rows<f>(qt, x), k[x], x ? p : zeros16());
+          if constexpr (kDk) dp = Operand<T>::product(at.template of_rows<f>(gt, x), v[x], dp);
         }
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-          const f32x4 l4 = *(const f32x4 *)&lses[B][f + row_of(r, half)];
+          const f32x4 l4 = *(const f32x4 *)&lses[B * 64 + f + row_of(r, half)];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r + e], a.scale_log2, bits - l4[e]));
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (__is_same(T, f16_t)) p[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r + e], a.scale_log2, kWeightBits - l4[e]));
+            else p[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r + e], a.scale_log2, -l4[e]));
+          }
         }
-        const bool whole = __all(inside);
         if (!whole) {
+          int from_here = left;
+          pin(from_here);  // (so that the comparisons stay here)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if ((unsigned)(left + row_of(r, half)) >= (unsigned)seen.count) p[r] = 0.0f;
+          for (int r = 0; r < 16; ++r) {
+            const bool hidden = (unsigned)(from_here + row_of(r, half)) >= (unsigned)seen.count;
+            if (hidden) p[r] = 0.0f;
+            if constexpr (kDk) {
+              if (hidden) dp[r] = 0.0f;  // (which may be infinite)
+            }
+          }
         }
         if constexpr (kDv) {
+          const operand_t<T> w0 = operand_of<T>(p, 0), w1 = operand_of<T>(p, 1);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const operand_t<T> w = operand_of<T>(p, u);
+          for (int x = 0; x < DP / 32; ++x) dv[x] = Operand<T>::product(at.template of_columns<f>(gt, x), w0, dv[x]);
 #pragma unroll
-            for (int x = 0; x < DP / 32; ++x) dv[x] = Operand<T>::product(G::columns(grads[B], f + 16 * u, x, lane), w, dv[x]);
-          }
+          for (int x = 0; x < DP / 32; ++x) dv[x] = Operand<T>::product(at.template of_columns<f + 16>(gt, x), w1, dv[x]);
         }
         if constexpr (kDk) {
 #pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            const f32x4 d4 = *(const f32x4 *)&deltas[B][f + row_of(r, half)];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[r + e] *= __builtin_fmaf(dp[r + e], lowering, -d4[e] * lowering);
+          for (int r = 0; r < 16; ++r) {
+            if constexpr (__is_same(T, f16_t)) p[r] *= lowering;
+            p[r] *= dp[r];
           }
-          if (!whole) {  // (a zero weight times an infinite gradient)
+          const operand_t<T> s0 = operand_of<T>(p, 0), s1 = operand_of<T>(p, 1);
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if ((unsigned)(left + row_of(r, half)) >= (unsigned)seen.count) p[r] = 0.0f;
-          }
+          for (int x = 0; x < DP / 32; ++x) dk[x] = Operand<T>::product(at.template of_columns<f>(qt, x), s0, dk[x]);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const operand_t<T> ds = operand_of<T>(p, u);
-#pragma unroll
-            for (int x = 0; x < DP / 32; ++x) dk[x] = Operand<T>::product(G::columns(queries[B], f + 16 * u, x, lane), ds, dk[x]);
-          }
+          for (int x = 0; x < DP / 32; ++x) dk[x] = Operand<T>::product(at.template of_columns<f + 16>(qt, x), s1, dk[x]);
         }
-      }
-      ++st;
+      };
+      part(std::integral_constant<int, 0>());
+      if constexpr (G::kRows == 64) part(std::integral_constant<int, 32>());
+      step = next;
     };
-    while (st < end) {
+    while (left_over > 0) {
       turn(std::integral_constant<int, 0>());
-      if (st >= end) break;
+      if (left_over <= 0) break;
       turn(std::integral_constant<int, 1>());
     }
   }

@@ -1,6 +1,5 @@
 // Kernels of the attention (gn_window.h) instantiated and launched for ONE element type, selected with -DGN_INST_DTYPE=0, 2 or 3
 // (f32, f16, bf16).
-#include <type_traits>
 #include "gn_window.h"
 
 #ifndef GN_INST_DTYPE

@@ -48,7 +48,7 @@ def _aligned(t):
     """t as the kernels read it: whole 16 bytes between its rows and in front; a copy where it is laid out otherwise."""
     n = 16 // t.element_size()
     if t.numel() == 0 or (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % n == 0 or m == 1 for m, s in zip(t.shape[:3], t.stride()))
-                          and (t.shape[1] == 1 or t.stride(1) * t.element_size() < 2 ** 31)):
+                          and (t.shape[1] == 1 or t.stride(1) * t.element_size() < 2 ** 25)):
         return t
     # (a contiguous tensor may start anywhere, too)
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)

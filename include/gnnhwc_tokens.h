@@ -137,7 +137,7 @@ int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const
  *   lse      : float (batch, heads, tokens): log2 of the softmax's sum, infinite for a query that sees nothing.  Written by the
  *              forward unless NULL, read by the backward.
  *   strides  : of batch, token and head in elements, each a whole multiple of 16 bytes (but for dimensions of size 1), as are the
- *              addresses; a token's below 2^31 bytes.  Channels of a head are contiguous.
+ *              addresses; a token's below 2^25 bytes.  Channels of a head are contiguous.
  * Backward (not with at_end): reads q, k, v, out, out_grad and lse, writes q_grad, k_grad and v_grad.
  * Outputs must not overlap inputs or each other.
  */

@@ -54,7 +54,7 @@ REFUSED = [(dict(dtype=F64), "dtype"), (dict(dtype=7), "dtype"), (dict(head_dim=
            (dict(keys=-1, tokens=0), "negative"), (dict(keys=2 ** 30 + 1), "2\\^30"), (dict(window=-2), "window"), (dict(sinks=-1), "sinks"), (dict(tokens=9), "more queries"),
            (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(scale=1e-60), "scale"),
            (dict(length_type=2), "length_type"), (dict(q=None), "q is null"), (dict(v=None), "v is null"), (dict(k="odd"), "aligned"), (dict(out="odd"), "aligned"),
-           (dict(q_stride=[4096, 257, 64]), "16 bytes"), (dict(k_stride=[4096, 2 ** 30, 64]), "2\\^31"), (dict(v_stride=[4096, -256, 64]), "stride"),
+           (dict(q_stride=[4096, 257, 64]), "16 bytes"), (dict(k_stride=[4096, 2 ** 30, 64]), "2\\^25"), (dict(v_stride=[4096, -256, 64]), "stride"),
            (dict(batch=2 ** 20, heads=64, kv_heads=64), "too many")]
 
 
