@@ -11,6 +11,7 @@ namespace gn {
 namespace {
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;
+constexpr int64_t kOverhead = 3, kJoin = 8;  // in steps
 constexpr int64_t kFewRows = 128, kFewItems = 512, kFewSteps = 8;
 constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
 
@@ -43,11 +44,23 @@ int put_rows(HeadRows &r, const void *base, const int64_t (&stride)[3], int64_t 
 }
 
 struct WindowPlan {
-  WindowArgs a, kv;  // queries' tiles, keys' tiles
-  bool empty, few;  // few: 32 rows of a key head at a time, see window_few_kernel
-  size_t join;      // forward's workspace: references and sums first
-  size_t delta, largest, part_k, part_v, bytes;  // backward's workspace
+  WindowArgs a, kv, sinks;  // queries' tiles, keys' tiles, sinks
+  bool empty, few;          // few: 32 rows of a key head at a time, see window_few_kernel
+  size_t delta, largest, part_q, part_k, part_v, bytes;  // the workspace (forward: part_k references and sums, part_v rows)
 };
+
+// Workgroups that share the work of each of `items`, of `steps` steps: a CU takes `thick` of them at once in the time of one, each
+// has kOverhead steps besides its share, and what they leave has to be joined.
+int64_t shares_of(int64_t items, int64_t steps, int64_t thick, int64_t most) {
+  if (items == 0) return 1;
+  auto cost = [&](int64_t s) {
+    return std::max(ceil_div(items * s, kNumCU), thick) * (ceil_div(steps, s) + kOverhead) + (s > 1 ? kJoin + items * s / 32 : 0);
+  };
+  int64_t best = 1;
+  for (int64_t s = 2; s <= most && s <= steps / 2; ++s)
+    if (cost(s) < cost(best)) best = s;
+  return best;
+}
 
 int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   if (!c) return invalid("null call");
@@ -57,6 +70,7 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   if (c->tokens > kMostTokens || c->keys > kMostTokens || c->batch > kMostTokens) return invalid("batch, tokens or keys out of range: at most 2^30");
   if (c->heads < 1 || c->kv_heads < 1 || c->heads > 65535 || c->heads % c->kv_heads) return invalid("heads must be 1 to 65535 and a multiple of kv_heads");
   if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8) return invalid("head_dim must be a multiple of 8 from 8 to 256");
+  if (es == 4 && c->head_dim > 128) return invalid("head_dim must be 128 or less in f32");
   if (c->window < -1 || c->sinks < 0) return invalid("window must be -1 or more, and sinks not negative");
   if (c->length_type != 0 && c->length_type != 1) return invalid("length_type must be 0 (int32) or 1 (int64)");
   if (!(c->scale > 0 && c->scale < INFINITY)) return invalid("scale must be positive and finite");
@@ -89,53 +103,74 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   a.scale = (float)c->scale;
   a.scale_log2 = (float)(c->scale * 1.4426950408889634);
   if (!(a.scale > 0 && a.scale_log2 < INFINITY)) return invalid("scale must be positive and finite");
+  if (a.sinks >= a.S || (a.left >= a.S - 1 && a.right >= (a.causal ? 0 : a.S - 1))) {  // all see all
+    a.left = kMostTokens;
+    a.right = a.causal ? 0 : a.left;
+    a.sinks = 0;
+  }
   a.tiles = (int)ceil_div(a.L, kQueries);
-  const int64_t items = (int64_t)a.tiles * a.H * a.B;
+  a.splits = a.shares = 1;
+  const int64_t items = (int64_t)a.tiles * a.H * a.B, lse = (int64_t)a.B * a.H * a.L;
   if (items > kMostItems || (int64_t)a.H * a.B > kMostItems) return invalid("too many tokens and heads for one call");
   a.items = (int)items;
   p.empty = items == 0;
+  const int64_t width = window_width(a.D), step = es == 2 ? 64 : 32;  // tokens of the other side that a step takes
+  // workgroups that a CU takes at once: as many as hide each other's latencies (float32 is bound by its products)
+  const int64_t thick = es == 4 ? 1 : width <= 64 ? 3 : width <= 128 ? 2 : 1;
+  const int64_t reach = (int64_t)a.left + a.right + kQueries;
+  const int64_t keys = ceil_div(std::min<int64_t>(a.S, reach + a.sinks), step), queries = ceil_div(std::min<int64_t>(a.L, reach), step) * a.group;
+  p.bytes = 256;
   if (!backward) {
     const int64_t few_rows = (int64_t)a.L * a.group;
     p.few = few_rows <= kFewRows;
-    p.bytes = 256;
-    if (p.few && !p.empty) {
+    if (p.empty) return GNNHWC_OK;
+    if (p.few) {
       a.tiles = (int)ceil_div(few_rows, 32);
       const int64_t heads = (int64_t)a.B * a.K * a.tiles;
-      // keys that a tile's rows see at most, in tiles of 32; a share is four or more of them
-      const int64_t seen = std::min<int64_t>(a.S, (int64_t)a.left + a.right + a.L + a.sinks + 64), steps = ceil_div(seen, 32);
-      a.splits = (int)std::clamp<int64_t>(ceil_div(kFewItems, heads), 1, std::min<int64_t>(64, std::max<int64_t>(1, steps / kFewSteps)));
+      // keys that a tile's rows see at most, in tiles of 32; a share is kFewSteps or more of them
+      const int64_t seen = std::min<int64_t>(a.S, (int64_t)a.left + a.right + a.L + a.sinks + 64);
+      a.splits = (int)std::clamp<int64_t>(ceil_div(kFewItems, heads), 1, std::min<int64_t>(64, std::max<int64_t>(1, ceil_div(seen, 32) / kFewSteps)));
       a.items = (int)(heads * a.splits);
-      if (a.splits > 1) {
-        p.join = round_up((size_t)a.items * 32 * 2 * sizeof(float));
-        p.bytes += p.join + (size_t)a.items * 32 * a.D * sizeof(float);
-      }
+    } else {
+      a.splits = (int)shares_of(items, keys, thick, 16);
+      a.items = (int)(items * a.splits);
+    }
+    if (a.splits > 1) {
+      p.part_v = round_up((size_t)a.splits * lse * 2 * sizeof(float));
+      p.bytes += p.part_v + (size_t)a.splits * lse * a.D * sizeof(float);
     }
     return GNNHWC_OK;
   }
-
-  // Workgroups of dk and dv.  A key that all queries see (a sink) has many times the others' work, and a short batch has fewer tiles
-  // than the device has room for: several workgroups then share a tile's queries.
-  p.kv = a;
-  WindowArgs &w = p.kv;
+  p.kv = p.sinks = a;
+  if (items) {
+    a.splits = (int)shares_of(items, keys, thick, 16);
+    a.items = (int)(items * a.splits);
+  }
+  WindowArgs &w = p.kv, &k = p.sinks;
   w.tiles = (int)ceil_div(a.S, kQueries);
-  w.sink_tiles = (int)std::min<int64_t>(w.tiles, ceil_div(a.sinks, kQueries));
-  const int64_t step = es == 2 ? 64 : 32, all = ceil_div(a.L, step) * a.group;  // queries that a step takes, steps of a sink's tile
-  const int64_t reach = std::min<int64_t>((int64_t)a.left + a.right + kQueries, a.L);
-  const int64_t usual = std::min(all, (ceil_div(reach, step) + 1) * a.group);
-  const int64_t heads = (int64_t)a.B * a.K, work = heads * (w.sink_tiles * all + (w.tiles - w.sink_tiles) * usual);
-  const int64_t most = std::max<int64_t>(4, work / (8 * kNumCU));  // steps of a workgroup: a quarter of what is for each of two per CU
-  w.shares = (int)std::clamp<int64_t>(ceil_div(usual, most), 1, 256);
-  w.sink_shares = w.sink_tiles ? (int)std::clamp<int64_t>(ceil_div(all, most), 1, 256) : 1;
-  const int64_t per = (int64_t)w.sink_tiles * w.sink_shares + (int64_t)(w.tiles - w.sink_tiles) * w.shares;
-  if (per * heads > kMostItems) return invalid("too many tokens and heads for one call");
-  w.items = (int)(per * heads);
-  w.parts = (int)((w.sink_shares > 1 ? (int64_t)w.sink_tiles * w.sink_shares : 0) + (w.shares > 1 ? (int64_t)(w.tiles - w.sink_tiles) * w.shares : 0));
-  const size_t lse = round_up((size_t)a.B * a.H * a.L * sizeof(float)), part = round_up((size_t)w.parts * heads * kQueries * a.D * sizeof(float));
+  const int64_t heads = (int64_t)a.B * a.K, tiles = heads * w.tiles;
+  w.shares = (int)shares_of(tiles, queries, es == 4 ? 1 : width <= 64 ? 2 : 1, 32);
+  if (tiles * w.shares > kMostItems) return invalid("too many tokens and heads for one call");
+  w.items = (int)(tiles * w.shares);
+  k.items = w.sink_sets = w.sink_parts = 0;
+  if (w.sinks > 0 && w.items > 0) {
+    const int waves = few_waves((int)width, (int)es);
+    w.sink_sets = (int)ceil_div(w.sinks, 32);
+    const int64_t sets = heads * w.sink_sets, steps = ceil_div(a.L, 32) * a.group;
+    const int64_t sink_shares = std::clamp<int64_t>(ceil_div(kNumCU, sets), 1, std::max<int64_t>(1, steps / (4 * waves)));
+    if (sets * sink_shares > kMostItems) return invalid("too many tokens and heads for one call");
+    w.sink_parts = (int)(sink_shares * waves);
+    k = w;
+    k.items = (int)(sets * sink_shares);
+  }
+  const size_t floats = round_up((size_t)lse * sizeof(float));
+  const size_t part = round_up(((size_t)heads * w.sink_sets * w.sink_parts * 32 + (w.shares > 1 ? (size_t)tiles * w.shares * kQueries : 0)) * a.D * sizeof(float));
   p.delta = 0;
-  p.largest = lse;
-  p.part_k = p.largest + (c->dtype == GN_F16 ? lse : 0);
+  p.largest = floats;
+  p.part_q = p.largest + (c->dtype == GN_F16 ? floats : 0);
+  p.part_k = p.part_q + (a.splits > 1 ? round_up((size_t)a.splits * lse * a.D * sizeof(float)) : 0);
   p.part_v = p.part_k + part;
-  p.bytes = 256 + p.part_v + part;
+  p.bytes += p.part_v + part;
   return GNNHWC_OK;
 }
 
@@ -160,9 +195,9 @@ int gnnhwc_window(const gnnhwc_window_call *c, void *workspace, size_t workspace
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes)
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_workspace_bytes");
   if (p.empty) return GNNHWC_OK;
+  p.a.part_k = (float *)workspace;
+  p.a.part_v = (float *)((char *)workspace + p.part_v);
   if (p.few) {
-    p.a.part_k = (float *)workspace;
-    p.a.part_v = (float *)((char *)workspace + p.join);
 #define GN_CALL(S) launch_window_few_##S(p.a, (hipStream_t)stream)
     return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window");
 #undef GN_CALL
@@ -183,14 +218,15 @@ int gnnhwc_window_bwd(const gnnhwc_window_call *c, void *workspace, size_t works
   if (const int rc = plan_window(c, true, p)) return rc;
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes)
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_bwd_workspace_bytes");
-  for (WindowArgs *a : {&p.a, &p.kv}) {
+  for (WindowArgs *a : {&p.a, &p.kv, &p.sinks}) {
     a->delta = (float *)((char *)workspace + p.delta);
     a->largest = (float *)((char *)workspace + p.largest);
+    a->part_q = (float *)((char *)workspace + p.part_q);
     a->part_k = (float *)((char *)workspace + p.part_k);
     a->part_v = (float *)((char *)workspace + p.part_v);
   }
-  if (p.a.items == 0 && p.kv.items == 0) return GNNHWC_OK;
-#define GN_CALL(S) launch_window_backward_##S(p.a, p.kv, (hipStream_t)stream)
+  if (p.kv.items == 0) return GNNHWC_OK;  // (then there are no queries either)
+#define GN_CALL(S) launch_window_backward_##S(p.a, p.kv, p.sinks, (hipStream_t)stream)
   return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window_bwd");
 #undef GN_CALL
 }

@@ -549,7 +549,9 @@ bool window_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor
   const at::ScalarType type = q.scalar_type();
   const int code = code_of(type);
   if (code < 0 || code == GNNHWC_F64 || !rows16(q, device, type) || !rows16(k, device, type) || !rows16(v, device, type)) return false;
-  if (k.size(0) != q.size(0) || k.size(3) != q.size(3) || v.sizes() != k.sizes() || q.size(2) % k.size(2) || q.size(3) % 8 || q.size(3) > 256) return false;
+  if (k.size(0) != q.size(0) || k.size(3) != q.size(3) || v.sizes() != k.sizes() || q.size(2) % k.size(2) || q.size(3) % 8 ||
+      q.size(3) > (code == GNNHWC_F32 ? 128 : 256))
+    return false;
   if (lengths.defined()) {
     if (!plain(lengths, device) || lengths.dim() != 1 || lengths.size(0) != q.size(0) || !lengths.is_contiguous()) return false;
     if (lengths.scalar_type() != at::kInt && lengths.scalar_type() != at::kLong) return false;

@@ -103,11 +103,27 @@ template <typename T, int DP> struct Tile {
 template <typename T, int DP> struct LaneOffsets {
   using G = Tile<T, DP>;
   static constexpr int kRowBytes = G::kChunks * 16;
-  int rows[sizeof(T) == 2 ? 1 : 2][DP / 16], columns[DP / 32][sizeof(T) == 2 ? 2 : 8];
+  // Wide heads keep one step's offsets and make the others of them: the steps' bits are the rows' to neither side.
+  static constexpr bool kCompact = DP * (int)sizeof(T) >= 512;
+  static_assert(!kCompact || (kRowBytes & (kRowBytes - 1)) == 0, "a row's bytes are a power of two");
+  static constexpr int kSteps = kCompact ? 1 : DP / 16, kParts = kCompact ? 1 : DP / 32;
+  int rows[sizeof(T) == 2 ? 1 : 2][kSteps], columns[kParts][sizeof(T) == 2 ? 2 : 8];
+  static __device__ __forceinline__ int step_of(int first, int x, int bytes) {
+    pin(first);  // (or they would all be made ahead of the loop, and kept)
+    return first ^ x * bytes;
+  }
+  __device__ __forceinline__ int row_offset(int i, int x) const {
+    if constexpr (kCompact) return step_of(rows[i][0], x, 16 * (int)sizeof(T));
+    else return rows[i][x];
+  }
+  __device__ __forceinline__ int column_offset(int x, int i) const {
+    if constexpr (kCompact) return step_of(columns[0][i], x, 32 * (int)sizeof(T));
+    else return columns[x][i];
+  }
   __device__ __forceinline__ void init() {
     const int lane = threadIdx.x & 63, h = lane >> 5, row = lane & 31;
 #pragma unroll
-    for (int x = 0; x < DP / 16; ++x) {
+    for (int x = 0; x < kSteps; ++x) {
       if constexpr (sizeof(T) == 2) {
         rows[0][x] = row * kRowBytes + G::chunk_of(row, 2 * x + h) * 16;
       } else {
@@ -116,7 +132,7 @@ template <typename T, int DP> struct LaneOffsets {
       }
     }
 #pragma unroll
-    for (int x = 0; x < DP / 32; ++x) {
+    for (int x = 0; x < kParts; ++x) {
       if constexpr (sizeof(T) == 2) {
         // a group of 16 lanes reads four rows of 16 channels, four to a lane, and each lane is left with a channel
         const int m = lane & 15, r = 4 * h + (m >> 2), chunk = 4 * x + (lane >> 4 & 1) * 2 + (m >> 1 & 1);
@@ -131,9 +147,9 @@ template <typename T, int DP> struct LaneOffsets {
   // Operand whose rows are the tile's rows FIRST .. FIRST + 31 (a multiple of 32), summands 16 x + 8 h ..
   template <int FIRST> __device__ __forceinline__ operand_t<T> of_rows(const char *tile, int x) const {
     if constexpr (sizeof(T) == 2) {
-      return *(const operand_t<T> *)(tile + rows[0][x] + FIRST * kRowBytes);
+      return *(const operand_t<T> *)(tile + row_offset(0, x) + FIRST * kRowBytes);
     } else {
-      const f32x4 a = *(const f32x4 *)(tile + rows[0][x] + FIRST * kRowBytes), b = *(const f32x4 *)(tile + rows[1][x] + FIRST * kRowBytes);
+      const f32x4 a = *(const f32x4 *)(tile + row_offset(0, x) + FIRST * kRowBytes), b = *(const f32x4 *)(tile + row_offset(1, x) + FIRST * kRowBytes);
       return f32x8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
@@ -141,13 +157,13 @@ template <typename T, int DP> struct LaneOffsets {
   template <int FIRST> __device__ __forceinline__ operand_t<T> of_columns(char *tile, int x) const {
     if constexpr (sizeof(T) == 2) {
       typedef __attribute__((address_space(3))) s16x4_t lds4;
-      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + columns[x][0] + FIRST * kRowBytes));
-      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + columns[x][1] + FIRST * kRowBytes));
+      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + column_offset(x, 0) + FIRST * kRowBytes));
+      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + column_offset(x, 1) + FIRST * kRowBytes));
       return __builtin_bit_cast(operand_t<T>, s16x8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     } else {
       f32x8_t r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = *(const float *)(tile + columns[x][i] + FIRST * kRowBytes);
+      for (int i = 0; i < 8; ++i) r[i] = *(const float *)(tile + column_offset(x, i) + FIRST * kRowBytes);
       return r;
     }
   }
@@ -157,6 +173,7 @@ template <typename T, int DP> struct LaneOffsets {
 // for all of them.  (The compiler would have every transposing read wait for all copies that are on their way, other buffers'
 // too: it is not told of these.  Nothing is written to a register but m0, which nothing else here uses; tiles_turn waits.)
 template <int BYTES> __device__ __forceinline__ void copy_to_lds(const char *base, unsigned offset, unsigned to) {
+  to = __builtin_amdgcn_readfirstlane(to);
   if constexpr (BYTES == 16)
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(offset), "s"(to), "s"(base) : "memory");
   else
@@ -252,7 +269,7 @@ __device__ __forceinline__ Seen seen_of(const WindowArgs &a, const Sample &s, in
   Seen g = {0, 0};
   if (j < s.n && s.last > s.first) {
     int lo = j - a.right, hi = j + a.left;
-    if (j < a.sinks) {
+    if (j < a.sinks) {  // by all
       if (!a.causal) lo = 0;
       hi = s.n - 1;
     }
@@ -267,9 +284,6 @@ __device__ __forceinline__ Seen seen_of(const WindowArgs &a, const Sample &s, in
 // Tiles of `rows` keys that a workgroup with queries at places low .. high has to visit: those of the sinks, then the window's.
 struct Walk {
   int sinks, first, last;  // tiles of the sinks; the window's tiles behind them: first .. last
-  __device__ __forceinline__ int start() const { return sinks > 0 ? 0 : first; }
-  __device__ __forceinline__ int next(int t) const { return t + 1 == sinks ? first : t + 1; }
-  __device__ __forceinline__ bool more(int t) const { return t < sinks || t <= last; }
 };
 __device__ __forceinline__ Walk walk_of(const WindowArgs &a, const Sample &s, int low, int high, int rows) {
   Walk w;
@@ -547,14 +561,30 @@ template <typename T, int DP, int N, typename ST> __device__ __forceinline__ voi
   }
 }
 
-// A workgroup: 128 queries of one head, 32 a wavefront.
-template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
+// Steps of a walk that one of `splits` workgroups takes: begin .. end - 1.
+struct Stretch {
+  Walk w;
+  int begin, end;
+  __device__ __forceinline__ int tile(int u) const { return u < w.sinks ? u : w.first + (u - w.sinks); }
+};
+__device__ __forceinline__ Stretch stretch_of(const Walk &w, int split, int splits) {
+  const int steps = w.sinks + (w.last >= w.first ? w.last - w.first + 1 : 0);
+  return {w, (int)((int64_t)steps * split / splits), (int)((int64_t)steps * (split + 1) / splits)};
+}
+// Rows of the results of workgroups that share a row's keys: a split's rows behind each other, then the next split's.
+__device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int b, int h, int i) {
+  return (((int64_t)split * a.B + b) * a.H + h) * a.L + i;
+}
+
+// A workgroup: 128 queries of one head, 32 a wavefront, against one of `splits` shares of the keys that they see.
+template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a.items);
   if (item >= a.items) return;
   // (the heads of a group are neighbours, then the tiles of queries, the last ones, which see most, first)
-  const int g = item % a.group, rest = item / a.group, tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
+  const int g = item % a.group, split = item / a.group % a.splits, rest = item / a.group / a.splits;
+  const int tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
   const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = tile * kQueries + wave * 32 + (lane & 31);
@@ -569,7 +599,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2
   if (from < to) {
     const int ic = i < from ? from : i < to ? i : to - 1;
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
-    const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows);
+    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.splits);
     TileCopy<T, DP, G::kRows, kBlock> ck, cv;
     ck.init(a.D, a.k.token_bytes);
     cv.init(a.D, a.v.token_bytes);
@@ -577,35 +607,43 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2
     at.init();
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
     const unsigned lds = lds_address(tiles) + wave * 1024;
+    auto issue = [&](int u, int buffer) {
+      const int first = w.tile(u) * G::kRows;
+      ck.issue(kb, first, s.n - 1, lds + buffer * 2 * G::kBytes, a.D);
+      cv.issue(vb, first, s.n - 1, lds + buffer * 2 * G::kBytes + G::kBytes, a.D);
+    };
     settle(st.q);
-    int t = w.start();
-    if (w.more(t)) {
-      ck.issue(kb, t * G::kRows, s.n - 1, lds, a.D);
-      cv.issue(vb, t * G::kRows, s.n - 1, lds + G::kBytes, a.D);
-    }
+    int u = w.begin;
+    if (u < w.end) issue(u, 0);
     auto turn = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
-      const int next = w.next(t);
-      if (w.more(next)) {
-        ck.issue(kb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes, a.D);
-        cv.issue(vb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes + G::kBytes, a.D);
-      }
-      forward_tile<T, DP, G::kRows / 32>(st, at, tiles + B * 2 * G::kBytes, tiles + B * 2 * G::kBytes + G::kBytes, t * G::kRows, a.scale_log2);
-      t = next;
+      if (u + 1 < w.end) issue(u + 1, 1 - B);
+      forward_tile<T, DP, G::kRows / 32>(st, at, tiles + B * 2 * G::kBytes, tiles + B * 2 * G::kBytes + G::kBytes, w.tile(u) * G::kRows, a.scale_log2);
+      ++u;
     };
-    while (w.more(t)) {
+    while (u < w.end) {
       turn(std::integral_constant<int, 0>());
-      if (!w.more(t)) break;
+      if (u >= w.end) break;
       turn(std::integral_constant<int, 1>());
     }
   }
   const float sum = st.sum + other_half(st.sum);
-  const bool nothing = st.reference == -INFINITY && sum == 0.0f;  // (of no key seen, or scores of -inf alone: the latter is computed again)
-  const float factor = nothing ? 0.0f : 1.0f / sum;
   const bool there = i < a.L, seeing = st.sight.count > 0 || st.sight.sinks > 0;
-  bool again = any_not_finite(st.o) || !(factor < INFINITY) || nothing;
-  again = either_half(again) && seeing;
+  if (a.splits > 1) {
+    if (there) {
+      const int64_t row = part_row(a, split, b, h, i);
+      store_token<float, DP>(a.part_v + row * a.D, a.D, st.o, 1.0f);
+      if (lane < 32) {
+        store_global<float>(a.part_k + 2 * row, st.reference);
+        store_global<float>(a.part_k + 2 * row + 1, sum);
+      }
+    }
+    return;
+  }
+  const bool nothing = !(sum > 0.0f);  // (no key seen, or no score above -inf: those that see one are computed again)
+  const float factor = nothing ? 0.0f : 1.0f / sum;
+  const bool again = either_half(any_not_finite(st.o) || !(factor < INFINITY) || nothing) && seeing;
   if (there) {
     store_token<T, DP>((T *)a.out.row(b, i, h), a.D, st.o, factor);
     if (a.lse && lane < 32) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, nothing ? INFINITY : st.reference + __builtin_amdgcn_logf(sum));
@@ -625,14 +663,22 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 ? 2
 // several workgroups share a head's keys (splits) and window_join_kernel joins them.
 template <typename T, int DP> struct Few {
   static constexpr int kStage = 2 * 32 * DP * (int)sizeof(T);  // bytes of a tile of keys and one of values
-  static constexpr int kMost = 131072 / (2 * kStage);
-  static constexpr int kWaves = kMost >= 8 ? 8 : kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
+  static constexpr int kWaves = few_waves(DP, sizeof(T));
   static constexpr int kPitch = DP + 4;                     // floats of a row while results are joined
   static_assert(32 * kPitch * 4 <= 2 * kStage, "a wavefront's results fit its tiles");
 };
-template <int COPIES> __device__ __forceinline__ void wait_for_copies(bool newest_too) {
-  if (newest_too) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES < 63 ? COPIES : 63) : "memory");
+// Takes the next tile of a wavefront's own walk: COPIES copies of another one, if there is one, are issued by issue(), into the place of
+// the one before.  Two tiles are on their way while the wavefront waits for the older one.  (That counts the newest copies: nothing
+// else may be among them, so that these kernels must keep no register in scratch memory.)
+template <int COPIES, typename F> __device__ __forceinline__ void next_copies(bool more, F &&issue) {
+  static_assert(COPIES < 64, "what the counter holds");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (reads of the tile that is now overwritten)
+  if (more) {
+    issue();
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES) : "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
 }
 
 // Weight and result of a row that is joined of parts: (reference, sum).
@@ -664,11 +710,8 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   if (from < to) {
     const int ic = i < from ? from : i < to ? i : to - 1;
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
-    const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, 32);
-    const int window = w.last >= w.first ? w.last - w.first + 1 : 0, steps = w.sinks + window;
-    const int begin = (int)((int64_t)steps * split / a.splits), end = (int)((int64_t)steps * (split + 1) / a.splits);
+    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, 32), split, a.splits);
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
-    auto tile_at = [&](int u) { return u < w.sinks ? u : w.first + (u - w.sinks); };
     using Copy = TileCopy<T, DP, 32, 64>;
     Copy ck, cv;
     ck.init(a.D, a.k.token_bytes);
@@ -678,20 +721,17 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
     const unsigned lds = lds_address(tiles) + wave * 2 * W::kStage;
     settle(st.q);
     auto issue = [&](int u, int buffer) {
-      const int first = tile_at(u) * 32;
+      const int first = w.tile(u) * 32;
       ck.issue(kb, first, s.n - 1, lds + buffer * W::kStage, a.D);
       cv.issue(vb, first, s.n - 1, lds + buffer * W::kStage + W::kStage / 2, a.D);
     };
-    int u = begin + wave, turn = 0;
-    if (u < end) issue(u, 0);
-    for (; u < end; u += kWaves) {
+    int u = w.begin + wave, turn = 0;
+    if (u < w.end) issue(u, 0);
+    for (; u < w.end; u += kWaves) {
       char *tile = tiles + (wave * 2 + turn) * W::kStage;
       turn ^= 1;
-      const bool more = u + kWaves < end;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (reads of the tile that is now overwritten)
-      if (more) issue(u + kWaves, turn);
-      wait_for_copies<2 * Copy::kCopies>(!more);
-      forward_tile<T, DP, 1>(st, at, tile, tile + W::kStage / 2, tile_at(u) * 32, a.scale_log2);
+      next_copies<2 * Copy::kCopies>(u + kWaves < w.end, [&] { issue(u + kWaves, turn); });
+      forward_tile<T, DP, 1>(st, at, tile, tile + W::kStage / 2, w.tile(u) * 32, a.scale_log2);
     }
   }
   // join the wavefronts
@@ -729,7 +769,7 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
 #pragma unroll
     for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)(tiles + n * 2 * W::kStage) + r * W::kPitch + d);
     if (a.splits > 1) {
-      store_global<f32x4>(a.part_v + ((int64_t)item * 32 + r) * a.D + d, v);
+      store_global<f32x4>(a.part_v + part_row(a, split, b, kh * a.group + rr % a.group, rr / a.group) * a.D + d, v);
       continue;
     }
     const float total = sums[0][r], factor = total > 0.0f ? 1.0f / total : 0.0f;
@@ -739,8 +779,9 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
     LV::store((T *)a.out.row(b, rr / a.group, kh * a.group + rr % a.group) + d, LV::pack(t));
   }
   if (a.splits > 1) {
-    if (threadIdx.x < 32) {
-      float *p = a.part_k + ((int64_t)item * 32 + threadIdx.x) * 2;
+    const int rr = block * 32 + (int)threadIdx.x;
+    if (threadIdx.x < 32 && rr < rows) {
+      float *p = a.part_k + 2 * part_row(a, split, b, kh * a.group + rr % a.group, rr / a.group);
       store_global<float>(p, references[0][threadIdx.x]);
       store_global<float>(p + 1, sums[0][threadIdx.x]);
     }
@@ -758,24 +799,22 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   }
 }
 
-// Rows that several workgroups share: a wavefront each.
+// Rows whose keys several workgroups shared: a wavefront each.
 template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kernel(const WindowArgs a) {
-  const int lane = threadIdx.x & 63, rows = a.L * a.group;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t bk64 = id / rows;
-  if (bk64 >= (int64_t)a.B * a.K) return;
-  const int bk = (int)bk64, row = (int)(id % rows), b = bk / a.K, kh = bk % a.K, i = row / a.group, h = kh * a.group + row % a.group;
-  const int64_t slot = (((int64_t)bk * a.tiles + row / 32) * a.splits) * 32 + row % 32;
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.B * a.H * a.L;
+  if (id >= rows) return;
+  const int i = (int)(id % a.L), h = (int)(id / a.L % a.H), b = (int)(id / a.L / a.H);
   // (a lane holds a split's reference and sum: at most 64 splits)
-  const float reference = lane < a.splits ? load_global<float>(a.part_k + (slot + lane * 32) * 2) : -INFINITY;
-  const float part = lane < a.splits ? load_global<float>(a.part_k + (slot + lane * 32) * 2 + 1) : 0.0f;
+  const float reference = lane < a.splits ? load_global<float>(a.part_k + 2 * (id + lane * rows)) : -INFINITY;
+  const float part = lane < a.splits ? load_global<float>(a.part_k + 2 * (id + lane * rows) + 1) : 0.0f;
   const float most = wave_max(reference), weight = part_weight(reference, most), sum = wave_sum(part * weight);
   float o[4] = {}, bad = 0.0f;
   for (int n = 0; n < a.splits; ++n) {
     const float w = __shfl(weight, n);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      if (x * 64 + lane < a.D) o[x] = __builtin_fmaf(w, load_global<float>(a.part_v + (slot + (int64_t)n * 32) * a.D + x * 64 + lane), o[x]);
+      if (x * 64 + lane < a.D) o[x] = __builtin_fmaf(w, load_global<float>(a.part_v + (id + n * rows) * a.D + x * 64 + lane), o[x]);
   }
   const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
@@ -785,10 +824,11 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
       const float t[1] = {o[x] * factor};
       LaneVec<T, 1>::store((T *)a.out.row(b, i, h) + x * 64 + lane, LaneVec<T, 1>::pack(t));
     }
-  if (a.lse && lane == 0) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, sum > 0.0f ? most + __builtin_amdgcn_logf(sum) : INFINITY);
+  if (a.lse && lane == 0) store_global<float>(a.lse + id, sum > 0.0f ? most + __builtin_amdgcn_logf(sum) : INFINITY);
+  if (!__any(!(bad == 0.0f)) && sum > 0.0f) return;
   const Sample s = sample_of(a, b);
   const Sight g = sight_of(a, s, i);
-  if ((__any(!(bad == 0.0f)) || !(sum > 0.0f)) && (g.count > 0 || g.sinks > 0)) row_again<T>(a, s, b, h, i);
+  if (g.count > 0 || g.sinks > 0) row_again<T>(a, s, b, h, i);
 }
 
 // ---- backward: dq ----
@@ -806,7 +846,8 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a.items);
   if (item >= a.items) return;
-  const int g = item % a.group, rest = item / a.group, tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
+  const int g = item % a.group, split = item / a.group % a.splits, rest = item / a.group / a.splits;
+  const int tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
   const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, i = tile * kQueries + wave * 32 + (lane & 31);
@@ -834,14 +875,14 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
       delta += other_half(delta);
       most = fmaxf(most, other_half(most));
       unit = gradient_unit<T>(most);
-      if (i >= from && i < to && lane < 32) {
+      if (split == 0 && i >= from && i < to && lane < 32) {
         store_global<float>(a.delta + row, -delta);
         if constexpr (__is_same(T, f16_t)) store_global<float>(a.largest + row, most);
       }
     }
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, q);
     if (i >= from && i < to) lse = load_global<float>(a.lse + row);
-    const Walk w = walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows);
+    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.splits);
     TileCopy<T, DP, G::kRows, kBlock> ck, cv;
     ck.init(a.D, a.k.token_bytes);
     cv.init(a.D, a.v.token_bytes);
@@ -859,23 +900,22 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
     settle(q);
     settle(dout);
     pin(lift);
-    int t = w.start();
-    if (w.more(t)) {
-      ck.issue(kb, t * G::kRows, s.n - 1, lds, a.D);
-      cv.issue(vb, t * G::kRows, s.n - 1, lds + G::kBytes, a.D);
-    }
+    auto issue = [&](int u, int buffer) {
+      const int first = w.tile(u) * G::kRows;
+      ck.issue(kb, first, s.n - 1, lds + buffer * 2 * G::kBytes, a.D);
+      cv.issue(vb, first, s.n - 1, lds + buffer * 2 * G::kBytes + G::kBytes, a.D);
+    };
+    int u = w.begin;
+    if (u < w.end) issue(u, 0);
     auto turn = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
-      const int next = w.next(t);
-      if (w.more(next)) {
-        ck.issue(kb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes, a.D);
-        cv.issue(vb, next * G::kRows, s.n - 1, lds + (1 - B) * 2 * G::kBytes + G::kBytes, a.D);
-      }
+      if (u + 1 < w.end) issue(u + 1, 1 - B);
+      const int place0 = w.tile(u) * G::kRows;
       char *kt = tiles + B * 2 * G::kBytes, *vt = kt + G::kBytes;
       auto part = [&](auto first) {
         constexpr int f = decltype(first)::value;
-        const int j0 = t * G::kRows + f, left = j0 - sight.low;
+        const int j0 = place0 + f, left = j0 - sight.low;
         const bool inside = (left >= 0 && left + 32 <= sight.count) || j0 + 32 <= sight.sinks;
         const bool whole = __all(inside);
         if (!whole && !__any((left + 32 > 0 && left < sight.count) || j0 < sight.sinks)) return;
@@ -902,20 +942,23 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
       };
       part(std::integral_constant<int, 0>());
       if constexpr (G::kRows == 64) part(std::integral_constant<int, 32>());
-      t = next;
+      ++u;
     };
-    while (w.more(t)) {
+    while (u < w.end) {
       turn(std::integral_constant<int, 0>());
-      if (!w.more(t)) break;
+      if (u >= w.end) break;
       turn(std::integral_constant<int, 1>());
     }
   }
   const bool there = i < a.L, seeing = sight.count > 0 || sight.sinks > 0;
-  bool again = any_not_finite(acc);
-  again = either_half(again) && seeing && there;
+  const bool again = either_half(any_not_finite(acc)) && seeing && there;
   if (there) {
-    const float factor = a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f);
-    store_token<T, DP>((T *)a.dq.row(b, i, h), a.D, acc, seeing ? factor : 0.0f);
+    const float factor = seeing ? a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f) : 0.0f;
+    if (a.splits > 1) {
+      store_token<float, DP>(a.part_q + part_row(a, split, b, h, i) * a.D, a.D, acc, factor);
+      return;
+    }
+    store_token<T, DP>((T *)a.dq.row(b, i, h), a.D, acc, factor);
   }
   uint64_t rows = __ballot(again) & 0xffffffffu;
   while (rows) {
@@ -926,183 +969,254 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
 }
 static_assert(kGradBits == 5.0f, "the factors of 1 / 32 undo it");
 
-// ---- backward: dk and dv ----
-// Where the workgroup `at` of a head leaves its sums: those of tiles that several share have a place.
-__device__ __forceinline__ int64_t part_slot(const WindowArgs &a, int bk, int at) {
-  const int sink_items = a.sink_tiles * a.sink_shares;
-  return (int64_t)bk * a.parts + (at < sink_items || a.sink_shares > 1 ? at : at - sink_items);
+// dq of rows whose keys several workgroups shared: four channels of a row each thread.
+template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_kernel(const WindowArgs a) {
+  __shared__ int bad[kBlock];
+  const int quads = a.D / 4, rows_here = kBlock / quads, r = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+  const int64_t rows = (int64_t)a.B * a.H * a.L, id = (int64_t)blockIdx.x * rows_here + r;
+  bad[threadIdx.x] = 0;
+  __syncthreads();
+  if (r < rows_here && id < rows) {
+    f32x4 q = {};
+#pragma unroll 4
+    for (int n = 0; n < a.splits; ++n) q += load_global<f32x4>(a.part_q + (id + n * rows) * a.D + d);
+    const float t[4] = {q[0], q[1], q[2], q[3]};
+    using LV = LaneVec<T, 4>;
+    LV::store((T *)a.dq.row((int)(id / a.L / a.H), (int)(id % a.L), (int)(id / a.L % a.H)) + d, LV::pack(t));
+    if (!(q[0] * 0.0f + q[1] * 0.0f + q[2] * 0.0f + q[3] * 0.0f == 0.0f)) bad[r] = 1;
+  }
+  __syncthreads();
+  for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
+    if (!bad[n]) continue;
+    const int64_t row = (int64_t)blockIdx.x * rows_here + n;
+    const int i = (int)(row % a.L), h = (int)(row / a.L % a.H), b = (int)(row / a.L / a.H);
+    const Sample s = sample_of(a, b);
+    const Sight g = sight_of(a, s, i);
+    if (g.count > 0 || g.sinks > 0) dq_again<T>(a, s, b, h, i, load_global<float>(a.lse + row), -load_global<float>(a.delta + row));
+  }
 }
-// A workgroup: 128 keys of one head, 32 a wavefront, against a share of the queries that see any of them, of all heads of the
-// group.  PARTS: 1 dv, 2 dk, 3 both (heads of more than 128 channels do not fit the registers at once).  Where several workgroups
-// share a tile's queries, each leaves float32 sums, which window_sum_kernel adds in their order.
+
+// ---- backward: dk and dv ----
+// Ends a phase of a kernel that reads its operands from shared memory a phase ahead of the products that take them: nothing is
+// moved across (the compiler would read each right in front of its product and wait).
+template <bool AHEAD> __device__ __forceinline__ void phase_end() {
+  if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+}
+
+// 32 keys of a wavefront, one a lane.  PARTS: 1 dv, 2 dk, 3 both (heads of more than 128 channels do not fit the registers at once).
+template <typename T, int DP, int PARTS> struct KeySide {
+  static constexpr bool kDv = PARTS & 1, kDk = PARTS & 2;
+  static constexpr bool kAhead = DP <= (sizeof(T) == 2 ? 128 : 64);
+  operand_t<T> k[DP / 16], v[kDk ? DP / 16 : 1];
+  f32x16_t dk[kDk ? DP / 32 : 1], dv[kDv ? DP / 32 : 1];
+  Seen seen;
+  float c, lowering;  // scale; float16: 2^(kGradBits - kWeightBits) times the unit of the gradients
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) {
+      if constexpr (kDk) dk[x] = zeros16();
+      if constexpr (kDv) dv[x] = zeros16();
+    }
+  }
+  __device__ __forceinline__ void load(const WindowArgs &a, int b, int j, int kh) {
+    load_token<T, DP>((const T *)a.k.row(b, j, kh), a.D, k);
+    if constexpr (kDk) load_token<T, DP>((const T *)a.v.row(b, j, kh), a.D, v);
+  }
+  __device__ __forceinline__ void settle_operands() {
+    settle(k);
+    if constexpr (kDk) settle(v);
+  }
+  // ROWS queries, the first at place `place`; their lse and -delta lie beside the tiles.
+  template <int ROWS> __device__ __forceinline__ void tile(const LaneOffsets<T, DP> &at, char *qt, char *gt, const float *lses, const float *deltas, int place) {
+    const int half = (threadIdx.x & 63) >> 5;
+    if (!__any(place + ROWS > seen.from && place < seen.from + seen.count)) return;
+    operand_t<T> qr[DP / 16], gr[kDk ? DP / 16 : 1];
+    f32x16_t dp;
+    auto read_rows = [&](auto first_row) {
+      constexpr int f = decltype(first_row)::value;
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x) qr[x] = at.template of_rows<f>(qt, x);
+      if constexpr (kDk) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {  // (the product starts from -delta)
+          const f32x4 d4 = *(const f32x4 *)&deltas[f + row_of(r, half)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[r + e] = d4[e];
+        }
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) gr[x] = at.template of_rows<f>(gt, x);
+      }
+    };
+    auto part = [&](auto first_row, auto is_last) {
+      constexpr int f = decltype(first_row)::value;
+      f32x16_t p, lse;
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x) p = Operand<T>::product(qr[x], k[x], x ? p : zeros16());
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4 l4 = *(const f32x4 *)&lses[f + row_of(r, half)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lse[r + e] = l4[e];
+      }
+      operand_t<T> gc[kDv ? DP / 32 : 1][2], qc[kDk ? DP / 32 : 1][2];
+      if constexpr (kDv) {
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) gc[x][0] = at.template of_columns<f>(gt, x), gc[x][1] = at.template of_columns<f + 16>(gt, x);
+      }
+      phase_end<kAhead>();
+      if constexpr (kDk) {
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) dp = Operand<T>::product(gr[x], v[x], dp);
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) qc[x][0] = at.template of_columns<f>(qt, x), qc[x][1] = at.template of_columns<f + 16>(qt, x);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], c, __is_same(T, f16_t) ? kWeightBits - lse[r] : -lse[r]));
+      if (!__all(place + f >= seen.from && place + f + 32 <= seen.from + seen.count)) {
+        int left = place + f - seen.from;
+        pin(left);  // (so that the comparisons stay here)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool hidden = (unsigned)(left + row_of(r, half)) >= (unsigned)seen.count;
+          if (hidden) p[r] = 0.0f;
+          if constexpr (kDk) {
+            if (hidden) dp[r] = 0.0f;  // (which may be infinite)
+          }
+        }
+      }
+      phase_end<kAhead>();
+      if constexpr (kDv) {
+        const operand_t<T> w[2] = {operand_of<T>(p, 0), operand_of<T>(p, 1)};
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) dv[x] = Operand<T>::product(gc[x][u], w[u], dv[x]);
+      }
+      if constexpr (kDk) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if constexpr (__is_same(T, f16_t)) p[r] *= lowering;
+          p[r] *= dp[r];
+        }
+      }
+      if constexpr (!decltype(is_last)::value) read_rows(std::integral_constant<int, f + 32>());
+      phase_end<kAhead>();
+      if constexpr (kDk) {
+        const operand_t<T> w[2] = {operand_of<T>(p, 0), operand_of<T>(p, 1)};
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) dk[x] = Operand<T>::product(qc[x][u], w[u], dk[x]);
+      }
+    };
+    read_rows(std::integral_constant<int, 0>());
+    if constexpr (ROWS == 64) {
+      part(std::integral_constant<int, 0>(), std::false_type());
+      part(std::integral_constant<int, 32>(), std::true_type());
+    } else {
+      part(std::integral_constant<int, 0>(), std::true_type());
+    }
+  }
+  static __device__ __forceinline__ float v_factor() { return __is_same(T, f16_t) ? 1.0f / 4096.0f : 1.0f; }
+  static __device__ __forceinline__ float k_factor(const WindowArgs &a, float unit) { return a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f); }
+};
+static_assert(kWeightBits == 12.0f, "the factors of 1 / 4096 and 1 / 128 undo it");
+
+// The queries that see any of the keys j0 .. top - 1 (of the window, or as sinks): from .. to.
+struct Queries {
+  int from, to;
+};
+__device__ __forceinline__ Queries queries_of(const WindowArgs &a, const Sample &s, int j0, int top, bool sinks) {
+  if (j0 >= top || s.first >= s.last) return {0, -1};
+  const int least = s.first + s.off, most = s.last - 1 + s.off;
+  const int lo = sinks ? (a.causal ? j0 : 0) : j0 - a.right, hi = sinks ? s.n - 1 : top - 1 + a.left;
+  return {(lo > least ? lo : least) - s.off, (hi < most ? hi : most) - s.off};
+}
+// A step of a walk over queries: a head of the group, a tile.
+struct Step {
+  int g, t;
+  __device__ __forceinline__ void advance(int by, int tiles) {
+    t += by;
+    while (t >= tiles) {
+      t -= tiles;
+      ++g;
+    }
+  }
+};
+// Where workgroups that share keys leave their sums of rows: first the sinks', 32 keys at a time, then those of tiles.
+__device__ __forceinline__ int64_t sink_slot(const WindowArgs &a, int bk, int set, int part) { return (((int64_t)bk * a.sink_sets + set) * a.sink_parts + part) * 32; }
+__device__ __forceinline__ int64_t tile_slot(const WindowArgs &a, int bk, int tile, int share) {
+  return (int64_t)a.B * a.K * a.sink_sets * a.sink_parts * 32 + (((int64_t)bk * a.tiles + tile) * a.shares + share) * kQueries;
+}
+
+// A workgroup: 128 keys of one head, 32 a wavefront, against a share of the queries whose windows have any of them, of all heads of
+// the group.  Where several share a tile's queries, each leaves float32 sums, which window_sum_kernel adds in their order.  Sinks,
+// which all queries see, are left to window_sink_kernel.
 template <typename T, int DP, int PARTS>
-__global__ __launch_bounds__(kBlock, DP <= 96 && sizeof(T) == 2 ? 2 : 1) void window_dkv_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void window_dkv_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
-  constexpr bool kDv = PARTS & 1, kDk = PARTS & 2;
+  using KS = KeySide<T, DP, PARTS>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // queries and gradients, two deep
   __shared__ __attribute__((aligned(16))) float lses[2 * 64], deltas[2 * 64];
   __shared__ float reduce[4];
   const int item = work_item(a.items);
   if (item >= a.items) return;
-  // first the shares of the sinks' tiles, then the others
-  const int sink_items = a.sink_tiles * a.sink_shares, per = sink_items + (a.tiles - a.sink_tiles) * a.shares;
-  const int bk = item / per, at = item % per, b = bk / a.K, kh = bk % a.K;
-  int tile, share, shares;
-  if (at < sink_items) {
-    shares = a.sink_shares;
-    tile = at / shares;
-    share = at % shares;
-  } else {
-    shares = a.shares;
-    tile = a.sink_tiles + (at - sink_items) / shares;
-    share = (at - sink_items) % shares;
-  }
+  const int share = item % a.shares, tile = item / a.shares % a.tiles, bk = item / a.shares / a.tiles, b = bk / a.K, kh = bk % a.K;
   const Sample s = sample_of(a, b);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, j = tile * kQueries + wave * 32 + (lane & 31);
-  const Seen seen = seen_of(a, s, j);
-  f32x16_t dk[kDk ? DP / 32 : 1], dv[kDv ? DP / 32 : 1];
-#pragma unroll
-  for (int x = 0; x < DP / 32; ++x) {
-    if constexpr (kDk) dk[x] = zeros16();
-    if constexpr (kDv) dv[x] = zeros16();
-  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), j = tile * kQueries + wave * 32 + (lane & 31);
+  const bool ours = j >= a.sinks && j < a.S;
+  KS key;
+  key.clear();
+  key.seen = ours ? seen_of(a, s, j) : Seen{0, 0};
+  key.c = a.scale_log2;
   float unit = 1.0f;
-  // the queries that see any key of the tile: those of its first key, of its last, and what is between
-  const int top = (tile + 1) * kQueries < s.n ? (tile + 1) * kQueries : s.n;
-  int from = 0, to = -1;
-  if (tile * kQueries < top && s.first < s.last) {
-    const int j0 = tile * kQueries, least = s.first + s.off, most = s.last - 1 + s.off;
-    from = j0 > a.right ? j0 - a.right : 0;
-    to = top - 1 + a.left;
-    if (j0 < a.sinks) {
-      if (!a.causal) from = 0;
-      to = s.n - 1;
-    }
-    from = (from > least ? from : least) - s.off;
-    to = (to < most ? to : most) - s.off;
-  }
-  if (from <= to) {
-    const int first = from / G::kRows, tiles_of = to / G::kRows - first + 1, steps = tiles_of * a.group;
-    const int begin = (int)((int64_t)steps * share / shares), end = (int)((int64_t)steps * (share + 1) / shares);
+  const int j0 = tile * kQueries > a.sinks ? tile * kQueries : a.sinks, top = (tile + 1) * kQueries < s.n ? (tile + 1) * kQueries : s.n;
+  const Queries range = queries_of(a, s, j0, top, false);
+  if (range.from <= range.to) {
+    const int first = range.from / G::kRows, tiles_of = range.to / G::kRows - first + 1, steps = tiles_of * a.group, to = range.to;
+    const int begin = (int)((int64_t)steps * share / a.shares), end = (int)((int64_t)steps * (share + 1) / a.shares);
     if constexpr (__is_same(T, f16_t)) {
       float most = 0.0f;
-      for (int st = begin; st < end; ++st) {
+      for (int st = begin + wave; st < end; st += 4) {
         const int64_t rows = ((int64_t)b * a.H + kh * a.group + st / tiles_of) * a.L;
-        const int i = (first + st % tiles_of) * G::kRows + (int)(threadIdx.x & 63);
-        if (wave == (st & 3) && i >= from && i <= to) most = fmaxf(most, load_global<float>(a.largest + rows + i));
+        const int i = (first + st % tiles_of) * G::kRows + lane;
+        if (i >= range.from && i <= to) most = fmaxf(most, load_global<float>(a.largest + rows + i));
       }
       most = wave_max(most);
       if (lane == 0) reduce[wave] = most;
       __syncthreads();
-      most = fmaxf(fmaxf(reduce[0], reduce[1]), fmaxf(reduce[2], reduce[3]));
-      unit = gradient_unit<T>(most);
+      unit = gradient_unit<T>(fmaxf(fmaxf(reduce[0], reduce[1]), fmaxf(reduce[2], reduce[3])));
     }
-    operand_t<T> k[DP / 16], v[kDk ? DP / 16 : 1];
-    const int jc = j < s.n ? j : s.n - 1;
-    load_token<T, DP>((const T *)a.k.row(b, jc, kh), a.D, k);
-    if constexpr (kDk) load_token<T, DP>((const T *)a.v.row(b, jc, kh), a.D, v);
+    key.lowering = unit * (1.0f / 128.0f);
+    key.load(a, b, j < s.n ? j : s.n - 1, kh);
     TileCopy<T, DP, G::kRows, kBlock> cq, cg;
     cq.init(a.D, a.q.token_bytes);
     cg.init(a.D, a.dout.token_bytes);
     LaneOffsets<T, DP> at;
     at.init();
     const unsigned lds = lds_address(tiles) + wave * 1024, lds_lse = lds_address(lses), lds_delta = lds_address(deltas);
-    settle(k);
-    if constexpr (kDk) settle(v);
-    // step: a head of the group, a tile of queries
-    struct Step {
-      int g, t;
-    };
-    auto advance = [&](Step w) {
-      ++w.t;
-      if (w.t == tiles_of) {
-        w.t = 0;
-        ++w.g;
-      }
-      return w;
-    };
+    key.settle_operands();
     auto issue = [&](Step w, int buffer) {
       const int h = kh * a.group + w.g, i0 = (first + w.t) * G::kRows;
       cq.issue((const char *)a.q.row(b, 0, h), i0, to, lds + buffer * 2 * G::kBytes, a.D);
       cg.issue((const char *)a.dout.row(b, 0, h), i0, to, lds + buffer * 2 * G::kBytes + G::kBytes, a.D);
-      if (wave < (kDk ? 2 : 1)) {
+      if (wave < (KS::kDk ? 2 : 1)) {
         const int r = lane < to - i0 ? lane : to - i0;
-        const char *from = (const char *)((wave ? a.delta : a.lse) + ((int64_t)b * a.H + h) * a.L + i0);
-        copy_to_lds<4>(uniform(from), (unsigned)r * 4, (wave ? lds_delta : lds_lse) + buffer * 256);
+        const char *rows = (const char *)((wave ? a.delta : a.lse) + ((int64_t)b * a.H + h) * a.L + i0);
+        copy_to_lds<4>(uniform(rows), (unsigned)r * 4, (wave ? lds_delta : lds_lse) + buffer * 256);
       }
     };
-    const float lowering = __is_same(T, f16_t) ? unit * (1.0f / 128.0f) : 1.0f;  // 2^(kGradBits - kWeightBits)
     int left_over = end - begin;
-    Step step = {begin / tiles_of, begin % tiles_of};
+    Step step = {begin / tiles_of, begin % tiles_of}, next = step;
     if (left_over > 0) issue(step, 0);
     auto turn = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
-      const Step next = advance(step);
+      next.advance(1, tiles_of);
       if (--left_over > 0) issue(next, 1 - B);
-      char *qt = tiles + B * 2 * G::kBytes, *gt = qt + G::kBytes;
-      auto part = [&](auto first_row) {
-        constexpr int f = decltype(first_row)::value;
-        const int left = (first + step.t) * G::kRows + f + s.off - seen.from;
-        const bool inside = left >= 0 && left + 32 <= seen.count, whole = __all(inside);
-        if (!whole && !__any(left + 32 > 0 && left < seen.count)) return;
-        f32x16_t p, dp;
-        if constexpr (kDk) {
-#pragma unroll
-          for (int r = 0; r < 16; r += 4) {  // (the product starts from -delta)
-            const f32x4 d4 = *(const f32x4 *)&deltas[B * 64 + f + row_of(r, half)];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dp[r + e] = d4[e];
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < DP / 16; ++x) {
-          p = Operand<T>::product(at.template of_rows<f>(qt, x), k[x], x ? p : zeros16());
-          if constexpr (kDk) dp = Operand<T>::product(at.template of_rows<f>(gt, x), v[x], dp);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const f32x4 l4 = *(const f32x4 *)&lses[B * 64 + f + row_of(r, half)];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (__is_same(T, f16_t)) p[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r + e], a.scale_log2, kWeightBits - l4[e]));
-            else p[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r + e], a.scale_log2, -l4[e]));
-          }
-        }
-        if (!whole) {
-          int from_here = left;
-          pin(from_here);  // (so that the comparisons stay here)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const bool hidden = (unsigned)(from_here + row_of(r, half)) >= (unsigned)seen.count;
-            if (hidden) p[r] = 0.0f;
-            if constexpr (kDk) {
-              if (hidden) dp[r] = 0.0f;  // (which may be infinite)
-            }
-          }
-        }
-        if constexpr (kDv) {
-          const operand_t<T> w0 = operand_of<T>(p, 0), w1 = operand_of<T>(p, 1);
-#pragma unroll
-          for (int x = 0; x < DP / 32; ++x) dv[x] = Operand<T>::product(at.template of_columns<f>(gt, x), w0, dv[x]);
-#pragma unroll
-          for (int x = 0; x < DP / 32; ++x) dv[x] = Operand<T>::product(at.template of_columns<f + 16>(gt, x), w1, dv[x]);
-        }
-        if constexpr (kDk) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            if constexpr (__is_same(T, f16_t)) p[r] *= lowering;
-            p[r] *= dp[r];
-          }
-          const operand_t<T> s0 = operand_of<T>(p, 0), s1 = operand_of<T>(p, 1);
-#pragma unroll
-          for (int x = 0; x < DP / 32; ++x) dk[x] = Operand<T>::product(at.template of_columns<f>(qt, x), s0, dk[x]);
-#pragma unroll
-          for (int x = 0; x < DP / 32; ++x) dk[x] = Operand<T>::product(at.template of_columns<f + 16>(qt, x), s1, dk[x]);
-        }
-      };
-      part(std::integral_constant<int, 0>());
-      if constexpr (G::kRows == 64) part(std::integral_constant<int, 32>());
+      char *qt = tiles + B * 2 * G::kBytes;
+      key.template tile<G::kRows>(at, qt, qt + G::kBytes, lses + B * 64, deltas + B * 64, (first + step.t) * G::kRows + s.off);
       step = next;
     };
     while (left_over > 0) {
@@ -1111,71 +1225,135 @@ __global__ __launch_bounds__(kBlock, DP <= 96 && sizeof(T) == 2 ? 2 : 1) void wi
       turn(std::integral_constant<int, 1>());
     }
   }
-  const bool there = j < a.S;
-  const float v_factor = __is_same(T, f16_t) ? 1.0f / 4096.0f : 1.0f, k_factor = a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f);
-  if (shares > 1) {
-    // (rows of D floats, the shares of a tile behind each other)
-    const int64_t slot = part_slot(a, bk, at) * kQueries + wave * 32 + (lane & 31);
-    if constexpr (kDk) store_token<float, DP>(a.part_k + slot * a.D, a.D, dk, k_factor);
-    if constexpr (kDv) store_token<float, DP>(a.part_v + slot * a.D, a.D, dv, v_factor);
+  if (a.shares > 1) {
+    const int64_t slot = tile_slot(a, bk, tile, share) + wave * 32 + (lane & 31);
+    if constexpr (KS::kDk) store_token<float, DP>(a.part_k + slot * a.D, a.D, key.dk, KS::k_factor(a, unit));
+    if constexpr (KS::kDv) store_token<float, DP>(a.part_v + slot * a.D, a.D, key.dv, KS::v_factor());
     return;
   }
-  if (there) {
-    if constexpr (kDk) store_token<T, DP>((T *)a.dk.row(b, j, kh), a.D, dk, k_factor);
-    if constexpr (kDv) store_token<T, DP>((T *)a.dv.row(b, j, kh), a.D, dv, v_factor);
+  if (ours) {
+    if constexpr (KS::kDk) store_token<T, DP>((T *)a.dk.row(b, j, kh), a.D, key.dk, KS::k_factor(a, unit));
+    if constexpr (KS::kDv) store_token<T, DP>((T *)a.dv.row(b, j, kh), a.D, key.dv, KS::v_factor());
   }
-  bool bad_k = false, bad_v = false;
-  if constexpr (kDk) bad_k = any_not_finite(dk);
-  if constexpr (kDv) bad_v = any_not_finite(dv);
-  const bool counts = there && seen.count > 0;
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const bool bad = part ? bad_k : bad_v;
-    uint64_t rows = __ballot(either_half(bad) && counts) & 0xffffffffu;
+  bool bad[2] = {false, false};
+  if constexpr (KS::kDv) bad[0] = any_not_finite(key.dv);
+  if constexpr (KS::kDk) bad[1] = any_not_finite(key.dk);
+  for (int of_k = 0; of_k < 2; ++of_k) {
+    uint64_t rows = __ballot(either_half(of_k ? bad[1] : bad[0]) && key.seen.count > 0) & 0xffffffffu;
     while (rows) {
       const int r = __builtin_ctzll(rows);
       rows &= rows - 1;
-      dkv_again<T>(a, s, b, kh, tile * kQueries + wave * 32 + r, part == 1);
+      dkv_again<T>(a, s, b, kh, tile * kQueries + wave * 32 + r, of_k == 1);
     }
   }
 }
-static_assert(kWeightBits == 12.0f, "the factors of 1 / 4096 and 1 / 128 undo it");
 
-// The shares' sums: a wavefront per row.
-template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kernel(const WindowArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  // rows of the tiles that were shared: the sinks', or all
-  const int shared_tiles = a.shares > 1 ? a.tiles : a.sink_tiles, skipped = a.sink_shares > 1 ? 0 : a.sink_tiles;
-  const int rows = (shared_tiles - skipped) * kQueries;
-  const int bk = (int)(id / rows), r = (int)(id % rows);
-  const int tile = skipped + r / kQueries, j = tile * kQueries + r % kQueries, b = bk / a.K, kh = bk % a.K;
-  if (bk >= a.B * a.K || j >= a.S) return;
-  const int shares = tile < a.sink_tiles ? a.sink_shares : a.shares;
-  const int first = tile < a.sink_tiles ? tile * a.sink_shares : a.sink_tiles * a.sink_shares + (tile - a.sink_tiles) * a.shares;
-  const int64_t slot = part_slot(a, bk, first) * kQueries + r % kQueries;
+// dk and dv of the sinks: 32 keys, which all wavefronts hold, against a share of all queries, of which each wavefront walks its own
+// (a tile of 128 keys with a few sinks would have three of four wavefronts idle most of the way).  Every wavefront leaves sums.
+template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void window_sink_kernel(const WindowArgs a) {
+  using W = Few<T, DP>;
+  using KS = KeySide<T, DP, PARTS>;
+  constexpr int kWaves = W::kWaves;
+  __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * W::kStage];
+  __shared__ __attribute__((aligned(16))) float lses[kWaves * 2 * 64], deltas[kWaves * 2 * 64];
+  const int item = work_item(a.items);
+  if (item >= a.items) return;
+  const int shares = a.sink_parts / kWaves, share = item % shares, set = item / shares % a.sink_sets, bk = item / shares / a.sink_sets, b = bk / a.K, kh = bk % a.K;
   const Sample s = sample_of(a, b);
-  const Seen seen = seen_of(a, s, j);
-  float k[4] = {}, v[4] = {}, bad_k = 0.0f, bad_v = 0.0f;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int d = x * 64 + lane;
-    if (d < a.D) {
-      for (int n = 0; n < shares; ++n) {
-        const int64_t e = (slot + (int64_t)n * kQueries) * a.D + d;
-        k[x] += load_global<float>(a.part_k + e);
-        v[x] += load_global<float>(a.part_v + e);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), j = set * 32 + (lane & 31);
+  KS key;
+  key.clear();
+  key.seen = j < a.sinks ? seen_of(a, s, j) : Seen{0, 0};
+  key.c = a.scale_log2;
+  float unit = 1.0f;
+  int top = (set + 1) * 32 < s.n ? (set + 1) * 32 : s.n;
+  top = top < a.sinks ? top : a.sinks;
+  const Queries range = queries_of(a, s, set * 32, top, true);
+  if (range.from <= range.to) {
+    const int first = range.from / 32, tiles_of = range.to / 32 - first + 1, steps = tiles_of * a.group, to = range.to;
+    const int begin = (int)((int64_t)steps * share / shares) + wave, end = (int)((int64_t)steps * (share + 1) / shares);
+    if constexpr (__is_same(T, f16_t)) {
+      float most = 0.0f;
+      for (int st = begin; st < end; st += kWaves) {
+        const int64_t rows = ((int64_t)b * a.H + kh * a.group + st / tiles_of) * a.L;
+        const int i = (first + st % tiles_of) * 32 + (lane & 31);
+        if (i >= range.from && i <= to) most = fmaxf(most, load_global<float>(a.largest + rows + i));
       }
-      bad_k = __builtin_fmaf(k[x], 0.0f, bad_k);
-      bad_v = __builtin_fmaf(v[x], 0.0f, bad_v);
-      const float tk[1] = {k[x]}, tv[1] = {v[x]};
-      LaneVec<T, 1>::store((T *)a.dk.row(b, j, kh) + d, LaneVec<T, 1>::pack(tk));
-      LaneVec<T, 1>::store((T *)a.dv.row(b, j, kh) + d, LaneVec<T, 1>::pack(tv));
+      unit = gradient_unit<T>(wave_max(most));
+    }
+    key.lowering = unit * (1.0f / 128.0f);
+    key.load(a, b, j < s.n ? j : s.n - 1, kh);
+    using Copy = TileCopy<T, DP, 32, 64>;
+    Copy cq, cg;
+    cq.init(a.D, a.q.token_bytes);
+    cg.init(a.D, a.dout.token_bytes);
+    LaneOffsets<T, DP> at;
+    at.init();
+    const unsigned lds = lds_address(tiles) + wave * 2 * W::kStage, lds_lse = lds_address(lses) + wave * 512, lds_delta = lds_address(deltas) + wave * 512;
+    key.settle_operands();
+    auto issue = [&](Step w, int buffer) {
+      const int h = kh * a.group + w.g, i0 = (first + w.t) * 32;
+      cq.issue((const char *)a.q.row(b, 0, h), i0, to, lds + buffer * W::kStage, a.D);
+      cg.issue((const char *)a.dout.row(b, 0, h), i0, to, lds + buffer * W::kStage + W::kStage / 2, a.D);
+      const unsigned r = (unsigned)(lane < to - i0 ? lane : to - i0) * 4;
+      const int64_t row = ((int64_t)b * a.H + h) * a.L + i0;
+      copy_to_lds<4>(uniform((const char *)(a.lse + row)), r, lds_lse + buffer * 256);
+      copy_to_lds<4>(uniform((const char *)(a.delta + row)), r, lds_delta + buffer * 256);
+    };
+    Step step = {begin / tiles_of, begin % tiles_of}, next = step;
+    int turn = 0;
+    if (begin < end) issue(step, 0);
+    for (int st = begin; st < end; st += kWaves) {
+      const int now = turn;
+      turn ^= 1;
+      next.advance(kWaves, tiles_of);
+      next_copies<2 * Copy::kCopies + 2>(st + kWaves < end, [&] { issue(next, turn); });
+      char *qt = tiles + (wave * 2 + now) * W::kStage;
+      key.template tile<32>(at, qt, qt + W::kStage / 2, lses + (wave * 2 + now) * 64, deltas + (wave * 2 + now) * 64, (first + step.t) * 32 + s.off);
+      step = next;
     }
   }
-  if (seen.count > 0) {
-    if (__any(!(bad_v == 0.0f))) dkv_again<T>(a, s, b, kh, j, false);
-    if (__any(!(bad_k == 0.0f))) dkv_again<T>(a, s, b, kh, j, true);
+  const int64_t slot = sink_slot(a, bk, set, share * kWaves + wave) + (lane & 31);
+  if constexpr (KS::kDk) store_token<float, DP>(a.part_k + slot * a.D, a.D, key.dk, KS::k_factor(a, unit));
+  if constexpr (KS::kDv) store_token<float, DP>(a.part_v + slot * a.D, a.D, key.dv, KS::v_factor());
+}
+
+// Sums of the keys that several workgroups shared, all keys or the sinks: four channels of a row each thread.
+template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kernel(const WindowArgs a) {
+  __shared__ int bad_k[kBlock], bad_v[kBlock];
+  const int quads = a.D / 4, rows_here = kBlock / quads, r = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+  const int rows = a.shares > 1 ? a.S : a.sinks < a.S ? a.sinks : a.S;
+  bad_k[threadIdx.x] = bad_v[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t id = (int64_t)blockIdx.x * rows_here + r;
+  if (r < rows_here && id < (int64_t)a.B * a.K * rows) {
+    const int bk = (int)(id / rows), j = (int)(id % rows), b = bk / a.K, kh = bk % a.K;
+    const bool sink = j < a.sinks;
+    const int64_t slot = sink ? sink_slot(a, bk, j / 32, 0) + j % 32 : tile_slot(a, bk, j / kQueries, 0) + j % kQueries;
+    const int64_t at = slot * a.D + d, step = (int64_t)(sink ? 32 : kQueries) * a.D;
+    const int parts = sink ? a.sink_parts : a.shares;
+    f32x4 k = {}, v = {};
+#pragma unroll 4
+    for (int n = 0; n < parts; ++n) {
+      k += load_global<f32x4>(a.part_k + at + n * step);
+      v += load_global<f32x4>(a.part_v + at + n * step);
+    }
+    const float tk[4] = {k[0], k[1], k[2], k[3]}, tv[4] = {v[0], v[1], v[2], v[3]};
+    using LV = LaneVec<T, 4>;
+    LV::store((T *)a.dk.row(b, j, kh) + d, LV::pack(tk));
+    LV::store((T *)a.dv.row(b, j, kh) + d, LV::pack(tv));
+    if (!(k[0] * 0.0f + k[1] * 0.0f + k[2] * 0.0f + k[3] * 0.0f == 0.0f)) bad_k[r] = 1;
+    if (!(v[0] * 0.0f + v[1] * 0.0f + v[2] * 0.0f + v[3] * 0.0f == 0.0f)) bad_v[r] = 1;
+  }
+  __syncthreads();
+  for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
+    if (!(bad_k[n] | bad_v[n])) continue;
+    const int64_t row = (int64_t)blockIdx.x * rows_here + n;
+    const int bk = (int)(row / rows), key = (int)(row % rows), b = bk / a.K;
+    const Sample s = sample_of(a, b);
+    if (seen_of(a, s, key).count == 0) continue;
+    if (bad_v[n]) dkv_again<T>(a, s, b, bk % a.K, key, false);
+    if (bad_k[n]) dkv_again<T>(a, s, b, bk % a.K, key, true);
   }
 }
 

@@ -25,17 +25,30 @@ namespace {
 
 // Calls f with the width that a head of D channels is padded to.
 template <typename F> void with_width(int D, F &&f) {
-  if (D <= 64) f(std::integral_constant<int, 64>());
-  else if (D <= 96) f(std::integral_constant<int, 96>());
-  else if (D <= 128) f(std::integral_constant<int, 128>());
-  else f(std::integral_constant<int, 256>());
+  switch (window_width(D)) {
+    case 64: return f(std::integral_constant<int, 64>());
+    case 96: return f(std::integral_constant<int, 96>());
+    case 128: return f(std::integral_constant<int, 128>());
+    default:
+      if constexpr (sizeof(elem_t) == 2) f(std::integral_constant<int, 256>());  // (float32: the plan takes heads of 128 at most)
+  }
 }
 dim3 grid_of(int items) { return dim3((unsigned)((items + 7) / 8 * 8)); }
+void join(const WindowArgs &a, hipStream_t stream) {
+  if (a.splits <= 1) return;
+  const int64_t rows = (int64_t)a.B * a.H * a.L;
+  hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)((rows + 3) / 4)), dim3(kBlock), 0, stream, a);
+}
+dim3 sum_grid(int64_t rows, int D) {
+  const int64_t here = kBlock / (D / 4);
+  return dim3((unsigned)((rows + here - 1) / here));
+}
 
 }  // namespace
 
 hipError_t GN_CAT(launch_window_forward_, GN_SUFFIX)(const WindowArgs &a, hipStream_t stream) {
   with_width(a.D, [&](auto w) { hipLaunchKernelGGL((window_forward_kernel<elem_t, decltype(w)::value>), grid_of(a.items), dim3(kBlock), 0, stream, a); });
+  join(a, stream);
   return hipGetLastError();
 }
 
@@ -44,28 +57,31 @@ hipError_t GN_CAT(launch_window_few_, GN_SUFFIX)(const WindowArgs &a, hipStream_
     constexpr int DP = decltype(w)::value;
     hipLaunchKernelGGL((window_few_kernel<elem_t, DP>), grid_of(a.items), dim3(64 * Few<elem_t, DP>::kWaves), 0, stream, a);
   });
-  if (a.splits > 1) {
-    const int64_t rows = (int64_t)a.B * a.H * a.L;
-    hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)((rows + 3) / 4)), dim3(kBlock), 0, stream, a);
-  }
+  join(a, stream);
   return hipGetLastError();
 }
 
-hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const WindowArgs &kv, hipStream_t stream) {
+hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const WindowArgs &kv, const WindowArgs &sinks, hipStream_t stream) {
   with_width(a.D, [&](auto w) {
     constexpr int DP = decltype(w)::value;
     if (a.items) hipLaunchKernelGGL((window_dq_kernel<elem_t, DP>), grid_of(a.items), dim3(kBlock), 0, stream, a);
+    if (a.items && a.splits > 1)
+      hipLaunchKernelGGL((window_dq_sum_kernel<elem_t>), sum_grid((int64_t)a.B * a.H * a.L, a.D), dim3(kBlock), 0, stream, a);
+    auto keys = [&](auto parts) {
+      constexpr int P = decltype(parts)::value;
+      hipLaunchKernelGGL((window_dkv_kernel<elem_t, DP, P>), grid_of(kv.items), dim3(kBlock), 0, stream, kv);
+      if (sinks.items) hipLaunchKernelGGL((window_sink_kernel<elem_t, DP, P>), grid_of(sinks.items), dim3(64 * Few<elem_t, DP>::kWaves), 0, stream, sinks);
+    };
     if constexpr (DP <= 128) {
-      hipLaunchKernelGGL((window_dkv_kernel<elem_t, DP, 3>), grid_of(kv.items), dim3(kBlock), 0, stream, kv);
+      keys(std::integral_constant<int, 3>());
     } else {
-      hipLaunchKernelGGL((window_dkv_kernel<elem_t, DP, 1>), grid_of(kv.items), dim3(kBlock), 0, stream, kv);
-      hipLaunchKernelGGL((window_dkv_kernel<elem_t, DP, 2>), grid_of(kv.items), dim3(kBlock), 0, stream, kv);
+      keys(std::integral_constant<int, 1>());
+      keys(std::integral_constant<int, 2>());
     }
   });
-  if (kv.shares > 1 || kv.sink_shares > 1) {
-    const int64_t tiles = (kv.shares > 1 ? kv.tiles : kv.sink_tiles) - (kv.sink_shares > 1 ? 0 : kv.sink_tiles);
-    const int64_t rows = (int64_t)kv.B * kv.K * tiles * kQueries;
-    if (rows > 0) hipLaunchKernelGGL((window_sum_kernel<elem_t>), dim3((unsigned)((rows + 3) / 4)), dim3(kBlock), 0, stream, kv);
+  if (kv.shares > 1 || kv.sinks > 0) {
+    const int64_t rows = (int64_t)kv.B * kv.K * (kv.shares > 1 ? kv.S : kv.sinks < kv.S ? kv.sinks : kv.S);
+    hipLaunchKernelGGL((window_sum_kernel<elem_t>), sum_grid(rows, kv.D), dim3(kBlock), 0, stream, kv);
   }
   return hipGetLastError();
 }

@@ -22,22 +22,29 @@ struct HeadRows {
 };
 struct WindowArgs {
   HeadRows q, k, v, out, dout, dq, dk, dv;
-  float *lse, *delta, *largest, *part_k, *part_v;
+  float *lse, *delta, *largest, *part_q, *part_k, *part_v;
   const void *lengths;
   int length_type, at_end;  // at_end: the queries are the last of a sample's own tokens, not of all S
   int B, L, S, H, K, D, group;
   int left, right, sinks, causal;
-  int tiles, items;                        // tiles of a head, workgroups with work
-  int sink_tiles, sink_shares, shares;     // dk / dv: tiles that hold sinks; workgroups that share a tile of those, of the others
-  int splits;                              // few queries: workgroups that share a head's keys
-  int parts;                               // ... and of a head, those that leave sums for window_sum_kernel
+  int tiles, items;           // tiles of a head, workgroups with work
+  int splits;                 // out, dq: workgroups that share a row's keys
+  int shares;                 // dk, dv: workgroups that share a tile's queries
+  int sink_sets, sink_parts;  // dk, dv of the sinks: 32 keys each; wavefronts that share the queries
   float scale, scale_log2;
 };
+
+// Wavefronts of a workgroup whose wavefronts have two pairs of tiles of 32 rows each, for a head padded to `width` channels.
+constexpr int window_width(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
+constexpr int few_waves(int width, int elem_size) {
+  const int most = 131072 / (4 * 32 * width * elem_size);
+  return most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
+}
 
 #define GN_DECLARE_WINDOW(S)                                                            \
   hipError_t launch_window_forward_##S(const WindowArgs &a, hipStream_t stream);        \
   hipError_t launch_window_few_##S(const WindowArgs &a, hipStream_t stream);            \
-  hipError_t launch_window_backward_##S(const WindowArgs &a, const WindowArgs &kv, hipStream_t stream);
+  hipError_t launch_window_backward_##S(const WindowArgs &a, const WindowArgs &kv, const WindowArgs &sinks, hipStream_t stream);
 GN_DECLARE_WINDOW(f32)
 GN_DECLARE_WINDOW(f16)
 GN_DECLARE_WINDOW(bf16)

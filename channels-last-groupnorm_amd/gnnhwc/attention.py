@@ -32,8 +32,9 @@ def _check_attention(q, k, v, lengths, window, sinks, at_end, opname):
         raise RuntimeError("%s: k and v must have shape (%d, tokens, kv_heads, %d), got %s and %s" % (opname, B, D, tuple(k.shape), tuple(v.shape)))
     if K < 1 or H < 1 or H % K:
         raise RuntimeError("%s: q's %d heads must be a multiple of k's %d" % (opname, H, K))
-    if not 1 <= D <= 256:
-        raise RuntimeError("%s: heads of %d channels: 1 to 256 are supported" % (opname, D))
+    most = 128 if q.dtype == torch.float32 else 256
+    if not 1 <= D <= most:
+        raise RuntimeError("%s: heads of %d channels: 1 to %d are supported in %s" % (opname, D, most, q.dtype))
     if not at_end and L > S:
         raise RuntimeError("%s: %d queries and %d keys: the queries are the last of the keys' tokens" % (opname, L, S))
     if window < -1 or sinks < 0:
@@ -192,7 +193,7 @@ def window_attention(q, k, v, window=None, sinks=0, causal=False, lengths=None, 
     """softmax(scale q k^T) v over the tokens that each token sees: those within `window` to either side (None: all), and the
     first `sinks` of its sample, such as registers or a prompt's beginning; none behind it if `causal`.
 
-    q: (B, L, heads, D), k, v: (B, S, kv_heads, D) in float32, float16 or bfloat16, D up to 256, heads a multiple of kv_heads
+    q: (B, L, heads, D), k, v: (B, S, kv_heads, D) in float32, float16 or bfloat16, D up to 256 (float32: 128), heads a multiple of kv_heads
     (heads / kv_heads neighbouring heads of q share one of k).  The queries are the last L of the S tokens: L = S is a whole
     sequence, L < S its end.  lengths: (B,) int32 or int64, tokens that a sample has (clamped to 0 .. S): the others are padding,
     which nobody sees, whose rows of the result are zeros, and whose gradients are zeros.  A token that sees nothing gets zeros.

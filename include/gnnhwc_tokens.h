@@ -150,7 +150,7 @@ typedef struct gnnhwc_window_call {
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
   int64_t out_grad_stride[3], q_grad_stride[3], k_grad_stride[3], v_grad_stride[3];
   int64_t batch, tokens, keys, heads, kv_heads;
-  int64_t head_dim;             /* a multiple of 8, to 256 */
+  int64_t head_dim;             /* a multiple of 8, to 256 (F32: 128) */
   int64_t window;               /* -1: no bound */
   int64_t sinks, causal;
   const void *lengths;          /* batch values, or NULL */

@@ -49,7 +49,7 @@ def _call(**change):
     return c, raw
 
 
-REFUSED = [(dict(dtype=F64), "dtype"), (dict(dtype=7), "dtype"), (dict(head_dim=0), "head_dim"), (dict(head_dim=12), "head_dim"), (dict(head_dim=264), "head_dim"),
+REFUSED = [(dict(dtype=F64), "dtype"), (dict(dtype=7), "dtype"), (dict(head_dim=0), "head_dim"), (dict(head_dim=12), "head_dim"), (dict(head_dim=264), "head_dim"), (dict(head_dim=136, dtype=F32), "head_dim"),
            (dict(heads=3), "heads"), (dict(kv_heads=0), "heads"), (dict(heads=65536, kv_heads=1), "heads"), (dict(batch=-1), "negative"), (dict(tokens=-1), "negative"),
            (dict(keys=-1, tokens=0), "negative"), (dict(keys=2 ** 30 + 1), "2\\^30"), (dict(window=-2), "window"), (dict(sinks=-1), "sinks"), (dict(tokens=9), "more queries"),
            (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(scale=1e-60), "scale"),

@@ -46,13 +46,18 @@ SHAPES = [
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_forward_and_backward(shape, dtype, device):
+    if dtype == F32 and shape[5] > 128:
+        with pytest.raises(RuntimeError, match="1 to 128"):
+            run(dtype, device, *shape)
+        return
     run(dtype, device, *shape)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("D", [1, 4, 10, 66, 130])
+@pytest.mark.parametrize("D", [1, 4, 10, 66, 126, 130])
 def test_heads_that_no_lane_vector_divides(D, dtype, device):
-    run(dtype, device, 2, 70, 70, 2, 1, D, 9, 2, False)
+    if dtype != F32 or D <= 128:
+        run(dtype, device, 2, 70, 70, 2, 1, D, 9, 2, False)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])

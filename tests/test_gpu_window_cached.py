@@ -28,6 +28,8 @@ CASES = [
 def test_newest_tokens(case, dtype, device):
     """What lies behind a request's length is NaN."""
     B, T, S, H, K, D, window, sinks, lengths = case
+    if dtype == F32 and D > 128:
+        D = 128
     print("cached", dtype, case, flush=True)
     q, k, v = (normal((B, n, h, D), dtype, device, i) for i, (n, h) in enumerate(((T, H), (S, K), (S, K))))
     n = torch.tensor(lengths, dtype=torch.int32, device=device)
@@ -142,7 +144,8 @@ def test_refusals(device):
                        (lambda: window_attention_cached(q, k, k, n, sinks=-1), "sinks"), (lambda: window_attention_cached(q, k, k, n, scale=0.0), "scale"),
                        (lambda: window_attention_cached(q, k, k, n, scale=math.nan), "scale"), (lambda: window_attention(k, q, q), "multiple|queries"),
                        (lambda: window_attention(k.expand(2, 9, 2, 64), k[:, :8], k[:, :8]), "queries"), (lambda: window_attention(q[0], k, k), "shape"),
-                       (lambda: window_attention(torch.zeros((1, 1, 1, 264), device=device), *(torch.zeros((1, 1, 1, 264), device=device),) * 2), "256")):
+                       (lambda: window_attention(*(torch.zeros((1, 1, 1, 257), device=device).half(),) * 3), "256"),
+                       (lambda: window_attention(*(torch.zeros((1, 1, 1, 129), device=device),) * 3), "128")):
         with pytest.raises(RuntimeError, match=text):
             call()
     with torch.no_grad():
