@@ -11,8 +11,13 @@ namespace gn {
 namespace {
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;
-constexpr int64_t kOverhead = 3, kJoin = 8;  // in steps
-constexpr int64_t kFewRows = 128, kFewItems = 512, kFewSteps = 8;
+#ifndef GN_EXP_FS
+#define GN_EXP_FS 8
+#endif
+#ifndef GN_EXP_FI
+#define GN_EXP_FI 512
+#endif
+constexpr int64_t kFewRows = 128, kFewItems = GN_EXP_FI, kFewSteps = GN_EXP_FS;
 constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
 
 int invalid(const char *what) { return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s", what); }
@@ -43,6 +48,13 @@ int put_rows(HeadRows &r, const void *base, const int64_t (&stride)[3], int64_t 
   return GNNHWC_OK;
 }
 
+// The order in which the workgroups' work goes to the dies.
+void put_order(WindowArgs &a) {
+  const int heads = a.B * a.K;
+  a.per_head = heads ? a.items / heads : 0;
+  a.order = heads % 8 == 0 ? kHeadsInTurn : a.lengths ? kInTurn : kStretches;
+}
+
 struct WindowPlan {
   WindowArgs a, kv, sinks;  // queries' tiles, keys' tiles, sinks
   bool empty, few;          // few: 32 rows of a key head at a time, see window_few_kernel
@@ -50,11 +62,14 @@ struct WindowPlan {
 };
 
 // Workgroups that share the work of each of `items`, of `steps` steps: a CU takes `thick` of them at once in the time of one, each
-// has kOverhead steps besides its share, and what they leave has to be joined.
+// has some steps' time of its own, and what they leave has to be joined.
 int64_t shares_of(int64_t items, int64_t steps, int64_t thick, int64_t most) {
   if (items == 0) return 1;
+  // (in steps of which a CU takes `thick` at once: 1.7 us for float32, 0.5 for 16 bits, where the second launch is 4 us and a share's
+  // rows, written and read, 13 ns)
+  const int64_t join = thick == 1 ? 3 : 8, rows = thick == 1 ? 128 : 32, overhead = thick == 1 ? 1 : 3;
   auto cost = [&](int64_t s) {
-    return std::max(ceil_div(items * s, kNumCU), thick) * (ceil_div(steps, s) + kOverhead) + (s > 1 ? kJoin + items * s / 32 : 0);
+    return std::max(ceil_div(items * s, kNumCU), thick) * (ceil_div(steps, s) + overhead) + (s > 1 ? join + items * s / rows : 0);
   };
   int64_t best = 1;
   for (int64_t s = 2; s <= most && s <= steps / 2; ++s)
@@ -135,6 +150,7 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
       a.splits = (int)shares_of(items, keys, thick, 16);
       a.items = (int)(items * a.splits);
     }
+    put_order(a);
     if (a.splits > 1) {
       p.part_v = round_up((size_t)a.splits * lse * 2 * sizeof(float));
       p.bytes += p.part_v + (size_t)a.splits * lse * a.D * sizeof(float);
@@ -146,12 +162,14 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     a.splits = (int)shares_of(items, keys, thick, 16);
     a.items = (int)(items * a.splits);
   }
+  put_order(a);
   WindowArgs &w = p.kv, &k = p.sinks;
   w.tiles = (int)ceil_div(a.S, kQueries);
   const int64_t heads = (int64_t)a.B * a.K, tiles = heads * w.tiles;
   w.shares = (int)shares_of(tiles, queries, es == 4 ? 1 : width <= 64 ? 2 : 1, 32);
   if (tiles * w.shares > kMostItems) return invalid("too many tokens and heads for one call");
   w.items = (int)(tiles * w.shares);
+  put_order(w);
   k.items = w.sink_sets = w.sink_parts = 0;
   if (w.sinks > 0 && w.items > 0) {
     const int waves = few_waves((int)width, (int)es);
@@ -159,9 +177,10 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     const int64_t sets = heads * w.sink_sets, steps = ceil_div(a.L, 32) * a.group;
     const int64_t sink_shares = std::clamp<int64_t>(ceil_div(kNumCU, sets), 1, std::max<int64_t>(1, steps / (4 * waves)));
     if (sets * sink_shares > kMostItems) return invalid("too many tokens and heads for one call");
-    w.sink_parts = (int)(sink_shares * waves);
+    w.sink_parts = (int)sink_shares;
     k = w;
     k.items = (int)(sets * sink_shares);
+    put_order(k);
   }
   const size_t floats = round_up((size_t)lse * sizeof(float));
   const size_t part = round_up(((size_t)heads * w.sink_sets * w.sink_parts * 32 + (w.shares > 1 ? (size_t)tiles * w.shares * kQueries : 0)) * a.D * sizeof(float));

@@ -297,10 +297,14 @@ __device__ __forceinline__ Walk walk_of(const WindowArgs &a, const Sample &s, in
   return w;
 }
 
-// Workgroups are dealt to the eight dies in turn, each with a cache of its own: neighbours in the work's order go to one die.
-__device__ __forceinline__ int work_item(int items) {
-  const int id = blockIdx.x, share = (items + 7) >> 3;
-  return (id & 7) * share + (id >> 3);  // (items and beyond: nothing to do)
+// The work of this workgroup, of a.items ordered by key head; a.items and beyond: none.  Workgroups are dealt to the eight dies in
+// turn, each with a cache of its own that a head's keys and values are to be in once: heads are dealt to the dies in turn, or, where
+// they do not come out even, each die has a stretch of the work, or, where samples have lengths that would make those uneven, all
+// is dealt in turn.  (padded float32 (3, 1961, 6 heads over 2, 40): forward 112 us with stretches)
+__device__ __forceinline__ int work_item(const WindowArgs &a) {
+  const int id = blockIdx.x, die = id & 7, n = id >> 3;
+  if (a.order == kHeadsInTurn) return (n / a.per_head * 8 + die) * a.per_head + n % a.per_head;
+  return a.order == kStretches ? die * ((a.items + 7) >> 3) + n : id;
 }
 
 // ---- rows by their formulas, for results that are not finite ----
@@ -580,7 +584,7 @@ __device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int 
 template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
-  const int item = work_item(a.items);
+  const int item = work_item(a);
   if (item >= a.items) return;
   // (the heads of a group are neighbours, then the tiles of queries, the last ones, which see most, first)
   const int g = item % a.group, split = item / a.group % a.splits, rest = item / a.group / a.splits;
@@ -690,7 +694,7 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * W::kStage];
   __shared__ float references[kWaves][32], sums[kWaves][32];
   __shared__ int bad[32];
-  const int item = work_item(a.items);
+  const int item = work_item(a);
   if (item >= a.items) return;
   const int split = item % a.splits, rest = item / a.splits, block = rest % a.tiles, bk = rest / a.tiles;
   const int b = bk / a.K, kh = bk % a.K;
@@ -799,36 +803,44 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   }
 }
 
-// Rows whose keys several workgroups shared: a wavefront each.
+// Rows whose keys several workgroups shared: four channels of a row each thread.
 template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kernel(const WindowArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.B * a.H * a.L;
-  if (id >= rows) return;
-  const int i = (int)(id % a.L), h = (int)(id / a.L % a.H), b = (int)(id / a.L / a.H);
-  // (a lane holds a split's reference and sum: at most 64 splits)
-  const float reference = lane < a.splits ? load_global<float>(a.part_k + 2 * (id + lane * rows)) : -INFINITY;
-  const float part = lane < a.splits ? load_global<float>(a.part_k + 2 * (id + lane * rows) + 1) : 0.0f;
-  const float most = wave_max(reference), weight = part_weight(reference, most), sum = wave_sum(part * weight);
-  float o[4] = {}, bad = 0.0f;
-  for (int n = 0; n < a.splits; ++n) {
-    const float w = __shfl(weight, n);
+  __shared__ int bad[kBlock];
+  const int quads = a.D / 4, rows_here = kBlock / quads, r = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+  const int64_t rows = (int64_t)a.B * a.H * a.L, id = (int64_t)blockIdx.x * rows_here + r;
+  bad[threadIdx.x] = 0;
+  __syncthreads();
+  if (r < rows_here && id < rows) {
+    float most = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+    for (int n = 0; n < a.splits; ++n) most = fmaxf(most, load_global<float>(a.part_k + 2 * (id + n * rows)));
+    f32x4 o = {};
+#pragma unroll 4
+    for (int n = 0; n < a.splits; ++n) {
+      const f32x2 part = load_global<f32x2>(a.part_k + 2 * (id + n * rows));
+      const float w = part_weight(part.x, most);
+      const f32x4 v = load_global<f32x4>(a.part_v + (id + n * rows) * a.D + d);
+      sum = __builtin_fmaf(w, part.y, sum);
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (x * 64 + lane < a.D) o[x] = __builtin_fmaf(w, load_global<float>(a.part_v + (id + n * rows) * a.D + x * 64 + lane), o[x]);
-  }
-  const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-    if (x * 64 + lane < a.D) {
-      bad = __builtin_fmaf(o[x] * factor, 0.0f, bad);
-      const float t[1] = {o[x] * factor};
-      LaneVec<T, 1>::store((T *)a.out.row(b, i, h) + x * 64 + lane, LaneVec<T, 1>::pack(t));
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
     }
-  if (a.lse && lane == 0) store_global<float>(a.lse + id, sum > 0.0f ? most + __builtin_amdgcn_logf(sum) : INFINITY);
-  if (!__any(!(bad == 0.0f)) && sum > 0.0f) return;
-  const Sample s = sample_of(a, b);
-  const Sight g = sight_of(a, s, i);
-  if (g.count > 0 || g.sinks > 0) row_again<T>(a, s, b, h, i);
+    const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float t[4] = {o[0] * factor, o[1] * factor, o[2] * factor, o[3] * factor};
+    const int i = (int)(id % a.L), h = (int)(id / a.L % a.H), b = (int)(id / a.L / a.H);
+    using LV = LaneVec<T, 4>;
+    LV::store((T *)a.out.row(b, i, h) + d, LV::pack(t));
+    if (a.lse && d == 0) store_global<float>(a.lse + id, sum > 0.0f ? most + __builtin_amdgcn_logf(sum) : INFINITY);
+    if (!(t[0] * 0.0f + t[1] * 0.0f + t[2] * 0.0f + t[3] * 0.0f == 0.0f) || !(sum > 0.0f)) bad[r] = 1;
+  }
+  __syncthreads();
+  for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
+    if (!bad[n]) continue;
+    const int64_t row = (int64_t)blockIdx.x * rows_here + n;
+    const int i = (int)(row % a.L), h = (int)(row / a.L % a.H), b = (int)(row / a.L / a.H);
+    const Sample s = sample_of(a, b);
+    const Sight g = sight_of(a, s, i);
+    if (g.count > 0 || g.sinks > 0) row_again<T>(a, s, b, h, i);
+  }
 }
 
 // ---- backward: dq ----
@@ -844,7 +856,7 @@ template <typename T> __device__ __forceinline__ float gradient_unit(float most)
 template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && sizeof(T) == 2 ? 2 : 1) void window_dq_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
-  const int item = work_item(a.items);
+  const int item = work_item(a);
   if (item >= a.items) return;
   const int g = item % a.group, split = item / a.group % a.splits, rest = item / a.group / a.splits;
   const int tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
@@ -1160,7 +1172,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // queries and gradients, two deep
   __shared__ __attribute__((aligned(16))) float lses[2 * 64], deltas[2 * 64];
   __shared__ float reduce[4];
-  const int item = work_item(a.items);
+  const int item = work_item(a);
   if (item >= a.items) return;
   const int share = item % a.shares, tile = item / a.shares % a.tiles, bk = item / a.shares / a.tiles, b = bk / a.K, kh = bk % a.K;
   const Sample s = sample_of(a, b);
@@ -1249,16 +1261,16 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
 }
 
 // dk and dv of the sinks: 32 keys, which all wavefronts hold, against a share of all queries, of which each wavefront walks its own
-// (a tile of 128 keys with a few sinks would have three of four wavefronts idle most of the way).  Every wavefront leaves sums.
+// (a tile of 128 keys with a few sinks would have three of four wavefronts idle most of the way).
 template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void window_sink_kernel(const WindowArgs a) {
   using W = Few<T, DP>;
   using KS = KeySide<T, DP, PARTS>;
   constexpr int kWaves = W::kWaves;
   __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * W::kStage];
   __shared__ __attribute__((aligned(16))) float lses[kWaves * 2 * 64], deltas[kWaves * 2 * 64];
-  const int item = work_item(a.items);
+  const int item = work_item(a);
   if (item >= a.items) return;
-  const int shares = a.sink_parts / kWaves, share = item % shares, set = item / shares % a.sink_sets, bk = item / shares / a.sink_sets, b = bk / a.K, kh = bk % a.K;
+  const int shares = a.sink_parts, share = item % shares, set = item / shares % a.sink_sets, bk = item / shares / a.sink_sets, b = bk / a.K, kh = bk % a.K;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), j = set * 32 + (lane & 31);
   KS key;
@@ -1313,9 +1325,29 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
       step = next;
     }
   }
-  const int64_t slot = sink_slot(a, bk, set, share * kWaves + wave) + (lane & 31);
-  if constexpr (KS::kDk) store_token<float, DP>(a.part_k + slot * a.D, a.D, key.dk, KS::k_factor(a, unit));
-  if constexpr (KS::kDv) store_token<float, DP>(a.part_v + slot * a.D, a.D, key.dv, KS::v_factor());
+  // the wavefronts' sums, through the tiles' place
+  float *mine = (float *)(tiles + wave * 2 * W::kStage);
+  const int64_t slot = sink_slot(a, bk, set, share);
+  auto add = [&](const auto &acc, float factor, float *to) {
+    __syncthreads();  // (no copy is on its way: each wavefront has waited for its last one)
+    #pragma unroll
+    for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(f32x4 *)(mine + (lane & 31) * W::kPitch + 32 * x + row_of(r, lane >> 5)) =
+            f32x4{acc[x][r] * factor, acc[x][r + 1] * factor, acc[x][r + 2] * factor, acc[x][r + 3] * factor};
+    __syncthreads();
+    for (int e = threadIdx.x; e < 32 * DP / 4; e += 64 * kWaves) {
+      const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+      if (d >= a.D) continue;
+      f32x4 v = *(const f32x4 *)((const float *)tiles + r * W::kPitch + d);
+#pragma unroll
+      for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)(tiles + n * 2 * W::kStage) + r * W::kPitch + d);
+      store_global<f32x4>(to + (slot + r) * a.D + d, v);
+    }
+  };
+  if constexpr (KS::kDk) add(key.dk, KS::k_factor(a, unit), a.part_k);
+  if constexpr (KS::kDv) add(key.dv, KS::v_factor(), a.part_v);
 }
 
 // Sums of the keys that several workgroups shared, all keys or the sinks: four channels of a row each thread.
@@ -1333,7 +1365,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kerne
     const int64_t at = slot * a.D + d, step = (int64_t)(sink ? 32 : kQueries) * a.D;
     const int parts = sink ? a.sink_parts : a.shares;
     f32x4 k = {}, v = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int n = 0; n < parts; ++n) {
       k += load_global<f32x4>(a.part_k + at + n * step);
       v += load_global<f32x4>(a.part_v + at + n * step);

@@ -34,14 +34,12 @@ template <typename F> void with_width(int D, F &&f) {
   }
 }
 dim3 grid_of(int items) { return dim3((unsigned)((items + 7) / 8 * 8)); }
-void join(const WindowArgs &a, hipStream_t stream) {
-  if (a.splits <= 1) return;
-  const int64_t rows = (int64_t)a.B * a.H * a.L;
-  hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)((rows + 3) / 4)), dim3(kBlock), 0, stream, a);
-}
 dim3 sum_grid(int64_t rows, int D) {
   const int64_t here = kBlock / (D / 4);
   return dim3((unsigned)((rows + here - 1) / here));
+}
+void join(const WindowArgs &a, hipStream_t stream) {
+  if (a.splits > 1) hipLaunchKernelGGL((window_join_kernel<elem_t>), sum_grid((int64_t)a.B * a.H * a.L, a.D), dim3(kBlock), 0, stream, a);
 }
 
 }  // namespace

@@ -20,6 +20,7 @@ struct HeadRows {
     return (char *)const_cast<void *>(base) + (int64_t)b * batch_bytes + (int64_t)i * token_bytes + (int64_t)h * head_bytes;
   }
 };
+enum { kInTurn = 0, kStretches = 1, kHeadsInTurn = 2 };  // which work a die takes (work_item)
 struct WindowArgs {
   HeadRows q, k, v, out, dout, dq, dk, dv;
   float *lse, *delta, *largest, *part_q, *part_k, *part_v;
@@ -28,9 +29,10 @@ struct WindowArgs {
   int B, L, S, H, K, D, group;
   int left, right, sinks, causal;
   int tiles, items;           // tiles of a head, workgroups with work
+  int order, per_head;        // ... of a key head
   int splits;                 // out, dq: workgroups that share a row's keys
   int shares;                 // dk, dv: workgroups that share a tile's queries
-  int sink_sets, sink_parts;  // dk, dv of the sinks: 32 keys each; wavefronts that share the queries
+  int sink_sets, sink_parts;  // dk, dv of the sinks: 32 keys each; workgroups that share the queries
   float scale, scale_log2;
 };
 
