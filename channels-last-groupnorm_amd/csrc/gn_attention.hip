@@ -11,13 +11,7 @@ namespace gn {
 namespace {
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;
-#ifndef GN_EXP_FS
-#define GN_EXP_FS 8
-#endif
-#ifndef GN_EXP_FI
-#define GN_EXP_FI 512
-#endif
-constexpr int64_t kFewRows = 128, kFewItems = GN_EXP_FI, kFewSteps = GN_EXP_FS;
+constexpr int64_t kFewRows = 128;
 constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
 
 int invalid(const char *what) { return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s", what); }
@@ -142,9 +136,13 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     if (p.few) {
       a.tiles = (int)ceil_div(few_rows, 32);
       const int64_t heads = (int64_t)a.B * a.K * a.tiles;
-      // keys that a tile's rows see at most, in tiles of 32; a share is kFewSteps or more of them
-      const int64_t seen = std::min<int64_t>(a.S, (int64_t)a.left + a.right + a.L + a.sinks + 64);
-      a.splits = (int)std::clamp<int64_t>(ceil_div(kFewItems, heads), 1, std::min<int64_t>(64, std::max<int64_t>(1, ceil_div(seen, 32) / kFewSteps)));
+      // Keys that a tile's rows see at most, in tiles of 32 and of a wavefront one takes 1.5 us of waiting for it, until the memory is
+      // what is waited for; a workgroup has 2 us besides, and joining takes a second launch of 4.  (one token of 24 heads over 8 of
+      // 128, 517 keys: one workgroup a head 14.3 us, two 11.3 + 3.5, nine 8.3 + 4.4)
+      const int64_t tiles = ceil_div(std::min<int64_t>(a.S, (int64_t)a.left + a.right + a.L + a.sinks + 64), 32), waves = few_waves((int)width, (int)es);
+      auto cost = [&](int64_t s) { return ceil_div(heads * s, kNumCU) * (4 + 3 * ceil_div(tiles, s * waves)) + (s > 1 ? 8 : 0); };
+      for (int64_t s = 2; s <= 64 && s <= tiles; ++s)
+        if (cost(s) < cost(a.splits)) a.splits = (int)s;
       a.items = (int)(heads * a.splits);
     } else {
       a.splits = (int)shares_of(items, keys, thick, 16);
@@ -175,7 +173,7 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     const int waves = few_waves((int)width, (int)es);
     w.sink_sets = (int)ceil_div(w.sinks, 32);
     const int64_t sets = heads * w.sink_sets, steps = ceil_div(a.L, 32) * a.group;
-    const int64_t sink_shares = std::clamp<int64_t>(ceil_div(kNumCU, sets), 1, std::max<int64_t>(1, steps / (4 * waves)));
+    const int64_t sink_shares = std::clamp<int64_t>(kNumCU / std::max<int64_t>(1, sets), 1, std::max<int64_t>(1, steps / (4 * waves)));
     if (sets * sink_shares > kMostItems) return invalid("too many tokens and heads for one call");
     w.sink_parts = (int)sink_shares;
     k = w;

@@ -46,7 +46,6 @@ template <> struct Operand<float> {  // eight products of two summands each
   }
 };
 template <typename T> using operand_t = typename Operand<T>::type;
-
 // Values 8 t .. 8 t + 7 of a lane's column, rounded to T once: what the products' results cost beside float32 operands, half a
 // unit in the last place of each summand, like the operands that come from memory.
 template <typename T> __device__ __forceinline__ operand_t<T> operand_of(const f32x16_t &v, int t) {
@@ -108,6 +107,12 @@ template <typename T, int DP> struct LaneOffsets {
   static_assert(!kCompact || (kRowBytes & (kRowBytes - 1)) == 0, "a row's bytes are a power of two");
   static constexpr int kSteps = kCompact ? 1 : DP / 16, kParts = kCompact ? 1 : DP / 32;
   int rows[sizeof(T) == 2 ? 1 : 2][kSteps], columns[kParts][sizeof(T) == 2 ? 2 : 8];
+  int steps;
+  // Whether step x of a product over a head's channels has any of them.  (16 bits: a step past the head costs less than to ask)
+  __device__ __forceinline__ bool has(int x) const {
+    if constexpr (sizeof(T) == 2) return true;
+    else return x == 0 || x < steps;
+  }
   static __device__ __forceinline__ int step_of(int first, int x, int bytes) {
     pin(first);  // (or they would all be made ahead of the loop, and kept)
     return first ^ x * bytes;
@@ -120,7 +125,8 @@ template <typename T, int DP> struct LaneOffsets {
     if constexpr (kCompact) return step_of(columns[0][i], x, 32 * (int)sizeof(T));
     else return columns[x][i];
   }
-  __device__ __forceinline__ void init() {
+  __device__ __forceinline__ void init(int D) {
+    steps = (D + 15) / 16;
     const int lane = threadIdx.x & 63, h = lane >> 5, row = lane & 31;
 #pragma unroll
     for (int x = 0; x < kSteps; ++x) {
@@ -169,22 +175,24 @@ template <typename T, int DP> struct LaneOffsets {
   }
 };
 
+template <typename P> __device__ __forceinline__ P *uniform(P *p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (P *)((uint64_t)hi << 32 | lo);
+}
+
 // Each lane's BYTES from memory (base + offset) into shared memory, the lanes' behind each other from `to` on; base and `to` are the same
 // for all of them.  (The compiler would have every transposing read wait for all copies that are on their way, other buffers'
 // too: it is not told of these.  Nothing is written to a register but m0, which nothing else here uses; tiles_turn waits.)
 template <int BYTES> __device__ __forceinline__ void copy_to_lds(const char *base, unsigned offset, unsigned to) {
   to = __builtin_amdgcn_readfirstlane(to);
+  base = uniform(base);
   if constexpr (BYTES == 16)
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(offset), "s"(to), "s"(base) : "memory");
   else
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, %2" ::"v"(offset), "s"(to), "s"(base) : "memory");
 }
 __device__ __forceinline__ unsigned lds_address(const void *p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)p; }
-template <typename P> __device__ __forceinline__ P *uniform(P *p) {
-  const uint64_t v = (uint64_t)p;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-  return (P *)((uint64_t)hi << 32 | lo);
-}
 
 // Copies tiles of ROWS rows into shared memory, by LANES lanes.  Rows past `last` and chunks past the head are other rows and chunks
 // of the same tensor (memory that is there, and values whose products are left out).
@@ -208,14 +216,14 @@ template <typename T, int DP, int ROWS, int LANES> struct TileCopy {
       offset[i] = (unsigned)row_at(i, lane) * (unsigned)stride + byte_at(i, lane, D);
     }
   }
-  // `to`: where the tile goes, plus 1024 times the wavefront's number among those that copy it
-  __device__ __forceinline__ void issue(const char *base, int first, int last, unsigned to, int D) const {
-    const char *from = uniform(base + (int64_t)first * stride);
-    if (first + ROWS - 1 <= last) {
+  // from: the tile's first row; left: its last row, counted from there; `to`: where the tile goes, plus 1024 times the wavefront's
+  // number among those that copy it.
+  __device__ __forceinline__ void issue(const char *from, int left, unsigned to, int D) const {
+    if (left >= ROWS - 1) {
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) copy_to_lds<16>(from, offset[i], to + i * LANES * 16);
     } else {
-      int lane = threadIdx.x % LANES, left = last - first;
+      int lane = threadIdx.x % LANES;
       pin(lane);  // (so that nothing of this lies in registers all along)
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
@@ -223,6 +231,32 @@ template <typename T, int DP, int ROWS, int LANES> struct TileCopy {
         copy_to_lds<16>(from, (unsigned)(r < left ? r : left) * (unsigned)stride + byte_at(i, lane, D), to + i * LANES * 16);
       }
     }
+  }
+};
+// Two tensors' tiles at once, one walk's after the other: the places in memory move on by additions.
+template <typename T, int DP, int ROWS, int LANES> struct TilePair {
+  TileCopy<T, DP, ROWS, LANES> x, y;
+  const char *at_x, *at_y;
+  int last, D, first;  // last row, the next tile's first
+  __device__ __forceinline__ void init(int D_, int x_bytes, int y_bytes, int last_) {
+    D = D_;
+    last = last_;
+    x.init(D_, x_bytes);
+    y.init(D_, y_bytes);
+  }
+  __device__ __forceinline__ void go_to(const char *base_x, const char *base_y, int row) {
+    first = row;
+    at_x = uniform(base_x + (int64_t)row * x.stride);
+    at_y = uniform(base_y + (int64_t)row * y.stride);
+  }
+  __device__ __forceinline__ void issue(unsigned to, unsigned apart) const {
+    x.issue(at_x, last - first, to, D);
+    y.issue(at_y, last - first, to + apart, D);
+  }
+  __device__ __forceinline__ void advance(int tiles) {
+    first += tiles * ROWS;
+    at_x += (int64_t)tiles * ROWS * x.stride;
+    at_y += (int64_t)tiles * ROWS * y.stride;
   }
 };
 // All of this workgroup's copies have arrived and all of its reads of shared memory are done.
@@ -238,7 +272,7 @@ __device__ __forceinline__ Sample sample_of(const WindowArgs &a, int b) {
   s.n = a.S;
   if (a.lengths) {
     const int64_t n = a.length_type ? load_global<int64_t>((const int64_t *)a.lengths + b) : (int64_t)load_global<int>((const int *)a.lengths + b);
-    s.n = n < 0 ? 0 : n < a.S ? (int)n : a.S;
+    s.n = __builtin_amdgcn_readfirstlane(n < 0 ? 0 : n < a.S ? (int)n : a.S);  // (all that a workgroup does by it is scalar)
   }
   s.off = (a.at_end ? s.n : a.S) - a.L;
   s.first = s.off < 0 ? -s.off : 0;
@@ -516,6 +550,7 @@ template <typename T, int DP, int N, typename ST> __device__ __forceinline__ voi
   f32x16_t s[N];
 #pragma unroll
   for (int x = 0; x < DP / 16; ++x) {
+    if (!at.has(x)) break;
     s[0] = Operand<T>::product(at.template of_rows<0>(kt, x), st.q[x], x ? s[0] : zeros16());
     if constexpr (N == 2) s[N - 1] = Operand<T>::product(at.template of_rows<32>(kt, x), st.q[x], x ? s[N - 1] : zeros16());
   }
@@ -570,6 +605,8 @@ struct Stretch {
   Walk w;
   int begin, end;
   __device__ __forceinline__ int tile(int u) const { return u < w.sinks ? u : w.first + (u - w.sinks); }
+  // Whether step u + by does not come `by` tiles behind step u.
+  __device__ __forceinline__ bool jumps(int u, int by) const { return u < w.sinks && u + by >= w.sinks && w.first != w.sinks; }
 };
 __device__ __forceinline__ Stretch stretch_of(const Walk &w, int split, int splits) {
   const int steps = w.sinks + (w.last >= w.first ? w.last - w.first + 1 : 0);
@@ -604,18 +641,18 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof
     const int ic = i < from ? from : i < to ? i : to - 1;
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
     const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.splits);
-    TileCopy<T, DP, G::kRows, kBlock> ck, cv;
-    ck.init(a.D, a.k.token_bytes);
-    cv.init(a.D, a.v.token_bytes);
+    TilePair<T, DP, G::kRows, kBlock> copy;
+    copy.init(a.D, a.k.token_bytes, a.v.token_bytes, s.n - 1);
     LaneOffsets<T, DP> at;
-    at.init();
+    at.init(a.D);
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
     const unsigned lds = lds_address(tiles) + wave * 1024;
-    auto issue = [&](int u, int buffer) {
-      const int first = w.tile(u) * G::kRows;
-      ck.issue(kb, first, s.n - 1, lds + buffer * 2 * G::kBytes, a.D);
-      cv.issue(vb, first, s.n - 1, lds + buffer * 2 * G::kBytes + G::kBytes, a.D);
+    auto issue = [&](int u, int buffer) {  // tile u, which is the next one; then the one behind it is
+      copy.issue(lds + buffer * 2 * G::kBytes, G::kBytes);
+      if (w.jumps(u, 1)) copy.go_to(kb, vb, w.tile(u + 1) * G::kRows);
+      else copy.advance(1);
     };
+    copy.go_to(kb, vb, w.tile(w.begin) * G::kRows);
     settle(st.q);
     int u = w.begin;
     if (u < w.end) issue(u, 0);
@@ -716,25 +753,24 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
     const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, 32), split, a.splits);
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
-    using Copy = TileCopy<T, DP, 32, 64>;
-    Copy ck, cv;
-    ck.init(a.D, a.k.token_bytes);
-    cv.init(a.D, a.v.token_bytes);
+    TilePair<T, DP, 32, 64> copy;
+    copy.init(a.D, a.k.token_bytes, a.v.token_bytes, s.n - 1);
     LaneOffsets<T, DP> at;
-    at.init();
+    at.init(a.D);
     const unsigned lds = lds_address(tiles) + wave * 2 * W::kStage;
     settle(st.q);
     auto issue = [&](int u, int buffer) {
-      const int first = w.tile(u) * 32;
-      ck.issue(kb, first, s.n - 1, lds + buffer * W::kStage, a.D);
-      cv.issue(vb, first, s.n - 1, lds + buffer * W::kStage + W::kStage / 2, a.D);
+      copy.issue(lds + buffer * W::kStage, W::kStage / 2);
+      if (w.jumps(u, kWaves)) copy.go_to(kb, vb, w.tile(u + kWaves) * 32);
+      else copy.advance(kWaves);
     };
+    copy.go_to(kb, vb, w.tile(w.begin + wave) * 32);
     int u = w.begin + wave, turn = 0;
     if (u < w.end) issue(u, 0);
     for (; u < w.end; u += kWaves) {
       char *tile = tiles + (wave * 2 + turn) * W::kStage;
       turn ^= 1;
-      next_copies<2 * Copy::kCopies>(u + kWaves < w.end, [&] { issue(u + kWaves, turn); });
+      next_copies<2 * TileCopy<T, DP, 32, 64>::kCopies>(u + kWaves < w.end, [&] { issue(u + kWaves, turn); });
       forward_tile<T, DP, 1>(st, at, tile, tile + W::kStage / 2, w.tile(u) * 32, a.scale_log2);
     }
   }
@@ -895,11 +931,10 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, q);
     if (i >= from && i < to) lse = load_global<float>(a.lse + row);
     const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.splits);
-    TileCopy<T, DP, G::kRows, kBlock> ck, cv;
-    ck.init(a.D, a.k.token_bytes);
-    cv.init(a.D, a.v.token_bytes);
+    TilePair<T, DP, G::kRows, kBlock> copy;
+    copy.init(a.D, a.k.token_bytes, a.v.token_bytes, s.n - 1);
     LaneOffsets<T, DP> at;
-    at.init();
+    at.init(a.D);
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
     const unsigned lds = lds_address(tiles) + wave * 1024;
     // P 2^bits (dP - delta) unit: the product starts from -delta
@@ -912,11 +947,12 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
     settle(q);
     settle(dout);
     pin(lift);
-    auto issue = [&](int u, int buffer) {
-      const int first = w.tile(u) * G::kRows;
-      ck.issue(kb, first, s.n - 1, lds + buffer * 2 * G::kBytes, a.D);
-      cv.issue(vb, first, s.n - 1, lds + buffer * 2 * G::kBytes + G::kBytes, a.D);
+    auto issue = [&](int u, int buffer) {  // tile u, which is the next one; then the one behind it is
+      copy.issue(lds + buffer * 2 * G::kBytes, G::kBytes);
+      if (w.jumps(u, 1)) copy.go_to(kb, vb, w.tile(u + 1) * G::kRows);
+      else copy.advance(1);
     };
+    copy.go_to(kb, vb, w.tile(w.begin) * G::kRows);
     int u = w.begin;
     if (u < w.end) issue(u, 0);
     auto turn = [&](auto buffer) {
@@ -934,6 +970,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
         f32x16_t p, dp;
 #pragma unroll
         for (int x = 0; x < DP / 16; ++x) {
+          if (!at.has(x)) break;
           p = Operand<T>::product(at.template of_rows<f>(kt, x), q[x], x ? p : zeros16());
           dp = Operand<T>::product(at.template of_rows<f>(vt, x), dout[x], x ? dp : start);
         }
@@ -1015,7 +1052,7 @@ template <bool AHEAD> __device__ __forceinline__ void phase_end() {
   if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
 }
 
-// 32 keys of a wavefront, one a lane.  PARTS: 1 dv, 2 dk, 3 both (heads of more than 128 channels do not fit the registers at once).
+// 32 keys of a wavefront, one a lane.  PARTS: 1 dv, 2 dk, 3 both (heads of more than 128 channels, in float32 96, do not fit the registers at once).
 template <typename T, int DP, int PARTS> struct KeySide {
   static constexpr bool kDv = PARTS & 1, kDk = PARTS & 2;
   static constexpr bool kAhead = DP <= (sizeof(T) == 2 ? 128 : 64);
@@ -1064,7 +1101,10 @@ template <typename T, int DP, int PARTS> struct KeySide {
       constexpr int f = decltype(first_row)::value;
       f32x16_t p, lse;
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) p = Operand<T>::product(qr[x], k[x], x ? p : zeros16());
+      for (int x = 0; x < DP / 16; ++x) {
+        if (!at.has(x)) break;
+        p = Operand<T>::product(qr[x], k[x], x ? p : zeros16());
+      }
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const f32x4 l4 = *(const f32x4 *)&lses[f + row_of(r, half)];
@@ -1079,7 +1119,10 @@ template <typename T, int DP, int PARTS> struct KeySide {
       phase_end<kAhead>();
       if constexpr (kDk) {
 #pragma unroll
-        for (int x = 0; x < DP / 16; ++x) dp = Operand<T>::product(gr[x], v[x], dp);
+        for (int x = 0; x < DP / 16; ++x) {
+          if (!at.has(x)) break;
+          dp = Operand<T>::product(gr[x], v[x], dp);
+        }
 #pragma unroll
         for (int x = 0; x < DP / 32; ++x) qc[x][0] = at.template of_columns<f>(qt, x), qc[x][1] = at.template of_columns<f + 16>(qt, x);
       }
@@ -1202,34 +1245,45 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
     }
     key.lowering = unit * (1.0f / 128.0f);
     key.load(a, b, j < s.n ? j : s.n - 1, kh);
-    TileCopy<T, DP, G::kRows, kBlock> cq, cg;
-    cq.init(a.D, a.q.token_bytes);
-    cg.init(a.D, a.dout.token_bytes);
+    TilePair<T, DP, G::kRows, kBlock> copy;
+    copy.init(a.D, a.q.token_bytes, a.dout.token_bytes, to);
     LaneOffsets<T, DP> at;
-    at.init();
+    at.init(a.D);
     const unsigned lds = lds_address(tiles) + wave * 1024, lds_lse = lds_address(lses), lds_delta = lds_address(deltas);
     key.settle_operands();
-    auto issue = [&](Step w, int buffer) {
+    const float *at_row = nullptr;  // lse for the first wavefront, -delta for the second
+    auto go_to = [&](Step w) {
       const int h = kh * a.group + w.g, i0 = (first + w.t) * G::kRows;
-      cq.issue((const char *)a.q.row(b, 0, h), i0, to, lds + buffer * 2 * G::kBytes, a.D);
-      cg.issue((const char *)a.dout.row(b, 0, h), i0, to, lds + buffer * 2 * G::kBytes + G::kBytes, a.D);
-      if (wave < (KS::kDk ? 2 : 1)) {
-        const int r = lane < to - i0 ? lane : to - i0;
-        const char *rows = (const char *)((wave ? a.delta : a.lse) + ((int64_t)b * a.H + h) * a.L + i0);
-        copy_to_lds<4>(uniform(rows), (unsigned)r * 4, (wave ? lds_delta : lds_lse) + buffer * 256);
-      }
+      copy.go_to((const char *)a.q.row(b, 0, h), (const char *)a.dout.row(b, 0, h), i0);
+      at_row = uniform((wave ? a.delta : a.lse) + ((int64_t)b * a.H + h) * a.L + i0);
     };
+    const unsigned lds_row = (wave ? lds_delta : lds_lse);
     int left_over = end - begin;
     Step step = {begin / tiles_of, begin % tiles_of}, next = step;
-    if (left_over > 0) issue(step, 0);
+    auto issue = [&](int buffer) {  // tile `next`; then the one behind it is next
+      copy.issue(lds + buffer * 2 * G::kBytes, G::kBytes);
+      if (wave < (KS::kDk ? 2 : 1)) {
+        const int r = to - copy.first;
+        copy_to_lds<4>((const char *)at_row, (unsigned)(lane < r ? lane : r) * 4, lds_row + buffer * 256);
+      }
+      next.advance(1, tiles_of);
+      if (next.t == 0) {
+        go_to(next.g < a.group ? next : step);
+      } else {
+        copy.advance(1);
+        at_row += G::kRows;
+      }
+    };
+    go_to(step);
+    if (left_over > 0) issue(0);
     auto turn = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
-      next.advance(1, tiles_of);
-      if (--left_over > 0) issue(next, 1 - B);
-      char *qt = tiles + B * 2 * G::kBytes;
-      key.template tile<G::kRows>(at, qt, qt + G::kBytes, lses + B * 64, deltas + B * 64, (first + step.t) * G::kRows + s.off);
+      const Step now = step;
       step = next;
+      if (--left_over > 0) issue(1 - B);
+      char *qt = tiles + B * 2 * G::kBytes;
+      key.template tile<G::kRows>(at, qt, qt + G::kBytes, lses + B * 64, deltas + B * 64, (first + now.t) * G::kRows + s.off);
     };
     while (left_over > 0) {
       turn(std::integral_constant<int, 0>());
@@ -1295,18 +1349,16 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
     }
     key.lowering = unit * (1.0f / 128.0f);
     key.load(a, b, j < s.n ? j : s.n - 1, kh);
-    using Copy = TileCopy<T, DP, 32, 64>;
-    Copy cq, cg;
-    cq.init(a.D, a.q.token_bytes);
-    cg.init(a.D, a.dout.token_bytes);
+    TilePair<T, DP, 32, 64> copy;
+    copy.init(a.D, a.q.token_bytes, a.dout.token_bytes, to);
     LaneOffsets<T, DP> at;
-    at.init();
+    at.init(a.D);
     const unsigned lds = lds_address(tiles) + wave * 2 * W::kStage, lds_lse = lds_address(lses) + wave * 512, lds_delta = lds_address(deltas) + wave * 512;
     key.settle_operands();
     auto issue = [&](Step w, int buffer) {
       const int h = kh * a.group + w.g, i0 = (first + w.t) * 32;
-      cq.issue((const char *)a.q.row(b, 0, h), i0, to, lds + buffer * W::kStage, a.D);
-      cg.issue((const char *)a.dout.row(b, 0, h), i0, to, lds + buffer * W::kStage + W::kStage / 2, a.D);
+      copy.go_to((const char *)a.q.row(b, 0, h), (const char *)a.dout.row(b, 0, h), i0);
+      copy.issue(lds + buffer * W::kStage, W::kStage / 2);
       const unsigned r = (unsigned)(lane < to - i0 ? lane : to - i0) * 4;
       const int64_t row = ((int64_t)b * a.H + h) * a.L + i0;
       copy_to_lds<4>(uniform((const char *)(a.lse + row)), r, lds_lse + buffer * 256);
@@ -1319,7 +1371,7 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
       const int now = turn;
       turn ^= 1;
       next.advance(kWaves, tiles_of);
-      next_copies<2 * Copy::kCopies + 2>(st + kWaves < end, [&] { issue(next, turn); });
+      next_copies<2 * TileCopy<T, DP, 32, 64>::kCopies + 2>(st + kWaves < end, [&] { issue(next, turn); });
       char *qt = tiles + (wave * 2 + now) * W::kStage;
       key.template tile<32>(at, qt, qt + W::kStage / 2, lses + (wave * 2 + now) * 64, deltas + (wave * 2 + now) * 64, (first + step.t) * 32 + s.off);
       step = next;

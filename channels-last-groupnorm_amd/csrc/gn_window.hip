@@ -30,7 +30,10 @@ template <typename F> void with_width(int D, F &&f) {
     case 96: return f(std::integral_constant<int, 96>());
     case 128: return f(std::integral_constant<int, 128>());
     default:
-      if constexpr (sizeof(elem_t) == 2) f(std::integral_constant<int, 256>());  // (float32: the plan takes heads of 128 at most)
+      if constexpr (sizeof(elem_t) == 2) {  // (float32: the plan takes heads of 128 at most)
+        if (D <= 160) f(std::integral_constant<int, 160>());
+        else f(std::integral_constant<int, 256>());
+      }
   }
 }
 dim3 grid_of(int items) { return dim3((unsigned)((items + 7) / 8 * 8)); }
@@ -70,7 +73,7 @@ hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const
       hipLaunchKernelGGL((window_dkv_kernel<elem_t, DP, P>), grid_of(kv.items), dim3(kBlock), 0, stream, kv);
       if (sinks.items) hipLaunchKernelGGL((window_sink_kernel<elem_t, DP, P>), grid_of(sinks.items), dim3(64 * Few<elem_t, DP>::kWaves), 0, stream, sinks);
     };
-    if constexpr (DP <= 128) {
+    if constexpr (DP <= (sizeof(elem_t) == 2 ? 128 : 96)) {
       keys(std::integral_constant<int, 3>());
     } else {
       keys(std::integral_constant<int, 1>());

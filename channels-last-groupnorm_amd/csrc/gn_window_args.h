@@ -37,7 +37,7 @@ struct WindowArgs {
 };
 
 // Wavefronts of a workgroup whose wavefronts have two pairs of tiles of 32 rows each, for a head padded to `width` channels.
-constexpr int window_width(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
+constexpr int window_width(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 160 ? 160 : 256; }
 constexpr int few_waves(int width, int elem_size) {
   const int most = 131072 / (4 * 32 * width * elem_size);
   return most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
