@@ -344,7 +344,8 @@ __device__ __forceinline__ int work_item(const WindowArgs &a) {
 // ---- rows by their formulas, for results that are not finite ----
 // A tile's products reach over all of its rows: what a token does not see has the weight 0 there, and 0 times an infinity or a NaN
 // of such a token is NaN.  A row that comes out infinite or NaN is therefore computed again over the pairs that see each other
-// alone, by one wavefront, in float32.  (Rows that have to be so, as in a training that has diverged, take this path too.)
+// alone, by one wavefront, in float32.  Rows that have to be NaN whatever they see (their own q is not finite: so are all scores,
+// and infinite ones differ by NaN) are seen to be at once: a training that has diverged has nothing but those.
 template <typename T> __device__ __forceinline__ float dot(const T *a, const T *b, int D) {
   float s = 0.0f;
 #pragma unroll 4
@@ -370,10 +371,29 @@ template <typename F> __device__ __forceinline__ void for_keys(const Sight &g, F
   if (g.count > 0 && g.low + g.count < g.sinks)
     for (int j0 = g.low + g.count; j0 < g.sinks; j0 += 64) f(j0, j0 + lane < g.sinks ? j0 + lane : -1);
 }
+// Whether a row of D channels holds a NaN, or with `infinite` anything that is not finite; all lanes of a wavefront ask together.
+template <typename T> __device__ __forceinline__ bool holds_nan(const T *p, int D, bool infinite) {
+  const int lane = threadIdx.x & 63;
+  bool bad = false;
+  for (int d = lane; d < D; d += 64) {
+    const float v = to_float(p + d);
+    bad = bad || (infinite ? !(v * 0.0f == 0.0f) : v != v);
+  }
+  return __any(bad);
+}
+template <typename T> __device__ __forceinline__ void fill_nan(T *p, int D) {
+  const float t[1] = {__builtin_nanf("")};
+  for (int d = threadIdx.x & 63; d < D; d += 64) LaneVec<T, 1>::store(p + d, LaneVec<T, 1>::pack(t));
+}
 template <typename T> __device__ void row_again(const WindowArgs &a, const Sample &s, int b, int h, int i) {
   const int lane = threadIdx.x & 63, kh = h / a.group;
   const Sight g = sight_of(a, s, i);
   const T *q = (const T *)a.q.row(b, i, h);
+  if (holds_nan(q, a.D, true)) {
+    fill_nan((T *)a.out.row(b, i, h), a.D);
+    if (a.lse && lane == 0) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, __builtin_nanf(""));
+    return;
+  }
   float most = -INFINITY, nan = 0.0f;
   for_keys(g, [&](int, int j) {
     if (j >= 0) {
@@ -415,6 +435,7 @@ template <typename T> __device__ void row_again(const WindowArgs &a, const Sampl
 template <typename T> __device__ void dq_again(const WindowArgs &a, const Sample &s, int b, int h, int i, float lse, float delta) {
   const int lane = threadIdx.x & 63, kh = h / a.group;
   const T *q = (const T *)a.q.row(b, i, h), *g = (const T *)a.dout.row(b, i, h);
+  if (lse != lse || delta != delta) return fill_nan((T *)a.dq.row(b, i, h), a.D);
   float acc[4] = {};
   for_keys(sight_of(a, s, i), [&](int, int j) {
     float ds = 0.0f;
@@ -445,6 +466,7 @@ template <typename T> __device__ void dkv_again(const WindowArgs &a, const Sampl
   const int lane = threadIdx.x & 63;
   const T *k = (const T *)a.k.row(b, j, kh), *v = (const T *)a.v.row(b, j, kh);
   const Seen w = seen_of(a, s, j);
+  if (holds_nan(k, a.D, false) || (of_k && holds_nan(v, a.D, false))) return fill_nan((T *)(of_k ? a.dk.row(b, j, kh) : a.dv.row(b, j, kh)), a.D);
   float acc[4] = {};
   for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
     const int64_t rows = ((int64_t)b * a.H + h) * a.L;
@@ -513,6 +535,13 @@ template <typename T, int DP> __device__ __forceinline__ void store_token(T *p, 
         LV::store(p + d, LV::pack(t));
       }
     }
+}
+// A token that sees nothing, or that nobody sees, gets zeros, whatever its tile held: its weights are 0, and 0 times NaN is NaN.
+template <int N> __device__ __forceinline__ void clear_unless(bool kept, f32x16_t (&acc)[N]) {
+#pragma unroll
+  for (int x = 0; x < N; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[x][r] = kept ? acc[x][r] : 0.0f;
 }
 template <int N> __device__ __forceinline__ bool any_not_finite(const f32x16_t (&acc)[N]) {
   float t = 0.0f;
@@ -671,6 +700,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof
   }
   const float sum = st.sum + other_half(st.sum);
   const bool there = i < a.L, seeing = st.sight.count > 0 || st.sight.sinks > 0;
+  clear_unless(seeing, st.o);
   if (a.splits > 1) {
     if (there) {
       const int64_t row = part_row(a, split, b, h, i);
@@ -775,6 +805,7 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
     }
   }
   // join the wavefronts
+  clear_unless(st.sight.count > 0 || st.sight.sinks > 0, st.o);
   st.sum += other_half(st.sum);
   if (lane < 32) {
     references[wave][lane] = st.reference;
@@ -1000,6 +1031,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
     }
   }
   const bool there = i < a.L, seeing = sight.count > 0 || sight.sinks > 0;
+  clear_unless(seeing, acc);
   const bool again = either_half(any_not_finite(acc)) && seeing && there;
   if (there) {
     const float factor = seeing ? a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f) : 0.0f;
@@ -1067,6 +1099,10 @@ template <typename T, int DP, int PARTS> struct KeySide {
       if constexpr (kDk) dk[x] = zeros16();
       if constexpr (kDv) dv[x] = zeros16();
     }
+  }
+  __device__ __forceinline__ void clear_unseen() {
+    if constexpr (kDk) clear_unless(seen.count > 0, dk);
+    if constexpr (kDv) clear_unless(seen.count > 0, dv);
   }
   __device__ __forceinline__ void load(const WindowArgs &a, int b, int j, int kh) {
     load_token<T, DP>((const T *)a.k.row(b, j, kh), a.D, k);
@@ -1291,6 +1327,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
       turn(std::integral_constant<int, 1>());
     }
   }
+  key.clear_unseen();
   if (a.shares > 1) {
     const int64_t slot = tile_slot(a, bk, tile, share) + wave * 32 + (lane & 31);
     if constexpr (KS::kDk) store_token<float, DP>(a.part_k + slot * a.D, a.D, key.dk, KS::k_factor(a, unit));
@@ -1377,6 +1414,7 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
       step = next;
     }
   }
+  key.clear_unseen();
   // the wavefronts' sums, through the tiles' place
   float *mine = (float *)(tiles + wave * 2 * W::kStage);
   const int64_t slot = sink_slot(a, bk, set, share);

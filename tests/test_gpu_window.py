@@ -112,6 +112,31 @@ def test_values_that_are_not_finite_reach_those_that_see_them(bad, causal, dtype
             assert not torch.isfinite(got["out"][:, by_key, :, 5]).any()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 150, 4, 2, 64, 100), (2, 900, 8, 8, 128, 800), (6, 1500, 6, 3, 64, 1450)])  # with and without shared keys
+def test_padding_next_to_values_that_are_not_finite(shape, dtype, device):
+    """Tokens of one tile, one NaN or infinite and others padding: those still get zeros."""
+    B, L, H, K, D, n = shape
+    lengths = torch.full((B,), n, device=device)
+    for i, bad in enumerate((math.nan, math.inf, math.nan, math.nan)):
+        tensors = [normal((B, L, h, D), dtype, device, j) for j, h in enumerate((H, K, K, H))]
+        tensors[i][:, [1, n - 8]] = bad
+        q, k, v = (t.requires_grad_(True) for t in tensors[:3])
+        out = window_attention(q, k, v, 21, 3, False, lengths)
+        for name, t in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, [q, k, v], tensors[3]))):
+            assert not t[:, n:].any(), (name, i)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_a_training_that_has_diverged(dtype, device):
+    """Where all is NaN, all of the results are, without a row by row search that would take seconds."""
+    q, k, v = (torch.full((2, 700, h, 64), math.nan, dtype=dtype, device=device).requires_grad_(True) for h in (8, 4, 4))
+    for window, sinks in ((None, 0), (50, 4)):
+        out = window_attention(q, k, v, window, sinks)
+        for t in (out, *torch.autograd.grad(out, [q, k, v], torch.full_like(out, math.nan))):
+            assert t.isnan().all()
+
+
 @pytest.mark.parametrize("gain", [2.0 ** -20, 2.0 ** 12])
 def test_gradients_of_any_scale_in_half_precision(gain, device):
     """float16 gradients of a scaled or an averaged loss: dS is held relative to the largest."""

@@ -84,6 +84,16 @@ def test_values_that_are_not_finite(S, dtype, device):
         ref.check(out[0, 1], tuple(t[0, 1] for t in want), "out")
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T,S", [(40, 60), (40, 5000), (200, 300)])
+def test_rows_in_front_of_a_short_request_are_zeros_whatever_it_holds(T, S, dtype, device):
+    q, k, v = (normal((2, n, h, 64), dtype, device, i) for i, (n, h) in enumerate(((T, 2), (S, 2), (S, 2))))
+    for t in (q, k, v):
+        t[0] = math.nan
+    out = window_attention_cached(q, k, v, torch.tensor([10, S], device=device), 20, 3)
+    assert not out[0, :T - 10].any() and out[0, T - 10:].isnan().all() and torch.isfinite(out[1]).all()
+
+
 def test_a_step_gives_what_the_whole_sequence_gives(device):
     """Codes one at a time against a cache that grows, and all of them at once: both round to bfloat16 what is within the bound."""
     B, S, H, K, D, window, sinks = 2, 70, 4, 2, 64, 20, 3
