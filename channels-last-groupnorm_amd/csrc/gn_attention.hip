@@ -99,6 +99,8 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     if (const int rc = put_rows(a.dv, c->v_grad, c->v_grad_stride, c->batch, c->keys, kv, es, "v_grad")) return rc;
     if (c->batch && c->tokens && !c->lse) return invalid("lse is null");
   }
+  if ((uintptr_t)c->out_rest % 16) return invalid("out_rest must be 16-byte aligned");
+  a.rest = es == 2 ? c->out_rest : nullptr;
   a.lse = c->lse;
   a.lengths = c->lengths;
   a.length_type = (int)c->length_type;

@@ -573,16 +573,20 @@ bool window_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor
   c.dtype = code;
   return true;
 }
-void run_window(const Tensor &q, gnnhwc_window_call &c, bool want_lse, Tensor &out, Tensor &lse) {
+// lse and rest are what the backward reads besides; both or neither, but float32 has no rest (a tensor without elements).
+void run_window(const Tensor &q, gnnhwc_window_call &c, Tensor &out, Tensor *lse, Tensor *rest) {
   const c10::DeviceGuard guard(q.device());
   const at::AutoDispatchBelowADInplaceOrView below;
   const OperatorRange range("gnop::window_attention");
   out = fresh(q.sizes(), q.scalar_type(), q);
   c.out = out.data_ptr();
   put_strides(out, c.out_stride);
-  if (want_lse) {
-    lse = fresh({q.size(0), q.size(2), q.size(1)}, at::kFloat, q);
-    c.lse = (float *)lse.data_ptr();
+  if (lse) {
+    *lse = fresh({q.size(0), q.size(2), q.size(1)}, at::kFloat, q);
+    c.lse = (float *)lse->data_ptr();
+    const bool has_rest = q.scalar_type() != at::kFloat;
+    *rest = has_rest ? fresh(q.sizes(), q.scalar_type(), q) : fresh({0}, q.scalar_type(), q);
+    c.out_rest = has_rest ? rest->data_ptr() : nullptr;
   }
   const size_t bytes = abi.window_workspace_bytes(&c);
   const Tensor ws = workspace(bytes, q, "gnop::window_attention");
@@ -592,9 +596,9 @@ void run_window(const Tensor &q, gnnhwc_window_call &c, bool want_lse, Tensor &o
 struct WindowNode : public torch::autograd::Function<WindowNode> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v,
                                                 const optional<Tensor> &lengths, gnnhwc_window_call *c) {
-    Tensor out, lse;
-    run_window(q, *c, true, out, lse);
-    ctx->save_for_backward({q, k, v, out, lse, defined(lengths)});
+    Tensor out, lse, rest;
+    run_window(q, *c, out, &lse, &rest);
+    ctx->save_for_backward({q, k, v, out, lse, rest, defined(lengths)});
     ctx->saved_data["window"] = c->window;
     ctx->saved_data["sinks"] = c->sinks;
     ctx->saved_data["causal"] = (bool)c->causal;
@@ -603,7 +607,7 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor q = saved[0], k = saved[1], v = saved[2], out = saved[3], lse = saved[4], lengths = saved[5], dout = grads[0];
+    const Tensor q = saved[0], k = saved[1], v = saved[2], out = saved[3], lse = saved[4], rest = saved[5], lengths = saved[6], dout = grads[0];
     const c10::Device device = dout.device();
     gnnhwc_window_call c = {};
     c.window = ctx->saved_data["window"].toInt();
@@ -614,11 +618,12 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
     // (as for the norm: whatever is not plain goes through the operator)
     if (at::GradMode::is_enabled() || !ordinary_dispatch() || !plain(q, device) || !window_call(q, k, v, lengths, c) ||
         !rows16(dout, device, q.scalar_type()) || dout.sizes() != q.sizes() || !rows16(out, device, q.scalar_type()) || out.sizes() != q.sizes() ||
-        !plain(lse, device) || !lse.is_contiguous() || lse.scalar_type() != at::kFloat || lse.numel() != q.size(0) * q.size(1) * q.size(2)) {
+        !plain(lse, device) || !lse.is_contiguous() || lse.scalar_type() != at::kFloat || lse.numel() != q.size(0) * q.size(1) * q.size(2) ||
+        (rest.numel() && (!rows16(rest, device, q.scalar_type()) || rest.sizes() != q.sizes() || !rest.is_contiguous()))) {
       using Signature = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
-                                                           const optional<Tensor> &, int64_t, int64_t, bool, double);
+                                                           const Tensor &, const optional<Tensor> &, int64_t, int64_t, bool, double);
       const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnop::window_attention_bwd", "").typed<Signature>();
-      std::tie(dq, dk, dv) = op.call(dout, q, k, v, out, lse, lengths.defined() ? optional<Tensor>(lengths) : std::nullopt, c.window, c.sinks, c.causal, c.scale);
+      std::tie(dq, dk, dv) = op.call(dout, q, k, v, out, lse, rest, lengths.defined() ? optional<Tensor>(lengths) : std::nullopt, c.window, c.sinks, c.causal, c.scale);
     } else {
       const c10::DeviceGuard guard(device);
       const at::AutoDispatchBelowADInplaceOrView below;
@@ -628,6 +633,7 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
       dv = fresh(v.sizes(), v.scalar_type(), v);
       c.out = out.data_ptr();
       c.lse = (float *)lse.data_ptr();
+      c.out_rest = rest.numel() ? rest.data_ptr() : nullptr;
       c.out_grad = dout.data_ptr();
       c.q_grad = dq.data_ptr();
       c.k_grad = dk.data_ptr();
@@ -681,11 +687,11 @@ PyObject *window_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
   if (!(c.scale > 1e-30 && c.scale < 1e30) || (!c.at_end && c.tokens > c.keys) || (c.at_end && differentiates) || c.keys > (1 << 30) || c.tokens > (1 << 30) ||
       c.heads > 65535 || c.batch * c.heads * (c.tokens / 128 + 1) > 1 << 22)
     return decline();
-  Tensor out, lse;
+  Tensor out;
   {
     const WithoutGil released;
     if (differentiates) out = WindowNode::apply(q, k, v, lengths_, &c)[0];
-    else run_window(q, c, false, out, lse);
+    else run_window(q, c, out, nullptr, nullptr);
   }
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS

@@ -341,6 +341,13 @@ __device__ __forceinline__ int work_item(const WindowArgs &a) {
   return a.order == kStretches ? die * ((a.items + 7) >> 3) + n : id;
 }
 
+// The kernel's arguments, read again behind a loop, so that those of the results take no registers in it.
+__device__ __forceinline__ const WindowArgs &arguments_again() {
+  auto p = (const __attribute__((address_space(4))) WindowArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const WindowArgs *)p;
+}
+
 // ---- rows by their formulas, for results that are not finite ----
 // A tile's products reach over all of its rows: what a token does not see has the weight 0 there, and 0 times an infinity or a NaN
 // of such a token is NaN.  A row that comes out infinite or NaN is therefore computed again over the pairs that see each other
@@ -385,6 +392,22 @@ template <typename T> __device__ __forceinline__ void fill_nan(T *p, int D) {
   const float t[1] = {__builtin_nanf("")};
   for (int d = threadIdx.x & 63; d < D; d += 64) LaneVec<T, 1>::store(p + d, LaneVec<T, 1>::pack(t));
 }
+// Channels d .. d + N - 1 of a row of out, rounded, and what the rounding left.  (The backward's delta, the sum of do * out, is made
+// of both: dP - delta of a token that sees a few others is a small difference, and 2^-9 of out is not small against it.)
+template <typename T, int N> __device__ __forceinline__ void store_out(const WindowArgs &a, int b, int h, int i, int d, const float (&t)[N]) {
+  using LV = LaneVec<T, N>;
+  const auto raw = LV::pack(t);
+  LV::store((T *)a.out.row(b, i, h) + d, raw);
+  if constexpr (sizeof(T) == 2) {
+    if (a.rest) {
+      float r[N];
+      LV::unpack(raw, r);
+#pragma unroll
+      for (int e = 0; e < N; ++e) r[e] = t[e] - r[e];
+      LV::store((T *)a.rest + (((int64_t)b * a.L + i) * a.H + h) * a.D + d, LV::pack(r));
+    }
+  }
+}
 template <typename T> __device__ void row_again(const WindowArgs &a, const Sample &s, int b, int h, int i) {
   const int lane = threadIdx.x & 63, kh = h / a.group;
   const Sight g = sight_of(a, s, i);
@@ -422,12 +445,11 @@ template <typename T> __device__ void row_again(const WindowArgs &a, const Sampl
         if (x * 64 + lane < a.D) o[x] = __builtin_fmaf(pu, to_float(v + x * 64 + lane), o[x]);
     }
   });
-  T *to = (T *)a.out.row(b, i, h);
 #pragma unroll
   for (int x = 0; x < 4; ++x)
     if (x * 64 + lane < a.D) {
       const float t[1] = {o[x]};
-      LaneVec<T, 1>::store(to + x * 64 + lane, LaneVec<T, 1>::pack(t));
+      store_out<T, 1>(a, b, h, i, x * 64 + lane, t);
     }
   if (a.lse && lane == 0) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, most + __builtin_amdgcn_logf(sum));
 }
@@ -647,7 +669,7 @@ __device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int 
 }
 
 // A workgroup: 128 queries of one head, 32 a wavefront, against one of `splits` shares of the keys that they see.
-template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
+template <typename T, int DP> __global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a);
@@ -698,16 +720,17 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof
       turn(std::integral_constant<int, 1>());
     }
   }
+  const WindowArgs &z = arguments_again();
   const float sum = st.sum + other_half(st.sum);
-  const bool there = i < a.L, seeing = st.sight.count > 0 || st.sight.sinks > 0;
+  const bool there = i < z.L, seeing = st.sight.count > 0 || st.sight.sinks > 0;
   clear_unless(seeing, st.o);
-  if (a.splits > 1) {
+  if (z.splits > 1) {
     if (there) {
-      const int64_t row = part_row(a, split, b, h, i);
-      store_token<float, DP>(a.part_v + row * a.D, a.D, st.o, 1.0f);
+      const int64_t row = part_row(z, split, b, h, i);
+      store_token<float, DP>(z.part_v + row * z.D, z.D, st.o, 1.0f);
       if (lane < 32) {
-        store_global<float>(a.part_k + 2 * row, st.reference);
-        store_global<float>(a.part_k + 2 * row + 1, sum);
+        store_global<float>(z.part_k + 2 * row, st.reference);
+        store_global<float>(z.part_k + 2 * row + 1, sum);
       }
     }
     return;
@@ -716,14 +739,21 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof
   const float factor = nothing ? 0.0f : 1.0f / sum;
   const bool again = either_half(any_not_finite(st.o) || !(factor < INFINITY) || nothing) && seeing;
   if (there) {
-    store_token<T, DP>((T *)a.out.row(b, i, h), a.D, st.o, factor);
-    if (a.lse && lane < 32) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, nothing ? INFINITY : st.reference + __builtin_amdgcn_logf(sum));
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * c + row_of(r, lane >> 5);
+        const float t[4] = {st.o[c][r] * factor, st.o[c][r + 1] * factor, st.o[c][r + 2] * factor, st.o[c][r + 3] * factor};
+        if (d < z.D) store_out<T, 4>(z, b, h, i, d, t);
+      }
+    if (z.lse && lane < 32) store_global<float>(z.lse + ((int64_t)b * z.H + h) * z.L + i, nothing ? INFINITY : st.reference + __builtin_amdgcn_logf(sum));
   }
   uint64_t rows = __ballot(again && there) & 0xffffffffu;
   while (rows) {
     const int r = __builtin_ctzll(rows);
     rows &= rows - 1;
-    row_again<T>(a, s, b, h, tile * kQueries + wave * 32 + r);
+    row_again<T>(z, s, b, h, tile * kQueries + wave * 32 + r);
   }
 }
 
@@ -804,6 +834,7 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
       forward_tile<T, DP, 1>(st, at, tile, tile + W::kStage / 2, w.tile(u) * 32, a.scale_log2);
     }
   }
+  const WindowArgs &z = arguments_again();
   // join the wavefronts
   clear_unless(st.sight.count > 0 || st.sight.sinks > 0, st.o);
   st.sum += other_half(st.sum);
@@ -835,24 +866,23 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   __syncthreads();
   for (int e = threadIdx.x; e < 32 * DP / 4; e += 64 * kWaves) {
     const int r = e / (DP / 4), d = e % (DP / 4) * 4, rr = block * 32 + r;
-    if (rr >= rows || d >= a.D) continue;
+    if (rr >= rows || d >= z.D) continue;
     f32x4 v = *(const f32x4 *)((const float *)tiles + r * W::kPitch + d);
 #pragma unroll
     for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)(tiles + n * 2 * W::kStage) + r * W::kPitch + d);
-    if (a.splits > 1) {
-      store_global<f32x4>(a.part_v + part_row(a, split, b, kh * a.group + rr % a.group, rr / a.group) * a.D + d, v);
+    if (z.splits > 1) {
+      store_global<f32x4>(z.part_v + part_row(z, split, b, kh * z.group + rr % z.group, rr / z.group) * z.D + d, v);
       continue;
     }
     const float total = sums[0][r], factor = total > 0.0f ? 1.0f / total : 0.0f;
     const float t[4] = {v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor};
     if (!(v[0] * 0.0f + v[1] * 0.0f + v[2] * 0.0f + v[3] * 0.0f + factor * 0.0f == 0.0f) || !(total > 0.0f)) bad[r] = 1;
-    using LV = LaneVec<T, 4>;
-    LV::store((T *)a.out.row(b, rr / a.group, kh * a.group + rr % a.group) + d, LV::pack(t));
+    store_out<T, 4>(z, b, kh * z.group + rr % z.group, rr / z.group, d, t);
   }
-  if (a.splits > 1) {
+  if (z.splits > 1) {
     const int rr = block * 32 + (int)threadIdx.x;
     if (threadIdx.x < 32 && rr < rows) {
-      float *p = a.part_k + 2 * part_row(a, split, b, kh * a.group + rr % a.group, rr / a.group);
+      float *p = z.part_k + 2 * part_row(z, split, b, kh * z.group + rr % z.group, rr / z.group);
       store_global<float>(p, references[0][threadIdx.x]);
       store_global<float>(p + 1, sums[0][threadIdx.x]);
     }
@@ -862,11 +892,11 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   for (int r = wave; r < 32; r += kWaves) {
     const int rr = block * 32 + r;
     if (rr >= rows) break;
-    const int ir = rr / a.group, hr = kh * a.group + rr % a.group;
-    const Sight g = sight_of(a, s, ir);
-    if (a.lse && lane == 0)
-      store_global<float>(a.lse + ((int64_t)b * a.H + hr) * a.L + ir, sums[0][r] > 0.0f ? references[0][r] + __builtin_amdgcn_logf(sums[0][r]) : INFINITY);
-    if (bad[r] && (g.count > 0 || g.sinks > 0)) row_again<T>(a, s, b, hr, ir);
+    const int ir = rr / z.group, hr = kh * z.group + rr % z.group;
+    const Sight g = sight_of(z, s, ir);
+    if (z.lse && lane == 0)
+      store_global<float>(z.lse + ((int64_t)b * z.H + hr) * z.L + ir, sums[0][r] > 0.0f ? references[0][r] + __builtin_amdgcn_logf(sums[0][r]) : INFINITY);
+    if (bad[r] && (g.count > 0 || g.sinks > 0)) row_again<T>(z, s, b, hr, ir);
   }
 }
 
@@ -894,19 +924,19 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
     const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
     const float t[4] = {o[0] * factor, o[1] * factor, o[2] * factor, o[3] * factor};
     const int i = (int)(id % a.L), h = (int)(id / a.L % a.H), b = (int)(id / a.L / a.H);
-    using LV = LaneVec<T, 4>;
-    LV::store((T *)a.out.row(b, i, h) + d, LV::pack(t));
+    store_out<T, 4>(a, b, h, i, d, t);
     if (a.lse && d == 0) store_global<float>(a.lse + id, sum > 0.0f ? most + __builtin_amdgcn_logf(sum) : INFINITY);
     if (!(t[0] * 0.0f + t[1] * 0.0f + t[2] * 0.0f + t[3] * 0.0f == 0.0f) || !(sum > 0.0f)) bad[r] = 1;
   }
   __syncthreads();
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!bad[n]) continue;
+    const WindowArgs &z = arguments_again();
     const int64_t row = (int64_t)blockIdx.x * rows_here + n;
-    const int i = (int)(row % a.L), h = (int)(row / a.L % a.H), b = (int)(row / a.L / a.H);
-    const Sample s = sample_of(a, b);
-    const Sight g = sight_of(a, s, i);
-    if (g.count > 0 || g.sinks > 0) row_again<T>(a, s, b, h, i);
+    const int i = (int)(row % z.L), h = (int)(row / z.L % z.H), b = (int)(row / z.L / z.H);
+    const Sample s = sample_of(z, b);
+    const Sight g = sight_of(z, s, i);
+    if (g.count > 0 || g.sinks > 0) row_again<T>(z, s, b, h, i);
   }
 }
 
@@ -951,6 +981,15 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
           delta = __builtin_fmaf((float)dout[x][e], (float)q[x][e], delta);
           most = fmaxf(most, fabsf((float)dout[x][e]));
         }
+      if constexpr (sizeof(T) == 2) {
+        if (a.rest) {
+          load_token<T, DP>((const T *)a.rest + (((int64_t)b * a.L + ic) * a.H + h) * a.D, a.D, q);
+#pragma unroll
+          for (int x = 0; x < DP / 16; ++x)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)dout[x][e], (float)q[x][e], delta);
+        }
+      }
       delta += other_half(delta);
       most = fmaxf(most, other_half(most));
       unit = gradient_unit<T>(most);
@@ -1030,22 +1069,23 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
       turn(std::integral_constant<int, 1>());
     }
   }
-  const bool there = i < a.L, seeing = sight.count > 0 || sight.sinks > 0;
+  const WindowArgs &z = arguments_again();
+  const bool there = i < z.L, seeing = sight.count > 0 || sight.sinks > 0;
   clear_unless(seeing, acc);
   const bool again = either_half(any_not_finite(acc)) && seeing && there;
   if (there) {
-    const float factor = seeing ? a.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f) : 0.0f;
-    if (a.splits > 1) {
-      store_token<float, DP>(a.part_q + part_row(a, split, b, h, i) * a.D, a.D, acc, factor);
+    const float factor = seeing ? z.scale * (__is_same(T, f16_t) ? 1.0f / 32.0f / unit : 1.0f) : 0.0f;
+    if (z.splits > 1) {
+      store_token<float, DP>(z.part_q + part_row(z, split, b, h, i) * z.D, z.D, acc, factor);
       return;
     }
-    store_token<T, DP>((T *)a.dq.row(b, i, h), a.D, acc, factor);
+    store_token<T, DP>((T *)z.dq.row(b, i, h), z.D, acc, factor);
   }
   uint64_t rows = __ballot(again) & 0xffffffffu;
   while (rows) {
     const int r = __builtin_ctzll(rows);
     rows &= rows - 1;
-    dq_again<T>(a, s, b, h, tile * kQueries + wave * 32 + r, __shfl(lse, r), __shfl(delta, r));
+    dq_again<T>(z, s, b, h, tile * kQueries + wave * 32 + r, __shfl(lse, r), __shfl(delta, r));
   }
 }
 static_assert(kGradBits == 5.0f, "the factors of 1 / 32 undo it");
@@ -1069,11 +1109,12 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_ke
   __syncthreads();
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!bad[n]) continue;
+    const WindowArgs &z = arguments_again();
     const int64_t row = (int64_t)blockIdx.x * rows_here + n;
-    const int i = (int)(row % a.L), h = (int)(row / a.L % a.H), b = (int)(row / a.L / a.H);
-    const Sample s = sample_of(a, b);
-    const Sight g = sight_of(a, s, i);
-    if (g.count > 0 || g.sinks > 0) dq_again<T>(a, s, b, h, i, load_global<float>(a.lse + row), -load_global<float>(a.delta + row));
+    const int i = (int)(row % z.L), h = (int)(row / z.L % z.H), b = (int)(row / z.L / z.H);
+    const Sample s = sample_of(z, b);
+    const Sight g = sight_of(z, s, i);
+    if (g.count > 0 || g.sinks > 0) dq_again<T>(z, s, b, h, i, load_global<float>(z.lse + row), -load_global<float>(z.delta + row));
   }
 }
 
@@ -1327,16 +1368,17 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
       turn(std::integral_constant<int, 1>());
     }
   }
+  const WindowArgs &z = arguments_again();
   key.clear_unseen();
-  if (a.shares > 1) {
-    const int64_t slot = tile_slot(a, bk, tile, share) + wave * 32 + (lane & 31);
-    if constexpr (KS::kDk) store_token<float, DP>(a.part_k + slot * a.D, a.D, key.dk, KS::k_factor(a, unit));
-    if constexpr (KS::kDv) store_token<float, DP>(a.part_v + slot * a.D, a.D, key.dv, KS::v_factor());
+  if (z.shares > 1) {
+    const int64_t slot = tile_slot(z, bk, tile, share) + wave * 32 + (lane & 31);
+    if constexpr (KS::kDk) store_token<float, DP>(z.part_k + slot * z.D, z.D, key.dk, KS::k_factor(z, unit));
+    if constexpr (KS::kDv) store_token<float, DP>(z.part_v + slot * z.D, z.D, key.dv, KS::v_factor());
     return;
   }
   if (ours) {
-    if constexpr (KS::kDk) store_token<T, DP>((T *)a.dk.row(b, j, kh), a.D, key.dk, KS::k_factor(a, unit));
-    if constexpr (KS::kDv) store_token<T, DP>((T *)a.dv.row(b, j, kh), a.D, key.dv, KS::v_factor());
+    if constexpr (KS::kDk) store_token<T, DP>((T *)z.dk.row(b, j, kh), z.D, key.dk, KS::k_factor(z, unit));
+    if constexpr (KS::kDv) store_token<T, DP>((T *)z.dv.row(b, j, kh), z.D, key.dv, KS::v_factor());
   }
   bool bad[2] = {false, false};
   if constexpr (KS::kDv) bad[0] = any_not_finite(key.dv);
@@ -1346,7 +1388,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
     while (rows) {
       const int r = __builtin_ctzll(rows);
       rows &= rows - 1;
-      dkv_again<T>(a, s, b, kh, tile * kQueries + wave * 32 + r, of_k == 1);
+      dkv_again<T>(z, s, b, kh, tile * kQueries + wave * 32 + r, of_k == 1);
     }
   }
 }
@@ -1414,10 +1456,11 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
       step = next;
     }
   }
+  const WindowArgs &z = arguments_again();
   key.clear_unseen();
   // the wavefronts' sums, through the tiles' place
   float *mine = (float *)(tiles + wave * 2 * W::kStage);
-  const int64_t slot = sink_slot(a, bk, set, share);
+  const int64_t slot = sink_slot(z, bk, set, share);
   auto add = [&](const auto &acc, float factor, float *to) {
     __syncthreads();  // (no copy is on its way: each wavefront has waited for its last one)
     #pragma unroll
@@ -1429,15 +1472,15 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
     __syncthreads();
     for (int e = threadIdx.x; e < 32 * DP / 4; e += 64 * kWaves) {
       const int r = e / (DP / 4), d = e % (DP / 4) * 4;
-      if (d >= a.D) continue;
+      if (d >= z.D) continue;
       f32x4 v = *(const f32x4 *)((const float *)tiles + r * W::kPitch + d);
 #pragma unroll
       for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)(tiles + n * 2 * W::kStage) + r * W::kPitch + d);
-      store_global<f32x4>(to + (slot + r) * a.D + d, v);
+      store_global<f32x4>(to + (slot + r) * z.D + d, v);
     }
   };
-  if constexpr (KS::kDk) add(key.dk, KS::k_factor(a, unit), a.part_k);
-  if constexpr (KS::kDv) add(key.dv, KS::v_factor(), a.part_v);
+  if constexpr (KS::kDk) add(key.dk, KS::k_factor(z, unit), z.part_k);
+  if constexpr (KS::kDv) add(key.dv, KS::v_factor(), z.part_v);
 }
 
 // Sums of the keys that several workgroups shared, all keys or the sinks: four channels of a row each thread.
@@ -1470,12 +1513,13 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kerne
   __syncthreads();
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!(bad_k[n] | bad_v[n])) continue;
+    const WindowArgs &z = arguments_again();
     const int64_t row = (int64_t)blockIdx.x * rows_here + n;
-    const int bk = (int)(row / rows), key = (int)(row % rows), b = bk / a.K;
-    const Sample s = sample_of(a, b);
-    if (seen_of(a, s, key).count == 0) continue;
-    if (bad_v[n]) dkv_again<T>(a, s, b, bk % a.K, key, false);
-    if (bad_k[n]) dkv_again<T>(a, s, b, bk % a.K, key, true);
+    const int bk = (int)(row / rows), key = (int)(row % rows), b = bk / z.K;
+    const Sample s = sample_of(z, b);
+    if (seen_of(z, s, key).count == 0) continue;
+    if (bad_v[n]) dkv_again<T>(z, s, b, bk % z.K, key, false);
+    if (bad_k[n]) dkv_again<T>(z, s, b, bk % z.K, key, true);
   }
 }
 

@@ -23,6 +23,7 @@ struct HeadRows {
 enum { kInTurn = 0, kStretches = 1, kHeadsInTurn = 2 };  // which work a die takes (work_item)
 struct WindowArgs {
   HeadRows q, k, v, out, dout, dq, dk, dv;
+  void *rest;  // what rounding left of out, contiguous, or null
   float *lse, *delta, *largest, *part_q, *part_k, *part_v;
   const void *lengths;
   int length_type, at_end;  // at_end: the queries are the last of a sample's own tokens, not of all S

@@ -80,7 +80,7 @@ class WindowCall(ctypes.Structure):
     """gnnhwc_window_call of include/gnnhwc_tokens.h."""
 
     _fields_ = (
-        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "out_grad", "q_grad", "k_grad", "v_grad")]
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "out_rest", "out_grad", "q_grad", "k_grad", "v_grad")]
         + [(n + "_stride", ctypes.c_int64 * 3) for n in ("q", "k", "v", "out", "out_grad", "q_grad", "k_grad", "v_grad")]
         + [(n, ctypes.c_int64) for n in ("batch", "tokens", "keys", "heads", "kv_heads", "head_dim", "window", "sinks", "causal")]
         + [("lengths", ctypes.c_void_p), ("length_type", ctypes.c_int64), ("at_end", ctypes.c_int64), ("scale", ctypes.c_double),

@@ -77,14 +77,17 @@ def _call(q, k, v, lengths, window, sinks, causal, at_end, scale, keep):
 
 
 def _window_attention(q, k, v, lengths, window, sinks, causal, at_end, scale, want_lse):
-    """gnop::window_attention.  Returns (out, lse); lse has no elements unless it is wanted."""
+    """gnop::window_attention.  Returns (out, lse, rest): what the backward reads; the last two have no elements unless it is to run
+    (want_lse), rest, which is what rounding left of out, none in float32 either."""
     opname = "gnop::window_attention"
     _check_attention(q, k, v, lengths, window, sinks, at_end, opname)
     keep = []
     c = _call(q, k, v, lengths, window, sinks, causal, at_end, scale, keep)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]) if want_lse else (0,), dtype=torch.float32, device=q.device)
+    rest = torch.empty(_rest_shape(q, want_lse), dtype=q.dtype, device=q.device)
     c.out, c.out_stride, c.lse = out.data_ptr(), _strides3(out), lse.data_ptr() if want_lse else None
+    c.out_rest = rest.data_ptr() if rest.numel() else None
     lib = _cabi.lib
     with _on_device(q.device):
         nbytes = lib.gnnhwc_window_workspace_bytes(ctypes.byref(c))
@@ -93,10 +96,14 @@ def _window_attention(q, k, v, lengths, window, sinks, causal, at_end, scale, wa
         ws = _workspace(nbytes, q.device)
         rc = lib.gnnhwc_window(ctypes.byref(c), ws.data_ptr(), ws.numel(), _current_stream_ptr(q.device))
     _cabi.check(rc, opname)
-    return out, lse
+    return out, lse, rest
 
 
-def _window_attention_bwd(dout, q, k, v, out, lse, lengths, window, sinks, causal, scale):
+def _rest_shape(q, want_lse):
+    return q.shape if want_lse and q.dtype != torch.float32 else (0,)
+
+
+def _window_attention_bwd(dout, q, k, v, out, lse, rest, lengths, window, sinks, causal, scale):
     """gnop::window_attention_bwd.  Returns (dq, dk, dv)."""
     opname = "gnop::window_attention_bwd"
     _check_attention(q, k, v, lengths, window, sinks, False, opname)
@@ -104,9 +111,13 @@ def _window_attention_bwd(dout, q, k, v, out, lse, lengths, window, sinks, causa
         _check_device(t, name)
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
             raise RuntimeError("%s: %s must be like q" % (opname, name))
+    if rest.numel() and (rest.shape != q.shape or rest.dtype != q.dtype or rest.device != q.device):
+        raise RuntimeError("%s: rest must be like q, or empty" % opname)
     keep = []
     c = _call(q, k, v, lengths, window, sinks, causal, False, scale, keep)
     dout, out, lse = _aligned(dout), _aligned(out), lse.contiguous()
+    rest = _aligned(rest.contiguous())
+    c.out_rest = rest.data_ptr() if rest.numel() else None
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     c.out, c.out_stride, c.out_grad, c.out_grad_stride, c.lse = out.data_ptr(), _strides3(out), dout.data_ptr(), _strides3(dout), lse.data_ptr()
     c.q_grad, c.q_grad_stride, c.k_grad, c.k_grad_stride = dq.data_ptr(), _strides3(dq), dk.data_ptr(), _strides3(dk)
@@ -123,8 +134,8 @@ def _window_attention_bwd(dout, q, k, v, out, lse, lengths, window, sinks, causa
 
 
 _op_lib.define("window_attention(Tensor q, Tensor k, Tensor v, Tensor? lengths, int window, int sinks, bool causal, bool at_end, float scale, "
-               "bool want_lse) -> (Tensor, Tensor)")
-_op_lib.define("window_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor? lengths, int window, int sinks, "
+               "bool want_lse) -> (Tensor, Tensor, Tensor)")
+_op_lib.define("window_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor rest, Tensor? lengths, int window, int sinks, "
                "bool causal, float scale) -> (Tensor, Tensor, Tensor)")
 _op_lib.impl("window_attention", _window_attention, "CompositeExplicitAutograd")
 _op_lib.impl("window_attention_bwd", _window_attention_bwd, "CompositeExplicitAutograd")
@@ -132,10 +143,11 @@ _op_lib.impl("window_attention_bwd", _window_attention_bwd, "CompositeExplicitAu
 
 def _window_attention_meta(q, k, v, lengths, window, sinks, causal, at_end, scale, want_lse):
     return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-            torch.empty((q.shape[0], q.shape[2], q.shape[1]) if want_lse else (0,), dtype=torch.float32, device=q.device))
+            torch.empty((q.shape[0], q.shape[2], q.shape[1]) if want_lse else (0,), dtype=torch.float32, device=q.device),
+            torch.empty(_rest_shape(q, want_lse), dtype=q.dtype, device=q.device))
 
 
-def _window_attention_bwd_meta(dout, q, k, v, out, lse, lengths, window, sinks, causal, scale):
+def _window_attention_bwd_meta(dout, q, k, v, out, lse, rest, lengths, window, sinks, causal, scale):
     return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
 
 
@@ -145,18 +157,18 @@ _op_lib.impl("window_attention_bwd", _window_attention_bwd_meta, "Meta")
 
 def _setup_context(ctx, inputs, output):
     q, k, v, lengths, ctx.window, ctx.sinks, ctx.causal, ctx.at_end, ctx.scale, ctx.have_lse = inputs
-    ctx.save_for_backward(q, k, v, output[0], output[1], lengths)
-    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(q, k, v, *output, lengths)
+    ctx.mark_non_differentiable(output[1], output[2])
     ctx.set_materialize_grads(False)
 
 
-def _backward(ctx, dout, _dlse):
+def _backward(ctx, dout, _dlse, _drest):
     if ctx.at_end or not ctx.have_lse:
         raise RuntimeError("gnop::window_attention: attention against a cache, or without lse, has no derivative")
     if dout is None:
         return (None,) * 10
-    q, k, v, out, lse, lengths = ctx.saved_tensors
-    grads = torch.ops.gnop.window_attention_bwd(dout, q, k, v, out, lse, lengths, ctx.window, ctx.sinks, ctx.causal, ctx.scale)
+    q, k, v, out, lse, rest, lengths = ctx.saved_tensors
+    grads = torch.ops.gnop.window_attention_bwd(dout, q, k, v, out, lse, rest, lengths, ctx.window, ctx.sinks, ctx.causal, ctx.scale)
     return (*grads, None, None, None, None, None, None, None)
 
 

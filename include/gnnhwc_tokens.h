@@ -136,15 +136,19 @@ int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const
  * once, as operands of the second product.  dtype: F32, F16 or BF16.
  *   lse      : float (batch, heads, tokens): log2 of the softmax's sum, infinite for a query that sees nothing.  Written by the
  *              forward unless NULL, read by the backward.
+ *   out_rest : (batch, tokens, heads, head_dim) of dtype, no gaps, 16-byte aligned: what rounding left of out.  Written by the forward
+ *              and read by the backward unless NULL; F32 has none.  Without it gradients of queries that see a few tokens are less
+ *              exact (they are differences that the rounding of out is large against).
  *   strides  : of batch, token and head in elements, each a whole multiple of 16 bytes (but for dimensions of size 1), as are the
  *              addresses; a token's below 2^25 bytes.  Channels of a head are contiguous.
- * Backward (not with at_end): reads q, k, v, out, out_grad and lse, writes q_grad, k_grad and v_grad.
+ * Backward (not with at_end): reads q, k, v, out, out_grad, lse and out_rest, writes q_grad, k_grad and v_grad.
  * Outputs must not overlap inputs or each other.
  */
 typedef struct gnnhwc_window_call {
   const void *q, *k, *v;        /* (batch, tokens, heads, head_dim), (batch, keys, kv_heads, head_dim) twice */
   void *out;                    /* like q; read by the backward */
   float *lse;
+  void *out_rest;               /* or NULL */
   const void *out_grad;
   void *q_grad, *k_grad, *v_grad;
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];

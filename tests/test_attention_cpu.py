@@ -104,10 +104,10 @@ def test_host_tensors_and_bad_shapes_are_refused():
 
 def test_meta_kernels():
     q, k = torch.zeros((2, 3, 4, 64), device="meta", dtype=torch.bfloat16), torch.zeros((2, 5, 2, 64), device="meta", dtype=torch.bfloat16)
-    out, lse = torch.ops.gnop.window_attention(q, k, k, None, 4, 1, True, False, 0.125, True)
+    out, lse, rest = torch.ops.gnop.window_attention(q, k, k, None, 4, 1, True, False, 0.125, True)
     assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (2, 4, 3) and lse.dtype == torch.float32
     assert torch.ops.gnop.window_attention(q, k, k, None, 4, 1, True, True, 0.125, False)[1].numel() == 0
-    dq, dk, dv = torch.ops.gnop.window_attention_bwd(out, q, k, k, out, lse, None, 4, 1, True, 0.125)
+    dq, dk, dv = torch.ops.gnop.window_attention_bwd(out, q, k, k, out, lse, rest, None, 4, 1, True, 0.125)
     assert dq.shape == q.shape and dk.shape == dv.shape == k.shape
     assert torch.ops.gnop.dropout(q, None, 0.1, 1, None, 0).shape == q.shape
 

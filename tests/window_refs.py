@@ -8,8 +8,8 @@ more: U w, and in float16 at least half the spacing of subnormals, 2^-25 of the 
 2^8 and the sum of weights is 1 or more; in the backward as 2^12 w).
   out:  sum_j |v_j| (error of w_j)                                                  + U |out|
   dv:   sum_i |do_i| (error of w_ij)                                                + U |dv|
-  dS:   the error of w times |dP - delta|, w times those of dP (D + 4) u sum |do v| and of delta (U + (D + 4) u) sum |do o| (which
-        comes from the rounded out, off by another D u), and U dS for its own rounding; in float16 2^-25 of the unit: |dS| is held as 32 dS /
+  dS:   the error of w times |dP - delta|, w times those of dP (D + 4) u sum |do v| and of delta (U^2 + 3 (D + 4) u) sum |do o| (which
+        comes from the rounded out and from what rounding left of it, itself rounded: off by U^2, in float16 by half a subnormal or more), and U dS for its own rounding; in float16 2^-25 of the unit: |dS| is held as 32 dS /
         (largest |do|), within a factor of two
   dq:   scale sum_j |k_j| (error of dS_ij) + U |dq|,   dk: scale sum_i |q_i| (error of dS_ij) + U |dk|
 and the float32 sums of the second products add (n / 16 + 64) u of the magnitudes that they add up."""
@@ -84,7 +84,8 @@ def attention(q, k, v, seen, scale, dout=None):
     dp, delta = G @ V.transpose(-1, -2), (G * out).sum(-1, keepdim=True)
     ds = w * (dp - delta)
     unit = G.abs().amax()
-    d_off = off * (dp - delta).abs() + w * ((D + 4) * u * (G.abs() @ V.abs().transpose(-1, -2)) + (rounded + 3 * (D + 4) * u) * (G.abs() * out.abs()).sum(-1, keepdim=True))
+    d_off = off * (dp - delta).abs() + w * ((D + 4) * u * (G.abs() @ V.abs().transpose(-1, -2)) + (rounded ** 2 + 3 * (D + 4) * u) * (G.abs() * out.abs()).sum(-1, keepdim=True)
+                                              + least * G.abs().sum(-1, keepdim=True))
     # (out's own error, as far as delta is made of it)
     d_off = d_off + w * (G.abs() * ((w_off + summed * w) @ V.abs())).sum(-1, keepdim=True)
     d_off = (d_off + rounded * (ds.abs() + d_off) + least * unit / 16 * m) * m
