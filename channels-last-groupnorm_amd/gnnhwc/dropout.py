@@ -91,8 +91,8 @@ def dropout(x, p, seed, offset=0, residual=None, channel_dim=-1):
 class Dropout(nn.Dropout):
     """Module of `dropout`: forward(x) or forward(x, residual), which is residual + dropout(x).  While training, every call draws
     a seed from torch's CPU generator (torch.manual_seed makes it repeatable, and a recomputed forward whose generator state is
-    restored draws the same); otherwise x passes, plus the residual.  A captured graph keeps the seed it was captured with: use
-    `dropout` with a seed tensor there."""
+    restored draws the same); otherwise x passes, plus the residual.  Where a graph is captured or traced, the seed is a tensor that
+    torch's generator of the device fills, with another number at each replay."""
 
     def __init__(self, p=0.5, channel_dim=-1):
         super().__init__(p)
@@ -101,7 +101,10 @@ class Dropout(nn.Dropout):
     def forward(self, x, residual=None):
         if not self.training or self.p == 0.0:
             return x if residual is None else x + residual
-        seed = int(torch.empty((), dtype=torch.int64).random_())
+        if torch.compiler.is_compiling() or (x.is_cuda and torch.cuda.is_current_stream_capturing()):
+            seed = torch.randint(2 ** 63 - 1, (), dtype=torch.int64, device=x.device)
+        else:
+            seed = int(torch.empty((), dtype=torch.int64).random_())
         return dropout(x, float(self.p), seed, 0, residual, self.channel_dim)
 
     def extra_repr(self):
