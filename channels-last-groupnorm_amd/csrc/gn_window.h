@@ -900,20 +900,59 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   }
 }
 
-// Rows whose keys several workgroups shared: four channels of a row each thread.
+// ---- joining ----
+// Rows of results that several workgroups left parts of.  A thread has four channels of a row and about four of its parts (a few
+// reads on their way at once); where there are more threads than one for that, they add up in shared memory, in their order.  43
+// parts of the sinks' gradients, 3 samples of 2 heads of 40 channels in float32: 20 us by one thread, 7 by eleven.
+__host__ __device__ __forceinline__ int joiners_of(int D, int parts) {
+  const int wanted = (parts + 3) / 4, room = kBlock / (D / 4);
+  const int n = wanted < room ? wanted : room;
+  return n < 1 ? 1 : n > 16 ? 16 : n;
+}
+struct Joiner {
+  int joiners;             // threads that share the parts
+  int rows, row, part, d;  // rows of the workgroup, the thread's own, its first part and first channel
+  int quads;
+  __device__ __forceinline__ Joiner(const WindowArgs &a, int parts) {
+    joiners = joiners_of(a.D, parts);
+    quads = a.D / 4;
+    const int lanes = quads * joiners, left = threadIdx.x % lanes;
+    rows = kBlock / lanes;
+    row = threadIdx.x / lanes;
+    part = left / quads;
+    d = left % quads * 4;
+  }
+};
+template <typename V, typename F> __device__ __forceinline__ V joined(const Joiner &at, V v, V *place, F &&f) {
+  if (at.joiners == 1) return v;
+  __syncthreads();
+  place[threadIdx.x] = v;
+  __syncthreads();
+  const V *first = place + (threadIdx.x - at.part * at.quads);
+  v = first[0];
+  for (int n = 1; n < at.joiners; ++n) v = f(v, first[n * at.quads]);
+  return v;
+}
+
 template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kernel(const WindowArgs a) {
   __shared__ int bad[kBlock];
-  const int quads = a.D / 4, rows_here = kBlock / quads, r = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+  __shared__ f32x4 place[kBlock];
+  const Joiner at(a, a.splits);
+  const int r = at.row, d = at.d, rows_here = at.rows;
   const int64_t rows = (int64_t)a.B * a.H * a.L, id = (int64_t)blockIdx.x * rows_here + r;
+  const bool there = r < rows_here && id < rows;
   bad[threadIdx.x] = 0;
-  __syncthreads();
-  if (r < rows_here && id < rows) {
-    float most = -INFINITY, sum = 0.0f;
+  const auto add = [](auto x, auto y) { return x + y; };
+  float most = -INFINITY, sum = 0.0f;
+  f32x4 o = {};
+  if (there) {
 #pragma unroll 4
-    for (int n = 0; n < a.splits; ++n) most = fmaxf(most, load_global<float>(a.part_k + 2 * (id + n * rows)));
-    f32x4 o = {};
+    for (int n = at.part; n < a.splits; n += at.joiners) most = fmaxf(most, load_global<float>(a.part_k + 2 * (id + n * rows)));
+  }
+  most = joined(at, most, (float *)place, [](float x, float y) { return fmaxf(x, y); });
+  if (there) {
 #pragma unroll 4
-    for (int n = 0; n < a.splits; ++n) {
+    for (int n = at.part; n < a.splits; n += at.joiners) {
       const f32x2 part = load_global<f32x2>(a.part_k + 2 * (id + n * rows));
       const float w = part_weight(part.x, most);
       const f32x4 v = load_global<f32x4>(a.part_v + (id + n * rows) * a.D + d);
@@ -921,6 +960,10 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
     }
+  }
+  sum = joined(at, sum, (float *)place, add);
+  o = joined(at, o, place, add);
+  if (there && at.part == 0) {
     const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
     const float t[4] = {o[0] * factor, o[1] * factor, o[2] * factor, o[3] * factor};
     const int i = (int)(id % a.L), h = (int)(id / a.L % a.H), b = (int)(id / a.L / a.H);
@@ -1090,20 +1133,25 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
 }
 static_assert(kGradBits == 5.0f, "the factors of 1 / 32 undo it");
 
-// dq of rows whose keys several workgroups shared: four channels of a row each thread.
+// dq of rows whose keys several workgroups shared.
 template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_kernel(const WindowArgs a) {
   __shared__ int bad[kBlock];
-  const int quads = a.D / 4, rows_here = kBlock / quads, r = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+  __shared__ f32x4 place[kBlock];
+  const Joiner at(a, a.splits);
+  const int r = at.row, rows_here = at.rows;
   const int64_t rows = (int64_t)a.B * a.H * a.L, id = (int64_t)blockIdx.x * rows_here + r;
+  const bool there = r < rows_here && id < rows;
   bad[threadIdx.x] = 0;
-  __syncthreads();
-  if (r < rows_here && id < rows) {
-    f32x4 q = {};
+  f32x4 q = {};
+  if (there) {
 #pragma unroll 4
-    for (int n = 0; n < a.splits; ++n) q += load_global<f32x4>(a.part_q + (id + n * rows) * a.D + d);
+    for (int n = at.part; n < a.splits; n += at.joiners) q += load_global<f32x4>(a.part_q + (id + n * rows) * a.D + at.d);
+  }
+  q = joined(at, q, place, [](f32x4 x, f32x4 y) { return x + y; });
+  if (there && at.part == 0) {
     const float t[4] = {q[0], q[1], q[2], q[3]};
     using LV = LaneVec<T, 4>;
-    LV::store((T *)a.dq.row((int)(id / a.L / a.H), (int)(id % a.L), (int)(id / a.L % a.H)) + d, LV::pack(t));
+    LV::store((T *)a.dq.row((int)(id / a.L / a.H), (int)(id % a.L), (int)(id / a.L % a.H)) + at.d, LV::pack(t));
     if (!(q[0] * 0.0f + q[1] * 0.0f + q[2] * 0.0f + q[3] * 0.0f == 0.0f)) bad[r] = 1;
   }
   __syncthreads();
@@ -1483,26 +1531,34 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
   if constexpr (KS::kDv) add(key.dv, KS::v_factor(), z.part_v);
 }
 
-// Sums of the keys that several workgroups shared, all keys or the sinks: four channels of a row each thread.
+// Sums of the keys that several workgroups shared, all keys or the sinks.
 template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kernel(const WindowArgs a) {
   __shared__ int bad_k[kBlock], bad_v[kBlock];
-  const int quads = a.D / 4, rows_here = kBlock / quads, r = threadIdx.x / quads, d = threadIdx.x % quads * 4;
-  const int rows = a.shares > 1 ? a.S : a.sinks < a.S ? a.sinks : a.S;
+  __shared__ f32x4 place[kBlock];
+  // (the first workgroups have the sinks, the others, if there are any, the other keys)
+  const bool sink = (int)blockIdx.x < a.sink_blocks;
+  const Joiner with(a, sink ? a.sink_parts : a.shares);
+  const int r = with.row, d = with.d, rows_here = with.rows;
+  const int first = sink ? 0 : a.sinks, rows = sink ? a.sinks : a.S - a.sinks;
   bad_k[threadIdx.x] = bad_v[threadIdx.x] = 0;
-  __syncthreads();
-  const int64_t id = (int64_t)blockIdx.x * rows_here + r;
-  if (r < rows_here && id < (int64_t)a.B * a.K * rows) {
-    const int bk = (int)(id / rows), j = (int)(id % rows), b = bk / a.K, kh = bk % a.K;
-    const bool sink = j < a.sinks;
+  const int64_t block = (int)blockIdx.x - (sink ? 0 : a.sink_blocks), id = block * rows_here + r;
+  const bool there = r < rows_here && id < (int64_t)a.B * a.K * rows;
+  const int bk = (int)(id / rows), j = first + (int)(id % rows), b = bk / a.K, kh = bk % a.K;
+  f32x4 k = {}, v = {};
+  if (there) {
     const int64_t slot = sink ? sink_slot(a, bk, j / 32, 0) + j % 32 : tile_slot(a, bk, j / kQueries, 0) + j % kQueries;
     const int64_t at = slot * a.D + d, step = (int64_t)(sink ? 32 : kQueries) * a.D;
     const int parts = sink ? a.sink_parts : a.shares;
-    f32x4 k = {}, v = {};
 #pragma unroll 8
-    for (int n = 0; n < parts; ++n) {
+    for (int n = with.part; n < parts; n += with.joiners) {
       k += load_global<f32x4>(a.part_k + at + n * step);
       v += load_global<f32x4>(a.part_v + at + n * step);
     }
+  }
+  const auto add = [](f32x4 x, f32x4 y) { return x + y; };
+  k = joined(with, k, place, add);
+  v = joined(with, v, place, add);
+  if (there && with.part == 0) {
     const float tk[4] = {k[0], k[1], k[2], k[3]}, tv[4] = {v[0], v[1], v[2], v[3]};
     using LV = LaneVec<T, 4>;
     LV::store((T *)a.dk.row(b, j, kh) + d, LV::pack(tk));
@@ -1514,8 +1570,8 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kerne
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!(bad_k[n] | bad_v[n])) continue;
     const WindowArgs &z = arguments_again();
-    const int64_t row = (int64_t)blockIdx.x * rows_here + n;
-    const int bk = (int)(row / rows), key = (int)(row % rows), b = bk / z.K;
+    const int64_t row = block * rows_here + n;
+    const int bk = (int)(row / rows), key = first + (int)(row % rows), b = bk / z.K;
     const Sample s = sample_of(z, b);
     if (seen_of(z, s, key).count == 0) continue;
     if (bad_v[n]) dkv_again<T>(z, s, b, bk % z.K, key, false);

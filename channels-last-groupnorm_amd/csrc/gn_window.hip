@@ -37,12 +37,14 @@ template <typename F> void with_width(int D, F &&f) {
   }
 }
 dim3 grid_of(int items) { return dim3((unsigned)((items + 7) / 8 * 8)); }
-dim3 sum_grid(int64_t rows, int D) {
-  const int64_t here = kBlock / (D / 4);
-  return dim3((unsigned)((rows + here - 1) / here));
+int64_t join_blocks(int64_t rows, int D, int parts) {
+  const int64_t here = kBlock / (D / 4 * joiners_of(D, parts));
+  return (rows + here - 1) / here;
 }
 void join(const WindowArgs &a, hipStream_t stream) {
-  if (a.splits > 1) hipLaunchKernelGGL((window_join_kernel<elem_t>), sum_grid((int64_t)a.B * a.H * a.L, a.D), dim3(kBlock), 0, stream, a);
+  if (a.splits <= 1) return;
+  const int64_t rows = (int64_t)a.B * a.H * a.L;
+  hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)join_blocks(rows, a.D, a.splits)), dim3(kBlock), 0, stream, a);
 }
 
 }  // namespace
@@ -66,8 +68,10 @@ hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const
   with_width(a.D, [&](auto w) {
     constexpr int DP = decltype(w)::value;
     if (a.items) hipLaunchKernelGGL((window_dq_kernel<elem_t, DP>), grid_of(a.items), dim3(kBlock), 0, stream, a);
-    if (a.items && a.splits > 1)
-      hipLaunchKernelGGL((window_dq_sum_kernel<elem_t>), sum_grid((int64_t)a.B * a.H * a.L, a.D), dim3(kBlock), 0, stream, a);
+    if (a.items && a.splits > 1) {
+      const int64_t rows = (int64_t)a.B * a.H * a.L;
+      hipLaunchKernelGGL((window_dq_sum_kernel<elem_t>), dim3((unsigned)join_blocks(rows, a.D, a.splits)), dim3(kBlock), 0, stream, a);
+    }
     auto keys = [&](auto parts) {
       constexpr int P = decltype(parts)::value;
       hipLaunchKernelGGL((window_dkv_kernel<elem_t, DP, P>), grid_of(kv.items), dim3(kBlock), 0, stream, kv);
@@ -81,8 +85,11 @@ hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const
     }
   });
   if (kv.shares > 1 || kv.sinks > 0) {
-    const int64_t rows = (int64_t)kv.B * kv.K * (kv.shares > 1 ? kv.S : kv.sinks < kv.S ? kv.sinks : kv.S);
-    hipLaunchKernelGGL((window_sum_kernel<elem_t>), sum_grid(rows, kv.D), dim3(kBlock), 0, stream, kv);
+    WindowArgs sum = kv;
+    const int64_t heads = (int64_t)kv.B * kv.K;
+    sum.sink_blocks = kv.sinks > 0 ? (int)join_blocks(heads * kv.sinks, kv.D, kv.sink_parts) : 0;
+    const int64_t others = kv.shares > 1 ? join_blocks(heads * (kv.S - kv.sinks), kv.D, kv.shares) : 0;
+    hipLaunchKernelGGL((window_sum_kernel<elem_t>), dim3((unsigned)(sum.sink_blocks + others)), dim3(kBlock), 0, stream, sum);
   }
   return hipGetLastError();
 }

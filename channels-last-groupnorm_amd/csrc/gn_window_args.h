@@ -35,6 +35,7 @@ struct WindowArgs {
   int shares;                 // dk, dv: workgroups that share a tile's queries
   int sink_sets, sink_parts;  // dk, dv of the sinks: 32 keys each; workgroups that share the queries
   float scale, scale_log2;
+  int sink_blocks;            // window_sum_kernel: workgroups that add up the sinks' parts
 };
 
 // Wavefronts of a workgroup whose wavefronts have two pairs of tiles of 32 rows each, for a head padded to `width` channels.
