@@ -42,11 +42,21 @@ int put_rows(HeadRows &r, const void *base, const int64_t (&stride)[3], int64_t 
   return GNNHWC_OK;
 }
 
-// The order in which the workgroups' work goes to the dies.
+// The order in which the workgroups' work goes to the dies, and what they divide by to find theirs: once all else of a is set.
 void put_order(WindowArgs &a) {
   const int heads = a.B * a.K;
   a.per_head = heads ? a.items / heads : 0;
   a.order = heads % 8 == 0 ? kHeadsInTurn : a.lengths ? kInTurn : kStretches;
+  a.by_group = make_divisor(std::max(1, a.group), 0);
+  a.by_splits = make_divisor(std::max(1, a.splits), 0);
+  a.by_tiles = make_divisor(std::max(1, a.tiles), 0);
+  a.by_K = make_divisor(std::max(1, a.K), 0);
+  a.by_shares = make_divisor(std::max(1, a.shares), 0);
+  a.by_sink_parts = make_divisor(std::max(1, a.sink_parts), 0);
+  a.by_sink_sets = make_divisor(std::max(1, a.sink_sets), 0);
+  a.by_per_head = make_divisor(std::max(1, a.per_head), 0);
+  a.by_L = make_divisor(std::max(1, a.L), 0);
+  a.by_H = make_divisor(std::max(1, a.H), 0);
 }
 
 struct WindowPlan {
@@ -169,7 +179,6 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   w.shares = (int)shares_of(tiles, queries, es == 4 ? 1 : width <= 64 ? 2 : 1, 32);
   if (tiles * w.shares > kMostItems) return invalid("too many tokens and heads for one call");
   w.items = (int)(tiles * w.shares);
-  put_order(w);
   k.items = w.sink_sets = w.sink_parts = 0;
   if (w.sinks > 0 && w.items > 0) {
     const int waves = few_waves((int)width, (int)es);
@@ -183,6 +192,7 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     k.items = (int)(sets * sink_shares);
     put_order(k);
   }
+  put_order(w);
   const size_t floats = round_up((size_t)lse * sizeof(float));
   const size_t part = round_up(((size_t)heads * w.sink_sets * w.sink_parts * 32 + (w.shares > 1 ? (size_t)tiles * w.shares * kQueries : 0)) * a.D * sizeof(float));
   p.delta = 0;

@@ -331,13 +331,15 @@ __device__ __forceinline__ Walk walk_of(const WindowArgs &a, const Sample &s, in
   return w;
 }
 
+__device__ __forceinline__ int rest_by(int n, const Divisor &v) { return n - div_by(n, v) * v.d; }
+
 // The work of this workgroup, of a.items ordered by key head; a.items and beyond: none.  Workgroups are dealt to the eight dies in
 // turn, each with a cache of its own that a head's keys and values are to be in once: heads are dealt to the dies in turn, or, where
 // they do not come out even, each die has a stretch of the work, or, where samples have lengths that would make those uneven, all
 // is dealt in turn.  (padded float32 (3, 1961, 6 heads over 2, 40): forward 112 us with stretches)
 __device__ __forceinline__ int work_item(const WindowArgs &a) {
   const int id = blockIdx.x, die = id & 7, n = id >> 3;
-  if (a.order == kHeadsInTurn) return (n / a.per_head * 8 + die) * a.per_head + n % a.per_head;
+  if (a.order == kHeadsInTurn) return (div_by(n, a.by_per_head) * 8 + die) * a.per_head + rest_by(n, a.by_per_head);
   return a.order == kStretches ? die * ((a.items + 7) >> 3) + n : id;
 }
 
@@ -409,7 +411,7 @@ template <typename T, int N> __device__ __forceinline__ void store_out(const Win
   }
 }
 template <typename T> __device__ void row_again(const WindowArgs &a, const Sample &s, int b, int h, int i) {
-  const int lane = threadIdx.x & 63, kh = h / a.group;
+  const int lane = threadIdx.x & 63, kh = div_by(h, a.by_group);
   const Sight g = sight_of(a, s, i);
   const T *q = (const T *)a.q.row(b, i, h);
   if (holds_nan(q, a.D, true)) {
@@ -455,7 +457,7 @@ template <typename T> __device__ void row_again(const WindowArgs &a, const Sampl
 }
 // dq of one row.
 template <typename T> __device__ void dq_again(const WindowArgs &a, const Sample &s, int b, int h, int i, float lse, float delta) {
-  const int lane = threadIdx.x & 63, kh = h / a.group;
+  const int lane = threadIdx.x & 63, kh = div_by(h, a.by_group);
   const T *q = (const T *)a.q.row(b, i, h), *g = (const T *)a.dout.row(b, i, h);
   if (lse != lse || delta != delta) return fill_nan((T *)a.dq.row(b, i, h), a.D);
   float acc[4] = {};
@@ -659,9 +661,14 @@ struct Stretch {
   // Whether step u + by does not come `by` tiles behind step u.
   __device__ __forceinline__ bool jumps(int u, int by) const { return u < w.sinks && u + by >= w.sinks && w.first != w.sinks; }
 };
-__device__ __forceinline__ Stretch stretch_of(const Walk &w, int split, int splits) {
+// Of `steps` steps the n-th share begins at this one (the first ones are longer by one where they do not come out even).
+__device__ __forceinline__ int share_begin(const Divisor &shares, int steps, int n) {
+  const int each = div_by(steps, shares), more = steps - each * shares.d;
+  return each * n + (n < more ? n : more);
+}
+__device__ __forceinline__ Stretch stretch_of(const Walk &w, int split, const Divisor &splits) {
   const int steps = w.sinks + (w.last >= w.first ? w.last - w.first + 1 : 0);
-  return {w, (int)((int64_t)steps * split / splits), (int)((int64_t)steps * (split + 1) / splits)};
+  return {w, share_begin(splits, steps, split), share_begin(splits, steps, split + 1)};
 }
 // Rows of the results of workgroups that share a row's keys: a split's rows behind each other, then the next split's.
 __device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int b, int h, int i) {
@@ -675,9 +682,9 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, sizeof(T) == 
   const int item = work_item(a);
   if (item >= a.items) return;
   // (the heads of a group are neighbours, then the tiles of queries, the last ones, which see most, first)
-  const int g = item % a.group, split = item / a.group % a.splits, rest = item / a.group / a.splits;
-  const int tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
-  const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
+  const int of_group = div_by(item, a.by_group), rest = div_by(of_group, a.by_splits), g = item - of_group * a.group, split = of_group - rest * a.splits;
+  const int bk = div_by(rest, a.by_tiles), tile = a.tiles - 1 - (rest - bk * a.tiles);
+  const int b = div_by(bk, a.by_K), kh = bk - b * a.K, h = kh * a.group + g;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = tile * kQueries + wave * 32 + (lane & 31);
   ForwardState<T, DP> st;
@@ -691,7 +698,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, sizeof(T) == 
   if (from < to) {
     const int ic = i < from ? from : i < to ? i : to - 1;
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
-    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.splits);
+    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.by_splits);
     TilePair<T, DP, G::kRows, kBlock> copy;
     copy.init(a.D, a.k.token_bytes, a.v.token_bytes, s.n - 1);
     LaneOffsets<T, DP> at;
@@ -793,11 +800,11 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   __shared__ int bad[32];
   const int item = work_item(a);
   if (item >= a.items) return;
-  const int split = item % a.splits, rest = item / a.splits, block = rest % a.tiles, bk = rest / a.tiles;
-  const int b = bk / a.K, kh = bk % a.K;
+  const int rest = div_by(item, a.by_splits), split = item - rest * a.splits, bk = div_by(rest, a.by_tiles), block = rest - bk * a.tiles;
+  const int b = div_by(bk, a.by_K), kh = bk - b * a.K;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int rows = a.L * a.group, row = block * 32 + (lane & 31), i = row < rows ? row / a.group : a.L, h = kh * a.group + row % a.group;
+  const int rows = a.L * a.group, row = block * 32 + (lane & 31), i = row < rows ? div_by(row, a.by_group) : a.L, h = kh * a.group + rest_by(row, a.by_group);
   ForwardState<T, DP> st;
   st.sight = sight_of(a, s, i);
   st.reference = -INFINITY;
@@ -805,13 +812,13 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
   st.sum = 0.0f;
 #pragma unroll
   for (int x = 0; x < DP / 32; ++x) st.o[x] = zeros16();
-  int from = block * 32 / a.group, to = (block * 32 + 31) / a.group + 1;
+  int from = div_by(block * 32, a.by_group), to = div_by(block * 32 + 31, a.by_group) + 1;
   from = from > s.first ? from : s.first;
   to = to < s.last ? to : s.last;
   if (from < to) {
     const int ic = i < from ? from : i < to ? i : to - 1;
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, st.q);
-    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, 32), split, a.splits);
+    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, 32), split, a.by_splits);
     const char *kb = (const char *)a.k.row(b, 0, kh), *vb = (const char *)a.v.row(b, 0, kh);
     TilePair<T, DP, 32, 64> copy;
     copy.init(a.D, a.k.token_bytes, a.v.token_bytes, s.n - 1);
@@ -871,32 +878,32 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
 #pragma unroll
     for (int n = 1; n < kWaves; ++n) v += *(const f32x4 *)((const float *)(tiles + n * 2 * W::kStage) + r * W::kPitch + d);
     if (z.splits > 1) {
-      store_global<f32x4>(z.part_v + part_row(z, split, b, kh * z.group + rr % z.group, rr / z.group) * z.D + d, v);
+      store_global<f32x4>(z.part_v + part_row(z, split, b, kh * z.group + rest_by(rr, z.by_group), div_by(rr, z.by_group)) * z.D + d, v);
       continue;
     }
     const float total = sums[0][r], factor = total > 0.0f ? 1.0f / total : 0.0f;
     const float t[4] = {v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor};
     if (!(v[0] * 0.0f + v[1] * 0.0f + v[2] * 0.0f + v[3] * 0.0f + factor * 0.0f == 0.0f) || !(total > 0.0f)) bad[r] = 1;
-    store_out<T, 4>(z, b, kh * z.group + rr % z.group, rr / z.group, d, t);
+    store_out<T, 4>(z, b, kh * z.group + rest_by(rr, z.by_group), div_by(rr, z.by_group), d, t);
   }
   if (z.splits > 1) {
     const int rr = block * 32 + (int)threadIdx.x;
     if (threadIdx.x < 32 && rr < rows) {
-      float *p = z.part_k + 2 * part_row(z, split, b, kh * z.group + rr % z.group, rr / z.group);
+      float *p = z.part_k + 2 * part_row(z, split, b, kh * z.group + rest_by(rr, z.by_group), div_by(rr, z.by_group));
       store_global<float>(p, references[0][threadIdx.x]);
       store_global<float>(p + 1, sums[0][threadIdx.x]);
     }
     return;
   }
   __syncthreads();
-  for (int r = wave; r < 32; r += kWaves) {
-    const int rr = block * 32 + r;
-    if (rr >= rows) break;
-    const int ir = rr / z.group, hr = kh * z.group + rr % z.group;
-    const Sight g = sight_of(z, s, ir);
-    if (z.lse && lane == 0)
-      store_global<float>(z.lse + ((int64_t)b * z.H + hr) * z.L + ir, sums[0][r] > 0.0f ? references[0][r] + __builtin_amdgcn_logf(sums[0][r]) : INFINITY);
-    if (bad[r] && (g.count > 0 || g.sinks > 0)) row_again<T>(z, s, b, hr, ir);
+  const bool ours = lane < 32 && row < rows;
+  if (z.lse && wave == 0 && ours)
+    store_global<float>(z.lse + ((int64_t)b * z.H + h) * z.L + i, sums[0][lane] > 0.0f ? references[0][lane] + __builtin_amdgcn_logf(sums[0][lane]) : INFINITY);
+  uint64_t again = __ballot(ours && bad[lane & 31] && (st.sight.count > 0 || st.sight.sinks > 0));
+  while (again) {
+    const int r = __builtin_ctzll(again);
+    again &= again - 1;
+    if (r % kWaves == wave) row_again<T>(z, s, b, __builtin_amdgcn_readlane(h, r), __builtin_amdgcn_readlane(i, r));
   }
 }
 
@@ -904,23 +911,27 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
 // Rows of results that several workgroups left parts of.  A thread has four channels of a row and about four of its parts (a few
 // reads on their way at once); where there are more threads than one for that, they add up in shared memory, in their order.  43
 // parts of the sinks' gradients, 3 samples of 2 heads of 40 channels in float32: 20 us by one thread, 7 by eleven.
-__host__ __device__ __forceinline__ int joiners_of(int D, int parts) {
-  const int wanted = (parts + 3) / 4, room = kBlock / (D / 4);
-  const int n = wanted < room ? wanted : room;
-  return n < 1 ? 1 : n > 16 ? 16 : n;
-}
+struct Joining {
+  int joiners, rows_here;  // threads that share the parts; rows of a workgroup
+  Divisor lanes, quads;    // threads of a row, of a part of it
+  Joining(int D, int parts) {
+    const int room = kBlock / (D / 4), wanted = (parts + 3) / 4, n = wanted < room ? wanted : room;
+    joiners = n < 1 ? 1 : n > 16 ? 16 : n;
+    quads = make_divisor(D / 4, 0);
+    lanes = make_divisor(quads.d * joiners, 0);
+    rows_here = kBlock / lanes.d;
+  }
+  int64_t blocks(int64_t rows) const { return (rows + rows_here - 1) / rows_here; }
+};
 struct Joiner {
-  int joiners;             // threads that share the parts
-  int rows, row, part, d;  // rows of the workgroup, the thread's own, its first part and first channel
-  int quads;
-  __device__ __forceinline__ Joiner(const WindowArgs &a, int parts) {
-    joiners = joiners_of(a.D, parts);
-    quads = a.D / 4;
-    const int lanes = quads * joiners, left = threadIdx.x % lanes;
-    rows = kBlock / lanes;
-    row = threadIdx.x / lanes;
-    part = left / quads;
-    d = left % quads * 4;
+  int joiners, row, part, d, quads;  // the thread's row of the workgroup's, its first part and first channel
+  __device__ __forceinline__ explicit Joiner(const Joining &j) {
+    joiners = j.joiners;
+    quads = j.quads.d;
+    row = div_by(threadIdx.x, j.lanes);
+    const int left = threadIdx.x - row * j.lanes.d;
+    part = div_by(left, j.quads);
+    d = (left - part * quads) * 4;
   }
 };
 template <typename V, typename F> __device__ __forceinline__ V joined(const Joiner &at, V v, V *place, F &&f) {
@@ -934,14 +945,16 @@ template <typename V, typename F> __device__ __forceinline__ V joined(const Join
   return v;
 }
 
-template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kernel(const WindowArgs a) {
-  __shared__ int bad[kBlock];
+template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kernel(const WindowArgs a, const Joining joining) {
+  __shared__ int bad[kBlock], any_bad;
   __shared__ f32x4 place[kBlock];
-  const Joiner at(a, a.splits);
-  const int r = at.row, d = at.d, rows_here = at.rows;
-  const int64_t rows = (int64_t)a.B * a.H * a.L, id = (int64_t)blockIdx.x * rows_here + r;
+  const Joiner at(joining);
+  const int r = at.row, d = at.d, rows_here = joining.rows_here;
+  const int64_t rows = (int64_t)a.B * a.H * a.L;
+  const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^24 workgroups)
   const bool there = r < rows_here && id < rows;
   bad[threadIdx.x] = 0;
+  if (threadIdx.x == 0) any_bad = 0;
   const auto add = [](auto x, auto y) { return x + y; };
   float most = -INFINITY, sum = 0.0f;
   f32x4 o = {};
@@ -963,20 +976,22 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
   }
   sum = joined(at, sum, (float *)place, add);
   o = joined(at, o, place, add);
+  if (at.joiners == 1) __syncthreads();  // (bad is cleared)
   if (there && at.part == 0) {
     const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
     const float t[4] = {o[0] * factor, o[1] * factor, o[2] * factor, o[3] * factor};
-    const int i = (int)(id % a.L), h = (int)(id / a.L % a.H), b = (int)(id / a.L / a.H);
+    const int bh = div_by(id, a.by_L), i = id - bh * a.L, b = div_by(bh, a.by_H), h = bh - b * a.H;
     store_out<T, 4>(a, b, h, i, d, t);
     if (a.lse && d == 0) store_global<float>(a.lse + id, sum > 0.0f ? most + __builtin_amdgcn_logf(sum) : INFINITY);
-    if (!(t[0] * 0.0f + t[1] * 0.0f + t[2] * 0.0f + t[3] * 0.0f == 0.0f) || !(sum > 0.0f)) bad[r] = 1;
+    if (!(t[0] * 0.0f + t[1] * 0.0f + t[2] * 0.0f + t[3] * 0.0f == 0.0f) || !(sum > 0.0f)) bad[r] = any_bad = 1;
   }
   __syncthreads();
+  if (!any_bad) return;
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!bad[n]) continue;
     const WindowArgs &z = arguments_again();
-    const int64_t row = (int64_t)blockIdx.x * rows_here + n;
-    const int i = (int)(row % z.L), h = (int)(row / z.L % z.H), b = (int)(row / z.L / z.H);
+    const int row = (int)blockIdx.x * rows_here + n;
+    const int bh = div_by(row, z.by_L), i = row - bh * z.L, b = div_by(bh, z.by_H), h = bh - b * z.H;
     const Sample s = sample_of(z, b);
     const Sight g = sight_of(z, s, i);
     if (g.count > 0 || g.sinks > 0) row_again<T>(z, s, b, h, i);
@@ -998,9 +1013,9 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a);
   if (item >= a.items) return;
-  const int g = item % a.group, split = item / a.group % a.splits, rest = item / a.group / a.splits;
-  const int tile = a.tiles - 1 - rest % a.tiles, bk = rest / a.tiles;
-  const int b = bk / a.K, kh = bk % a.K, h = kh * a.group + g;
+  const int of_group = div_by(item, a.by_group), rest = div_by(of_group, a.by_splits), g = item - of_group * a.group, split = of_group - rest * a.splits;
+  const int bk = div_by(rest, a.by_tiles), tile = a.tiles - 1 - (rest - bk * a.tiles);
+  const int b = div_by(bk, a.by_K), kh = bk - b * a.K, h = kh * a.group + g;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, i = tile * kQueries + wave * 32 + (lane & 31);
   const Sight sight = sight_of(a, s, i);
@@ -1043,7 +1058,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
     }
     load_token<T, DP>((const T *)a.q.row(b, ic, h), a.D, q);
     if (i >= from && i < to) lse = load_global<float>(a.lse + row);
-    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.splits);
+    const Stretch w = stretch_of(walk_of(a, s, from + s.off, to - 1 + s.off, G::kRows), split, a.by_splits);
     TilePair<T, DP, G::kRows, kBlock> copy;
     copy.init(a.D, a.k.token_bytes, a.v.token_bytes, s.n - 1);
     LaneOffsets<T, DP> at;
@@ -1134,32 +1149,37 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && 
 static_assert(kGradBits == 5.0f, "the factors of 1 / 32 undo it");
 
 // dq of rows whose keys several workgroups shared.
-template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_kernel(const WindowArgs a) {
-  __shared__ int bad[kBlock];
+template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_kernel(const WindowArgs a, const Joining joining) {
+  __shared__ int bad[kBlock], any_bad;
   __shared__ f32x4 place[kBlock];
-  const Joiner at(a, a.splits);
-  const int r = at.row, rows_here = at.rows;
-  const int64_t rows = (int64_t)a.B * a.H * a.L, id = (int64_t)blockIdx.x * rows_here + r;
+  const Joiner at(joining);
+  const int r = at.row, rows_here = joining.rows_here;
+  const int64_t rows = (int64_t)a.B * a.H * a.L;
+  const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^24 workgroups)
   const bool there = r < rows_here && id < rows;
   bad[threadIdx.x] = 0;
+  if (threadIdx.x == 0) any_bad = 0;
   f32x4 q = {};
   if (there) {
 #pragma unroll 4
     for (int n = at.part; n < a.splits; n += at.joiners) q += load_global<f32x4>(a.part_q + (id + n * rows) * a.D + at.d);
   }
   q = joined(at, q, place, [](f32x4 x, f32x4 y) { return x + y; });
+  if (at.joiners == 1) __syncthreads();  // (bad is cleared)
   if (there && at.part == 0) {
     const float t[4] = {q[0], q[1], q[2], q[3]};
     using LV = LaneVec<T, 4>;
-    LV::store((T *)a.dq.row((int)(id / a.L / a.H), (int)(id % a.L), (int)(id / a.L % a.H)) + at.d, LV::pack(t));
-    if (!(q[0] * 0.0f + q[1] * 0.0f + q[2] * 0.0f + q[3] * 0.0f == 0.0f)) bad[r] = 1;
+    const int bh = div_by(id, a.by_L), i = id - bh * a.L, b = div_by(bh, a.by_H), h = bh - b * a.H;
+    LV::store((T *)a.dq.row(b, i, h) + at.d, LV::pack(t));
+    if (!(q[0] * 0.0f + q[1] * 0.0f + q[2] * 0.0f + q[3] * 0.0f == 0.0f)) bad[r] = any_bad = 1;
   }
   __syncthreads();
+  if (!any_bad) return;
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!bad[n]) continue;
     const WindowArgs &z = arguments_again();
-    const int64_t row = (int64_t)blockIdx.x * rows_here + n;
-    const int i = (int)(row % z.L), h = (int)(row / z.L % z.H), b = (int)(row / z.L / z.H);
+    const int row = (int)blockIdx.x * rows_here + n;
+    const int bh = div_by(row, z.by_L), i = row - bh * z.L, b = div_by(bh, z.by_H), h = bh - b * z.H;
     const Sample s = sample_of(z, b);
     const Sight g = sight_of(z, s, i);
     if (g.count > 0 || g.sinks > 0) dq_again<T>(z, s, b, h, i, load_global<float>(z.lse + row), -load_global<float>(z.delta + row));
@@ -1342,7 +1362,8 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
   __shared__ float reduce[4];
   const int item = work_item(a);
   if (item >= a.items) return;
-  const int share = item % a.shares, tile = item / a.shares % a.tiles, bk = item / a.shares / a.tiles, b = bk / a.K, kh = bk % a.K;
+  const int rest = div_by(item, a.by_shares), share = item - rest * a.shares, bk = div_by(rest, a.by_tiles), tile = rest - bk * a.tiles;
+  const int b = div_by(bk, a.by_K), kh = bk - b * a.K;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), j = tile * kQueries + wave * 32 + (lane & 31);
   const bool ours = j >= a.sinks && j < a.S;
@@ -1355,7 +1376,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
   const Queries range = queries_of(a, s, j0, top, false);
   if (range.from <= range.to) {
     const int first = range.from / G::kRows, tiles_of = range.to / G::kRows - first + 1, steps = tiles_of * a.group, to = range.to;
-    const int begin = (int)((int64_t)steps * share / a.shares), end = (int)((int64_t)steps * (share + 1) / a.shares);
+    const int begin = share_begin(a.by_shares, steps, share), end = share_begin(a.by_shares, steps, share + 1);
     if constexpr (__is_same(T, f16_t)) {
       float most = 0.0f;
       for (int st = begin + wave; st < end; st += 4) {
@@ -1451,7 +1472,8 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
   __shared__ __attribute__((aligned(16))) float lses[kWaves * 2 * 64], deltas[kWaves * 2 * 64];
   const int item = work_item(a);
   if (item >= a.items) return;
-  const int shares = a.sink_parts, share = item % shares, set = item / shares % a.sink_sets, bk = item / shares / a.sink_sets, b = bk / a.K, kh = bk % a.K;
+  const int rest = div_by(item, a.by_sink_parts), share = item - rest * a.sink_parts, bk = div_by(rest, a.by_sink_sets), set = rest - bk * a.sink_sets;
+  const int b = div_by(bk, a.by_K), kh = bk - b * a.K;
   const Sample s = sample_of(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), j = set * 32 + (lane & 31);
   KS key;
@@ -1464,7 +1486,7 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
   const Queries range = queries_of(a, s, set * 32, top, true);
   if (range.from <= range.to) {
     const int first = range.from / 32, tiles_of = range.to / 32 - first + 1, steps = tiles_of * a.group, to = range.to;
-    const int begin = (int)((int64_t)steps * share / shares) + wave, end = (int)((int64_t)steps * (share + 1) / shares);
+    const int begin = share_begin(a.by_sink_parts, steps, share) + wave, end = share_begin(a.by_sink_parts, steps, share + 1);
     if constexpr (__is_same(T, f16_t)) {
       float most = 0.0f;
       for (int st = begin; st < end; st += kWaves) {
@@ -1532,18 +1554,19 @@ template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<
 }
 
 // Sums of the keys that several workgroups shared, all keys or the sinks.
-template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kernel(const WindowArgs a) {
-  __shared__ int bad_k[kBlock], bad_v[kBlock];
+template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kernel(const WindowArgs a, const Joining of_sinks, const Joining of_others) {
+  __shared__ int bad_k[kBlock], bad_v[kBlock], any_bad;
   __shared__ f32x4 place[kBlock];
   // (the first workgroups have the sinks, the others, if there are any, the other keys)
   const bool sink = (int)blockIdx.x < a.sink_blocks;
-  const Joiner with(a, sink ? a.sink_parts : a.shares);
-  const int r = with.row, d = with.d, rows_here = with.rows;
+  const Joiner with(sink ? of_sinks : of_others);
+  const int r = with.row, d = with.d, rows_here = (sink ? of_sinks : of_others).rows_here;
   const int first = sink ? 0 : a.sinks, rows = sink ? a.sinks : a.S - a.sinks;
   bad_k[threadIdx.x] = bad_v[threadIdx.x] = 0;
-  const int64_t block = (int)blockIdx.x - (sink ? 0 : a.sink_blocks), id = block * rows_here + r;
+  if (threadIdx.x == 0) any_bad = 0;
+  const int block = (int)blockIdx.x - (sink ? 0 : a.sink_blocks), id = block * rows_here + r;
   const bool there = r < rows_here && id < (int64_t)a.B * a.K * rows;
-  const int bk = (int)(id / rows), j = first + (int)(id % rows), b = bk / a.K, kh = bk % a.K;
+  const int bk = (unsigned)id / (unsigned)rows, j = first + (id - bk * rows), b = div_by(bk, a.by_K), kh = bk - b * a.K;
   f32x4 k = {}, v = {};
   if (there) {
     const int64_t slot = sink ? sink_slot(a, bk, j / 32, 0) + j % 32 : tile_slot(a, bk, j / kQueries, 0) + j % kQueries;
@@ -1558,24 +1581,26 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kerne
   const auto add = [](f32x4 x, f32x4 y) { return x + y; };
   k = joined(with, k, place, add);
   v = joined(with, v, place, add);
+  if (with.joiners == 1) __syncthreads();  // (bad is cleared)
   if (there && with.part == 0) {
     const float tk[4] = {k[0], k[1], k[2], k[3]}, tv[4] = {v[0], v[1], v[2], v[3]};
     using LV = LaneVec<T, 4>;
     LV::store((T *)a.dk.row(b, j, kh) + d, LV::pack(tk));
     LV::store((T *)a.dv.row(b, j, kh) + d, LV::pack(tv));
-    if (!(k[0] * 0.0f + k[1] * 0.0f + k[2] * 0.0f + k[3] * 0.0f == 0.0f)) bad_k[r] = 1;
-    if (!(v[0] * 0.0f + v[1] * 0.0f + v[2] * 0.0f + v[3] * 0.0f == 0.0f)) bad_v[r] = 1;
+    if (!(k[0] * 0.0f + k[1] * 0.0f + k[2] * 0.0f + k[3] * 0.0f == 0.0f)) bad_k[r] = any_bad = 1;
+    if (!(v[0] * 0.0f + v[1] * 0.0f + v[2] * 0.0f + v[3] * 0.0f == 0.0f)) bad_v[r] = any_bad = 1;
   }
   __syncthreads();
+  if (!any_bad) return;
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!(bad_k[n] | bad_v[n])) continue;
     const WindowArgs &z = arguments_again();
-    const int64_t row = block * rows_here + n;
-    const int bk = (int)(row / rows), key = first + (int)(row % rows), b = bk / z.K;
+    const int row = block * rows_here + n;
+    const int bk = (unsigned)row / (unsigned)rows, key = first + (row - bk * rows), b = div_by(bk, z.by_K), kh = bk - b * z.K;
     const Sample s = sample_of(z, b);
     if (seen_of(z, s, key).count == 0) continue;
-    if (bad_v[n]) dkv_again<T>(z, s, b, bk % z.K, key, false);
-    if (bad_k[n]) dkv_again<T>(z, s, b, bk % z.K, key, true);
+    if (bad_v[n]) dkv_again<T>(z, s, b, kh, key, false);
+    if (bad_k[n]) dkv_again<T>(z, s, b, kh, key, true);
   }
 }
 

@@ -37,14 +37,11 @@ template <typename F> void with_width(int D, F &&f) {
   }
 }
 dim3 grid_of(int items) { return dim3((unsigned)((items + 7) / 8 * 8)); }
-int64_t join_blocks(int64_t rows, int D, int parts) {
-  const int64_t here = kBlock / (D / 4 * joiners_of(D, parts));
-  return (rows + here - 1) / here;
-}
 void join(const WindowArgs &a, hipStream_t stream) {
   if (a.splits <= 1) return;
   const int64_t rows = (int64_t)a.B * a.H * a.L;
-  hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)join_blocks(rows, a.D, a.splits)), dim3(kBlock), 0, stream, a);
+  const Joining joining(a.D, a.splits);
+  hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)joining.blocks(rows)), dim3(kBlock), 0, stream, a, joining);
 }
 
 }  // namespace
@@ -70,7 +67,8 @@ hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const
     if (a.items) hipLaunchKernelGGL((window_dq_kernel<elem_t, DP>), grid_of(a.items), dim3(kBlock), 0, stream, a);
     if (a.items && a.splits > 1) {
       const int64_t rows = (int64_t)a.B * a.H * a.L;
-      hipLaunchKernelGGL((window_dq_sum_kernel<elem_t>), dim3((unsigned)join_blocks(rows, a.D, a.splits)), dim3(kBlock), 0, stream, a);
+      const Joining joining(a.D, a.splits);
+      hipLaunchKernelGGL((window_dq_sum_kernel<elem_t>), dim3((unsigned)joining.blocks(rows)), dim3(kBlock), 0, stream, a, joining);
     }
     auto keys = [&](auto parts) {
       constexpr int P = decltype(parts)::value;
@@ -87,9 +85,10 @@ hipError_t GN_CAT(launch_window_backward_, GN_SUFFIX)(const WindowArgs &a, const
   if (kv.shares > 1 || kv.sinks > 0) {
     WindowArgs sum = kv;
     const int64_t heads = (int64_t)kv.B * kv.K;
-    sum.sink_blocks = kv.sinks > 0 ? (int)join_blocks(heads * kv.sinks, kv.D, kv.sink_parts) : 0;
-    const int64_t others = kv.shares > 1 ? join_blocks(heads * (kv.S - kv.sinks), kv.D, kv.shares) : 0;
-    hipLaunchKernelGGL((window_sum_kernel<elem_t>), dim3((unsigned)(sum.sink_blocks + others)), dim3(kBlock), 0, stream, sum);
+    const Joining of_sinks(kv.D, kv.sink_parts), of_others(kv.D, kv.shares);
+    sum.sink_blocks = kv.sinks > 0 ? (int)of_sinks.blocks(heads * kv.sinks) : 0;
+    const int64_t others = kv.shares > 1 ? of_others.blocks(heads * (kv.S - kv.sinks)) : 0;
+    hipLaunchKernelGGL((window_sum_kernel<elem_t>), dim3((unsigned)(sum.sink_blocks + others)), dim3(kBlock), 0, stream, sum, of_sinks, of_others);
   }
   return hipGetLastError();
 }

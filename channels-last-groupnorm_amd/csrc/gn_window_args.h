@@ -35,6 +35,7 @@ struct WindowArgs {
   int shares;                 // dk, dv: workgroups that share a tile's queries
   int sink_sets, sink_parts;  // dk, dv of the sinks: 32 keys each; workgroups that share the queries
   float scale, scale_log2;
+  Divisor by_group, by_splits, by_tiles, by_K, by_shares, by_sink_parts, by_sink_sets, by_per_head, by_L, by_H;
   int sink_blocks;            // window_sum_kernel: workgroups that add up the sinks' parts
 };
 
