@@ -560,6 +560,41 @@ template <typename T, int DP> __device__ __forceinline__ void store_token(T *p, 
       }
     }
 }
+// The same of 16-bit results, with REST what their rounding leaves instead, through a wavefront's own 64 DP bytes of shared memory, so
+// that a row leaves in whole lines: row r goes to `to` + r row_bytes if r < last.  (Two results of 16 samples of 128 tokens, 8 heads
+// of 128: the forward takes 9.0 us so, 10.0 by 8 bytes of a row at a time; the backward, with one result a kernel, is no faster.)
+template <typename T, int DP, bool REST>
+__device__ __forceinline__ void store_rows(char *place, const f32x16_t (&acc)[DP / 32], float factor, int D, char *to, int64_t row_bytes, int last) {
+  static_assert(sizeof(T) == 2, "");
+  using LV = LaneVec<T, 4>;
+  constexpr int kChunks = DP / 8, kMask = (kChunks & -kChunks) - 1;  // (rows' chunks turned, so that they are not all in the same banks)
+  const int lane = threadIdx.x & 63, h = lane >> 5, row = lane & 31;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const float t[4] = {acc[c][r] * factor, acc[c][r + 1] * factor, acc[c][r + 2] * factor, acc[c][r + 3] * factor};
+      auto raw = LV::pack(t);
+      if constexpr (REST) {
+        float left[4];
+        LV::unpack(raw, left);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) left[e] = t[e] - left[e];
+        raw = LV::pack(left);
+      }
+      *(decltype(raw) *)(place + (row * kChunks + ((4 * c + r / 4) ^ (row & kMask))) * 16 + h * 8) = raw;
+    }
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int n = 0; n < kChunks / 2; ++n) {
+    const int e = n * 64 + lane, r = e / kChunks, ch = e % kChunks;
+    const u32x4 v = *(const u32x4 *)(place + (r * kChunks + (ch ^ (r & kMask))) * 16);
+    if (r < last && ch * 8 < D) store_global<u32x4>(to + r * row_bytes + ch * 16, v);
+  }
+  asm volatile("" ::: "memory");
+}
+// Rows are written again, by other lanes: what they hold has to be there before.
+__device__ __forceinline__ void rows_written() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // A token that sees nothing, or that nobody sees, gets zeros, whatever its tile held: its weights are 0, and 0 times NaN is NaN.
 template <int N> __device__ __forceinline__ void clear_unless(bool kept, f32x16_t (&acc)[N]) {
 #pragma unroll
@@ -729,6 +764,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, sizeof(T) == 
   }
   const WindowArgs &z = arguments_again();
   const float sum = st.sum + other_half(st.sum);
+  const int i0 = tile * kQueries + wave * 32;
   const bool there = i < z.L, seeing = st.sight.count > 0 || st.sight.sinks > 0;
   clear_unless(seeing, st.o);
   if (z.splits > 1) {
@@ -745,22 +781,24 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, sizeof(T) == 
   const bool nothing = !(sum > 0.0f);  // (no key seen, or no score above -inf: those that see one are computed again)
   const float factor = nothing ? 0.0f : 1.0f / sum;
   const bool again = either_half(any_not_finite(st.o) || !(factor < INFINITY) || nothing) && seeing;
-  if (there) {
-#pragma unroll
-    for (int c = 0; c < DP / 32; ++c)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int d = 32 * c + row_of(r, lane >> 5);
-        const float t[4] = {st.o[c][r] * factor, st.o[c][r + 1] * factor, st.o[c][r + 2] * factor, st.o[c][r + 3] * factor};
-        if (d < z.D) store_out<T, 4>(z, b, h, i, d, t);
-      }
-    if (z.lse && lane < 32) store_global<float>(z.lse + ((int64_t)b * z.H + h) * z.L + i, nothing ? INFINITY : st.reference + __builtin_amdgcn_logf(sum));
+  if constexpr (sizeof(T) == 2) {
+    char *place = tiles + wave * G::kBytes;
+    __syncthreads();  // (the tiles have been read)
+    if (i0 < z.L) {
+      store_rows<T, DP, false>(place, st.o, factor, z.D, z.out.row(b, i0, h), z.out.token_bytes, z.L - i0);
+      if (z.rest)
+        store_rows<T, DP, true>(place, st.o, factor, z.D, (char *)((T *)z.rest + (((int64_t)b * z.L + i0) * z.H + h) * z.D), (int64_t)z.H * z.D * 2, z.L - i0);
+    }
+  } else if (there) {
+    store_token<T, DP>((T *)z.out.row(b, i, h), z.D, st.o, factor);
   }
+  if (z.lse && there && lane < 32) store_global<float>(z.lse + ((int64_t)b * z.H + h) * z.L + i, nothing ? INFINITY : st.reference + __builtin_amdgcn_logf(sum));
   uint64_t rows = __ballot(again && there) & 0xffffffffu;
+  if (rows) rows_written();
   while (rows) {
     const int r = __builtin_ctzll(rows);
     rows &= rows - 1;
-    row_again<T>(z, s, b, h, tile * kQueries + wave * 32 + r);
+    row_again<T>(z, s, b, h, i0 + r);
   }
 }
 
