@@ -148,11 +148,13 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     if (p.few) {
       a.tiles = (int)ceil_div(few_rows, 32);
       const int64_t heads = (int64_t)a.B * a.K * a.tiles;
-      // Keys that a tile's rows see at most, in tiles of 32 and of a wavefront one takes 1.5 us of waiting for it, until the memory is
-      // what is waited for; a workgroup has 2 us besides, and joining takes a second launch of 4.  (one token of 24 heads over 8 of
-      // 128, 517 keys: one workgroup a head 14.3 us, two 11.3 + 3.5, nine 8.3 + 4.4)
+      // Keys that a tile's rows see at most, in tiles of 32 and of a wavefront one takes 1.5 us of waiting for it (float32: 3, of its
+      // products), until the memory is what is waited for; a workgroup has 2 us besides, and joining takes a second launch of 4.  (one
+      // token of 8 heads of 128 against 2000: one workgroup a head 18 us, two 15.5, five 12.2, nine, as here, 11.1; 8 heads of 64
+      // against 300: one, as here, 6.2, three 8.2; in float32 one 14.6, three, as here, 10.8)
       const int64_t tiles = ceil_div(std::min<int64_t>(a.S, (int64_t)a.left + a.right + a.L + a.sinks + 64), 32), waves = few_waves((int)width, (int)es);
-      auto cost = [&](int64_t s) { return ceil_div(heads * s, kNumCU) * (4 + 3 * ceil_div(tiles, s * waves)) + (s > 1 ? 8 : 0); };
+      const int64_t each = es == 4 ? 6 : 3;
+      auto cost = [&](int64_t s) { return ceil_div(heads * s, kNumCU) * (4 + each * ceil_div(tiles, s * waves)) + (s > 1 ? 8 : 0); };
       for (int64_t s = 2; s <= 64 && s <= tiles; ++s)
         if (cost(s) < cost(a.splits)) a.splits = (int)s;
       a.items = (int)(heads * a.splits);
