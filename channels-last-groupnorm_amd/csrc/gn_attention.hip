@@ -12,6 +12,7 @@ namespace {
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;
 constexpr int64_t kFewRows = 128;
+constexpr int64_t kFineKeys = 64;  // (where 64 are seen, 1.44 without)
 constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
 
 int invalid(const char *what) { return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s", what); }
@@ -129,6 +130,10 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     a.right = a.causal ? 0 : a.left;
     a.sinks = 0;
   }
+  // Rounding the weights of the second product leaves the forward's result inexact by more than its own rounding where they are few,
+  // and the gradients, which are small differences there, by half as much again: two tokens of 64 channels in bfloat16 1.58 times
+  // what rounding dq alone leaves, 1.41 with the weights and what rounding them left.
+  a.fine = es == 2 && std::min<int64_t>(a.S, (int64_t)a.left + a.right + 1 + a.sinks) <= kFineKeys;
   a.tiles = (int)ceil_div(a.L, kQueries);
   a.splits = a.shares = 1;
   const int64_t items = (int64_t)a.tiles * a.H * a.B, lse = (int64_t)a.B * a.H * a.L;
@@ -229,12 +234,7 @@ int gnnhwc_window(const gnnhwc_window_call *c, void *workspace, size_t workspace
   if (p.empty) return GNNHWC_OK;
   p.a.part_k = (float *)workspace;
   p.a.part_v = (float *)((char *)workspace + p.part_v);
-  if (p.few) {
-#define GN_CALL(S) launch_window_few_##S(p.a, (hipStream_t)stream)
-    return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window");
-#undef GN_CALL
-  }
-#define GN_CALL(S) launch_window_forward_##S(p.a, (hipStream_t)stream)
+#define GN_CALL(S) launch_window_forward_##S(p.a, p.few, (hipStream_t)stream)
   return launched(GN_BY_TYPE(c->dtype, GN_CALL), "gnnhwc_window");
 #undef GN_CALL
 }

@@ -628,8 +628,10 @@ template <typename T, int DP> struct ForwardState {
   Sight sight;
 };
 
-// 32 N keys against the wavefront's 32 queries: scores, then weights in their place, then their products with the values.
-template <typename T, int DP, int N, typename ST> __device__ __forceinline__ void forward_tile(ST &st, const LaneOffsets<T, DP> &at, const char *kt, char *vt, int j0, float c) {
+// 32 N keys against the wavefront's 32 queries: scores, then weights in their place, then their products with the values.  SUMS:
+// float32 scores as sums of 16 channels' sums (half the error of adding channel to channel, for 16 additions a step, which a wavefront
+// that waits for its keys has time for).
+template <typename T, int DP, int N, bool SUMS, typename ST> __device__ __forceinline__ void forward_tile(ST &st, const LaneOffsets<T, DP> &at, const char *kt, char *vt, int j0, float c, bool fine) {
   const int h = (threadIdx.x & 63) >> 5;
   const Sight &g = st.sight;
   const int left = j0 - g.low;
@@ -639,7 +641,12 @@ template <typename T, int DP, int N, typename ST> __device__ __forceinline__ voi
 #pragma unroll
   for (int x = 0; x < DP / 16; ++x) {
     if (!at.has(x)) break;
-    s[0] = Operand<T>::product(at.template of_rows<0>(kt, x), st.q[x], x ? s[0] : zeros16());
+    if constexpr (sizeof(T) == 4 && SUMS) {
+      const f32x16_t t = Operand<T>::product(at.template of_rows<0>(kt, x), st.q[x], zeros16());
+      s[0] = x ? s[0] + t : t;
+    } else {
+      s[0] = Operand<T>::product(at.template of_rows<0>(kt, x), st.q[x], x ? s[0] : zeros16());
+    }
     if constexpr (N == 2) s[N - 1] = Operand<T>::product(at.template of_rows<32>(kt, x), st.q[x], x ? s[N - 1] : zeros16());
   }
   if (!__all(inside)) {
@@ -679,6 +686,15 @@ template <typename T, int DP, int N, typename ST> __device__ __forceinline__ voi
     const operand_t<T> w = operand_of<T>(p, u % 2);
 #pragma unroll
     for (int x = 0; x < DP / 32; ++x) st.o[x] = Operand<T>::product(at.template of_columns<16 * u>(vt, x), w, st.o[x]);
+    if constexpr (sizeof(T) == 2) {
+      if (fine) {  // and what the weights' rounding left
+#pragma unroll
+        for (int r = 0; r < 8; ++r) p[8 * (u % 2) + r] -= (float)w[r];
+        const operand_t<T> left = operand_of<T>(p, u % 2);
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) st.o[x] = Operand<T>::product(at.template of_columns<16 * u>(vt, x), left, st.o[x]);
+      }
+    }
   };
   part(std::integral_constant<int, 0>());
   part(std::integral_constant<int, 1>());
@@ -710,8 +726,10 @@ __device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int 
   return (((int64_t)split * a.B + b) * a.H + h) * a.L + i;
 }
 
-// A workgroup: 128 queries of one head, 32 a wavefront, against one of `splits` shares of the keys that they see.
-template <typename T, int DP> __global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
+// A workgroup: 128 queries of one head, 32 a wavefront, against one of `splits` shares of the keys that they see.  FINE: a.fine, as a
+// kernel of its own (float16 heads of 64 have no registers left for both in one, and few queries are 3 % slower with both).
+template <typename T, int DP, bool FINE>
+__global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : DP <= 64 && !FINE ? 4 : DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a);
@@ -753,7 +771,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, sizeof(T) == 
       constexpr int B = decltype(buffer)::value;
       tiles_turn();
       if (u + 1 < w.end) issue(u + 1, 1 - B);
-      forward_tile<T, DP, G::kRows / 32>(st, at, tiles + B * 2 * G::kBytes, tiles + B * 2 * G::kBytes + G::kBytes, w.tile(u) * G::kRows, a.scale_log2);
+      forward_tile<T, DP, G::kRows / 32, false>(st, at, tiles + B * 2 * G::kBytes, tiles + B * 2 * G::kBytes + G::kBytes, w.tile(u) * G::kRows, a.scale_log2, FINE);
       ++u;
     };
     while (u < w.end) {
@@ -830,7 +848,7 @@ template <int COPIES, typename F> __device__ __forceinline__ void next_copies(bo
 // Weight and result of a row that is joined of parts: (reference, sum).
 __device__ __forceinline__ float part_weight(float reference, float most) { return most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(reference - most); }
 
-template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void window_few_kernel(const WindowArgs a) {
+template <typename T, int DP, bool FINE> __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void window_few_kernel(const WindowArgs a) {
   using W = Few<T, DP>;
   constexpr int kWaves = W::kWaves;
   __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * W::kStage];
@@ -876,7 +894,7 @@ template <typename T, int DP> __global__ __launch_bounds__((64 * Few<T, DP>::kWa
       char *tile = tiles + (wave * 2 + turn) * W::kStage;
       turn ^= 1;
       next_copies<2 * TileCopy<T, DP, 32, 64>::kCopies>(u + kWaves < w.end, [&] { issue(u + kWaves, turn); });
-      forward_tile<T, DP, 1>(st, at, tile, tile + W::kStage / 2, w.tile(u) * 32, a.scale_log2);
+      forward_tile<T, DP, 1, true>(st, at, tile, tile + W::kStage / 2, w.tile(u) * 32, a.scale_log2, FINE);
     }
   }
   const WindowArgs &z = arguments_again();

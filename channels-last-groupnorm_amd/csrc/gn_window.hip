@@ -37,27 +37,25 @@ template <typename F> void with_width(int D, F &&f) {
   }
 }
 dim3 grid_of(int items) { return dim3((unsigned)((items + 7) / 8 * 8)); }
-void join(const WindowArgs &a, hipStream_t stream) {
-  if (a.splits <= 1) return;
-  const int64_t rows = (int64_t)a.B * a.H * a.L;
-  const Joining joining(a.D, a.splits);
-  hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)joining.blocks(rows)), dim3(kBlock), 0, stream, a, joining);
-}
-
 }  // namespace
 
-hipError_t GN_CAT(launch_window_forward_, GN_SUFFIX)(const WindowArgs &a, hipStream_t stream) {
-  with_width(a.D, [&](auto w) { hipLaunchKernelGGL((window_forward_kernel<elem_t, decltype(w)::value>), grid_of(a.items), dim3(kBlock), 0, stream, a); });
-  join(a, stream);
-  return hipGetLastError();
-}
-
-hipError_t GN_CAT(launch_window_few_, GN_SUFFIX)(const WindowArgs &a, hipStream_t stream) {
-  with_width(a.D, [&](auto w) {
+hipError_t GN_CAT(launch_window_forward_, GN_SUFFIX)(const WindowArgs &a, bool few, hipStream_t stream) {
+  auto launch = [&](auto w, auto fine) {
     constexpr int DP = decltype(w)::value;
-    hipLaunchKernelGGL((window_few_kernel<elem_t, DP>), grid_of(a.items), dim3(64 * Few<elem_t, DP>::kWaves), 0, stream, a);
+    constexpr bool FINE = decltype(fine)::value;
+    if (few) hipLaunchKernelGGL((window_few_kernel<elem_t, DP, FINE>), grid_of(a.items), dim3(64 * Few<elem_t, DP>::kWaves), 0, stream, a);
+    else hipLaunchKernelGGL((window_forward_kernel<elem_t, DP, FINE>), grid_of(a.items), dim3(kBlock), 0, stream, a);
+  };
+  with_width(a.D, [&](auto w) {
+    if constexpr (sizeof(elem_t) == 2) {
+      if (a.fine) return launch(w, std::true_type());
+    }
+    launch(w, std::false_type());
   });
-  join(a, stream);
+  if (a.splits > 1) {
+    const Joining joining(a.D, a.splits);
+    hipLaunchKernelGGL((window_join_kernel<elem_t>), dim3((unsigned)joining.blocks((int64_t)a.B * a.H * a.L)), dim3(kBlock), 0, stream, a, joining);
+  }
   return hipGetLastError();
 }
 

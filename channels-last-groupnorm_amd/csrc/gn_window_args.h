@@ -31,6 +31,7 @@ struct WindowArgs {
   int left, right, sinks, causal;
   int tiles, items;           // tiles of a head, workgroups with work
   int order, per_head;        // ... of a key head
+  int fine;                   // weights in twice the bits (plan_window)
   int splits;                 // out, dq: workgroups that share a row's keys
   int shares;                 // dk, dv: workgroups that share a tile's queries
   int sink_sets, sink_parts;  // dk, dv of the sinks: 32 keys each; workgroups that share the queries
@@ -46,9 +47,8 @@ constexpr int few_waves(int width, int elem_size) {
   return most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
 }
 
-#define GN_DECLARE_WINDOW(S)                                                            \
-  hipError_t launch_window_forward_##S(const WindowArgs &a, hipStream_t stream);        \
-  hipError_t launch_window_few_##S(const WindowArgs &a, hipStream_t stream);            \
+#define GN_DECLARE_WINDOW(S)                                                                  \
+  hipError_t launch_window_forward_##S(const WindowArgs &a, bool few, hipStream_t stream);    \
   hipError_t launch_window_backward_##S(const WindowArgs &a, const WindowArgs &kv, const WindowArgs &sinks, hipStream_t stream);
 GN_DECLARE_WINDOW(f32)
 GN_DECLARE_WINDOW(f16)

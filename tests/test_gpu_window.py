@@ -137,6 +137,22 @@ def test_a_training_that_has_diverged(dtype, device):
             assert t.isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape", [(16, 2, 2, 12, 12, 64, 1, 0, False), (16, 12, 12, 4, 2, 128, None, 0, True), (8, 300, 300, 4, 4, 80, 2, 0, True),
+                                   (2, 700, 700, 4, 2, 64, 9, 2, False)])
+def test_gradients_of_tokens_that_see_a_few(shape, dtype, device):
+    """Each gradient has dS rounded, as an operand, and itself: sqrt(2) times the error of the last rounding alone, in the norm, and
+    out that one only.  (dS is a small difference there: a result that is off by its weights' rounding would show.)  A tenth more for
+    how the few roundings of a small case fall."""
+    B, L, S, H, K, D, window, sinks, causal = shape
+    q, k, v, dout, n, got = run(dtype, device, *shape)
+    want = ref.attention(q, k, v, ref.sees(B, L, S, window, sinks, causal, None, False, device), D ** -0.5, dout)
+    for name, most in (("out", 1.0), ("dq", math.sqrt(2)), ("dk", math.sqrt(2)), ("dv", math.sqrt(2))):
+        value = want[name][0]
+        alone = float((value.to(dtype).double() - value).norm())
+        assert float((got[name].detach().double() - value).norm()) < 1.1 * most * alone, name
+
+
 @pytest.mark.parametrize("gain", [2.0 ** -20, 2.0 ** 12])
 def test_gradients_of_any_scale_in_half_precision(gain, device):
     """float16 gradients of a scaled or an averaged loss: dS is held relative to the largest."""
