@@ -11,7 +11,6 @@ namespace gn {
 namespace {
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;
-constexpr int64_t kFewRows = 128;
 constexpr int64_t kFineKeys = 64;  // (where 64 are seen, 1.44 without)
 constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
 
@@ -148,7 +147,15 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   p.bytes = 256;
   if (!backward) {
     const int64_t few_rows = (int64_t)a.L * a.group;
-    p.few = few_rows <= kFewRows;
+    // The kernel for few queries has tiles of 32 rows, all of a workgroup's wavefronts share a tile's keys, and its queries are
+    // read by nobody else; the other has 128 rows, a wavefront's 32 to itself, and reads keys once for all.  The first is faster
+    // while its tiles leave CUs without work, which float32, being bound by its products, does sooner, and wide heads, which have
+    // fewer wavefronts: bfloat16, 8 samples of 8 heads of 64, 100 queries, 2000 keys 14.5 us against 22.2, 4 samples of 128, 250
+    // queries 29.7 against 28.9, one of 20 heads of 64, 200 tokens 6.0 against 9.3; float32, 4 samples of 8 heads of 64, 2000
+    // keys, 128 queries 34.6 against 35.5, 250 60.6 against 52.6.  (16 samples of 16 heads of 128, 32 queries, 1000 keys 19.3
+    // against 25.1, 64 queries 33.6 against 26.4)
+    const int64_t few_tiles = (int64_t)a.B * a.K * ceil_div(few_rows, 32);
+    p.few = few_rows <= 32 || few_tiles <= (es == 2 ? (width <= 64 ? kNumCU : kNumCU * 3 / 4) : width <= 64 ? kNumCU / 2 : kNumCU / 8);
     if (p.empty) return GNNHWC_OK;
     if (p.few) {
       a.tiles = (int)ceil_div(few_rows, 32);

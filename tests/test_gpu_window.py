@@ -40,6 +40,11 @@ SHAPES = [
     (1, 515, 515, 2, 1, 96, 100, 129, False), (2, 640, 640, 2, 2, 64, 63, 16, False), (1, 1030, 1030, 4, 2, 64, 200, 4, True),
     (1, 700, 1500, 2, 1, 128, None, 0, True), (1, 130, 130, 2, 1, 160, 33, 3, False), (1, 200, 200, 2, 2, 256, None, 0, True),
     (1, 70, 70, 1, 1, 248, 20, 2, False),
+    # more heads than a kernel for few queries takes
+    (4, 128, 128, 16, 16, 8, 0, 0, False), (4, 129, 129, 16, 16, 64, None, 0, False), (4, 200, 260, 16, 16, 64, 30, 5, True),
+    (5, 150, 150, 16, 8, 128, 40, 3, False), (4, 257, 257, 16, 16, 96, 64, 33, True), (3, 140, 140, 20, 20, 160, 20, 1, False),
+    (4, 130, 130, 16, 16, 256, None, 0, True), (6, 300, 300, 16, 4, 40, 10, 2, False), (5, 131, 131, 16, 16, 128, 5, 0, True),
+    (9, 65, 100, 40, 20, 72, 70, 9, True),
 ]
 
 
@@ -63,9 +68,10 @@ def test_heads_that_no_lane_vector_divides(D, dtype, device):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("lengths", [[150, 0, 1], [64, 33, 149], [200, -5, 150]])
 @pytest.mark.parametrize("causal", [False, True])
-def test_padded_batches(lengths, causal, dtype, device):
+@pytest.mark.parametrize("heads", [(4, 2), (80, 40)])
+def test_padded_batches(heads, lengths, causal, dtype, device):
     """Padding holds NaN: it reaches nobody, and gets zeros."""
-    B, L, H, K, D = 3, 150, 4, 2, 64
+    (H, K), B, L, D = heads, 3, 150, 64
     q, k, v, dout = (normal((B, L, h, D), dtype, device, i) for i, h in enumerate((H, K, K, H)))
     n = torch.tensor(lengths, device=device)
     seen = ref.sees(B, L, L, 21, 3, causal, n, False, device)
@@ -86,9 +92,10 @@ def test_padded_batches(lengths, causal, dtype, device):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("causal", [False, True])
-def test_values_that_are_not_finite_reach_those_that_see_them(bad, causal, dtype, device):
+@pytest.mark.parametrize("heads", [(2, 1), (80, 40)])
+def test_values_that_are_not_finite_reach_those_that_see_them(heads, bad, causal, dtype, device):
     """One token of q, k, v or the gradient is NaN or infinite: what does not see it is as without it."""
-    B, L, H, K, D, window, sinks, at = 1, 200, 2, 1, 64, 20, 3, 100
+    (H, K), B, L, D, window, sinks, at = heads, 1, 200, 64, 20, 3, 100
     seen = ref.sees(B, L, L, window, sinks, causal, None, False, device)[0]
     tensors = [normal((B, L, h, D), dtype, device, i) for i, h in enumerate((H, K, K, H))]
     want = ref.attention(*tensors[:3], seen.unsqueeze(0), D ** -0.5, tensors[3])
@@ -113,7 +120,7 @@ def test_values_that_are_not_finite_reach_those_that_see_them(bad, causal, dtype
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("shape", [(1, 150, 4, 2, 64, 100), (2, 900, 8, 8, 128, 800), (6, 1500, 6, 3, 64, 1450)])  # with and without shared keys
+@pytest.mark.parametrize("shape", [(1, 150, 4, 2, 64, 100), (1, 150, 80, 80, 64, 100), (2, 900, 8, 8, 128, 800), (6, 1500, 6, 3, 64, 1450)])  # with and without shared keys
 def test_padding_next_to_values_that_are_not_finite(shape, dtype, device):
     """Tokens of one tile, one NaN or infinite and others padding: those still get zeros."""
     B, L, H, K, D, n = shape
