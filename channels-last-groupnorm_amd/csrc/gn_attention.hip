@@ -66,7 +66,8 @@ struct WindowPlan {
 };
 
 // Workgroups that share the work of each of `items`, of `steps` steps: a CU takes `thick` of them at once in the time of one, each
-// has some steps' time of its own, and what they leave has to be joined.
+// has some steps' time of its own, and what they leave has to be joined.  (training of 1500 tokens, 8 heads over 2 of 128, causal, in
+// bfloat16: 99 us, unshared 294; of a padded float32 batch, 3 x 1961, 6 over 2 of 40: 250 and 500)
 int64_t shares_of(int64_t items, int64_t steps, int64_t thick, int64_t most) {
   if (items == 0) return 1;
   // (in steps of which a CU takes `thick` at once: 1.7 us for float32, 0.5 for 16 bits, where the second launch is 4 us and a share's

@@ -336,7 +336,8 @@ __device__ __forceinline__ int rest_by(int n, const Divisor &v) { return n - div
 // The work of this workgroup, of a.items ordered by key head; a.items and beyond: none.  Workgroups are dealt to the eight dies in
 // turn, each with a cache of its own that a head's keys and values are to be in once: heads are dealt to the dies in turn, or, where
 // they do not come out even, each die has a stretch of the work, or, where samples have lengths that would make those uneven, all
-// is dealt in turn.  (padded float32 (3, 1961, 6 heads over 2, 40): forward 112 us with stretches)
+// is dealt in turn.  (training: 2 x 4096 tokens, 24 heads over 8 of 128, 535 us by heads or stretches, 590 in turn; 3 x 4096, padded,
+// 9 over 3, 475 us in turn, 760 by stretches)
 __device__ __forceinline__ int work_item(const WindowArgs &a) {
   const int id = blockIdx.x, die = id & 7, n = id >> 3;
   if (a.order == kHeadsInTurn) return (div_by(n, a.by_per_head) * 8 + die) * a.per_head + rest_by(n, a.by_per_head);
@@ -726,7 +727,10 @@ __device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int 
   return (((int64_t)split * a.B + b) * a.H + h) * a.L + i;
 }
 
-// A workgroup: 128 queries of one head, 32 a wavefront, against one of `splits` shares of the keys that they see.  FINE: a.fine, as a
+// A workgroup: 128 queries of one head, 32 a wavefront, against one of `splits` shares of the keys that they see.  128 queries share a
+// tile's copy; 64 keys a tile are as many as leave room for four workgroups of heads of 64 in a CU's registers, whose waits hide
+// each other.  float16 15600 tokens, 8 heads of 128, window 2400: 321 us, 880 TFLOP/s (a library's product 1070); bfloat16 4 x
+// 4096, 20 heads of 64: 810; with window 512, where a tenth of the pairs of its tiles is hidden, 675.  FINE: a.fine, as a
 // kernel of its own (float16 heads of 64 have no registers left for both in one, and few queries are 3 % slower with both).
 template <typename T, int DP, bool FINE>
 __global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : DP <= 64 && !FINE ? 4 : DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
@@ -823,7 +827,8 @@ __global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : DP <=
 // ---- forward of few queries: the newest tokens of requests ----
 // Rows (tokens times the heads of a group) fill one tile of 32, and the keys are what takes time: a workgroup is as many wavefronts
 // as have room for two tiles of 32 keys and values each, every one walks keys of its own, and what they found is joined at the end.
-// No barrier on the way: a wavefront waits for its own copies only.  Where there are fewer heads than the device has room for,
+// No barrier on the way: a wavefront waits for its own copies only.  64 requests of 32 heads over 8 of 128, 4100 keys: 184 us, 5.6 TB/s;
+// one of 24 heads over 8, 517 keys: 8 us, the latency of its arguments, its tile and the join, and 4 of the second launch.  Where there are fewer heads than the device has room for,
 // several workgroups share a head's keys (splits) and window_join_kernel joins them.
 template <typename T, int DP> struct Few {
   static constexpr int kStage = 2 * 32 * DP * (int)sizeof(T);  // bytes of a tile of keys and one of values
@@ -1064,6 +1069,9 @@ template <typename T> __device__ __forceinline__ float gradient_unit(float most)
   else return most > 0.0f && most < INFINITY ? __builtin_amdgcn_ldexpf(1.0f, -__builtin_amdgcn_frexp_expf(most)) : 1.0f;
 }
 
+// A workgroup: 128 queries of one head against a share of the keys that they see, like the forward, with q and do in registers and
+// three products a pair.  bfloat16, 4 x 4112 tokens, 20 heads of 64, window 512: 163 to 175 us, 121 GFLOP of the formula's at 0.7 PFLOP/s;
+// without its copies 5 % less, without the exponentials a tenth, without the products a fifth: no one unit bounds it.
 template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && sizeof(T) == 2 ? 2 : 1) void window_dq_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
@@ -1408,7 +1416,10 @@ __device__ __forceinline__ int64_t tile_slot(const WindowArgs &a, int bk, int ti
 
 // A workgroup: 128 keys of one head, 32 a wavefront, against a share of the queries whose windows have any of them, of all heads of
 // the group.  Where several share a tile's queries, each leaves float32 sums, which window_sum_kernel adds in their order.  Sinks,
-// which all queries see, are left to window_sink_kernel.
+// which all queries see, are left to window_sink_kernel.  k, v and both sums of 32 keys stay in registers, which leaves two wavefronts
+// a SIMD for heads of 64 (three would have registers in scratch memory: 321 us for 254) and one beyond, and operands are read a phase
+// ahead of their products instead.  bfloat16, 4 x 4112 tokens, 20 heads of 64, window 512: 197 to 212 us, 0.8 PFLOP/s; 2 x 4096, 24 over 8
+// of 128, causal, window 1024: 238 to 258.
 template <typename T, int DP, int PARTS>
 __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void window_dkv_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
@@ -1519,7 +1530,8 @@ __global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void wi
 }
 
 // dk and dv of the sinks: 32 keys, which all wavefronts hold, against a share of all queries, of which each wavefront walks its own
-// (a tile of 128 keys with a few sinks would have three of four wavefronts idle most of the way).
+// (a tile of 128 keys with a few sinks would have three of four wavefronts idle most of the way).  Reading q and do once more bounds
+// it: 4 x 4112 tokens of 20 heads of 64 in bfloat16 21 us, 4 TB/s.
 template <typename T, int DP, int PARTS> __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void window_sink_kernel(const WindowArgs a) {
   using W = Few<T, DP>;
   using KS = KeySide<T, DP, PARTS>;
