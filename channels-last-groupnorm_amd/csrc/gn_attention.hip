@@ -150,13 +150,17 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     const int64_t few_rows = (int64_t)a.L * a.group;
     // The kernel for few queries has tiles of 32 rows, all of a workgroup's wavefronts share a tile's keys, and its queries are
     // read by nobody else; the other has 128 rows, a wavefront's 32 to itself, and reads keys once for all.  The first is faster
-    // while its tiles leave CUs without work, which float32, being bound by its products, does sooner, and wide heads, which have
-    // fewer wavefronts: bfloat16, 8 samples of 8 heads of 64, 100 queries, 2000 keys 14.5 us against 22.2, 4 samples of 128, 250
-    // queries 29.7 against 28.9, one of 20 heads of 64, 200 tokens 6.0 against 9.3; float32, 4 samples of 8 heads of 64, 2000
-    // keys, 128 queries 34.6 against 35.5, 250 60.6 against 52.6.  (16 samples of 16 heads of 128, 32 queries, 1000 keys 19.3
-    // against 25.1, 64 queries 33.6 against 26.4)
+    // while its tiles leave CUs without work (wide heads have fewer wavefronts): bfloat16, 8 samples of 8 heads of 64, 100 queries,
+    // 2000 keys 14.5 us against 22.2, one of 20 heads of 64, 200 tokens 6.0 against 9.3; 4 samples of 8 heads of 128, 250 queries,
+    // 2000 keys 29.7 against 28.9.  float32 is bound by its products, which the first shares evenly: what counts are the tiles of keys
+    // that all its tiles of rows visit.  2 samples of 12 heads of 64, 200 queries, window 50 (840 of them) 8.6 us against 20.3, 4
+    // of 8 heads, 250 queries, 2000 keys (16000) 60.6 against 52.6; heads of 128: 840 23.1 against 47.1, 980 36.9 against 30.3.
+    // (16 samples of 16 heads of 128, 1000 keys: 32 queries 19.3 against 25.1, 64 queries 33.6 against 26.4)
     const int64_t few_tiles = (int64_t)a.B * a.K * ceil_div(few_rows, 32);
-    p.few = few_rows <= 32 || few_tiles <= (es == 2 ? (width <= 64 ? kNumCU : kNumCU * 3 / 4) : width <= 64 ? kNumCU / 2 : kNumCU / 8);
+    const int64_t visits = few_tiles * ceil_div(std::min<int64_t>(a.S, (int64_t)a.left + a.right + a.sinks + 32 / std::min(a.group, 32) + 32), 32);
+    if (es == 2) p.few = few_tiles <= (width <= 64 ? kNumCU : kNumCU * 3 / 4);
+    else p.few = few_tiles <= 2 * kNumCU && visits <= (width <= 64 ? 8192 : 900);
+    p.few |= few_rows <= 32;
     if (p.empty) return GNNHWC_OK;
     if (p.few) {
       a.tiles = (int)ceil_div(few_rows, 32);

@@ -985,9 +985,10 @@ struct Joining {
   int64_t blocks(int64_t rows) const { return (rows + rows_here - 1) / rows_here; }
 };
 struct Joiner {
-  int joiners, row, part, d, quads;  // the thread's row of the workgroup's, its first part and first channel
+  int joiners, rows_here, row, part, d, quads;  // the thread's row of the workgroup's, its first part and first channel
   __device__ __forceinline__ explicit Joiner(const Joining &j) {
     joiners = j.joiners;
+    rows_here = j.rows_here;
     quads = j.quads.d;
     row = div_by(threadIdx.x, j.lanes);
     const int left = threadIdx.x - row * j.lanes.d;
@@ -1000,6 +1001,7 @@ template <typename V, typename F> __device__ __forceinline__ V joined(const Join
   __syncthreads();
   place[threadIdx.x] = v;
   __syncthreads();
+  if (at.row >= at.rows_here) return v;  // (left over: no row, and no parts in reach)
   const V *first = place + (threadIdx.x - at.part * at.quads);
   v = first[0];
   for (int n = 1; n < at.joiners; ++n) v = f(v, first[n * at.quads]);
@@ -1010,7 +1012,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
   __shared__ int bad[kBlock], any_bad;
   __shared__ f32x4 place[kBlock];
   const Joiner at(joining);
-  const int r = at.row, d = at.d, rows_here = joining.rows_here;
+  const int r = at.row, d = at.d, rows_here = at.rows_here;
   const int64_t rows = (int64_t)a.B * a.H * a.L;
   const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^24 workgroups)
   const bool there = r < rows_here && id < rows;
@@ -1217,7 +1219,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_ke
   __shared__ int bad[kBlock], any_bad;
   __shared__ f32x4 place[kBlock];
   const Joiner at(joining);
-  const int r = at.row, rows_here = joining.rows_here;
+  const int r = at.row, rows_here = at.rows_here;
   const int64_t rows = (int64_t)a.B * a.H * a.L;
   const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^24 workgroups)
   const bool there = r < rows_here && id < rows;
@@ -1628,7 +1630,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kerne
   // (the first workgroups have the sinks, the others, if there are any, the other keys)
   const bool sink = (int)blockIdx.x < a.sink_blocks;
   const Joiner with(sink ? of_sinks : of_others);
-  const int r = with.row, d = with.d, rows_here = (sink ? of_sinks : of_others).rows_here;
+  const int r = with.row, d = with.d, rows_here = with.rows_here;
   const int first = sink ? 0 : a.sinks, rows = sink ? a.sinks : a.S - a.sinks;
   bad_k[threadIdx.x] = bad_v[threadIdx.x] = 0;
   if (threadIdx.x == 0) any_bad = 0;

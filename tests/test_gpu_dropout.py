@@ -7,6 +7,7 @@ import torch
 
 from gnnhwc import Dropout, dropout
 from tests.dropout_refs import bits_of
+from tests.left_alone import generators_left_alone  # noqa: F401 (a fixture)
 from tests.token_refs import LEAST, U
 
 pytestmark = pytest.mark.gpu

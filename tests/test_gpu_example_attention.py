@@ -7,6 +7,7 @@ import torch
 import torch.nn.functional as F
 
 from gnnhwc import dropout
+from tests.left_alone import generators_left_alone  # noqa: F401 (a fixture)
 from tests import window_refs as ref
 
 pytestmark = pytest.mark.gpu

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from gnnhwc import window_attention
+from tests.left_alone import generators_left_alone  # noqa: F401 (a fixture)
 from tests import window_refs as ref
 
 pytestmark = pytest.mark.gpu

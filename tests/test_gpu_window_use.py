@@ -7,6 +7,7 @@ import torch
 
 from gnnhwc import Dropout, window_attention, window_attention_cached
 from tests import window_refs as ref
+from tests.left_alone import generators_left_alone  # noqa: F401 (a fixture)
 from tests.test_gpu_window import normal
 
 pytestmark = pytest.mark.gpu
