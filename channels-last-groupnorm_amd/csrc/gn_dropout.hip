@@ -8,7 +8,7 @@
 //
 // Memory bounds it as long as the generator hides behind it: 7 rounds of two 64-bit products are about 50 cycles of a SIMD
 // for each of a lane's 8 elements of 16 bits, where 32 bits an element and 10 rounds would take three times as much.  float16 (65536,
-// 2560): 111 to 115 us, 5.8 TB/s (a copy of that size 5.1); bfloat16 (16384, 1280) with a residual 19 us; float32 (5883, 1001) 15.8.
+// 2560): 111 us, 6.0 TB/s (a copy of that size 5.1); bfloat16 (16384, 1280) with a residual 19 us; float32 (5883, 1001) 6.3.
 #include <math.h>
 #include <stdint.h>
 #include "gn_rms.h"
@@ -45,68 +45,74 @@ __device__ __forceinline__ u32x4 random_words(uint64_t counter, uint64_t offset,
 }
 __device__ __forceinline__ bool kept(const u32x4 &w, int i, uint32_t least) { return (i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu) >= least; }
 
-// Groups that a lane has on their way at once.
-template <typename T> constexpr int kAtOnce = sizeof(T) == 2 ? 4 : sizeof(T) == 4 ? 2 : 1;
+// The value of the lane beside this one: 0 and 1, 2 and 3, ...
+__device__ __forceinline__ uint32_t neighbours(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true); }
 
+// One group a lane: more of them on their way at once are slower (float16 (65536, 2560) 111 us, by four 117; float32 (5883, 1001) 6.3, by two
+// 8.1, by four 11).
 template <typename T, bool RES> __global__ __launch_bounds__(kBlock) void dropout_kernel(const DropoutArgs a) {
   using A = acc_of_t<T>;
-  constexpr int VEC = vec_of<T>::value, PARTS = kGroup / VEC, N = kAtOnce<T>;
+  constexpr int VEC = vec_of<T>::value, PARTS = kGroup / VEC;
   using LV = LaneVec<T, VEC>;
   const T *x = (const T *)a.x, *res = (const T *)a.residual;
   T *y = (T *)a.y;
   const uint64_t seed = a.seed_at ? (uint64_t)load_global<int64_t>(a.seed_at) : a.seed;
   const A scale = (A)a.scale;
-  const int64_t first = (int64_t)blockIdx.x * (kBlock * N) + threadIdx.x;
-  if ((int64_t)(blockIdx.x + 1) * (kBlock * N * kGroup) <= a.n) {
-    typename LV::raw_t rx[N][PARTS], rr[RES ? N : 1][RES ? PARTS : 1];
+  const int64_t group = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if ((int64_t)(blockIdx.x + 1) * (kBlock * kGroup) <= a.n) {
+    // Part v of a lane's elements, and the two halves of a word each that decide on them.  float32: a group's 32 bytes are two lanes',
+    // so that a wavefront reads and writes whole lines.  Of its 64 groups two neighbours make the bits of one of the first half and
+    // one of the second, and hand each other what the other's elements need.  (float32 (65536, 1280) 183 us by 32 bytes a lane,
+    // 110 so)
+    constexpr bool kPairs = sizeof(T) == 4;
+    const int lane = threadIdx.x & 63, odd = lane & 1;
+    const int64_t base = group - lane;
+    auto place = [&](int v) { return kPairs ? (base + v * 32) * kGroup + lane * 4 : group * kGroup + v * VEC; };
+    typename LV::raw_t rx[PARTS], rr[RES ? PARTS : 1];
 #pragma unroll
-    for (int k = 0; k < N; ++k)
+    for (int v = 0; v < PARTS; ++v) {
+      rx[v] = load_loose<LV>(x + place(v));
+      if constexpr (RES) rr[v] = load_loose<LV>(res + place(v));
+    }
+    u32x4 w = random_words((uint64_t)(kPairs ? base + odd * 32 + lane / 2 : group), a.offset, seed);
+    if constexpr (kPairs) {  // into the order of this lane's elements
+      const uint32_t own0 = odd ? w[2] : w[0], own1 = odd ? w[3] : w[1];
+      const uint32_t others0 = neighbours(odd ? w[0] : w[2]), others1 = neighbours(odd ? w[1] : w[3]);
+      w = u32x4{odd ? others0 : own0, odd ? others1 : own1, odd ? own0 : others0, odd ? own1 : others1};
+    }
 #pragma unroll
-      for (int v = 0; v < PARTS; ++v) {
-        const int64_t e = (first + k * kBlock) * kGroup + v * VEC;
-        rx[k][v] = load_loose<LV>(x + e);
-        if constexpr (RES) rr[k][v] = load_loose<LV>(res + e);
+    for (int v = 0; v < PARTS; ++v) {
+      A f[VEC], r[VEC];
+      LV::unpack(rx[v], f);
+      if constexpr (RES) LV::unpack(rr[v], r);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const bool keep = kept(w, v * VEC + i, a.least);
+        if constexpr (RES) f[i] = keep ? __builtin_elementwise_fma(f[i], scale, r[i]) : r[i];
+        else f[i] = keep ? f[i] * scale : (A)0;
       }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int64_t g = first + k * kBlock;
-      const u32x4 w = random_words((uint64_t)g, a.offset, seed);
-#pragma unroll
-      for (int v = 0; v < PARTS; ++v) {
-        A f[VEC], r[VEC];
-        LV::unpack(rx[k][v], f);
-        if constexpr (RES) LV::unpack(rr[k][v], r);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const bool keep = kept(w, v * VEC + i, a.least);
-          if constexpr (RES) f[i] = keep ? __builtin_elementwise_fma(f[i], scale, r[i]) : r[i];
-          else f[i] = keep ? f[i] * scale : (A)0;
-        }
-        store_loose<LV>(y + g * kGroup + v * VEC, LV::pack(f));
-      }
+      store_loose<LV>(y + place(v), LV::pack(f));
     }
     return;
   }
-  for (int k = 0; k < N; ++k) {
-    const int64_t g = first + k * kBlock, e0 = g * kGroup;
-    if (e0 >= a.n) break;
-    const u32x4 w = random_words((uint64_t)g, a.offset, seed);
+  const int64_t e0 = group * kGroup;
+  if (e0 >= a.n) return;
+  const u32x4 w = random_words((uint64_t)group, a.offset, seed);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-      if (e0 + i >= a.n) break;
-      using L1 = LaneVec<T, 1>;
-      A f[1], r[1] = {0};
-      L1::unpack(L1::load(x + e0 + i), f);
-      if constexpr (RES) L1::unpack(L1::load(res + e0 + i), r);
-      if constexpr (RES) f[0] = kept(w, i, a.least) ? __builtin_elementwise_fma(f[0], scale, r[0]) : r[0];
-      else f[0] = kept(w, i, a.least) ? f[0] * scale : (A)0;
-      L1::store(y + e0 + i, L1::pack(f));
-    }
+  for (int i = 0; i < kGroup; ++i) {
+    if (e0 + i >= a.n) break;
+    using L1 = LaneVec<T, 1>;
+    A f[1], r[1] = {0};
+    L1::unpack(L1::load(x + e0 + i), f);
+    if constexpr (RES) L1::unpack(L1::load(res + e0 + i), r);
+    if constexpr (RES) f[0] = kept(w, i, a.least) ? __builtin_elementwise_fma(f[0], scale, r[0]) : r[0];
+    else f[0] = kept(w, i, a.least) ? f[0] * scale : (A)0;
+    L1::store(y + e0 + i, L1::pack(f));
   }
 }
 
 template <typename T> void launch_dropout(DropoutArgs a, hipStream_t stream) {
-  constexpr int64_t per_block = (int64_t)kBlock * kAtOnce<T> * kGroup;
+  constexpr int64_t per_block = (int64_t)kBlock * kGroup;
   const dim3 grid((unsigned)((a.n + per_block - 1) / per_block));
   if (a.residual) hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(kBlock), 0, stream, a);
   else hipLaunchKernelGGL((dropout_kernel<T, false>), grid, dim3(kBlock), 0, stream, a);
