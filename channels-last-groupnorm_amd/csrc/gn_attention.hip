@@ -68,13 +68,17 @@ struct WindowPlan {
 // Workgroups that share the work of each of `items`, of `steps` steps: a CU takes `thick` of them at once in the time of one, each
 // has some steps' time of its own, and what they leave has to be joined.  (training of 1500 tokens, 8 heads over 2 of 128, causal, in
 // bfloat16: 99 us, unshared 294; of a padded float32 batch, 3 x 1961, 6 over 2 of 40: 250 and 500)
-int64_t shares_of(int64_t items, int64_t steps, int64_t thick, int64_t most) {
+// mean: steps of an item on average; where they are uneven, the CUs are as good as evenly loaded, but the longest item has to end, too.
+// (float32, 4 x 800 tokens, 8 heads over 2 of 96, causal: forward 94 us unshared, 78 by two; dk and dv 383 by four, 313 by eight)
+int64_t shares_of(int64_t items, int64_t steps, int64_t mean, int64_t thick, int64_t most) {
   if (items == 0) return 1;
   // (in steps of which a CU takes `thick` at once: 1.7 us for float32, 0.5 for 16 bits, where the second launch is 4 us and a share's
   // rows, written and read, 13 ns)
   const int64_t join = thick == 1 ? 3 : 8, rows = thick == 1 ? 128 : 32, overhead = thick == 1 ? 1 : 3;
   auto cost = [&](int64_t s) {
-    return std::max(ceil_div(items * s, kNumCU), thick) * (ceil_div(steps, s) + overhead) + (s > 1 ? join + items * s / rows : 0);
+    const int64_t joined = s > 1 ? join + items * s / rows : 0;
+    if (mean < steps) return std::max(items * (mean + overhead * s) / kNumCU, thick * (ceil_div(steps, s) + overhead)) + joined;
+    return std::max(ceil_div(items * s, kNumCU), thick) * (ceil_div(steps, s) + overhead) + joined;
   };
   int64_t best = 1;
   for (int64_t s = 2; s <= most && s <= steps / 2; ++s)
@@ -145,6 +149,9 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   const int64_t thick = es == 4 ? 1 : width <= 64 ? 3 : width <= 128 ? 2 : 1;
   const int64_t reach = (int64_t)a.left + a.right + kQueries;
   const int64_t keys = ceil_div(std::min<int64_t>(a.S, reach + a.sinks), step), queries = ceil_div(std::min<int64_t>(a.L, reach), step) * a.group;
+  // of a causal walk the first tiles see less: the mean over p of min(p, n) keys, n being the most that one sees
+  const int64_t seen = std::min<int64_t>(a.S, reach), lacking = a.causal ? seen * seen / (2 * std::max<int64_t>(1, a.S)) : 0;
+  const int64_t mean_keys = a.L < a.S ? keys : std::max<int64_t>(1, keys - lacking / step);
   p.bytes = 256;
   if (!backward) {
     const int64_t few_rows = (int64_t)a.L * a.group;
@@ -176,7 +183,7 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
         if (cost(s) < cost(a.splits)) a.splits = (int)s;
       a.items = (int)(heads * a.splits);
     } else {
-      a.splits = (int)shares_of(items, keys, thick, 16);
+      a.splits = (int)shares_of(items, keys, mean_keys, thick, 16);
       a.items = (int)(items * a.splits);
     }
     put_order(a);
@@ -188,14 +195,16 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   }
   p.kv = p.sinks = a;
   if (items) {
-    a.splits = (int)shares_of(items, keys, thick, 16);
+    a.splits = (int)shares_of(items, keys, mean_keys, thick, 16);
     a.items = (int)(items * a.splits);
   }
   put_order(a);
   WindowArgs &w = p.kv, &k = p.sinks;
   w.tiles = (int)ceil_div(a.S, kQueries);
   const int64_t heads = (int64_t)a.B * a.K, tiles = heads * w.tiles;
-  w.shares = (int)shares_of(tiles, queries, es == 4 ? 1 : width <= 64 ? 2 : 1, 32);
+  // (of 16 bits, where the joins weigh more, by the longest alone: 4500 tokens, 16 heads over 4 of 128, 679 us so, 711 by the mean)
+  const int64_t mean_queries = es == 2 || a.L < a.S ? queries : std::max<int64_t>(1, queries - lacking / step * a.group);
+  w.shares = (int)shares_of(tiles, queries, mean_queries, es == 4 ? 1 : width <= 64 ? 2 : 1, 32);
   if (tiles * w.shares > kMostItems) return invalid("too many tokens and heads for one call");
   w.items = (int)(tiles * w.shares);
   k.items = w.sink_sets = w.sink_parts = 0;
