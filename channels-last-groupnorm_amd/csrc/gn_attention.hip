@@ -12,7 +12,7 @@ namespace {
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;
 constexpr int64_t kFineKeys = 64;  // (where 64 are seen, 1.44 without)
-constexpr int64_t kMostItems = ((int64_t)1 << 24) - 64;  // workgroups: a launch has fewer than 2^32 threads
+constexpr int64_t kMostItems = ((int64_t)1 << 23) - 64;  // workgroups of up to 512 threads: a launch has fewer than 2^32
 
 int invalid(const char *what) { return fail(GNNHWC_ERR_INVALID_ARGUMENT, "%s", what); }
 int launched(hipError_t e, const char *what) {
@@ -214,7 +214,8 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
     const int64_t sets = heads * w.sink_sets, steps = ceil_div(a.L, 32) * a.group;
     // as many workgroups as there are CUs, down to one step a wavefront (float32, 6 sets of 186 steps: 11 shares 28.7 us, 43 16.3)
     const int64_t sink_shares = std::clamp<int64_t>(kNumCU / std::max<int64_t>(1, sets), 1, std::max<int64_t>(1, steps / waves));
-    if (sets * sink_shares > kMostItems) return invalid("too many tokens and heads for one call");
+    // (rows are added up by 256 threads or fewer each)
+    if (sets * sink_shares > kMostItems || heads * w.sinks / std::max(1, 64 / a.D) > 2 * kMostItems) return invalid("too many tokens and heads for one call");
     w.sink_parts = (int)sink_shares;
     k = w;
     k.items = (int)(sets * sink_shares);

@@ -1014,7 +1014,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
   const Joiner at(joining);
   const int r = at.row, d = at.d, rows_here = at.rows_here;
   const int64_t rows = (int64_t)a.B * a.H * a.L;
-  const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^24 workgroups)
+  const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^23 workgroups)
   const bool there = r < rows_here && id < rows;
   bad[threadIdx.x] = 0;
   if (threadIdx.x == 0) any_bad = 0;
@@ -1221,7 +1221,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_ke
   const Joiner at(joining);
   const int r = at.row, rows_here = at.rows_here;
   const int64_t rows = (int64_t)a.B * a.H * a.L;
-  const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^24 workgroups)
+  const int id = (int)blockIdx.x * rows_here + r;  // (fewer than 2^31: 128 of each of 2^23 workgroups)
   const bool there = r < rows_here && id < rows;
   bad[threadIdx.x] = 0;
   if (threadIdx.x == 0) any_bad = 0;

@@ -55,7 +55,7 @@ REFUSED = [(dict(dtype=F64), "dtype"), (dict(dtype=7), "dtype"), (dict(head_dim=
            (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(scale=1e-60), "scale"),
            (dict(length_type=2), "length_type"), (dict(q=None), "q is null"), (dict(v=None), "v is null"), (dict(k="odd"), "aligned"), (dict(out="odd"), "aligned"),
            (dict(q_stride=[4096, 257, 64]), "16 bytes"), (dict(k_stride=[4096, 2 ** 30, 64]), "2\\^25"), (dict(v_stride=[4096, -256, 64]), "stride"),
-           (dict(batch=2 ** 20, heads=64, kv_heads=64), "too many")]
+           (dict(batch=2 ** 20, heads=64, kv_heads=64), "too many"), (dict(batch=2 ** 18, heads=32, kv_heads=32), "too many"), (dict(out_rest="odd"), "out_rest")]
 
 
 @pytest.mark.parametrize("change,text", REFUSED)
@@ -78,6 +78,9 @@ def test_workspaces_and_backward_refuse():
     for change, text in ((dict(at_end=1), "cache"), (dict(lse=None), "lse"), (dict(out_grad=None), "out_grad"), (dict(k_grad="odd"), "aligned")):
         c, _keep = _call(**change)
         assert lib.gnnhwc_window_bwd(ctypes.byref(c), ws, 1 << 40, None) == -1 and text in _cabi.last_error()
+    c, _keep = _call(batch=2 ** 12, heads=64, kv_heads=64, keys=200, window=3, sinks=100)
+    assert lib.gnnhwc_window_workspace_bytes(ctypes.byref(c)) > 0
+    assert lib.gnnhwc_window_bwd(ctypes.byref(c), ws, 1 << 60, None) == -1 and "too many" in _cabi.last_error()
     # a batch of nothing launches nothing
     c, _keep = _call(batch=0)
     assert lib.gnnhwc_window(ctypes.byref(c), ws, 1 << 20, None) == 0 and lib.gnnhwc_window_bwd(ctypes.byref(c), ws, 1 << 40, None) == 0
