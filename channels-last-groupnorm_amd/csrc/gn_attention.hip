@@ -152,7 +152,7 @@ int plan_window(const gnnhwc_window_call *c, bool backward, WindowPlan &p) {
   // of a causal walk the first tiles see less: the mean over p of min(p, n) keys, n being the most that one sees
   const int64_t seen = std::min<int64_t>(a.S, reach), lacking = a.causal ? seen * seen / (2 * std::max<int64_t>(1, a.S)) : 0;
   const int64_t mean_keys = a.L < a.S ? keys : std::max<int64_t>(1, keys - lacking / step);
-  p.bytes = 256;
+  p.bytes = GNNHWC_WINDOW_NO_WORKSPACE;
   if (!backward) {
     const int64_t few_rows = (int64_t)a.L * a.group;
     // The kernel for few queries has tiles of 32 rows, all of a workgroup's wavefronts share a tile's keys, and its queries are
@@ -251,7 +251,7 @@ size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *c) {
 int gnnhwc_window(const gnnhwc_window_call *c, void *workspace, size_t workspace_bytes, void *stream) {
   WindowPlan p;
   if (const int rc = plan_window(c, false, p)) return rc;
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes)
+  if (p.bytes > GNNHWC_WINDOW_NO_WORKSPACE && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes))
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_workspace_bytes");
   if (p.empty) return GNNHWC_OK;
   p.a.part_k = (float *)workspace;

@@ -573,53 +573,66 @@ bool window_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor
   c.dtype = code;
   return true;
 }
-// lse and rest are what the backward reads besides; both or neither, but float32 has no rest (a tensor without elements).
-void run_window(const Tensor &q, gnnhwc_window_call &c, Tensor &out, Tensor *lse, Tensor *rest) {
+// What the backward reads beside the forward's tensors, in one allocation: lse, then, in 16 bits, what rounding left of out.
+struct WindowKept {
+  int64_t lse_bytes, bytes;
+  explicit WindowKept(const Tensor &q) {
+    lse_bytes = (q.size(0) * q.size(1) * q.size(2) * 4 + 15) / 16 * 16;
+    bytes = lse_bytes + (q.scalar_type() == at::kFloat ? 0 : q.numel() * 2);
+  }
+  void put(const Tensor &kept, gnnhwc_window_call &c) const {
+    c.lse = (float *)kept.data_ptr();
+    c.out_rest = bytes > lse_bytes ? (char *)kept.data_ptr() + lse_bytes : nullptr;
+  }
+};
+void run_window(const Tensor &q, gnnhwc_window_call &c, Tensor &out, Tensor *kept) {
   const c10::DeviceGuard guard(q.device());
   const at::AutoDispatchBelowADInplaceOrView below;
   const OperatorRange range("gnop::window_attention");
   out = fresh(q.sizes(), q.scalar_type(), q);
   c.out = out.data_ptr();
   put_strides(out, c.out_stride);
-  if (lse) {
-    *lse = fresh({q.size(0), q.size(2), q.size(1)}, at::kFloat, q);
-    c.lse = (float *)lse->data_ptr();
-    const bool has_rest = q.scalar_type() != at::kFloat;
-    *rest = has_rest ? fresh(q.sizes(), q.scalar_type(), q) : fresh({0}, q.scalar_type(), q);
-    c.out_rest = has_rest ? rest->data_ptr() : nullptr;
+  if (kept) {
+    const WindowKept parts(q);
+    *kept = fresh({parts.bytes}, at::kByte, q);
+    parts.put(*kept, c);
   }
   const size_t bytes = abi.window_workspace_bytes(&c);
-  const Tensor ws = workspace(bytes, q, "gnop::window_attention");
-  check(abi.window(&c, ws.data_ptr(), bytes, stream_of(q)), "gnop::window_attention");
+  Tensor ws;
+  if (bytes != GNNHWC_WINDOW_NO_WORKSPACE) ws = workspace(bytes, q, "gnop::window_attention");
+  check(abi.window(&c, ptr(ws), bytes, stream_of(q)), "gnop::window_attention");
 }
 
 struct WindowNode : public torch::autograd::Function<WindowNode> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v,
                                                 const optional<Tensor> &lengths, gnnhwc_window_call *c) {
-    Tensor out, lse, rest;
-    run_window(q, *c, out, &lse, &rest);
-    ctx->save_for_backward({q, k, v, out, lse, rest, defined(lengths)});
-    ctx->saved_data["window"] = c->window;
-    ctx->saved_data["sinks"] = c->sinks;
-    ctx->saved_data["causal"] = (bool)c->causal;
+    Tensor out, kept;
+    run_window(q, *c, out, &kept);
+    ctx->save_for_backward({q, k, v, out, kept, defined(lengths)});
+    ctx->saved_data["call"] = std::vector<int64_t>{c->window, c->sinks, c->causal};
     ctx->saved_data["scale"] = c->scale;
     return {out};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor q = saved[0], k = saved[1], v = saved[2], out = saved[3], lse = saved[4], rest = saved[5], lengths = saved[6], dout = grads[0];
+    const Tensor q = saved[0], k = saved[1], v = saved[2], out = saved[3], kept = saved[4], lengths = saved[5], dout = grads[0];
     const c10::Device device = dout.device();
     gnnhwc_window_call c = {};
-    c.window = ctx->saved_data["window"].toInt();
-    c.sinks = ctx->saved_data["sinks"].toInt();
-    c.causal = ctx->saved_data["causal"].toBool();
+    const auto numbers = ctx->saved_data["call"].toIntVector();
+    c.window = numbers[0];
+    c.sinks = numbers[1];
+    c.causal = numbers[2];
     c.scale = ctx->saved_data["scale"].toDouble();
+    const WindowKept parts(q);
     Tensor dq, dk, dv;
     // (as for the norm: whatever is not plain goes through the operator)
     if (at::GradMode::is_enabled() || !ordinary_dispatch() || !plain(q, device) || !window_call(q, k, v, lengths, c) ||
         !rows16(dout, device, q.scalar_type()) || dout.sizes() != q.sizes() || !rows16(out, device, q.scalar_type()) || out.sizes() != q.sizes() ||
-        !plain(lse, device) || !lse.is_contiguous() || lse.scalar_type() != at::kFloat || lse.numel() != q.size(0) * q.size(1) * q.size(2) ||
-        (rest.numel() && (!rows16(rest, device, q.scalar_type()) || rest.sizes() != q.sizes() || !rest.is_contiguous()))) {
+        !plain(kept, device) || !kept.is_contiguous() || kept.scalar_type() != at::kByte || kept.numel() != parts.bytes || (uintptr_t)kept.data_ptr() % 16) {
+      TORCH_CHECK(kept.dim() == 1 && kept.numel() == parts.bytes && kept.scalar_type() == at::kByte, "window_attention: a saved tensor came back as another");
+      const Tensor lse = kept.narrow(0, 0, q.size(0) * q.size(1) * q.size(2) * 4).view(at::kFloat).view({q.size(0), q.size(2), q.size(1)});
+      const Tensor rest = parts.bytes > parts.lse_bytes ? kept.narrow(0, parts.lse_bytes, q.numel() * 2).view(q.scalar_type()).view(q.sizes())
+                                                        : at::empty({0}, q.options());
       using Signature = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
                                                            const Tensor &, const optional<Tensor> &, int64_t, int64_t, bool, double);
       const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnop::window_attention_bwd", "").typed<Signature>();
@@ -632,8 +645,7 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
       dk = fresh(k.sizes(), k.scalar_type(), k);
       dv = fresh(v.sizes(), v.scalar_type(), v);
       c.out = out.data_ptr();
-      c.lse = (float *)lse.data_ptr();
-      c.out_rest = rest.numel() ? rest.data_ptr() : nullptr;
+      parts.put(kept, c);
       c.out_grad = dout.data_ptr();
       c.q_grad = dq.data_ptr();
       c.k_grad = dk.data_ptr();
@@ -691,7 +703,7 @@ PyObject *window_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
   {
     const WithoutGil released;
     if (differentiates) out = WindowNode::apply(q, k, v, lengths_, &c)[0];
-    else run_window(q, c, out, nullptr, nullptr);
+    else run_window(q, c, out, nullptr);
   }
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS

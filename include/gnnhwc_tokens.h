@@ -164,6 +164,8 @@ typedef struct gnnhwc_window_call {
   int64_t dtype;
 } gnnhwc_window_call;
 
+/* What gnnhwc_window_workspace_bytes returns for a call that needs none: its workspace may be NULL. */
+#define GNNHWC_WINDOW_NO_WORKSPACE ((size_t)256)
 size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *call);
 int gnnhwc_window(const gnnhwc_window_call *call, void *workspace, size_t workspace_bytes, void *stream);
 size_t gnnhwc_window_bwd_workspace_bytes(const gnnhwc_window_call *call);
