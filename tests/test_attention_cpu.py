@@ -71,7 +71,12 @@ def test_attention_refuses(change, text):
 
 def test_workspaces_and_backward_refuse():
     c, _keep = _call()
-    assert lib.gnnhwc_window(ctypes.byref(c), None, 1 << 20, None) == -2 and "workspace" in _cabi.last_error()
+    assert lib.gnnhwc_window_workspace_bytes(ctypes.byref(c)) == 256  # one workgroup a head: none is needed
+    c, _keep = _call(batch=1, keys=5000, window=-1)  # several share a head's keys
+    assert lib.gnnhwc_window_workspace_bytes(ctypes.byref(c)) > 256
+    assert lib.gnnhwc_window(ctypes.byref(c), None, 1 << 40, None) == -2 and "workspace" in _cabi.last_error()
+    assert lib.gnnhwc_window(ctypes.byref(c), _block()[1], 256, None) == -2
+    c, _keep = _call()
     small = lib.gnnhwc_window_bwd_workspace_bytes(ctypes.byref(c))
     _raw, ws = _block()
     assert small > 0 and lib.gnnhwc_window_bwd(ctypes.byref(c), ws, small - 1, None) == -2 and lib.gnnhwc_window_bwd(ctypes.byref(c), ws + 8, 1 << 40, None) == -2
