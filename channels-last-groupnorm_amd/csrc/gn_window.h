@@ -733,7 +733,7 @@ __device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int 
 // 4096, 20 heads of 64: 810; with window 512, where a tenth of the pairs of its tiles is hidden, 675.  FINE: a.fine, as a
 // kernel of its own (float16 heads of 64 have no registers left for both in one, and few queries are 3 % slower with both).
 template <typename T, int DP, bool FINE>
-__global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : DP <= 64 && !FINE ? 4 : DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? 2 : DP <= 64 && !FINE ? 4 : DP <= 128 ? 2 : 1) void window_forward_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a);
@@ -1074,7 +1074,7 @@ template <typename T> __device__ __forceinline__ float gradient_unit(float most)
 // A workgroup: 128 queries of one head against a share of the keys that they see, like the forward, with q and do in registers and
 // three products a pair.  bfloat16, 4 x 4112 tokens, 20 heads of 64, window 512: 163 to 175 us, 121 GFLOP of the formula's at 0.7 PFLOP/s;
 // without its copies 5 % less, without the exponentials a tenth, without the products a fifth: no one unit bounds it.
-template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= 128 && sizeof(T) == 2 ? 2 : 1) void window_dq_kernel(const WindowArgs a) {
+template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof(T) == 2 ? 128 : 96) ? 2 : 1) void window_dq_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // keys and values, two deep
   const int item = work_item(a);
