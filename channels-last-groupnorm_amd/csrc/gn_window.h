@@ -1423,7 +1423,7 @@ __device__ __forceinline__ int64_t tile_slot(const WindowArgs &a, int bk, int ti
 // ahead of their products instead.  bfloat16, 4 x 4112 tokens, 20 heads of 64, window 512: 197 to 212 us, 0.8 PFLOP/s; 2 x 4096, 24 over 8
 // of 128, causal, window 1024: 238 to 258.
 template <typename T, int DP, int PARTS>
-__global__ __launch_bounds__(kBlock, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void window_dkv_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(kBlock, (DP <= 64 && sizeof(T) == 2) || (sizeof(T) == 4 && PARTS == 1) ? 2 : 1) void window_dkv_kernel(const WindowArgs a) {
   using G = Tile<T, DP>;
   using KS = KeySide<T, DP, PARTS>;
   __shared__ __attribute__((aligned(16))) char tiles[4 * G::kBytes];  // queries and gradients, two deep
