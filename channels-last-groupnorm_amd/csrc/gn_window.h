@@ -596,6 +596,11 @@ __device__ __forceinline__ void store_rows(char *place, const f32x16_t (&acc)[DP
 }
 // Rows are written again, by other lanes: what they hold has to be there before.
 __device__ __forceinline__ void rows_written() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The same for rows that any wavefront has written.
+__device__ __forceinline__ void rows_of_all_written() {
+  rows_written();
+  __syncthreads();
+}
 // A token that sees nothing, or that nobody sees, gets zeros, whatever its tile held: its weights are 0, and 0 times NaN is NaN.
 template <int N> __device__ __forceinline__ void clear_unless(bool kept, f32x16_t (&acc)[N]) {
 #pragma unroll
@@ -960,7 +965,8 @@ template <typename T, int DP, bool FINE> __global__ __launch_bounds__((64 * Few<
   const bool ours = lane < 32 && row < rows;
   if (z.lse && wave == 0 && ours)
     store_global<float>(z.lse + ((int64_t)b * z.H + h) * z.L + i, sums[0][lane] > 0.0f ? references[0][lane] + __builtin_amdgcn_logf(sums[0][lane]) : INFINITY);
-  uint64_t again = __ballot(ours && bad[lane & 31] && (st.sight.count > 0 || st.sight.sinks > 0));
+  uint64_t again = __ballot(ours && bad[lane & 31] && (st.sight.count > 0 || st.sight.sinks > 0));  // (the same in all wavefronts)
+  if (again) rows_of_all_written();
   while (again) {
     const int r = __builtin_ctzll(again);
     again &= again - 1;
@@ -1050,6 +1056,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kern
   }
   __syncthreads();
   if (!any_bad) return;
+  rows_of_all_written();
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!bad[n]) continue;
     const WindowArgs &z = arguments_again();
@@ -1206,6 +1213,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof
     store_token<T, DP>((T *)z.dq.row(b, i, h), z.D, acc, factor);
   }
   uint64_t rows = __ballot(again) & 0xffffffffu;
+  if (rows) rows_written();
   while (rows) {
     const int r = __builtin_ctzll(rows);
     rows &= rows - 1;
@@ -1241,6 +1249,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_ke
   }
   __syncthreads();
   if (!any_bad) return;
+  rows_of_all_written();
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!bad[n]) continue;
     const WindowArgs &z = arguments_again();
@@ -1523,6 +1532,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 && sizeof(T) == 2) || (sizeof(T) 
   if constexpr (KS::kDk) bad[1] = any_not_finite(key.dk);
   for (int of_k = 0; of_k < 2; ++of_k) {
     uint64_t rows = __ballot(either_half(of_k ? bad[1] : bad[0]) && key.seen.count > 0) & 0xffffffffu;
+    if (rows) rows_written();
     while (rows) {
       const int r = __builtin_ctzll(rows);
       rows &= rows - 1;
@@ -1662,6 +1672,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void window_sum_kerne
   }
   __syncthreads();
   if (!any_bad) return;
+  rows_of_all_written();
   for (int n = threadIdx.x >> 6; n < rows_here; n += 4) {
     if (!(bad_k[n] | bad_v[n])) continue;
     const WindowArgs &z = arguments_again();
