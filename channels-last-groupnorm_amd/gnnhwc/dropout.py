@@ -104,7 +104,7 @@ class Dropout(nn.Dropout):
         if torch.compiler.is_compiling() or (x.is_cuda and torch.cuda.is_current_stream_capturing()):
             seed = torch.randint(2 ** 63 - 1, (), dtype=torch.int64, device=x.device)
         else:
-            seed = int(torch.empty((), dtype=torch.int64).random_())
+            seed = int(torch.empty((), dtype=torch.int64, device="cpu").random_())  # (whatever torch's default device is)
         return dropout(x, float(self.p), seed, 0, residual, self.channel_dim)
 
     def extra_repr(self):
