@@ -103,6 +103,15 @@ def _rest_shape(q, want_lse):
     return q.shape if want_lse and q.dtype != torch.float32 else (0,)
 
 
+def _check_kept(q, lse, rest, opname):
+    """What the forward left for the backward, which the kernels read by q's sizes."""
+    B, L, H, _ = q.shape
+    if tuple(lse.shape) != (B, H, L) or lse.dtype != torch.float32 or lse.device != q.device:
+        raise RuntimeError("%s: lse must be float32 of shape %s on %s, as the forward leaves it with want_lse" % (opname, (B, H, L), q.device))
+    if rest.numel() and (rest.shape != q.shape or rest.dtype != q.dtype or rest.device != q.device):
+        raise RuntimeError("%s: rest must be like q, or empty" % opname)
+
+
 def _window_attention_bwd(dout, q, k, v, out, lse, rest, lengths, window, sinks, causal, scale):
     """gnop::window_attention_bwd.  Returns (dq, dk, dv)."""
     opname = "gnop::window_attention_bwd"
@@ -111,8 +120,7 @@ def _window_attention_bwd(dout, q, k, v, out, lse, rest, lengths, window, sinks,
         _check_device(t, name)
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
             raise RuntimeError("%s: %s must be like q" % (opname, name))
-    if rest.numel() and (rest.shape != q.shape or rest.dtype != q.dtype or rest.device != q.device):
-        raise RuntimeError("%s: rest must be like q, or empty" % opname)
+    _check_kept(q, lse, rest, opname)
     keep = []
     c = _call(q, k, v, lengths, window, sinks, causal, False, scale, keep)
     dout, out, lse = _aligned(dout), _aligned(out), lse.contiguous()
