@@ -251,7 +251,7 @@ size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *c) {
 int gnnhwc_window(const gnnhwc_window_call *c, void *workspace, size_t workspace_bytes, void *stream) {
   WindowPlan p;
   if (const int rc = plan_window(c, false, p)) return rc;
-  if (p.bytes > GNNHWC_WINDOW_NO_WORKSPACE && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes))
+  if (p.bytes > GNNHWC_WINDOW_NO_WORKSPACE && (!workspace || (uintptr_t)workspace % GNNHWC_WINDOW_WORKSPACE_ALIGNMENT || workspace_bytes < p.bytes))
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_workspace_bytes");
   if (p.empty) return GNNHWC_OK;
   p.a.part_k = (float *)workspace;
@@ -270,7 +270,7 @@ size_t gnnhwc_window_bwd_workspace_bytes(const gnnhwc_window_call *c) {
 int gnnhwc_window_bwd(const gnnhwc_window_call *c, void *workspace, size_t workspace_bytes, void *stream) {
   WindowPlan p;
   if (const int rc = plan_window(c, true, p)) return rc;
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes)
+  if (!workspace || (uintptr_t)workspace % GNNHWC_WINDOW_WORKSPACE_ALIGNMENT || workspace_bytes < p.bytes)
     return fail(GNNHWC_ERR_WORKSPACE, "workspace null, misaligned or smaller than gnnhwc_window_bwd_workspace_bytes");
   for (WindowArgs *a : {&p.a, &p.kv, &p.sinks}) {
     a->delta = (float *)((char *)workspace + p.delta);

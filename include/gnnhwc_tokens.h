@@ -12,10 +12,11 @@
  *   gnnhwc_dropout     dropout from a counter-based generator, with the residual's addition
  *
  * Conventions are those of gnnhwc.h: device pointers on the current device, asynchronous on `stream`, no synchronisation, no
- * allocation, a caller-provided workspace whose contents on entry are ignored (8-byte aligned is enough here), GNNHWC_OK or
- * a negative code with the message in gnnhwc_last_error(), and nothing launched when an error is returned.  All of them may
- * be captured into a HIP graph; all results are reproducible bit for bit.  These operators keep no state between calls.
- * Tensors need the alignment of their element only.  Outputs must not overlap inputs unless stated.
+ * allocation, a caller-provided workspace whose contents on entry are ignored (8-byte aligned is enough here, but for the attention's:
+ * GNNHWC_WINDOW_WORKSPACE_ALIGNMENT), GNNHWC_OK or a negative code with the message in gnnhwc_last_error(), and nothing launched when
+ * an error is returned.  All of them may be captured into a HIP graph; all results are reproducible bit for bit.  These operators
+ * keep no state between calls.  Tensors need the alignment of their element only (the attention's: see there).  Outputs must not
+ * overlap inputs unless stated.
  */
 #ifndef GNNHWC_TOKENS_H
 #define GNNHWC_TOKENS_H
@@ -164,8 +165,10 @@ typedef struct gnnhwc_window_call {
   int64_t dtype;
 } gnnhwc_window_call;
 
-/* What gnnhwc_window_workspace_bytes returns for a call that needs none: its workspace may be NULL. */
+/* What gnnhwc_window_workspace_bytes returns for a call that needs none: its workspace may be NULL.  (The backward's may not.) */
 #define GNNHWC_WINDOW_NO_WORKSPACE ((size_t)256)
+/* What the address of these functions' workspace is a whole multiple of (it holds rows that are read 16 bytes at a time). */
+#define GNNHWC_WINDOW_WORKSPACE_ALIGNMENT ((size_t)16)
 size_t gnnhwc_window_workspace_bytes(const gnnhwc_window_call *call);
 int gnnhwc_window(const gnnhwc_window_call *call, void *workspace, size_t workspace_bytes, void *stream);
 size_t gnnhwc_window_bwd_workspace_bytes(const gnnhwc_window_call *call);
