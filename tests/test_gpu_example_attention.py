@@ -97,3 +97,10 @@ def test_a_block_and_its_gradients_against_formulas(p, device):
     want = torch.autograd.grad([y64, r64], [h64, *wide.parameters()], [dy.double(), dr.double()])
     for name, a, b in zip(["y", "residual", "h"] + [n for n, _ in block.named_parameters()], [y, r, *grads], [y64, r64, *want]):
         assert distance(a, b) < FLOAT32, (name, distance(a, b))
+
+
+@pytest.mark.parametrize("options", [dict(window=20, registers=4), dict(causal=True, dropout=0.1), dict(window=5, registers=1, causal=True, dropout=0.3)])
+def test_the_8_bit_form_stays_near_the_other(options, device):
+    """e4m3 values are off by 2.6 % in the mean; a block's products average over channels, and the residual stream is not quantised."""
+    model, _losses, _norms = example.train(steps=3, size=16, channels=128, blocks=2, images=2, device=device, **options)
+    assert example.compare_served(model, size=16, device=device) < 0.05

@@ -116,3 +116,27 @@ def test_two_threads(device):
     for t in threads:
         t.join()
     assert not faults, faults
+
+
+def test_all_nan_takes_no_search(device):
+    """A row that its own q or k makes NaN is filled.  Searched row by row, each would walk its keys three times, with scalar products, on
+    one wavefront: matrix instructions do 16 times as many products in that time and more, and the walk of finite values is one.  Filling
+    costs one more writing of the rows.  So the bound of 8 times the finite call's time is passed by far where rows are searched."""
+    def once(*tensors):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        q, k, v, dout = tensors
+        torch.cuda.synchronize()
+        start.record()
+        out = window_attention(q, k, v)
+        grads = torch.autograd.grad(out, [q, k, v], dout)
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end), (out, *grads)
+
+    finite = [normal((2, 3000, h, 64), BF16, device, i).requires_grad_(i < 3) for i, h in enumerate((8, 4, 4, 8))]
+    nothing = [torch.full_like(t, math.nan).requires_grad_(i < 3) for i, t in enumerate(finite)]
+    least = min(once(*finite)[0] for _ in range(5))
+    took, results = min((once(*nothing) for _ in range(5)), key=lambda r: r[0])
+    print("finite %.3f ms, NaN %.3f ms" % (least, took), flush=True)
+    assert all(t.isnan().all() for t in results)
+    assert took < 8 * least
