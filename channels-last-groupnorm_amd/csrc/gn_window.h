@@ -355,7 +355,9 @@ __device__ __forceinline__ const WindowArgs &arguments_again() {
 // A tile's products reach over all of its rows: what a token does not see has the weight 0 there, and 0 times an infinity or a NaN
 // of such a token is NaN.  A row that comes out infinite or NaN is therefore computed again over the pairs that see each other
 // alone, by one wavefront, in float32.  Rows that have to be NaN whatever they see (their own q is not finite: so are all scores,
-// and infinite ones differ by NaN) are seen to be at once: a training that has diverged has nothing but those.
+// and infinite ones differ by NaN) are seen to be at once: a training that has diverged has nothing but those.  A walk ends where all
+// that it adds up has become NaN, which nothing behind it changes: float16 gradients of a loss that was scaled too far are NaN as a
+// rule, while q, k and v are finite (4 x 4112 tokens, 20 heads of 64, window 512, all of the gradient NaN: 7 ms, 101 to the end).
 template <typename T> __device__ __forceinline__ float dot(const T *a, const T *b, int D) {
   float s = 0.0f;
 #pragma unroll 4
@@ -372,14 +374,17 @@ __device__ __forceinline__ float wave_sum(float v) {
   for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
   return v;
 }
-// Calls f(j0, j) for the keys that a query sees, 64 at a time: j of this lane, or -1.
+// Calls f(j0, j) for the keys that a query sees, 64 at a time: j of this lane, or -1.  Ends where f returns true.
 template <typename F> __device__ __forceinline__ void for_keys(const Sight &g, F &&f) {
   const int lane = threadIdx.x & 63;
   const int sinks = g.count > 0 && g.low < g.sinks ? g.low : g.sinks;  // (those of the window once)
-  for (int j0 = 0; j0 < sinks; j0 += 64) f(j0, j0 + lane < sinks ? j0 + lane : -1);
-  for (int j0 = g.low; j0 < g.low + g.count; j0 += 64) f(j0, j0 + lane < g.low + g.count ? j0 + lane : -1);
+  for (int j0 = 0; j0 < sinks; j0 += 64)
+    if (f(j0, j0 + lane < sinks ? j0 + lane : -1)) return;
+  for (int j0 = g.low; j0 < g.low + g.count; j0 += 64)
+    if (f(j0, j0 + lane < g.low + g.count ? j0 + lane : -1)) return;
   if (g.count > 0 && g.low + g.count < g.sinks)
-    for (int j0 = g.low + g.count; j0 < g.sinks; j0 += 64) f(j0, j0 + lane < g.sinks ? j0 + lane : -1);
+    for (int j0 = g.low + g.count; j0 < g.sinks; j0 += 64)
+      if (f(j0, j0 + lane < g.sinks ? j0 + lane : -1)) return;
 }
 // Whether a row of D channels holds a NaN, or with `infinite` anything that is not finite; all lanes of a wavefront ask together.
 template <typename T> __device__ __forceinline__ bool holds_nan(const T *p, int D, bool infinite) {
@@ -390,6 +395,16 @@ template <typename T> __device__ __forceinline__ bool holds_nan(const T *p, int 
     bad = bad || (infinite ? !(v * 0.0f == 0.0f) : v != v);
   }
   return __any(bad);
+}
+// A row's sums, channels lane, lane + 64, .. of a lane each; those past the head, which are left alone, are NaN.
+__device__ __forceinline__ void clear_row(float (&acc)[4], int D) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) acc[x] = x * 64 + (int)(threadIdx.x & 63) < D ? 0.0f : __builtin_nanf("");
+}
+// Whether all of them are NaN (a maximum is, if both of its operands are).
+__device__ __forceinline__ bool all_nan(const float (&acc)[4]) {
+  const float most = fmaxf(fmaxf(acc[0], acc[1]), fmaxf(acc[2], acc[3]));
+  return __all(most != most);
 }
 template <typename T> __device__ __forceinline__ void fill_nan(T *p, int D) {
   const float t[1] = {__builtin_nanf("")};
@@ -415,27 +430,30 @@ template <typename T> __device__ void row_again(const WindowArgs &a, const Sampl
   const int lane = threadIdx.x & 63, kh = div_by(h, a.by_group);
   const Sight g = sight_of(a, s, i);
   const T *q = (const T *)a.q.row(b, i, h);
-  if (holds_nan(q, a.D, true)) {
+  float most = -INFINITY;
+  bool nan = holds_nan(q, a.D, true);  // (so is the sum, and all of the row, where a score is NaN or +infinity)
+  if (!nan)
+    for_keys(g, [&](int, int j) {
+      const float v = j >= 0 ? dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2 : -INFINITY;
+      most = fmaxf(most, v);
+      nan = __any(!(v < INFINITY));
+      return nan;
+    });
+  if (nan) {
     fill_nan((T *)a.out.row(b, i, h), a.D);
     if (a.lse && lane == 0) store_global<float>(a.lse + ((int64_t)b * a.H + h) * a.L + i, __builtin_nanf(""));
     return;
   }
-  float most = -INFINITY, nan = 0.0f;
-  for_keys(g, [&](int, int j) {
-    if (j >= 0) {
-      const float v = dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2;
-      most = fmaxf(most, v);
-      nan += v == v ? 0.0f : v;  // (a maximum loses it)
-    }
-  });
   most = wave_max(most);
   most = most == -INFINITY ? 0.0f : most;
-  float sum = nan;
+  float sum = 0.0f;
   for_keys(g, [&](int, int j) {
     if (j >= 0) sum += __builtin_amdgcn_exp2f(dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2 - most);
+    return false;
   });
   sum = wave_sum(sum);
-  float o[4] = {};
+  float o[4];
+  clear_row(o, a.D);
   for_keys(g, [&](int j0, int j) {
     const float p = j >= 0 ? __builtin_amdgcn_exp2f(dot(q, (const T *)a.k.row(b, j, kh), a.D) * a.scale_log2 - most) / sum : 0.0f;
     for (int u = 0; u < 64; ++u) {
@@ -447,6 +465,7 @@ template <typename T> __device__ void row_again(const WindowArgs &a, const Sampl
       for (int x = 0; x < 4; ++x)
         if (x * 64 + lane < a.D) o[x] = __builtin_fmaf(pu, to_float(v + x * 64 + lane), o[x]);
     }
+    return all_nan(o);
   });
 #pragma unroll
   for (int x = 0; x < 4; ++x)
@@ -461,7 +480,8 @@ template <typename T> __device__ void dq_again(const WindowArgs &a, const Sample
   const int lane = threadIdx.x & 63, kh = div_by(h, a.by_group);
   const T *q = (const T *)a.q.row(b, i, h), *g = (const T *)a.dout.row(b, i, h);
   if (lse != lse || delta != delta) return fill_nan((T *)a.dq.row(b, i, h), a.D);
-  float acc[4] = {};
+  float acc[4];
+  clear_row(acc, a.D);
   for_keys(sight_of(a, s, i), [&](int, int j) {
     float ds = 0.0f;
     if (j >= 0) {
@@ -477,6 +497,7 @@ template <typename T> __device__ void dq_again(const WindowArgs &a, const Sample
       for (int x = 0; x < 4; ++x)
         if (x * 64 + lane < a.D) acc[x] = __builtin_fmaf(du, to_float(k + x * 64 + lane), acc[x]);
     }
+    return all_nan(acc);
   });
   T *to = (T *)a.dq.row(b, i, h);
 #pragma unroll
@@ -492,10 +513,12 @@ template <typename T> __device__ void dkv_again(const WindowArgs &a, const Sampl
   const T *k = (const T *)a.k.row(b, j, kh), *v = (const T *)a.v.row(b, j, kh);
   const Seen w = seen_of(a, s, j);
   if (holds_nan(k, a.D, false) || (of_k && holds_nan(v, a.D, false))) return fill_nan((T *)(of_k ? a.dk.row(b, j, kh) : a.dv.row(b, j, kh)), a.D);
-  float acc[4] = {};
-  for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
+  float acc[4];
+  clear_row(acc, a.D);
+  bool nan = false;
+  for (int h = kh * a.group; h < (kh + 1) * a.group && !nan; ++h) {
     const int64_t rows = ((int64_t)b * a.H + h) * a.L;
-    for (int i0 = 0; i0 < w.count; i0 += 64) {
+    for (int i0 = 0; i0 < w.count && !nan; i0 += 64) {
       const int i = i0 + lane < w.count ? w.from + i0 + lane - s.off : -1;
       float t = 0.0f;
       if (i >= 0) {
@@ -511,6 +534,7 @@ template <typename T> __device__ void dkv_again(const WindowArgs &a, const Sampl
         for (int x = 0; x < 4; ++x)
           if (x * 64 + lane < a.D) acc[x] = __builtin_fmaf(tu, to_float(r + x * 64 + lane), acc[x]);
       }
+      nan = all_nan(acc);
     }
   }
   T *to = (T *)(of_k ? a.dk.row(b, j, kh) : a.dv.row(b, j, kh));

@@ -140,3 +140,32 @@ def test_all_nan_takes_no_search(device):
     print("finite %.3f ms, NaN %.3f ms" % (least, took), flush=True)
     assert all(t.isnan().all() for t in results)
     assert took < 8 * least
+
+
+@pytest.mark.parametrize("which", ["gradient", "keys"])
+def test_a_walk_ends_where_all_is_nan(which, device):
+    """A gradient that has overflowed next to finite q, k and v, and a NaN that all queries see: all that walks such a row adds up is NaN
+    after its first 64 tokens, of 4000 here, so that walks that end there read a sixtieth of what whole ones do.  The finite call takes 0.5 ms
+    and a walk to the end of a row 0.3 ms for each of 32 rows that a wavefront has, twice over, 20 ms and more."""
+    q, k, v, dout = (normal((4, 4000, 8, 64), BF16, device, i) for i in range(4))
+    sinks = 1
+    if which == "gradient":
+        dout.fill_(math.nan)
+    else:
+        k[:, 0] = math.nan
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def once():
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        torch.cuda.synchronize()
+        start.record()
+        out = window_attention(*leaves, 1500, sinks)
+        grads = torch.autograd.grad(out, leaves, dout)
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end), (out, *grads)
+
+    took, (out, *grads) = min((once() for _ in range(3)), key=lambda r: r[0])
+    print("%s: %.3f ms" % (which, took), flush=True)
+    assert all(t.isnan().all() for t in grads) and bool(out.isnan().all()) == (which == "keys")
+    assert took < 20
