@@ -1038,7 +1038,9 @@ template <typename V, typename F> __device__ __forceinline__ V joined(const Join
   return v;
 }
 
-template <typename T> __global__ __launch_bounds__(kBlock) void window_join_kernel(const WindowArgs a, const Joining joining) {
+// (Eight workgroups a CU, which leaves 64 registers and 80 scalar ones: with a few more of either 30540 rows of 64 channels, three parts
+// each, take 8.4 us for 7.0.)
+template <typename T> __global__ __launch_bounds__(kBlock, 8) void window_join_kernel(const WindowArgs a, const Joining joining) {
   __shared__ int bad[kBlock], any_bad;
   __shared__ f32x4 place[kBlock];
   const Joiner at(joining);
@@ -1247,7 +1249,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kBlock, DP <= (sizeof
 static_assert(kGradBits == 5.0f, "the factors of 1 / 32 undo it");
 
 // dq of rows whose keys several workgroups shared.
-template <typename T> __global__ __launch_bounds__(kBlock) void window_dq_sum_kernel(const WindowArgs a, const Joining joining) {
+template <typename T> __global__ __launch_bounds__(kBlock, 8) void window_dq_sum_kernel(const WindowArgs a, const Joining joining) {
   __shared__ int bad[kBlock], any_bad;
   __shared__ f32x4 place[kBlock];
   const Joiner at(joining);
