@@ -1,14 +1,16 @@
 // Dropout from a counter-based generator, with the residual's addition behind it (declared in include/gnnhwc_tokens.h): kernel
 // and C ABI.
 //
-//   y[e] = (bits(e) >= t ? x[e] 65536 / (65536 - t) : 0) + r[e],   t = round(65536 p)
+//   y[e] = (bits(e) >= t ? x[e] f : 0) + r[e],   t = round(65536 p),  f = 65536 / (65536 - t), rounded to float32 (float64)
 // bits(e): 16 bits of Philox 4x32 with 7 rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011;
 // their tests find nothing against 7), counter (e / 8, offset), key the seed; element e has half e % 2, the lower first, of word
 // e / 2 % 4.  No mask is stored: the backward is the same call on the gradient, without a residual.
 //
 // Memory bounds it as long as the generator hides behind it: 7 rounds of two 64-bit products are about 50 cycles of a SIMD
 // for each of a lane's 8 elements of 16 bits, where 32 bits an element and 10 rounds would take three times as much.  float16 (65536,
-// 2560): 111 us, 6.0 TB/s (a copy of that size 5.1); bfloat16 (16384, 1280) with a residual 19 us; float32 (5883, 1001) 6.3.
+// 2560): 109 us, 6.1 TB/s (a copy of that size 5.1); bfloat16 (16384, 1280) with a residual 19 us; float32 (5883, 1001) 9.1 in a
+// training pass, 5.8 where x lies in the memory-side cache.  float64 (16384, 1280): 216 us, 1.6 TB/s (a lane's 64 bytes in four accesses
+// that a wavefront has 64 bytes apart).
 #include <math.h>
 #include <stdint.h>
 #include "gn_rms.h"
@@ -48,7 +50,7 @@ __device__ __forceinline__ bool kept(const u32x4 &w, int i, uint32_t least) { re
 // The value of the lane beside this one: 0 and 1, 2 and 3, ...
 __device__ __forceinline__ uint32_t neighbours(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true); }
 
-// One group a lane: more of them on their way at once are slower (float16 (65536, 2560) 111 us, by four 117; float32 (5883, 1001) 6.3, by two
+// One group a lane: more of them on their way at once are slower (float16 (65536, 2560) 111 us, by four 117; float32 (5883, 1001), x in the cache, 6.3, by two
 // 8.1, by four 11).
 template <typename T, bool RES> __global__ __launch_bounds__(kBlock) void dropout_kernel(const DropoutArgs a) {
   using A = acc_of_t<T>;

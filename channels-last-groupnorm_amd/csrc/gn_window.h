@@ -758,7 +758,7 @@ __device__ __forceinline__ int64_t part_row(const WindowArgs &a, int split, int 
 
 // A workgroup: 128 queries of one head, 32 a wavefront, against one of `splits` shares of the keys that they see.  128 queries share a
 // tile's copy; 64 keys a tile are as many as leave room for four workgroups of heads of 64 in a CU's registers, whose waits hide
-// each other.  float16 15600 tokens, 8 heads of 128, window 2400: 321 us, 880 TFLOP/s (a library's product 1070); bfloat16 4 x
+// each other.  float16 15600 tokens, 8 heads of 128, window 2400: 314 to 330 us a pass, 860 to 900 TFLOP/s (a library's product 1070); bfloat16 4 x
 // 4096, 20 heads of 64: 810; with window 512, where a tenth of the pairs of its tiles is hidden, 675.  FINE: a.fine, as a
 // kernel of its own (float16 heads of 64 have no registers left for both in one, and few queries are 3 % slower with both).
 template <typename T, int DP, bool FINE>

@@ -67,7 +67,8 @@ torch.library.register_autograd("gnop::dropout", _backward, setup_context=_setup
 
 
 def dropout(x, p, seed, offset=0, residual=None, channel_dim=-1):
-    """Each element of x dropped with probability p and otherwise divided by 1 - p, plus the residual, rounded once.
+    """Each element of x dropped with probability p and otherwise times 1 / (1 - p), plus the residual, in float32 (float64 for float64)
+    and rounded to x's type once.
 
     x: any shape, float32, float64, float16 or bfloat16; residual: a tensor like x, or None.  p is taken in whole multiples of
     2^-16.  The mask is a function of the seed, the offset and an element's place among x's, counted in x's order of dimensions with the one at

@@ -134,7 +134,9 @@ int gnnhwc_clip(const void *const *in, void *const *out, const int64_t *n, const
  * zeros; what lies behind n in k and v is not read, in q and out_grad has no effect, and gets zeros for gradients.  An infinity or a NaN reaches
  * only the tokens that see it.
  * Scores, softmax and sums are in float32; softmax weights (and in the backward their derivatives) are rounded to dtype
- * once, as operands of the second product.  dtype: F32, F16 or BF16.
+ * once, as operands of the second product.  dtype: F32, F16 or BF16.  F16 has small ones in fixed steps: weights are off by up to
+ * 2^-25 of their query's largest (in v_grad 2^-37 of one), the derivatives by up to 2^-29 of the largest |out_grad| of the query or,
+ * in k_grad, of the queries that a workgroup visits.
  *   lse      : float (batch, heads, tokens): log2 of the softmax's sum, infinite for a query that sees nothing.  Written by the
  *              forward unless NULL, read by the backward.
  *   out_rest : (batch, tokens, heads, head_dim) of dtype, no gaps, 16-byte aligned: what rounding left of out.  Written by the forward
@@ -175,7 +177,8 @@ size_t gnnhwc_window_bwd_workspace_bytes(const gnnhwc_window_call *call);
 int gnnhwc_window_bwd(const gnnhwc_window_call *call, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
- * Dropout:  y[e] = (kept ? x[e] / (1 - p') : 0) + residual[e],  rounded once, for e in 0 .. n - 1.
+ * Dropout:  y[e] = (kept ? x[e] f : 0) + residual[e],  f = 1 / (1 - p'),  for e in 0 .. n - 1, in float32 (float64 for F64) and rounded to
+ * dtype once.  f is rounded to float32 (float64) itself, so that of F32 and F64 the product is off by a unit in the last place or less.
  * p' is p in whole multiples of 2^-16, rounded to nearest.  Element e is kept if its 16 random bits are at least 65536 p': they are
  * half e % 2 (the lower first) of word (e / 2) % 4 of Philox 4x32 with 7 rounds, whose counter is (e / 8, offset), both 64 bits, the
  * lower word first, and whose key is the seed.  The same seed and offset give the same bits: the backward is this call on the gradient, without a
